@@ -18,6 +18,7 @@ LIB_PATH = os.path.join(HERE, "lib", "libbitsqz_llm.so")
 
 # enum values of include/bitsqz_llm.hpp
 NONE, NF4_DQ, NF4 = -1, 10, 11
+MXFP4, NVFP4 = 8, 9
 INPUT_HOST, INPUT_DEVICE = 0, 1
 SECTION_NONE, SECTION_FP32, SECTION_QUANT, SECTION_TOPK = 0, 1, 2, 3
 FLAG_SVD, FLAG_OUTLIER, FLAG_ERROR = 1, 2, 4
@@ -114,6 +115,16 @@ SIGNATURES = {
     "bsq_batch_lane": (_vp, [_vp, _i]),
     "bsq_batch_compress": (_i, [_vp, C.POINTER(_vp), _i, _i, C.POINTER(_vp), _u64, C.POINTER(_vp), _vp, C.POINTER(_u64)]),
     "bsq_batch_decompress": (_i, [_vp, C.POINTER(_vp), _i, _i, C.POINTER(_vp), _u64]),
+    "bsq_fp4_packed_bytes": (_u64, [_i, _u64, _u64]),
+    "bsq_fp4_scratch_bytes": (_sz, []),
+    "bsq_fp4_quantize": (_i, [_i, _vp, _i, _u64, _u64, _u64, _vp, _vp, _vp, _vp]),
+    "bsq_fp4_dequantize": (_i, [_i, _vp, _u64, _u64, _vp, _i, _u64, _vp]),
+    "bsq_fp4_matmul": (_i, [_i, _vp, _u64, _vp, _u64, _u64, _vp, _i, _u64, _vp, _vp]),
+    "bsq_fp4_grad_scratch_bytes": (_sz, [_vp, _u64, _u64, _u64]),
+    "bsq_fp4_grad_input": (_i, [_i, _vp, _u64, _u64, _vp, _u64, _u64, _vp, _i, _u64, _vp, _vp, _vp]),
+    "bsq_fp4_grad_weight": (_i, [_i, _vp, _u64, _u64, _u64, _vp, _u64, _vp, _i, _u64, _vp, _vp, _vp]),
+    "bsq_grad_norm_scratch_bytes": (_sz, []),
+    "bsq_grad_norm_clip": (_i, [C.POINTER(_vp), C.POINTER(_u64), C.POINTER(_i), _i, C.POINTER(_vp), C.c_double, _i, _vp, _vp, _vp]),
     "bsq_test_inject_status": (None, [_i, _u32]),
     "bsq_test_inject_lane_status": (None, [_vp, _i, _u32]),
     "bsq_build_info": (C.c_char_p, []),

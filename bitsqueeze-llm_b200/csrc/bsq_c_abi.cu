@@ -3,6 +3,8 @@
 #include <bitsqz_llm.hpp>
 #include <bitsqz_llm_c.h>
 
+#include "bsq_fp4.hpp"
+#include "bsq_grad_norm.hpp"
 #include "bsq_internal.hpp"
 
 using namespace bsq;
@@ -163,6 +165,70 @@ int bsq_reconstruct(const float *d_U, const float *d_S, const float *d_V, int m,
     if (!d_U || !d_S || !d_V || !d_out || m <= 0 || n <= 0 || k <= 0) return 1;
     if (d_minuend && !d_flag) return 1;
     return rc(reconstruct_lowrank(d_U, d_S, d_V, m, n, k, d_minuend, d_out, d_flag, d_status, nullptr, 0, device_sm_count(), as_stream(stream)));
+}
+
+// ---- microscaled 4-bit matrices ----
+static inline bool fp4_aligned(const void *packed) { return packed && reinterpret_cast<uintptr_t>(packed) % 16 == 0; }
+static inline bool op_rows_ok(const void *p, int type, uint64_t rows, uint64_t cols, uint64_t ld) {
+    const int size = op_bytes(type);
+    return size && p && reinterpret_cast<uintptr_t>(p) % size == 0 && (rows <= 1 || ld >= cols);
+}
+
+uint64_t bsq_fp4_packed_bytes(int format, uint64_t rows, uint64_t cols) { return fp4_shape_ok(format, rows, cols) ? fp4_packed_bytes(format, rows, cols) : 0; }
+size_t bsq_fp4_scratch_bytes(void) { return kFp4ScratchBytes; }
+int bsq_fp4_quantize(int format, const void *d_x, int type, uint64_t rows, uint64_t cols, uint64_t ld, const float *d_amax, void *d_packed, void *d_scratch,
+                     void *stream) {
+    if (!fp4_shape_ok(format, rows, cols) || !op_bytes(type) || !fp4_aligned(d_packed) || (rows && !op_rows_ok(d_x, type, rows, cols, ld))) return 1;
+    if (format == kNvFp4 && !d_amax && (!d_scratch || reinterpret_cast<uintptr_t>(d_scratch) % 4 != 0)) return 1;
+    return rc(fp4_quantize(format, d_x, type, rows, cols, rows > 1 ? ld : cols, d_amax, d_packed, d_scratch, device_sm_count(), as_stream(stream)));
+}
+int bsq_fp4_dequantize(int format, const void *d_packed, uint64_t rows, uint64_t cols, void *d_out, int type, uint64_t ld, void *stream) {
+    if (!fp4_shape_ok(format, rows, cols) || !op_bytes(type) || !fp4_aligned(d_packed) || (rows && !op_rows_ok(d_out, type, rows, cols, ld))) return 1;
+    return rc(fp4_dequantize(format, d_packed, rows, cols, d_out, type, rows > 1 ? ld : cols, device_sm_count(), as_stream(stream)));
+}
+int bsq_fp4_matmul(int format, const void *d_a, uint64_t M, const void *d_b, uint64_t N, uint64_t K, void *d_out, int type, uint64_t ld, uint32_t *d_status,
+                   void *stream) {
+    if (!fp4_shape_ok(format, M, K) || !fp4_shape_ok(format, N, K) || !op_bytes(type) || !fp4_aligned(d_a) || !fp4_aligned(d_b)) return 1;
+    if (M && N && !op_rows_ok(d_out, type, M, N, ld)) return 1;
+    return rc(fp4_matmul(format, d_a, M, d_b, N, K, d_out, type, M > 1 ? ld : N, d_status, device_sm_count(), as_stream(stream)));
+}
+size_t bsq_fp4_grad_scratch_bytes(const void *d_dy, uint64_t M, uint64_t N, uint64_t ld_dy) { return fp4_grad_scratch_bytes(M, N, d_dy, ld_dy); }
+static inline bool fp4_grad_ok(int format, const void *d_dy, uint64_t M, uint64_t N, uint64_t ld_dy, uint64_t packed_rows, uint64_t K, const void *packed,
+                               const void *d_out, uint64_t out_rows, int type, uint64_t ld, const void *d_scratch) {
+    if (!fp4_shape_ok(format, packed_rows, K) || M > kFp4MaxDim || N > kFp4MaxDim || !op_bytes(type) || !fp4_aligned(packed)) return false;
+    if (M && N && !op_rows_ok(d_dy, kBf16, M, N, ld_dy)) return false;
+    if (out_rows && !op_rows_ok(d_out, type, out_rows, K, ld)) return false;
+    return fp4_grad_scratch_bytes(M, N, d_dy, ld_dy) == 0 || (d_scratch && reinterpret_cast<uintptr_t>(d_scratch) % 16 == 0);
+}
+int bsq_fp4_grad_input(int format, const void *d_dy, uint64_t M, uint64_t ld_dy, const void *d_w, uint64_t N, uint64_t K, void *d_out, int type, uint64_t ld,
+                       void *d_scratch, uint32_t *d_status, void *stream) {
+    if (!fp4_grad_ok(format, d_dy, M, N, ld_dy, N, K, d_w, d_out, M, type, ld, d_scratch)) return 1;
+    return rc(fp4_grad_input(format, d_dy, M, ld_dy, d_w, N, K, d_out, type, M > 1 ? ld : K, d_scratch, d_status, device_sm_count(), as_stream(stream)));
+}
+int bsq_fp4_grad_weight(int format, const void *d_dy, uint64_t M, uint64_t N, uint64_t ld_dy, const void *d_x, uint64_t K, void *d_out, int type, uint64_t ld,
+                        void *d_scratch, uint32_t *d_status, void *stream) {
+    if (!fp4_grad_ok(format, d_dy, M, N, ld_dy, M, K, d_x, d_out, N, type, ld, d_scratch)) return 1;
+    return rc(fp4_grad_weight(format, d_dy, M, N, ld_dy, d_x, K, d_out, type, N > 1 ? ld : K, d_scratch, d_status, device_sm_count(), as_stream(stream)));
+}
+
+// ---- gradients of many tensors ----
+size_t bsq_grad_norm_scratch_bytes(void) { return kNormScratchBytes; }
+int bsq_grad_norm_clip(const void *const *d_grads, const uint64_t *counts, const int *types, int n, void *const *d_outs, double max_norm, int norm_kind, float *d_norm,
+                       void *d_scratch, void *stream) {
+    if (n < 0 || (n && (!d_grads || !counts || !types)) || (norm_kind != 0 && norm_kind != 2) || (d_outs && !(max_norm >= 0.0))) return 1;
+    if (!d_scratch || reinterpret_cast<uintptr_t>(d_scratch) % 8 != 0 || reinterpret_cast<uintptr_t>(d_norm) % 4 != 0 || (!d_outs && !d_norm)) return 1;
+    for (int i = 0; i < n; ++i) {
+        const int size = op_bytes(types[i]);
+        if (!size || counts[i] > (1ull << 44)) return 1;
+        if (counts[i] && (!d_grads[i] || reinterpret_cast<uintptr_t>(d_grads[i]) % size != 0)) return 1;
+        if (counts[i] && d_outs && (!d_outs[i] || reinterpret_cast<uintptr_t>(d_outs[i]) % size != 0)) return 1;
+    }
+    try {
+        if (!norm_layout_ok(d_grads, counts, types, n, d_outs)) return 1;
+        return rc(grad_norm_clip(d_grads, counts, types, n, d_outs, max_norm, norm_kind, d_norm, d_scratch, device_sm_count(), as_stream(stream)));
+    } catch (...) {
+        return 1;
+    }
 }
 
 const char *bsq_build_info(void) { return "bitsqz_llm sm_100a " __DATE__; }

@@ -28,11 +28,9 @@
 #include "bsq_device.cuh"
 #include "bsq_gemm.hpp"
 #include "bsq_gemm_tc.cuh"
-
-#include <cuda.h>
+#include "bsq_tma.cuh"
 
 #include <cstdlib>
-#include <mutex>
 
 namespace bsq {
 namespace {
@@ -44,26 +42,6 @@ constexpr int NTH = 11 * 32;                    // warp 0: A producer, 1: MMA is
 constexpr int XF = 128;                         // transform threads; as many epilogue threads
 constexpr int MAXR = 8;                         // most slots of A / images of B in their rings
 
-// K-major operand in 128-byte-swizzled shared memory: rows of 128 B, groups of 8 rows 1024 B apart (stride byte
-// offset), leading byte offset unused, descriptor version 1, layout type 2 (128-byte swizzle).  Steps of 8 along K
-// inside the 128-byte row are steps of 32 B of the start address.
-__device__ __forceinline__ uint64_t smem_desc_sw128(unsigned addr_bytes) {
-    return (uint64_t)((addr_bytes >> 4) & 0x3FFFu) | (1ull << 16) | ((uint64_t)(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
-}
-
-__device__ __forceinline__ void tma_load_2d(void *dst_smem, const CUtensorMap *map, int x, int y, uint64_t *bar) {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
-                     smem_u32(dst_smem)),
-                 "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar))
-                 : "memory");
-}
-__device__ __forceinline__ void tma_store_2d(const CUtensorMap *map, int x, int y, const void *src_smem) {
-    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y), "r"(smem_u32(src_smem))
-                 : "memory");
-}
-__device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
 // This thread has read its share of a raw slot: the producer's next copy may overwrite it.  The copy writes through the async proxy, which
 // the arrival alone does not order behind the reads: they may still be under way when it is seen.  (Without the fence, products of two
 // matrices side by side had single rows wrong, a few units of four k, in 3 to 6 % of the calls where waiting CTAs of the next kernels shared
@@ -72,22 +50,6 @@ __device__ __forceinline__ void raw_read_done(uint64_t *bar) {
     fence_proxy_async_smem();
     mbar_arrive(bar);
 }
-// Position in a ring of `n` stages and the parity of its current round.  Every role walks its rings with one of these:
-// a division and a remainder by the (run-time) ring length per stage were most of what the single threads that issue
-// the copies and the MMAs executed per stage.
-struct Ring {
-    int pos = 0, n;
-    unsigned par = 0;            // parity of the round `pos` is in
-    bool wrapped = false;        // the ring has been around at least once: the stage at `pos` has a previous use
-    __device__ __forceinline__ explicit Ring(int stages) : n(stages) {}
-    __device__ __forceinline__ void next() {
-        if (++pos == n) { pos = 0; par ^= 1u; wrapped = true; }
-    }
-};
-__device__ __forceinline__ void tc_commit(uint64_t *bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-
 constexpr unsigned RAW_BOX = 32 * 32 * 4;       // A contiguous along M: one box of 32 k x 32 rows, four per slot
 constexpr unsigned RAW_SLOT = 4 * RAW_BOX;
 constexpr unsigned C_BOX = 32 * 32 * 4;         // 32 rows x 32 columns of C on their way out (EPI_STORE, EPI_MINUEND: one box for each of the 8 epilogue warps)
@@ -667,24 +629,6 @@ __global__ void __launch_bounds__(NTH, 1) gemm_tc_tma_kernel(const __grid_consta
     if (warp == 1) {
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_d), "r"(tmem_cols) : "memory");
     }
-}
-
-// cuTensorMapEncodeTiled from the driver, looked up once (the library links the runtime only).
-typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
-                                  const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-EncodeTiledFn encode_tiled() {
-    static EncodeTiledFn fn = nullptr;
-    static std::once_flag once;
-    std::call_once(once, [] {
-        void *p = nullptr;
-        cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<EncodeTiledFn>(p);
-        else
-            cudaGetLastError();
-    });
-    return fn;
 }
 
 bool tma_enabled() {

@@ -1,0 +1,69 @@
+// What the TMA-fed tensor-core kernels share: tiled copies and their tensor maps, operand descriptors of 128-byte-swizzled
+// shared memory, positions in rings of stages.
+#pragma once
+
+#include <cuda.h>
+
+#include <mutex>
+
+#include "bsq_device.cuh"
+
+namespace bsq {
+namespace {
+
+// K-major operand in 128-byte-swizzled shared memory: rows of 128 B, groups of 8 rows 1024 B apart (stride byte
+// offset), leading byte offset unused, descriptor version 1, layout type 2 (128-byte swizzle).  Steps of 8 along K
+// inside the 128-byte row are steps of 32 B of the start address.
+__device__ __forceinline__ uint64_t smem_desc_sw128(unsigned addr_bytes) {
+    return (uint64_t)((addr_bytes >> 4) & 0x3FFFu) | (1ull << 16) | ((uint64_t)(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+__device__ __forceinline__ void tma_load_2d(void *dst_smem, const CUtensorMap *map, int x, int y, uint64_t *bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+                     smem_u32(dst_smem)),
+                 "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap *map, int x, int y, const void *src_smem) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y), "r"(smem_u32(src_smem))
+                 : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// Position in a ring of `n` stages and the parity of its current round.  Every role walks its rings with one of these:
+// a division and a remainder by the (run-time) ring length per stage were most of what the single threads that issue
+// the copies and the MMAs executed per stage.
+struct Ring {
+    int pos = 0, n;
+    unsigned par = 0;            // parity of the round `pos` is in
+    bool wrapped = false;        // the ring has been around at least once: the stage at `pos` has a previous use
+    __device__ __forceinline__ explicit Ring(int stages) : n(stages) {}
+    __device__ __forceinline__ void next() {
+        if (++pos == n) { pos = 0; par ^= 1u; wrapped = true; }
+    }
+};
+__device__ __forceinline__ void tc_commit(uint64_t *bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// cuTensorMapEncodeTiled from the driver, looked up once (the library links the runtime only).
+typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                                  const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+inline EncodeTiledFn encode_tiled() {
+    static EncodeTiledFn fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<EncodeTiledFn>(p);
+        else
+            cudaGetLastError();
+    });
+    return fn;
+}
+
+}  // namespace
+}  // namespace bsq

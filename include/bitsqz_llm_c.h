@@ -253,6 +253,48 @@ int bsq_batch_compress(bsq_batch_t *batch, const float *const *matrices, int cou
 int bsq_batch_decompress(bsq_batch_t *batch, const struct bitsqz_llm_array *const *headers, int count, int payload_on_device,
                          float *const *d_dsts, uint64_t dst_num_elements);
 
+/* ---- microscaled 4-bit matrices: MXFP4 (format 8) and NVFP4 (9), the enumerators of quantization_method_t ------------------------------
+ * (No counterpart in the reference's CUDA modules; its CPU library has formats of these names for flat arrays, legacy_modules/quantization/src/impl/
+ * mxfp4_impl.cpp and nvfp4_impl.cpp.)  An element is an e2m1 value (magnitudes 0 0.5 1 1.5 2 3 4 6) times its block's scale times the matrix's.  Blocks run
+ * along a row: MXFP4 32 elements with a scale 2^(byte - 127), matrix scale 1; NVFP4 16 elements with an E4M3 scale.
+ *
+ * Packed form, bsq_fp4_packed_bytes (0: no such matrix) on a 16-byte boundary: a head of 128 bytes whose first word is the matrix scale (float); the codes, 16
+ * bytes for 32 columns of a row, the even column in the low nibble; from the next multiple of 128 bytes on the scale bytes in tiles of 128 rows x 4 blocks (512
+ * bytes; row r, block b of a tile at (r % 32) * 16 + (r / 32) * 4 + b), tiles of the same rows one behind the other.  Codes behind the last column are 0 up to a
+ * multiple of 32 columns, scales behind the last block of a row 0 up to the end of the tile; scale bytes of rows behind the last one may hold anything.
+ *
+ * type: 0 FP32, 1 FP16, 2 BF16; ld: elements from one row to the next.  Rows may be 0.  All calls enqueue on `stream` and return; they allocate nothing and keep
+ * nothing, and may be captured.  d_status (nullable): bit 0 is set when a bounded wait gave up; the results concerned are NaN then. */
+uint64_t bsq_fp4_packed_bytes(int format, uint64_t rows, uint64_t cols);
+size_t bsq_fp4_scratch_bytes(void);
+/* Codes are x / (block scale * matrix scale) to the nearest, ties to even, saturated at 6, with the decision made exactly.  MXFP4: the block scale is
+ * 2^(floor(log2 m) - 2), at least 2^-127, m the block's largest magnitude.  NVFP4: the matrix scale is the power of two 2^t with the smallest t (-110 to 117) for
+ * which the largest finite magnitude of the matrix is at most 2688 * 2^t -- of the matrix, or *d_amax where that is given (elements above it saturate) -- and the
+ * block scale the nearest E4M3 to m / (6 * 2^t).  A block that holds Inf or NaN gets the scale NaN.  d_scratch: bsq_fp4_scratch_bytes, for NVFP4 without d_amax. */
+int bsq_fp4_quantize(int format, const void *d_x, int type, uint64_t rows, uint64_t cols, uint64_t ld, const float *d_amax, void *d_packed, void *d_scratch,
+                     void *stream);
+/* out = (element * block scale) * matrix scale, rounded once */
+int bsq_fp4_dequantize(int format, const void *d_packed, uint64_t rows, uint64_t cols, void *d_out, int type, uint64_t ld, void *stream);
+/* out[M x N] = A[M x K] B[N x K]^T, both packed in the same format; FP32 sums, the result rounded once */
+int bsq_fp4_matmul(int format, const void *d_a, uint64_t M, const void *d_b, uint64_t N, uint64_t K, void *d_out, int type, uint64_t ld, uint32_t *d_status,
+                   void *stream);
+/* Gradients of y[M x N] = x[M x K] W[N x K]^T from dy (BF16) and the operands as they are packed:  dx[M x K] = dy W,  dW[N x K] = dy^T x.  FP32 sums, the result
+ * rounded once.  d_scratch: bsq_fp4_grad_scratch_bytes on a 16-byte boundary (0 unless dy's rows do not all start on 16 bytes). */
+size_t bsq_fp4_grad_scratch_bytes(const void *d_dy, uint64_t M, uint64_t N, uint64_t ld_dy);
+int bsq_fp4_grad_input(int format, const void *d_dy, uint64_t M, uint64_t ld_dy, const void *d_w, uint64_t N, uint64_t K, void *d_out, int type, uint64_t ld,
+                       void *d_scratch, uint32_t *d_status, void *stream);
+int bsq_fp4_grad_weight(int format, const void *d_dy, uint64_t M, uint64_t N, uint64_t ld_dy, const void *d_x, uint64_t K, void *d_out, int type, uint64_t ld,
+                        void *d_scratch, uint32_t *d_status, void *stream);
+
+/* ---- gradients of many tensors (no counterpart in the reference) -------------------------------------------------------------------------
+ * *d_norm (nullable with d_outs) = the norm of n tensors taken as one vector: norm_kind 2 the square root of the sum of squares, 0 the largest magnitude.  With
+ * d_outs: d_outs[i] = d_grads[i] * min(1, max_norm / (norm + 1e-6)), each in the type of its tensor (type as above, counts[i] elements).  d_outs[i] may be
+ * d_grads[i]; otherwise it must not overlap any input or output (such calls return 1).  A NaN or Inf anywhere shows in the norm and goes through the factor.  The
+ * three arrays are read before the call returns.  d_scratch: bsq_grad_norm_scratch_bytes on an 8-byte boundary. */
+size_t bsq_grad_norm_scratch_bytes(void);
+int bsq_grad_norm_clip(const void *const *d_grads, const uint64_t *counts, const int *types, int n, void *const *d_outs, double max_norm, int norm_kind, float *d_norm,
+                       void *d_scratch, void *stream);
+
 /* Test hook (no counterpart in the reference): the next bsq_compress (which = 0) or bsq_decompress (which = 1) on the
  * current device starts with `bits` set in its device status word, as if a kernel had reported them; that call must
  * return 1.  Lets the error path be tested without making a kernel fail. */
