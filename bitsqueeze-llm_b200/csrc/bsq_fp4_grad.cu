@@ -3,43 +3,50 @@
 // with dY in BF16 and W, X packed (bsq_fp4.hpp).  Both are out[R x C] = op(dY)[R x D] B[D x C], where B's blocks lie along C, not along the
 // dimension D that is summed over, so the block-scaled instructions of bsq_fp4_gemm.cu do not apply: B is decoded to BF16.  A code
 // times its block scale has 6 significant bits and BF16's exponent covers every MXFP4 scale (NVFP4: held 2^12 smaller), so decoding is exact;
-// sums are FP32 in tensor memory, the matrix scale is multiplied in when a tile leaves, and the result is rounded once.  FP32 results are
-// summed in two accumulators, one for each half of D: the tensor core cuts every addition off, which is what such a sum is off by.
+// sums are FP32 in tensor memory, the matrix scale is multiplied in when a tile leaves, and the result is rounded once.  The tensor core
+// cuts every addition off instead of rounding it, and what is lost grows with the length of the chain: results in FP32 leave tensor memory every 1024 of D
+// and are added up rounded (4096 of D: 1.0e-6 off 64 bits in chains of 2048, %SPLITERR in chains of 1024, a rounded FP32 product 3e-7).
 //
-// One CTA per SM walks over tiles of 128 x 256; per 64 of D warp 0 brings a box of dY (128-byte swizzle, in the orientation that memory
-// has; the tensor core reads either) and the packed codes and scales of 64 rows of B (10 KB instead of 32), eight warps decode them into the
-// swizzled operand (contiguous along C), warp 1 issues the MMAs, four warps take finished tiles out.  Decoding costs about as many issue
-// slots as the MMAs take (64 x 256 elements at 3.4 instructions per 32 of them against 512 clocks), so it bounds the kernel together with them.
-// Fewer tiles than SMs: clusters share a tile along D as in bsq_fp4_gemm.cu.
+// Where there are enough tiles, a pair of CTAs on two SMs shares one of 256 x 256 (cta_group::2): each has 128 rows of dY and decodes 128 columns of B, so
+// an element is decoded once for 256 rows of the result.  Per 64 of D warp 0 brings the packed codes and scales of 64 rows of B (5 KB instead of
+// 16), warp 2 a box of dY (128-byte swizzle, in the orientation that memory has; the tensor core reads either), twelve warps decode, four at a stage, into
+// the swizzled operand (contiguous along C), warp 1 of the leader issues the MMAs, four warps take finished tiles out while the next
+// one is computed.  Small results: one CTA per tile of 128 x 128, and clusters that share a tile along D (partial sums through distributed shared memory).
 #include "bsq_fp4_tile.cuh"
 #include "bsq_internal.hpp"
 
 namespace bsq {
 namespace {
 
-constexpr int kGradThreads = 15 * 32;                            // warp 0: copies of B, 1: MMAs, 2-9: decode, 10-13: epilogue, 14: copies of dY
-constexpr int kDecodeWarps = 8;
-constexpr int kTileC = 256, kStageD = 64;
-constexpr int kRing = 3, kRawRing = 6;
+// warp 0: copies of B, 1: MMAs (in the other CTA of a pair: the word that a stage is ready), 2: copies of dY, 4-7: epilogue, 8-: decode
+constexpr int kDecodeWarps = 4, kDecodeGroups = 3;               // at one stage; stages that are decoded at a time
+constexpr int kEpilogueWarps = 4, kFirstDecode = 4 + kEpilogueWarps;
+constexpr int kGradThreads = (kFirstDecode + kDecodeWarps * kDecodeGroups) * 32;
+constexpr int kTileC = 128, kStageD = 64;                        // a CTA's columns of B; of D per stage
+constexpr int kRing = 5, kRawRing = 6;
+constexpr unsigned kBoxBytes = 32 * 128;                         // 32 rows x 128 bytes of the result on their way out: two for each epilogue warp
+constexpr unsigned kBoxesBytes = kEpilogueWarps * 2 * kBoxBytes;
 constexpr unsigned kABytes = 128 * kStageD * 2, kBBytes = kStageD * kTileC * 2, kOpBytes = kABytes + kBBytes;
-constexpr unsigned kCodeBytes = kStageD * kTileC / 2, kRawBytes = kCodeBytes + 2048;
+constexpr unsigned kCodeBytes = kStageD * kTileC / 2, kRawBytes = kCodeBytes + 1024;
 constexpr float kNvHold = 4096.0f;                               // NVFP4: decoded values are held 2^12 smaller
+constexpr int kChainStages = 1024 / kStageD;                     // FP32 results: longest chain of additions in tensor memory
 
 struct Fp4Grad {
     int R, C, D;                     // rows and columns of the result, the dimension that is summed over
     int r_tiles, c_tiles, d_stages, splits, stages_per_split;
     bool a_kmajor;                   // dY contiguous along D (input gradient) or along R (weight gradient)
-    bool halves;                     // two accumulators per tile, instead of two tiles in turn
+    int chain;                       // stages that are summed in one accumulator
     unsigned quads;                  // scale tiles along a row of B
     const uint8_t *scales;
     const float *head;
     void *out;
     long ld;
     int type;
+    bool boxes;                      // the result can be written by TMA
 };
 
 struct GradBars {
-    uint64_t a_full[kRing], ready[kRing], empty[kRing], raw_full[kRawRing], raw_empty[kRawRing], acc_full[2], acc_empty[2], drain;
+    uint64_t full[kRing], empty[kRing], ready[kRing], raw_full[kRawRing], raw_empty[kRawRing], acc_full[2], acc_empty[2], drain;
     unsigned tmem_base, failed;
 };
 
@@ -47,6 +54,15 @@ struct GradBars {
 // byte offset); within one, groups of 8 of K 1024 bytes apart (stride byte offset).  A step of 16 along K is 2048 bytes of the start address.
 __device__ __forceinline__ uint64_t smem_desc_mn_sw128(unsigned addr) {
     return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(8192u >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+__device__ __forceinline__ void mma_f16_pair(unsigned tmem_d, uint64_t desc_a, uint64_t desc_b, unsigned idesc, bool accumulate) {
+    const unsigned acc = accumulate ? 1u : 0u;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5, %5, %5, %5, %5}, p;\n\t}" ::"r"(tmem_d),
+        "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(acc), "r"(0u)
+        : "memory");
 }
 
 __device__ __forceinline__ unsigned mul_bf16x2(unsigned a, unsigned b) {
@@ -83,27 +99,40 @@ template <int FMT> __device__ __forceinline__ unsigned decode_scale(unsigned byt
     return h | (h << 16);
 }
 
-template <int FMT, bool SPLIT>
+// 16 columns of accumulators, decode8's order of columns undone
+__device__ __forceinline__ void read_columns(unsigned taddr, unsigned (&r)[16], bool ok) {
+    unsigned p[16];
+    read16(taddr, p, ok);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) r[j] = p[(j & 8) | ((j & 3) << 1) | ((j & 4) >> 2)];
+}
+
+// CTAS: 1, or 2 for a pair.  SPLIT: the CTAs of a cluster share a tile, each with a slice of D.
+template <int FMT, int CTAS, bool SPLIT>
 __global__ void __launch_bounds__(kGradThreads, 1) fp4_grad_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                                                                   const Fp4Grad g, unsigned *status) {
+                                                                   const __grid_constant__ CUtensorMap map_c, const Fp4Grad g, unsigned *status) {
+    static_assert(CTAS == 1 || !SPLIT, "pairs do not share tiles");
     chain_begin();
     extern __shared__ unsigned char smem_dyn[];
     unsigned char *base = smem_dyn + ((1024u - (smem_u32(smem_dyn) & 1023u)) & 1023u);
-    unsigned char *raw = base + kRing * kOpBytes;
-    GradBars &bars = *reinterpret_cast<GradBars *>(raw + kRawRing * kRawBytes);
-    constexpr int kQuads = FMT == kNvFp4 ? 4 : 2;                // scale tiles across a tile's 256 columns
+    unsigned char *raw = base + kRing * kOpBytes, *boxes = raw + kRawRing * kRawBytes;
+    GradBars &bars = *reinterpret_cast<GradBars *>(boxes + kBoxesBytes);
+    constexpr int kQuads = FMT == kNvFp4 ? 2 : 1;                // scale tiles across a CTA's 128 columns
+    constexpr unsigned kAccCols = CTAS * kTileC;                 // columns of an accumulator
+    constexpr int kSets = SPLIT ? 4 : 2;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int half = CTAS == 2 ? (int)(blockIdx.x & 1) : 0, unit = (int)(blockIdx.x / (SPLIT ? (unsigned)g.splits : (unsigned)CTAS));
     const int rank = SPLIT ? (int)(blockIdx.x % (unsigned)g.splits) : 0;
     const int tiles = g.r_tiles * g.c_tiles;
-    const int first = SPLIT ? (int)(blockIdx.x / (unsigned)g.splits) : (int)blockIdx.x, step = SPLIT ? tiles : (int)gridDim.x;
+    const int first = unit, step = SPLIT ? tiles : (int)(gridDim.x / CTAS);
     const int d0 = rank * g.stages_per_split, d1 = min(g.d_stages, d0 + g.stages_per_split);
-    const int sets = g.halves ? 1 : 2, d_half = g.halves ? d0 + (d1 - d0 + 1) / 2 : d1;
+    const bool leader = half == 0;
 
     if (tid == 0) {
         for (int i = 0; i < kRing; ++i) {
-            mbar_init(&bars.a_full[i], 1);
-            mbar_init(&bars.ready[i], kDecodeWarps);
+            mbar_init(&bars.full[i], 1 + kDecodeWarps + (CTAS == 2 ? 1 : 0));
             mbar_init(&bars.empty[i], 1);
+            mbar_init(&bars.ready[i], kDecodeWarps);
         }
         for (int i = 0; i < kRawRing; ++i) {
             mbar_init(&bars.raw_full[i], 1);
@@ -111,36 +140,36 @@ __global__ void __launch_bounds__(kGradThreads, 1) fp4_grad_kernel(const __grid_
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&bars.acc_full[i], 1);
-            mbar_init(&bars.acc_empty[i], 4);
+            mbar_init(&bars.acc_empty[i], CTAS * kEpilogueWarps);
         }
         mbar_init(&bars.drain, 1);
         bars.failed = 0;
         mbar_fence_init();
     }
-    if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars.tmem_base)), "r"(512u) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
+    if (warp == 1) tmem_alloc<CTAS>(&bars.tmem_base, 512u);
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    if constexpr (CTAS == 2) cg::this_cluster().sync();          // the other CTA's barriers are ready too
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const unsigned tmem = bars.tmem_base;
+    const unsigned lead = CTAS == 2 ? cluster_addr(smem_u32(base), 0u) - smem_u32(base) : 0u;       // from an address here to the leader's
     bool ok = true;
 
     if (warp == 0) {
-        // ---- codes and scales, up to kRawRing stages ahead ----
+        // ---- codes and scales of this CTA's columns, up to kRawRing stages ahead ----
         if (lane == 0) {
             Ring r(kRawRing);
             int filled = 0;
             for (int t = first; t < tiles && ok; t += step) {
-                const unsigned quad = (unsigned)(t / g.r_tiles) * kQuads, sf = min((unsigned)kQuads, g.quads - quad) * 512u;
+                const int c_tile = (t / g.r_tiles) * CTAS + half;
+                const unsigned quad = (unsigned)c_tile * kQuads, sf = quad < g.quads ? min((unsigned)kQuads, g.quads - quad) * 512u : 0u;
                 for (int d = d0; d < d1; ++d, ++filled, r.next()) {
                     if (r.wrapped) ok = mbar_wait_bounded(&bars.raw_empty[r.pos], r.par ^ 1u, status);
                     if (!ok) break;
                     unsigned char *s = raw + (size_t)r.pos * kRawBytes;
                     mbar_expect_tx(&bars.raw_full[r.pos], kCodeBytes + sf);
-                    tma_load_2d(s, &map_b, (t / g.r_tiles) * (kTileC / 2), d * kStageD, &bars.raw_full[r.pos]);
-                    bulk_g2s(s + kCodeBytes, g.scales + ((size_t)(d >> 1) * g.quads + quad) * 512, sf, &bars.raw_full[r.pos]);
+                    tma_load_2d(s, &map_b, c_tile * (kTileC / 2), d * kStageD, &bars.raw_full[r.pos]);
+                    if (sf) bulk_g2s(s + kCodeBytes, g.scales + ((size_t)(d >> 1) * g.quads + quad) * 512, sf, &bars.raw_full[r.pos]);
                 }
             }
             if (!ok) {                                           // copies in flight must have landed before this CTA's shared memory goes away
@@ -149,145 +178,246 @@ __global__ void __launch_bounds__(kGradThreads, 1) fp4_grad_kernel(const __grid_
             }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            // BF16 x BF16, FP32 sums, B contiguous along N, A along K or along M, N >> 3, M >> 4
-            const unsigned idesc = (1u << 4) | (1u << 7) | (1u << 10) | (g.a_kmajor ? 0u : 1u << 15) | (1u << 16) | ((unsigned)(kTileC >> 3) << 17) | ((128u >> 4) << 24);
-            Ring r(kRing), rs(sets);
-            for (int t = first; t < tiles && ok; t += step, rs.next()) {
-                if (rs.wrapped) ok = mbar_wait_bounded(&bars.acc_empty[rs.pos], rs.par ^ 1u, status);
-                if (!ok) break;
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (lane == 0 && !leader) {
+            // this CTA's decoded stages are announced to the leader by one thread: an arrival there waits for all stores in front of it
+            Ring r(kRing);
+            for (int t = first; t < tiles && ok; t += step)
                 for (int d = d0; d < d1; ++d, r.next()) {
-                    ok = mbar_wait_bounded(&bars.a_full[r.pos], r.par, status) && mbar_wait_bounded(&bars.ready[r.pos], r.par, status);
+                    ok = mbar_wait_bounded(&bars.ready[r.pos], r.par, status);
+                    if (!ok) break;
+                    mbar_arrive_pair(smem_u32(&bars.full[r.pos]) + lead);
+                }
+            if (!ok) atomicOr(&bars.failed, 1u);
+        }
+        if (lane == 0 && leader) {
+            // BF16 x BF16, FP32 sums, B contiguous along N, A along K or along M, N >> 3, M >> 4
+            const unsigned idesc = (1u << 4) | (1u << 7) | (1u << 10) | (g.a_kmajor ? 0u : 1u << 15) | (1u << 16) | (kAccCols >> 3 << 17) | ((CTAS * 128u >> 4) << 24);
+            const uint64_t a_step = g.a_kmajor ? 2u : 128u;
+            Ring r(kRing), rs(SPLIT ? 1 : 2);
+            for (int t = first; t < tiles && ok; t += step) {
+                for (int c0 = d0; c0 < d1 && ok; c0 += SPLIT ? d1 - d0 : g.chain, rs.next()) {
+                    const int c1 = SPLIT ? d1 : min(d1, c0 + g.chain);
+                    if (rs.wrapped) ok = mbar_wait_bounded(&bars.acc_empty[rs.pos], rs.par ^ 1u, status);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const unsigned s = smem_u32(base + (size_t)r.pos * kOpBytes);
-                    const uint64_t da = g.a_kmajor ? smem_desc_sw128(s) : smem_desc_mn_sw128(s), db = smem_desc_mn_sw128(s + kABytes);
-                    const uint64_t a_step = g.a_kmajor ? 2u : 128u;
-                    const unsigned acc = tmem + (g.halves ? (d >= d_half ? 256u : 0u) : (unsigned)rs.pos * 256u);
-                    const bool fresh = d == d0 || (g.halves && d == d_half);
+                    for (int d = c0; d < c1; ++d, r.next()) {
+                        ok = mbar_wait_bounded(&bars.full[r.pos], r.par, status);
+                        if (!ok) break;
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        const unsigned s = smem_u32(base + (size_t)r.pos * kOpBytes);
+                        const uint64_t da = g.a_kmajor ? smem_desc_sw128(s) : smem_desc_mn_sw128(s), db = smem_desc_mn_sw128(s + kABytes);
+                        const int set = SPLIT ? (d - c0) / g.chain : rs.pos;                 // (SPLIT: up to four accumulators, one behind the other)
+                        const bool fresh = SPLIT ? (d - c0) % g.chain == 0 : d == c0;
+                        const unsigned acc = tmem + (unsigned)set * kAccCols;
 #pragma unroll
-                    for (int kk = 0; kk < kStageD / 16; ++kk)
-                        mma_f16(acc, da + a_step * (uint64_t)kk, db + (uint64_t)(kk * 128), idesc, !fresh || kk > 0);
-                    tc_commit(&bars.empty[r.pos]);
+                        for (int kk = 0; kk < kStageD / 16; ++kk) {
+                            if (CTAS == 2) mma_f16_pair(acc, da + a_step * (uint64_t)kk, db + (uint64_t)(kk * 128), idesc, !fresh || kk > 0);
+                            else mma_f16(acc, da + a_step * (uint64_t)kk, db + (uint64_t)(kk * 128), idesc, !fresh || kk > 0);
+                        }
+                        if (CTAS == 2) tc_commit_pair(&bars.empty[r.pos], 3);
+                        else tc_commit(&bars.empty[r.pos]);
+                    }
+                    if (ok) {
+                        if (CTAS == 2) tc_commit_pair(&bars.acc_full[rs.pos], 3);
+                        else tc_commit(&bars.acc_full[rs.pos]);
+                    }
                 }
-                if (ok) tc_commit(&bars.acc_full[rs.pos]);
             }
             if (!ok) {
                 atomicOr(&bars.failed, 1u);
-                tc_commit(&bars.drain);                          // MMAs under way must be done before tensor memory is given back
+                if (CTAS == 2) tc_commit_pair(&bars.drain, 1);   // MMAs under way must be done before tensor memory is given back
+                else tc_commit(&bars.drain);
                 mbar_wait_bounded(&bars.drain, 0, status);
             }
         }
-    } else if (warp == 14) {
+    } else if (warp == 2) {
+        // ---- dY ----
         if (lane == 0) {
             Ring r(kRing);
             int filled = 0;
             for (int t = first; t < tiles && ok; t += step) {
-                const int row = (t % g.r_tiles) * 128;
+                const int row = ((t % g.r_tiles) * CTAS + half) * 128;
                 for (int d = d0; d < d1; ++d, ++filled, r.next()) {
                     if (r.wrapped) ok = mbar_wait_bounded(&bars.empty[r.pos], r.par ^ 1u, status);
                     if (!ok) break;
                     unsigned char *s = base + (size_t)r.pos * kOpBytes;
-                    mbar_expect_tx(&bars.a_full[r.pos], kABytes);
-                    if (g.a_kmajor) {
-                        tma_load_2d(s, &map_a, d * kStageD, row, &bars.a_full[r.pos]);
+                    uint64_t *bar = &bars.full[r.pos];
+                    if (leader) mbar_expect_tx(bar, CTAS * kABytes);
+                    if (CTAS == 2) {
+                        const unsigned lead_bar = smem_u32(bar) + lead;
+                        if (g.a_kmajor) {
+                            tma_load_2d_pair(s, &map_a, d * kStageD, row, lead_bar);
+                        } else {
+                            tma_load_2d_pair(s, &map_a, row, d * kStageD, lead_bar);
+                            tma_load_2d_pair(s + kABytes / 2, &map_a, row + 64, d * kStageD, lead_bar);
+                        }
+                    } else if (g.a_kmajor) {
+                        tma_load_2d(s, &map_a, d * kStageD, row, bar);
                     } else {
-                        tma_load_2d(s, &map_a, row, d * kStageD, &bars.a_full[r.pos]);
-                        tma_load_2d(s + kABytes / 2, &map_a, row + 64, d * kStageD, &bars.a_full[r.pos]);
+                        tma_load_2d(s, &map_a, row, d * kStageD, bar);
+                        tma_load_2d(s + kABytes / 2, &map_a, row + 64, d * kStageD, bar);
                     }
                 }
             }
             if (!ok) {
                 atomicOr(&bars.failed, 1u);
-                for (int c = max(0, filled - kRing); c < filled; ++c) mbar_wait_bounded(&bars.a_full[c % kRing], (unsigned)(c / kRing) & 1u, status);
+                if (leader)
+                    for (int c = max(0, filled - kRing); c < filled; ++c) mbar_wait_bounded(&bars.full[c % kRing], (unsigned)(c / kRing) & 1u, status);
             }
         }
-    } else if (warp < 2 + kDecodeWarps) {
-        // ---- decode: a thread has one row of B and, twice, 32 of its columns; the lanes of a warp have rows beside one another, so that neither the
-        // swizzled codes nor the swizzled operand see a bank conflict ----
-        const int w = warp - 2, d_in = (w & 1) * 32 + lane;
+    } else if (warp >= kFirstDecode) {
+        // ---- decode: three groups of four warps take the stages in turn.  A thread has one row of B and, twice, 32 of its columns; the lanes of a warp have
+        // rows beside one another, so that neither the swizzled codes nor the swizzled operand see a bank conflict ----
+        const int w = (warp - kFirstDecode) % kDecodeWarps, d_in = (w & 1) * 32 + lane, turn = (warp - kFirstDecode) / kDecodeWarps;
         Ring r(kRing), rr(kRawRing);
+        int n = 0;
         for (int t = first; t < tiles && ok; t += step) {
-            for (int d = d0; d < d1; ++d, r.next(), rr.next()) {
-                ok = mbar_wait_bounded(&bars.raw_full[rr.pos], rr.par, status);
-                if (ok && r.wrapped) ok = mbar_wait_bounded(&bars.empty[r.pos], r.par ^ 1u, status);
-                ok = __all_sync(kFullMask, ok) != 0;
+            for (int d = d0; d < d1; ++d, n = n + 1 == kDecodeGroups ? 0 : n + 1, r.next(), rr.next()) {
+                if (n != turn) continue;
+                constexpr int kUnits = 8 / kDecodeWarps;         // of 32 columns for each thread
+                ok = __all_sync(kFullMask, mbar_wait_bounded(&bars.raw_full[rr.pos], rr.par, status)) != 0;
                 if (!ok) break;
                 const unsigned char *s = raw + (size_t)rr.pos * kRawBytes;
-                unsigned char *b = base + (size_t)r.pos * kOpBytes + kABytes + d_in * 128;
                 const int row = (d & 1) * 64 + d_in;             // in its scale tile
                 const unsigned char *sf = s + kCodeBytes + (row & 31) * 16 + (row >> 5) * 4;
                 const bool live = d * kStageD + d_in < g.D;      // (scales behind the last row are anything)
+                uint4 v[kUnits][4];
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const int unit = (w >> 1) + 4 * j;
-                    const uint4 c = *reinterpret_cast<const uint4 *>(s + d_in * 128 + ((unit ^ (d_in & 7)) << 4));
+                for (int j = 0; j < kUnits; ++j) {
+                    const int u = (w >> 1) + j * (kDecodeWarps / 2);
+                    const uint4 c = *reinterpret_cast<const uint4 *>(s + d_in * 64 + ((u ^ ((d_in >> 1) & 3)) << 4));
                     unsigned s0, s1;
                     if (FMT == kMxFp4) {
-                        s0 = s1 = decode_scale<FMT>(live ? sf[(unit >> 2) * 512 + (unit & 3)] : 0u);
+                        s0 = s1 = decode_scale<FMT>(live ? sf[u] : 0u);
                     } else {
-                        const unsigned two = live ? *reinterpret_cast<const unsigned short *>(sf + (unit >> 1) * 512 + (unit & 1) * 2) : 0u;
+                        const unsigned two = live ? *reinterpret_cast<const unsigned short *>(sf + (u >> 1) * 512 + (u & 1) * 2) : 0u;
                         s0 = decode_scale<FMT>(two & 0xffu);
                         s1 = decode_scale<FMT>(two >> 8);
                     }
-                    unsigned char *dst = b + (unit >> 1) * 8192;
-                    const int chunk = (unit & 1) * 4, x = d_in & 7;
-                    *reinterpret_cast<uint4 *>(dst + (((chunk + 0) ^ x) << 4)) = decode8<FMT>(c.x, s0);
-                    *reinterpret_cast<uint4 *>(dst + (((chunk + 1) ^ x) << 4)) = decode8<FMT>(c.y, s0);
-                    *reinterpret_cast<uint4 *>(dst + (((chunk + 2) ^ x) << 4)) = decode8<FMT>(c.z, s1);
-                    *reinterpret_cast<uint4 *>(dst + (((chunk + 3) ^ x) << 4)) = decode8<FMT>(c.w, s1);
+                    v[j][0] = decode8<FMT>(c.x, s0);
+                    v[j][1] = decode8<FMT>(c.y, s0);
+                    v[j][2] = decode8<FMT>(c.z, s1);
+                    v[j][3] = decode8<FMT>(c.w, s1);
+                }
+                // only then the operand's place is waited for: what follows is all that a free stage waits for on this side
+                if (r.wrapped) ok = __all_sync(kFullMask, mbar_wait_bounded(&bars.empty[r.pos], r.par ^ 1u, status)) != 0;
+                if (!ok) break;
+                unsigned char *b = base + (size_t)r.pos * kOpBytes + kABytes + d_in * 128;
+#pragma unroll
+                for (int j = 0; j < kUnits; ++j) {
+                    const int u = (w >> 1) + j * (kDecodeWarps / 2);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4 *>(b + (u >> 1) * 8192 + ((((u & 1) * 4 + i) ^ (d_in & 7)) << 4)) = v[j][i];
                 }
                 fence_proxy_async_smem();                        // stores before the tensor core's reads, reads before the next copy's writes
                 __syncwarp();
                 if (lane == 0) {
-                    mbar_arrive(&bars.ready[r.pos]);
+                    mbar_arrive(leader ? &bars.full[r.pos] : &bars.ready[r.pos]);
                     mbar_arrive(&bars.raw_empty[rr.pos]);
                 }
             }
         }
         if (!ok && lane == 0) atomicOr(&bars.failed, 1u);
-    } else {
+    } else if (warp >= 4) {
         const int quarter = warp & 3;                            // the lanes of tensor memory this warp may read
         const float f0 = *g.head, f1 = FMT == kNvFp4 ? kNvHold : 1.0f;
         const int size = g.type == kF32 ? 4 : 2;
-        const bool wide = (reinterpret_cast<uintptr_t>(g.out) | (uintptr_t)(g.ld * size)) % 32 == 0;
-        Ring rs(sets);
-        for (int t = first; t < tiles; t += step, rs.next()) {
-            const int row = (t % g.r_tiles) * 128 + quarter * 32 + lane, col = (t / g.r_tiles) * kTileC;
-            if (ok) ok = __all_sync(kFullMask, mbar_wait_bounded(&bars.acc_full[rs.pos], rs.par, status)) != 0;
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const unsigned taddr = tmem + (unsigned)rs.pos * 256u + ((unsigned)(quarter * 32) << 16);
-            for (int c = 0; c < kTileC; c += 16) {
-                unsigned p[16], r[16];
-                read16(taddr + (unsigned)c, p, ok);
-                if (g.halves && d_half < d1) {
-                    unsigned q[16];
-                    read16(taddr + 256u + (unsigned)c, q, ok);
+        int which = 0;
+        Ring rs(SPLIT ? 1 : 2);
+        for (int t = first; t < tiles; t += step) {
+            const int row = ((t % g.r_tiles) * CTAS + half) * 128 + quarter * 32 + lane, col = (t / g.r_tiles) * (int)kAccCols;
+            for (int c0 = d0; c0 < d1; c0 += SPLIT ? d1 - d0 : g.chain, rs.next()) {
+                if (ok) ok = __all_sync(kFullMask, mbar_wait_bounded(&bars.acc_full[rs.pos], rs.par, status)) != 0;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const unsigned taddr = tmem + (SPLIT ? 0u : (unsigned)rs.pos * kAccCols) + ((unsigned)(quarter * 32) << 16);
+                const bool add = !SPLIT && c0 > d0;              // (FP32 only: to what this warp wrote before)
+                if constexpr (!SPLIT) {
+                    if (g.boxes) {
+                        // through boxes in shared memory, 16-byte pieces swizzled as the tensor map says, written (or added) by TMA as whole lines.  What was written
+                        // to this tile before has to be there before it is added to: in that order every time, the same bits every time.
+                        const int per = 128 / size, row0 = row - lane;
+                        if (add && lane == 0) bulk_wait_all();
+                        for (int c = 0; c < (int)kAccCols; c += per, which ^= 1) {
+                            unsigned char *box = boxes + (unsigned)((warp - 4) * 2 + which) * kBoxBytes;
+                            if (lane == 0) bulk_wait_read_1();   // this box's last copy has been read
+                            __syncwarp();
+                            uint4 *line = reinterpret_cast<uint4 *>(box + lane * 128);
+#pragma unroll 1
+                            for (int h = 0; h < per; h += 16) {
+                                unsigned r[16];
+                                read_columns(taddr + (unsigned)(c + h), r, ok);
+                                float v[16];
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) p[j] = __float_as_uint(__uint_as_float(p[j]) + __uint_as_float(q[j]));
+                                for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]) * f0 * f1;
+                                if (g.type == kF32) {
+#pragma unroll
+                                    for (int j = 0; j < 4; ++j) {
+                                        const float4 o = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+                                        line[(h / 4 + j) ^ (lane & 7)] = *reinterpret_cast<const uint4 *>(&o);
+                                    }
+                                } else {
+                                    unsigned w[8];
+#pragma unroll
+                                    for (int j = 0; j < 8; ++j) w[j] = g.type == kBf16 ? pack_pair<kBf16>(v[2 * j], v[2 * j + 1]) : pack_pair<kF16>(v[2 * j], v[2 * j + 1]);
+                                    line[(h / 8) ^ (lane & 7)] = make_uint4(w[0], w[1], w[2], w[3]);
+                                    line[(h / 8 + 1) ^ (lane & 7)] = make_uint4(w[4], w[5], w[6], w[7]);
+                                }
+                            }
+                            fence_proxy_async_smem();
+                            __syncwarp();
+                            if (lane == 0) {
+                                if (row0 < g.R && col + c < g.C) {
+                                    if (add) tma_add_2d(&map_c, col + c, row0, box);
+                                    else tma_store_2d(&map_c, col + c, row0, box);
+                                }
+                                bulk_commit();
+                            }
+                        }
+                    }
                 }
+                for (int c = 0; c < (SPLIT || !g.boxes ? (int)kAccCols : 0); c += 16) {
+                    unsigned r[16];
+                    read_columns(taddr + (unsigned)c, r, ok);
+                    if constexpr (SPLIT) {
+                        for (int i = 1; i < kSets && i * g.chain < d1 - d0; ++i) {
+                            unsigned q[16];
+                            read_columns(taddr + (unsigned)i * kAccCols + (unsigned)c, q, ok);
 #pragma unroll
-                for (int j = 0; j < 16; ++j) r[j] = p[(j & 8) | ((j & 3) << 1) | ((j & 4) >> 2)];        // decode8's order of columns
-                if constexpr (SPLIT) {
-                    // operand stages are free: every copy has landed and every MMA has read them
-                    float *part = reinterpret_cast<float *>(base) + (quarter * 32 + lane) * (kTileC + 4) + c;
+                            for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + __uint_as_float(q[j]));
+                        }
+                        // operand stages are free: every copy has landed and every MMA has read them
+                        float *part = reinterpret_cast<float *>(base) + (quarter * 32 + lane) * (kTileC + 4) + c;
 #pragma unroll
-                    for (int j = 0; j < 16; j += 4) *reinterpret_cast<uint4 *>(part + j) = make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]);
-                } else {
-                    if (row < g.R && col + c < g.C) store_run16(g.out, g.type, (long)row * g.ld + col + c, r, f0, f1, min(16, g.C - col - c), wide);
+                        for (int j = 0; j < 16; j += 4) *reinterpret_cast<uint4 *>(part + j) = make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]);
+                    } else if (row < g.R && col + c < g.C) {
+                        const int have = min(16, g.C - col - c);
+                        const long at = (long)row * g.ld + col + c;
+                        if (add) {
+                            float *dst = static_cast<float *>(g.out) + at;
+#pragma unroll
+                            for (int j = 0; j < 16; ++j)
+                                if (j < have) dst[j] += __uint_as_float(r[j]) * f0 * f1;
+                        } else {
+                            store_run16(g.out, g.type, at, r, f0, f1, have, false);
+                        }
+                    }
                     __syncwarp();
                 }
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) {
+                    if (CTAS == 2) mbar_arrive_pair(smem_u32(&bars.acc_empty[rs.pos]) + lead);
+                    else mbar_arrive(&bars.acc_empty[rs.pos]);
+                }
             }
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&bars.acc_empty[rs.pos]);
         }
+        if (!SPLIT && lane == 0) bulk_wait_all();
         if (!ok && lane == 0) atomicOr(&bars.failed, 1u);
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    if constexpr (CTAS == 2) cg::this_cluster().sync();          // the leader's MMAs are done with this CTA's memory, the other's arrivals have landed
+    if (warp == 1) tmem_free<CTAS>(tmem, 512u);
 
     if constexpr (SPLIT) {
         cg::cluster_group cluster = cg::this_cluster();
@@ -307,16 +437,23 @@ __global__ void __launch_bounds__(256) pad_rows_kernel(const unsigned short *in,
         for (uint64_t c = (uint64_t)blockIdx.x * 2048 + threadIdx.x; c < min(cols, (uint64_t)(blockIdx.x + 1) * 2048); c += 256) out[r * ld_out + c] = in[r * ld + c];
 }
 
-template <int FMT, bool SPLIT>
-cudaError_t launch_grad(const CUtensorMap &map_a, const CUtensorMap &map_b, const Fp4Grad &g, int sm_count, unsigned *status, cudaStream_t stream) {
-    constexpr size_t smem = 1024 + kRing * kOpBytes + kRawRing * kRawBytes + sizeof(GradBars) + 64;
+template <int FMT, int CTAS, bool SPLIT>
+cudaError_t launch_grad(const CUtensorMap &map_a, const CUtensorMap &map_b, const CUtensorMap &map_c, const Fp4Grad &g, int sm_count, unsigned *status, cudaStream_t stream) {
+    constexpr size_t smem = 1024 + kRing * kOpBytes + kRawRing * kRawBytes + kBoxesBytes + sizeof(GradBars) + 64;
     static_assert(smem <= 227 * 1024, "stages do not fit");
     static_assert((size_t)128 * (kTileC + 4) * 4 <= (size_t)kRing * kOpBytes, "partial tile does not fit");
-    cudaError_t err = cudaFuncSetAttribute(fp4_grad_kernel<FMT, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    cudaError_t err = cudaFuncSetAttribute(fp4_grad_kernel<FMT, CTAS, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (err != cudaSuccess) return err;
     const int tiles = g.r_tiles * g.c_tiles;
-    if (SPLIT) return launch_cluster(fp4_grad_kernel<FMT, SPLIT>, (unsigned)(tiles * g.splits), kGradThreads, g.splits, smem, stream, map_a, map_b, g, status);
-    return launch_chained(fp4_grad_kernel<FMT, SPLIT>, (unsigned)(tiles < sm_count ? tiles : sm_count), kGradThreads, smem, stream, map_a, map_b, g, status);
+    if (SPLIT) return launch_cluster(fp4_grad_kernel<FMT, CTAS, SPLIT>, (unsigned)(tiles * g.splits), kGradThreads, g.splits, smem, stream, map_a, map_b, map_c, g, status);
+    const int units = sm_count / CTAS, grid = (tiles < units ? tiles : units) * CTAS;
+    if (CTAS == 2) return launch_cluster(fp4_grad_kernel<FMT, CTAS, SPLIT>, (unsigned)grid, kGradThreads, CTAS, smem, stream, map_a, map_b, map_c, g, status);
+    return launch_chained(fp4_grad_kernel<FMT, CTAS, SPLIT>, (unsigned)grid, kGradThreads, smem, stream, map_a, map_b, map_c, g, status);
+}
+template <int FMT>
+cudaError_t launch_grad_format(int ctas, const CUtensorMap &map_a, const CUtensorMap &map_b, const CUtensorMap &map_c, const Fp4Grad &g, int sm_count, unsigned *status, cudaStream_t stream) {
+    if (ctas == 2) return launch_grad<FMT, 2, false>(map_a, map_b, map_c, g, sm_count, status, stream);
+    return g.splits > 1 ? launch_grad<FMT, 1, true>(map_a, map_b, map_c, g, sm_count, status, stream) : launch_grad<FMT, 1, false>(map_a, map_b, map_c, g, sm_count, status, stream);
 }
 
 bool needs_padding(const void *dy, uint64_t rows, uint64_t ld) { return reinterpret_cast<uintptr_t>(dy) % 16 != 0 || (rows > 1 && ld % 8 != 0); }
@@ -338,33 +475,45 @@ cudaError_t grad_product(int format, bool a_kmajor, const void *dy, uint64_t M, 
     }
     Fp4Grad g = {};
     g.R = (int)R; g.C = (int)C; g.D = (int)D;
-    const uint64_t r_tiles = (R + 127) / 128, c_tiles = (C + kTileC - 1) / kTileC;
-    if (r_tiles * c_tiles > 0x7fffffffull / 8) return cudaErrorInvalidValue;
-    g.r_tiles = (int)r_tiles; g.c_tiles = (int)c_tiles;
+    const uint64_t r128 = (R + 127) / 128, c128 = (C + kTileC - 1) / kTileC;
+    if (r128 * c128 > 0x7fffffffull / 8) return cudaErrorInvalidValue;
+    // a pair per tile of 256 x 256 where that fills the device
+    const int ctas = r128 > 1 && ((r128 + 1) / 2) * ((c128 + 1) / 2) * 2 >= (uint64_t)sm_count * 2 / 3 ? 2 : 1;
+    g.r_tiles = (int)((r128 + ctas - 1) / ctas); g.c_tiles = (int)((c128 + ctas - 1) / ctas);
     g.d_stages = (int)((D + kStageD - 1) / kStageD);
     g.a_kmajor = a_kmajor;
-    g.halves = type == kF32;
     g.quads = (unsigned)fp4_quads(format, C);
     g.scales = b + fp4_scales_at(D, C);
     g.head = reinterpret_cast<const float *>(b);
     g.out = out; g.ld = (long)ld; g.type = type;
     const int tiles = g.r_tiles * g.c_tiles;
     g.splits = 1;
-    while (g.splits < 8 && tiles * g.splits * 2 <= sm_count && g.d_stages >= g.splits * 4) g.splits *= 2;
+    if (ctas == 1)
+        while (g.splits < 8 && tiles * g.splits * 2 <= sm_count && g.d_stages >= g.splits * 4) g.splits *= 2;
     g.stages_per_split = (g.d_stages + g.splits - 1) / g.splits;
     g.splits = (g.d_stages + g.stages_per_split - 1) / g.stages_per_split;               // no slice is empty
-    CUtensorMap map_a, map_b;
+    g.chain = type != kF32 ? g.stages_per_split : g.splits > 1 ? (g.stages_per_split + 3) / 4 : kChainStages;
+    CUtensorMap map_a, map_b, map_c;
     const cuuint64_t dims_a[2] = {N, M}, strides_a[1] = {ld_a * 2}, dims_b[2] = {fp4_ld(C), D}, strides_b[1] = {fp4_ld(C)};
     const cuuint32_t box_a[2] = {64u, a_kmajor ? 128u : 64u}, box_b[2] = {kTileC / 2, kStageD}, estr[2] = {1, 1};
     if (!encode_tiled() ||
         encode_tiled()(&map_a, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void *>(dy), dims_a, strides_a, box_a, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS ||
         encode_tiled()(&map_b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t *>(b) + kFp4Head, dims_b, strides_b, box_b, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                       CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+                       CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         return cudaErrorInvalidValue;
-    if (format == kNvFp4)
-        return g.splits > 1 ? launch_grad<kNvFp4, true>(map_a, map_b, g, sm_count, status, stream) : launch_grad<kNvFp4, false>(map_a, map_b, g, sm_count, status, stream);
-    return g.splits > 1 ? launch_grad<kMxFp4, true>(map_a, map_b, g, sm_count, status, stream) : launch_grad<kMxFp4, false>(map_a, map_b, g, sm_count, status, stream);
+    map_c = map_a;                                               // (not looked at without boxes)
+    g.boxes = reinterpret_cast<uintptr_t>(out) % 16 == 0 && (R == 1 || ld * op_bytes(type) % 16 == 0);
+    if (g.boxes) {
+        const cuuint64_t dims_c[2] = {C, R}, strides_c[1] = {R == 1 ? (C * op_bytes(type) + 15) / 16 * 16 : ld * op_bytes(type)};
+        const cuuint32_t box_c[2] = {128u / (unsigned)op_bytes(type), 32u};
+        if (encode_tiled()(&map_c, type == kF32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : type == kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, out,
+                           dims_c, strides_c, box_c, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return cudaErrorInvalidValue;
+    }
+    return format == kNvFp4 ? launch_grad_format<kNvFp4>(ctas, map_a, map_b, map_c, g, sm_count, status, stream)
+                            : launch_grad_format<kMxFp4>(ctas, map_a, map_b, map_c, g, sm_count, status, stream);
 }
 
 }  // namespace

@@ -13,6 +13,21 @@ namespace {
 
 namespace cg = cooperative_groups;
 
+// Tensor memory of a CTA, or of both CTAs of a pair (a warp of each executes it)
+template <int CTAS> __device__ __forceinline__ void tmem_alloc(unsigned *base, unsigned cols) {
+    if (CTAS == 2) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(base)), "r"(cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(base)), "r"(cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+}
+template <int CTAS> __device__ __forceinline__ void tmem_free(unsigned base, unsigned cols) {
+    if (CTAS == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(cols) : "memory");
+    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(cols) : "memory");
+}
+
 // 16 neighbouring accumulators of this thread's row; NaN for a tile that was given up
 __device__ __forceinline__ void read16(unsigned taddr, unsigned (&r)[16], bool ok) {
     if (ok) tmem_ld16(taddr, r);

@@ -28,8 +28,26 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap *map, int x, int 
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y), "r"(smem_u32(src_smem))
                  : "memory");
 }
+// ... added to what is there (FP32)
+__device__ __forceinline__ void tma_add_2d(const CUtensorMap *map, int x, int y, const void *src_smem) {
+    asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y), "r"(smem_u32(src_smem))
+                 : "memory");
+}
 __device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// ---- pairs of CTAs (cta_group::2): one MMA over both, issued by the CTA of even rank in the cluster, the leader ----
+// A tiled copy into this CTA's shared memory that counts itself off on a barrier of either CTA of the pair (a shared::cluster address)
+__device__ __forceinline__ void tma_load_2d_pair(void *dst_smem, const CUtensorMap *map, int x, int y, unsigned bar) {
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst_smem)),
+                 "l"(map), "r"(x), "r"(y), "r"(bar)
+                 : "memory");
+}
+// An arrival on a barrier of either CTA of the pair.  What it announces stays where it is and is read by the tensor core of the SM that wrote it (operands in
+// this CTA's shared memory, behind a proxy fence; accumulators that have been read out): nothing has to become visible to threads of the other SM, so the
+// release stays within the CTA.  One of cluster scope waits some 900 clocks for all stores of the SM: a stage of 64 of K then took 2180 clocks instead of 960.
+__device__ __forceinline__ void mbar_arrive_pair(unsigned bar) {
+    asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 // Position in a ring of `n` stages and the parity of its current round.  Every role walks its rings with one of these:
 // a division and a remainder by the (run-time) ring length per stage were most of what the single threads that issue
@@ -45,6 +63,11 @@ struct Ring {
 };
 __device__ __forceinline__ void tc_commit(uint64_t *bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// ... on the barriers at this offset in both CTAs of the pair; `mask`: their ranks in the cluster
+__device__ __forceinline__ void tc_commit_pair(uint64_t *bar, unsigned short mask) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"(mask) : "memory");
 }
 
 // cuTensorMapEncodeTiled from the driver, looked up once (the library links the runtime only).
