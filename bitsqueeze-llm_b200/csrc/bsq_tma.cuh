@@ -36,6 +36,15 @@ __device__ __forceinline__ void tma_add_2d(const CUtensorMap *map, int x, int y,
 __device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+// One lane of a warp whose lanes are all here.  The warp that issues MMAs walks its loops with all lanes and lets one of them issue: addresses and
+// descriptors then stay in uniform registers, which is where these instructions take them from.  In a branch of one lane every operand was moved
+// there one by one, some 100 clocks for each instruction (12 copies of scales and 4 MMAs per stage: 2300 clocks instead of 960).
+__device__ __forceinline__ bool elect_one() {
+    unsigned p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+
 // ---- pairs of CTAs (cta_group::2): one MMA over both, issued by the CTA of even rank in the cluster, the leader ----
 // A tiled copy into this CTA's shared memory that counts itself off on a barrier of either CTA of the pair (a shared::cluster address)
 __device__ __forceinline__ void tma_load_2d_pair(void *dst_smem, const CUtensorMap *map, int x, int y, unsigned bar) {

@@ -159,7 +159,7 @@ def packed(ops, rng, rows, cols, fmt, exact=True, fill=0xFF):
 
 
 MATMUL = [(1, 16, 32), (1, 128, 64), (1, 1031, 300), (3, 257, 1000), (16, 300, 128), (17, 130, 96), (63, 640, 257), (64, 1000, 512), (65, 100, 31), (100, 129, 700),
-          (128, 256, 256), (129, 257, 258), (200, 1500, 640), (777, 515, 1030), (1, 4096, 2048), (40, 40, 4096), (300, 3000, 100), (2500, 2600, 64)]
+          (128, 256, 256), (129, 257, 258), (200, 1500, 640), (777, 515, 1030), (1, 4096, 2048), (40, 40, 4096), (300, 3000, 100), (2500, 2600, 64), (2049, 2600, 700), (1800, 2304, 1031)]
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
