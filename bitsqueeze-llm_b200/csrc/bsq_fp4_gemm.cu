@@ -83,7 +83,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(const __grid_
     const unsigned sp_at = p_bytes + ((q_bytes + 1023u) & ~1023u), sq_at = sp_at + kQuads * 512u;
     const unsigned stage_bytes = stage_bytes_of<FMT, CTAS>(g.q_tile);
     unsigned char *boxes = base + (size_t)g.ring * stage_bytes;
-    Fp4Bars &bars = *reinterpret_cast<Fp4Bars *>(boxes + (g.boxes ? kEpilogueWarps * kBoxBytes : 0u));
+    Fp4Bars &bars = *reinterpret_cast<Fp4Bars *>(boxes + (SPLIT || g.lanes_contiguous ? 0u : kEpilogueWarps * kBoxBytes));
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int side = CTAS == 2 ? (int)(blockIdx.x & 1) : 0;      // which CTA of the pair
     const bool leader = side == 0;
@@ -252,9 +252,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(const __grid_
                     if (CTAS == 2) mbar_arrive_pair(smem_u32(&bars.acc_empty[rs.pos]) + lead);
                     else mbar_arrive(&bars.acc_empty[rs.pos]);
                 }
-                if (g.boxes) {
+                if (!g.lanes_contiguous) {
                     // (tiles of Q of 128 or 256: a warp has 64 or 128 columns, boxes of 128 bytes a row, 16-byte pieces swizzled as the tensor map says)
-                    uint4 *line = reinterpret_cast<uint4 *>(boxes + (unsigned)(warp - 2) * kBoxBytes + (unsigned)lane * 128u);
+                    unsigned char *box = boxes + (unsigned)(warp - 2) * kBoxBytes;
+                    uint4 *line = reinterpret_cast<uint4 *>(box + lane * 128);
                     const int per = 8 / size;                    // chunks of 16 columns in a box
 #pragma unroll
                     for (int c = 0; c < 8; ++c) {
@@ -281,11 +282,19 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(const __grid_
                                 line[(in_box * 2 + 1) ^ (lane & 7)] = make_uint4(w[4], w[5], w[6], w[7]);
                             }
                             if (in_box == per - 1) {
-                                fence_proxy_async_smem();
-                                __syncwarp();
                                 const int col = q0 + (c_first + c + 1 - per) * 16;
-                                if (lane == 0 && p0 < g.P && col < g.Q) tma_store_2d(&maps.out, col, p0, line);
-                                if (lane == 0) bulk_commit();
+                                if (p0 < g.P && col < g.Q) {
+                                    if (g.boxes) {
+                                        fence_proxy_async_smem();
+                                        __syncwarp();
+                                        if (lane == 0) {
+                                            tma_store_2d(&maps.out, col, p0, line);
+                                            bulk_commit();
+                                        }
+                                    } else {
+                                        box_out(box, lane, g.out, size, (long)p0 * g.ld + col, g.ld, g.P - p0, g.Q - col);
+                                    }
+                                }
                             }
                         }
                     }
@@ -294,15 +303,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(const __grid_
 #pragma unroll
                     for (int c = 0; c < 8; ++c) {
                         const int q = q0 + (c_first + c) * 16, have = c < c_count ? min(16, g.Q - q) : 0;
-                        if (have > 0) {
-                            if (g.lanes_contiguous) {
 #pragma unroll
-                                for (int j = 0; j < 16; ++j)
-                                    if (j < have) store_one(g.out, g.type, (long)(q + j) * g.ld + p, __uint_as_float(r[c][j]) * f0 * f1);
-                            } else {
-                                store_run16(g.out, g.type, (long)p * g.ld + q, r[c], f0, f1, have, false);
-                            }
-                        }
+                        for (int j = 0; j < 16; ++j)
+                            if (j < have) store_one(g.out, g.type, (long)(q + j) * g.ld + p, __uint_as_float(r[c][j]) * f0 * f1);
                     }
                 }
             }
@@ -343,7 +346,7 @@ cudaError_t launch_fp4_gemm(GemmMaps &maps, Fp4Gemm &g, const uint8_t *p, const 
     if (!map_codes(&maps.p, p, (uint64_t)g.P, (uint64_t)g.K, 128u) || !map_codes(&maps.q, q, (uint64_t)g.Q, (uint64_t)g.K, (unsigned)(g.q_tile / CTAS)) ||
         !map_scales<FMT>(&maps.p_scales, p, (uint64_t)g.P, (uint64_t)g.K, 1u) || !map_scales<FMT>(&maps.q_scales, q, (uint64_t)g.Q, (uint64_t)g.K, (unsigned)(g.q_tile + 127) / 128))
         return cudaErrorInvalidValue;
-    const size_t stage = stage_bytes_of<FMT, CTAS>(g.q_tile), fixed = 1024 + sizeof(Fp4Bars) + 64 + (g.boxes ? kEpilogueWarps * kBoxBytes : 0);
+    const size_t stage = stage_bytes_of<FMT, CTAS>(g.q_tile), fixed = 1024 + sizeof(Fp4Bars) + 64 + (SPLIT || g.lanes_contiguous ? 0 : kEpilogueWarps * kBoxBytes);
     const size_t room = ((size_t)227 * 1024 - fixed) / stage;
     g.ring = (int)(room < (size_t)kMaxStages ? room : (size_t)kMaxStages);
     const size_t smem = fixed + g.ring * stage;

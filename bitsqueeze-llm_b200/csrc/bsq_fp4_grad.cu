@@ -9,7 +9,7 @@
 //
 // Where there are enough tiles, a pair of CTAs on two SMs shares one of 256 x 256 (cta_group::2): each has 128 rows of dY and decodes 128 columns of B, so
 // an element is decoded once for 256 rows of the result.  Per 64 of D warp 0 brings the packed codes and scales of 64 rows of B (5 KB instead of
-// 16), warp 2 a box of dY (128-byte swizzle, in the orientation that memory has; the tensor core reads either), twelve warps decode, four at a stage, into
+// 16), warp 2 a box of dY (128-byte swizzle, in the orientation that memory has; the tensor core reads either), sixteen warps decode, four at a stage, into
 // the swizzled operand (contiguous along C), warp 1 of the leader issues the MMAs, four warps take finished tiles out while the next
 // one is computed.  Small results: one CTA per tile of 128 x 128, and clusters that share a tile along D (partial sums through distributed shared memory).
 #include "bsq_fp4_tile.cuh"
@@ -19,7 +19,7 @@ namespace bsq {
 namespace {
 
 // warp 0: copies of B, 1: MMAs (in the other CTA of a pair: the word that a stage is ready), 2: copies of dY, 4-7: epilogue, 8-: decode
-constexpr int kDecodeWarps = 4, kDecodeGroups = 3;               // at one stage; stages that are decoded at a time
+constexpr int kDecodeWarps = 4, kDecodeGroups = 4;               // at one stage; stages that are decoded at a time
 constexpr int kEpilogueWarps = 4, kFirstDecode = 4 + kEpilogueWarps;
 constexpr int kGradThreads = (kFirstDecode + kDecodeWarps * kDecodeGroups) * 32;
 constexpr int kTileC = 128, kStageD = 64;                        // a CTA's columns of B; of D per stage
@@ -75,11 +75,13 @@ __device__ __forceinline__ unsigned mul_bf16x2(unsigned a, unsigned b) {
 // the first of its mantissa: read as BF16 that is the element times 2^-126 (also for 0 and 0.5, which are subnormal in both), and multiplying brings it
 // back.  Word i holds elements i and i + 4: columns of a group of 8 come out in the order 0 4 1 5 2 6 3 7, which the epilogue undoes for nothing.
 template <int FMT> __device__ __forceinline__ uint4 decode8(unsigned x, unsigned scale2) {
+    // (shifts to the left, which go to the multiply pipe: the integer pipe with its half rate is what decoding is short of)
+    const unsigned y = x >> 6;
     unsigned w[4];
     w[0] = ((x << 12) & 0x80008000u) | ((x << 6) & 0x01C001C0u);
     w[1] = ((x << 8) & 0x80008000u) | ((x << 2) & 0x01C001C0u);
-    w[2] = ((x << 4) & 0x80008000u) | ((x >> 2) & 0x01C001C0u);
-    w[3] = (x & 0x80008000u) | ((x >> 6) & 0x01C001C0u);
+    w[2] = ((x << 4) & 0x80008000u) | ((y << 4) & 0x01C001C0u);
+    w[3] = (x & 0x80008000u) | (y & 0x01C001C0u);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         if (FMT == kMxFp4) w[i] = mul_bf16x2(w[i], 0x7E807E80u);  // 2^126: the element itself, exact; the scale's range needs a product of its own
@@ -189,7 +191,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) fp4_grad_kernel(const __grid_
                 }
             if (!ok) atomicOr(&bars.failed, 1u);
         }
-        if (lane == 0 && leader) {
+        if (leader) {
             // BF16 x BF16, FP32 sums, B contiguous along N, A along K or along M, N >> 3, M >> 4
             const unsigned idesc = (1u << 4) | (1u << 7) | (1u << 10) | (g.a_kmajor ? 0u : 1u << 15) | (1u << 16) | (kAccCols >> 3 << 17) | ((CTAS * 128u >> 4) << 24);
             const uint64_t a_step = g.a_kmajor ? 2u : 128u;
@@ -197,33 +199,43 @@ __global__ void __launch_bounds__(kGradThreads, 1) fp4_grad_kernel(const __grid_
             for (int t = first; t < tiles && ok; t += step) {
                 for (int c0 = d0; c0 < d1 && ok; c0 += SPLIT ? d1 - d0 : g.chain, rs.next()) {
                     const int c1 = SPLIT ? d1 : min(d1, c0 + g.chain);
-                    if (rs.wrapped) ok = mbar_wait_bounded(&bars.acc_empty[rs.pos], rs.par ^ 1u, status);
+                    if (rs.wrapped) ok = __all_sync(kFullMask, mbar_wait_bounded(&bars.acc_empty[rs.pos], rs.par ^ 1u, status)) != 0;
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    int set = SPLIT ? 0 : rs.pos, left = g.chain;                            // (SPLIT: up to four accumulators, one behind the other)
+                    bool fresh = true;
                     for (int d = c0; d < c1; ++d, r.next()) {
-                        ok = mbar_wait_bounded(&bars.full[r.pos], r.par, status);
+                        ok = __all_sync(kFullMask, mbar_wait_bounded(&bars.full[r.pos], r.par, status)) != 0;
                         if (!ok) break;
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                        const unsigned s = smem_u32(base + (size_t)r.pos * kOpBytes);
+                        const unsigned s = smem_u32(base) + (unsigned)r.pos * kOpBytes;
                         const uint64_t da = g.a_kmajor ? smem_desc_sw128(s) : smem_desc_mn_sw128(s), db = smem_desc_mn_sw128(s + kABytes);
-                        const int set = SPLIT ? (d - c0) / g.chain : rs.pos;                 // (SPLIT: up to four accumulators, one behind the other)
-                        const bool fresh = SPLIT ? (d - c0) % g.chain == 0 : d == c0;
                         const unsigned acc = tmem + (unsigned)set * kAccCols;
+                        if (elect_one()) {
 #pragma unroll
-                        for (int kk = 0; kk < kStageD / 16; ++kk) {
-                            if (CTAS == 2) mma_f16_pair(acc, da + a_step * (uint64_t)kk, db + (uint64_t)(kk * 128), idesc, !fresh || kk > 0);
-                            else mma_f16(acc, da + a_step * (uint64_t)kk, db + (uint64_t)(kk * 128), idesc, !fresh || kk > 0);
+                            for (int kk = 0; kk < kStageD / 16; ++kk) {
+                                if (CTAS == 2) mma_f16_pair(acc, da + a_step * (uint64_t)kk, db + (uint64_t)(kk * 128), idesc, !fresh || kk > 0);
+                                else mma_f16(acc, da + a_step * (uint64_t)kk, db + (uint64_t)(kk * 128), idesc, !fresh || kk > 0);
+                            }
+                            if (CTAS == 2) tc_commit_pair(&bars.empty[r.pos], 3);
+                            else tc_commit(&bars.empty[r.pos]);
                         }
-                        if (CTAS == 2) tc_commit_pair(&bars.empty[r.pos], 3);
-                        else tc_commit(&bars.empty[r.pos]);
+                        __syncwarp();
+                        fresh = false;
+                        if (SPLIT && --left == 0) {
+                            ++set;
+                            left = g.chain;
+                            fresh = true;
+                        }
                     }
-                    if (ok) {
+                    if (ok && elect_one()) {
                         if (CTAS == 2) tc_commit_pair(&bars.acc_full[rs.pos], 3);
                         else tc_commit(&bars.acc_full[rs.pos]);
                     }
+                    __syncwarp();
                 }
             }
-            if (!ok) {
+            if (!ok && lane == 0) {
                 atomicOr(&bars.failed, 1u);
                 if (CTAS == 2) tc_commit_pair(&bars.drain, 1);   // MMAs under way must be done before tensor memory is given back
                 else tc_commit(&bars.drain);
@@ -266,7 +278,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) fp4_grad_kernel(const __grid_
             }
         }
     } else if (warp >= kFirstDecode) {
-        // ---- decode: three groups of four warps take the stages in turn.  A thread has one row of B and, twice, 32 of its columns; the lanes of a warp have
+        // ---- decode: four groups of four warps take the stages in turn.  A thread has one row of B and, twice, 32 of its columns; the lanes of a warp have
         // rows beside one another, so that neither the swizzled codes nor the swizzled operand see a bank conflict ----
         const int w = (warp - kFirstDecode) % kDecodeWarps, d_in = (w & 1) * 32 + lane, turn = (warp - kFirstDecode) / kDecodeWarps;
         Ring r(kRing), rr(kRawRing);
@@ -331,54 +343,10 @@ __global__ void __launch_bounds__(kGradThreads, 1) fp4_grad_kernel(const __grid_
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const unsigned taddr = tmem + (SPLIT ? 0u : (unsigned)rs.pos * kAccCols) + ((unsigned)(quarter * 32) << 16);
                 const bool add = !SPLIT && c0 > d0;              // (FP32 only: to what this warp wrote before)
-                if constexpr (!SPLIT) {
-                    if (g.boxes) {
-                        // through boxes in shared memory, 16-byte pieces swizzled as the tensor map says, written (or added) by TMA as whole lines.  What was written
-                        // to this tile before has to be there before it is added to: in that order every time, the same bits every time.
-                        const int per = 128 / size, row0 = row - lane;
-                        if (add && lane == 0) bulk_wait_all();
-                        for (int c = 0; c < (int)kAccCols; c += per, which ^= 1) {
-                            unsigned char *box = boxes + (unsigned)((warp - 4) * 2 + which) * kBoxBytes;
-                            if (lane == 0) bulk_wait_read_1();   // this box's last copy has been read
-                            __syncwarp();
-                            uint4 *line = reinterpret_cast<uint4 *>(box + lane * 128);
-#pragma unroll 1
-                            for (int h = 0; h < per; h += 16) {
-                                unsigned r[16];
-                                read_columns(taddr + (unsigned)(c + h), r, ok);
-                                float v[16];
-#pragma unroll
-                                for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]) * f0 * f1;
-                                if (g.type == kF32) {
-#pragma unroll
-                                    for (int j = 0; j < 4; ++j) {
-                                        const float4 o = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-                                        line[(h / 4 + j) ^ (lane & 7)] = *reinterpret_cast<const uint4 *>(&o);
-                                    }
-                                } else {
-                                    unsigned w[8];
-#pragma unroll
-                                    for (int j = 0; j < 8; ++j) w[j] = g.type == kBf16 ? pack_pair<kBf16>(v[2 * j], v[2 * j + 1]) : pack_pair<kF16>(v[2 * j], v[2 * j + 1]);
-                                    line[(h / 8) ^ (lane & 7)] = make_uint4(w[0], w[1], w[2], w[3]);
-                                    line[(h / 8 + 1) ^ (lane & 7)] = make_uint4(w[4], w[5], w[6], w[7]);
-                                }
-                            }
-                            fence_proxy_async_smem();
-                            __syncwarp();
-                            if (lane == 0) {
-                                if (row0 < g.R && col + c < g.C) {
-                                    if (add) tma_add_2d(&map_c, col + c, row0, box);
-                                    else tma_store_2d(&map_c, col + c, row0, box);
-                                }
-                                bulk_commit();
-                            }
-                        }
-                    }
-                }
-                for (int c = 0; c < (SPLIT || !g.boxes ? (int)kAccCols : 0); c += 16) {
-                    unsigned r[16];
-                    read_columns(taddr + (unsigned)c, r, ok);
-                    if constexpr (SPLIT) {
+                if constexpr (SPLIT) {
+                    for (int c = 0; c < (int)kAccCols; c += 16) {
+                        unsigned r[16];
+                        read_columns(taddr + (unsigned)c, r, ok);
                         for (int i = 1; i < kSets && i * g.chain < d1 - d0; ++i) {
                             unsigned q[16];
                             read_columns(taddr + (unsigned)i * kAccCols + (unsigned)c, q, ok);
@@ -389,19 +357,53 @@ __global__ void __launch_bounds__(kGradThreads, 1) fp4_grad_kernel(const __grid_
                         float *part = reinterpret_cast<float *>(base) + (quarter * 32 + lane) * (kTileC + 4) + c;
 #pragma unroll
                         for (int j = 0; j < 16; j += 4) *reinterpret_cast<uint4 *>(part + j) = make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]);
-                    } else if (row < g.R && col + c < g.C) {
-                        const int have = min(16, g.C - col - c);
-                        const long at = (long)row * g.ld + col + c;
-                        if (add) {
-                            float *dst = static_cast<float *>(g.out) + at;
+                    }
+                } else {
+                    // through boxes in shared memory, 16-byte pieces swizzled as the tensor map says, written (or added) by TMA as whole lines.  What was written to
+                    // this tile before has to be there before it is added to: in that order every time, the same bits every time.
+                    const int per = 128 / size, row0 = row - lane;
+                    if (add && lane == 0) bulk_wait_all();
+                    for (int c = 0; c < (int)kAccCols; c += per, which ^= 1) {
+                        unsigned char *box = boxes + (unsigned)((warp - 4) * 2 + which) * kBoxBytes;
+                        if (lane == 0) bulk_wait_read_1();       // this box's last copy has been read
+                        __syncwarp();
+                        uint4 *line = reinterpret_cast<uint4 *>(box + lane * 128);
+#pragma unroll 1
+                        for (int h = 0; h < per; h += 16) {
+                            unsigned r[16];
+                            read_columns(taddr + (unsigned)(c + h), r, ok);
+                            float v[16];
 #pragma unroll
-                            for (int j = 0; j < 16; ++j)
-                                if (j < have) dst[j] += __uint_as_float(r[j]) * f0 * f1;
+                            for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]) * f0 * f1;
+                            if (g.type == kF32) {
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) {
+                                    const float4 o = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+                                    line[(h / 4 + j) ^ (lane & 7)] = *reinterpret_cast<const uint4 *>(&o);
+                                }
+                            } else {
+                                unsigned w[8];
+#pragma unroll
+                                for (int j = 0; j < 8; ++j) w[j] = g.type == kBf16 ? pack_pair<kBf16>(v[2 * j], v[2 * j + 1]) : pack_pair<kF16>(v[2 * j], v[2 * j + 1]);
+                                line[(h / 8) ^ (lane & 7)] = make_uint4(w[0], w[1], w[2], w[3]);
+                                line[(h / 8 + 1) ^ (lane & 7)] = make_uint4(w[4], w[5], w[6], w[7]);
+                            }
+                        }
+                        if (row0 >= g.R || col + c >= g.C) continue;
+                        if (g.boxes) {
+                            fence_proxy_async_smem();
+                            __syncwarp();
+                            if (lane == 0) {
+                                if (add) tma_add_2d(&map_c, col + c, row0, box);
+                                else tma_store_2d(&map_c, col + c, row0, box);
+                                bulk_commit();
+                            }
+                        } else if (add) {
+                            box_add(box, lane, static_cast<float *>(g.out), (long)row0 * g.ld + col + c, g.ld, g.R - row0, g.C - col - c);
                         } else {
-                            store_run16(g.out, g.type, at, r, f0, f1, have, false);
+                            box_out(box, lane, g.out, size, (long)row0 * g.ld + col + c, g.ld, g.R - row0, g.C - col - c);
                         }
                     }
-                    __syncwarp();
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();

@@ -38,39 +38,40 @@ __device__ __forceinline__ void read16(unsigned taddr, unsigned (&r)[16], bool o
     }
 }
 
-// 16 neighbouring results (one row of the tile) to memory
-__device__ __forceinline__ void store_run16(void *out, int type, long at, const unsigned (&r)[16], float f0, float f1, int have, bool wide) {
-    float v[16];
-#pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]) * f0 * f1;
-    if (type == kF32) {
-        float *dst = static_cast<float *>(out) + at;
-        if (wide && have == 16) {
-            st_global_v8(dst, make_float4(v[0], v[1], v[2], v[3]), make_float4(v[4], v[5], v[6], v[7]));
-            st_global_v8(dst + 8, make_float4(v[8], v[9], v[10], v[11]), make_float4(v[12], v[13], v[14], v[15]));
-        } else {
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-                if (j < have) dst[j] = v[j];
-        }
-        return;
-    }
-    unsigned w[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) w[j] = type == kBf16 ? pack_pair<kBf16>(v[2 * j], v[2 * j + 1]) : pack_pair<kF16>(v[2 * j], v[2 * j + 1]);
-    unsigned short *dst = static_cast<unsigned short *>(out) + at;
-    if (wide && have == 16) {
-        st_words8(dst, w);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-            if (j < have) dst[j] = (unsigned short)(j & 1 ? w[j >> 1] >> 16 : w[j >> 1]);
-    }
-}
 __device__ __forceinline__ void store_one(void *out, int type, long at, float v) {
     if (type == kF32) store_elem<kF32>(out, (uint64_t)at, v);
     else if (type == kBf16) store_elem<kBf16>(out, (uint64_t)at, v);
     else store_elem<kF16>(out, (uint64_t)at, v);
+}
+
+// A box of 32 rows x 128 bytes, as the epilogues of the products leave it in shared memory (16-byte piece i of row r at piece i ^ (r & 7)), to a result whose rows
+// TMA cannot take (stride or start off 16 bytes): a row at a time, neighbouring lanes neighbouring elements.  (A row per lane and element after element, as it
+// lies in the registers, touches 32 lines with every store: 1031 x 3001 results of 1501 products took 57 us, this way %BOXUS.)
+__device__ __forceinline__ void box_out(const unsigned char *box, int lane, void *out, int size, long at, long ld, int rows, int cols) {
+    const int per_lane = 128 / size / 32;                        // elements of a row for each lane: 1 (FP32) or 2
+    __syncwarp();
+#pragma unroll 4
+    for (int r = 0; r < min(rows, 32); ++r) {
+        const unsigned w = *reinterpret_cast<const unsigned *>(box + r * 128 + ((((lane >> 2) ^ (r & 7)) << 4) | ((lane & 3) << 2)));
+        const long to = at + (long)r * ld + lane * per_lane;
+        if (size == 4) {
+            if (lane < cols) static_cast<unsigned *>(out)[to] = w;
+        } else {
+            if (2 * lane < cols) static_cast<unsigned short *>(out)[to] = (unsigned short)w;
+            if (2 * lane + 1 < cols) static_cast<unsigned short *>(out)[to + 1] = (unsigned short)(w >> 16);
+        }
+    }
+    __syncwarp();
+}
+// ... added to what is there (FP32)
+__device__ __forceinline__ void box_add(const unsigned char *box, int lane, float *out, long at, long ld, int rows, int cols) {
+    __syncwarp();
+#pragma unroll 4
+    for (int r = 0; r < min(rows, 32); ++r) {
+        const float v = *reinterpret_cast<const float *>(box + r * 128 + ((((lane >> 2) ^ (r & 7)) << 4) | ((lane & 3) << 2)));
+        if (lane < cols) out[at + (long)r * ld + lane] += v;
+    }
+    __syncwarp();
 }
 
 // The rows that fall to CTA `rank` of a tile whose partial sums lie in the shared memory of the `splits` CTAs of a cluster (each `rows` x `run`, `run`
