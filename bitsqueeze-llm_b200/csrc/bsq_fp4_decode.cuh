@@ -1,0 +1,48 @@
+// Decoding of 4-bit values to BF16, exact, eight at a time.
+#pragma once
+
+#include "bsq_fp4.cuh"
+
+namespace bsq {
+namespace {
+
+constexpr float kNvHold = 4096.0f;                               // NVFP4: decoded values are held 2^12 smaller
+
+__device__ __forceinline__ unsigned mul_bf16x2(unsigned a, unsigned b) {
+    unsigned r;
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+
+// Eight codes to BF16, times a scale.  Sign and the three magnitude bits are moved to where BF16 has its sign, the last two bits of its exponent and
+// the first of its mantissa: read as BF16 that is the element times 2^-126 (also for 0 and 0.5, which are subnormal in both), and multiplying brings it
+// back.  Word i holds elements i and i + 4: columns of a group of 8 come out in the order 0 4 1 5 2 6 3 7, which the epilogue undoes for nothing.
+template <int FMT> __device__ __forceinline__ uint4 decode8(unsigned x, unsigned scale2) {
+    // (shifts to the left, which go to the multiply pipe: the integer pipe with its half rate is what decoding is short of)
+    const unsigned y = x >> 6;
+    unsigned w[4];
+    w[0] = ((x << 12) & 0x80008000u) | ((x << 6) & 0x01C001C0u);
+    w[1] = ((x << 8) & 0x80008000u) | ((x << 2) & 0x01C001C0u);
+    w[2] = ((x << 4) & 0x80008000u) | ((y << 4) & 0x01C001C0u);
+    w[3] = (x & 0x80008000u) | (y & 0x01C001C0u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (FMT == kMxFp4) w[i] = mul_bf16x2(w[i], 0x7E807E80u);  // 2^126: the element itself, exact; the scale's range needs a product of its own
+        w[i] = mul_bf16x2(w[i], scale2);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// The factor of decode8 from a scale byte, in both halves of a word
+template <int FMT> __device__ __forceinline__ unsigned decode_scale(unsigned byte) {
+    unsigned h;
+    if (FMT == kMxFp4) {
+        h = byte == 0 ? 0x0040u : byte == 255 ? 0x7FFFu : byte << 7;
+    } else {
+        byte &= 0x7fu;                                           // s * 2^(126 - 12), exact in BF16
+        h = byte == 0x7fu ? 0x7FFFu : __float_as_uint(e4m3_decode(byte) * 2.076918743413931e34f) >> 16;
+    }
+    return h | (h << 16);
+}
+
+}  // namespace
+}  // namespace bsq

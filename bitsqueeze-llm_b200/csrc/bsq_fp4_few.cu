@@ -1,0 +1,204 @@
+// Gradient of the input for up to 16 rows of dY (a few tokens): out[R x C] = dY[R x D] W[D x C], W packed (bsq_fp4.hpp).
+//
+// W is read once and bounds it: 0.53 bytes an element from memory, and 3 instructions an element to decode it.  On the path of bsq_fp4_grad.cu every
+// decoded element goes through shared memory and three barriers to a tensor core that has next to nothing to do; here it is decoded in the register
+// that mma.sync takes it from.  A warp has 128 columns and 32 rows of W at a time; thread (g, t) of it has the 16 columns 16 g.. and the 8 rows 8 t.. .
+// The sum may take rows in any order, so the k of an MMA are dealt to fit: B wants pairs of k in a register, and the codes of rows 2 p and
+// 2 p + 1, their 16-bit halves put side by side, are decoded to just such pairs by decode8, column after column; A's pairs are neighbours in dY, so that
+// eight rows of W make one 16-byte load of dY.  Column i of every thread's 16 is one MMA's n, so a thread ends up with 32 neighbouring
+// columns of the result.
+//
+// Codes and scales come by cp.async, four stages of 32 rows ahead for each warp on its own (18 KB a CTA and stage, no barrier in the loop).  The warps of a CTA and
+// the CTAs of a cluster share the rows; their sums are added in a fixed order.
+#include "bsq_fp4_decode.cuh"
+#include "bsq_fp4_few.hpp"
+#include "bsq_fp4_tile.cuh"
+
+namespace bsq {
+namespace {
+
+constexpr int kFewThreads = 256, kFewWarps = kFewThreads / 32, kFewStages = 4, kFewCols = 128, kFewRows = 32;
+constexpr unsigned kFewCodes = kFewRows * kFewCols / 2, kFewStage = kFewCodes + 256;
+
+struct Fp4Few {
+    int R, C, D, chunks, splits, chunks_per_split;
+    const uint8_t *codes, *scales;
+    uint64_t ld_codes, quads;
+    const float *head;
+    const __nv_bfloat16 *dy;
+    uint64_t ld_dy;
+    void *out;
+    long ld;
+    int type;
+};
+
+// 16 or 4 bytes into shared memory in the background; zeros where `live` is false
+__device__ __forceinline__ void copy16(unsigned dst, const void *src, bool live) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy4(unsigned dst, const void *src, bool live) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(live ? 4 : 0) : "memory");
+}
+
+__device__ __forceinline__ void mma_16816(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Eight neighbouring elements of a row of dY from column d on; zeros behind the last one
+__device__ __forceinline__ uint4 load_dy(const __nv_bfloat16 *row, int d, int D, bool live) {
+    if (!live || d >= D) return make_uint4(0u, 0u, 0u, 0u);
+    if (d + 8 <= D) return *reinterpret_cast<const uint4 *>(row + d);
+    unsigned w[4] = {0u, 0u, 0u, 0u};
+    const unsigned short *p = reinterpret_cast<const unsigned short *>(row + d);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (d + i < D) w[i >> 1] |= (unsigned)p[i] << (16 * (i & 1));
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <int FMT> __global__ void __launch_bounds__(kFewThreads, 2) fp4_grad_few_kernel(const Fp4Few g) {
+    chain_begin();
+    extern __shared__ __align__(16) unsigned char smem_few[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, t = lane & 3;
+    const int rank = (int)(blockIdx.x % (unsigned)g.splits), col0 = (int)(blockIdx.x / (unsigned)g.splits) * kFewCols;
+    const int c_end = min(g.chunks, (rank + 1) * g.chunks_per_split);
+    constexpr int kQuads = FMT == kNvFp4 ? 2 : 1;
+    unsigned char *mine = smem_few + (unsigned)warp * kFewStages * kFewStage;
+    const unsigned mine_u = smem_u32(mine);
+
+    // row r of a chunk lies at place (r & 7) * 4 + (r >> 3): the four threads t that read rows 8 t + j at once read neighbouring places
+    const auto fetch = [&](int chunk, int stage) {
+        if (chunk < c_end) {
+            const uint64_t row0 = (uint64_t)chunk * kFewRows;
+            const unsigned dst = mine_u + (unsigned)stage * kFewStage;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int r = (lane >> 2) + 8 * i;
+                const uint64_t at = (uint64_t)(col0 / 2) + (uint64_t)(lane & 3) * 16;
+                const bool live = row0 + r < (uint64_t)g.D && at < g.ld_codes;
+                copy16(dst + (unsigned)(((r & 7) * 4 + (r >> 3)) * 64 + (lane & 3) * 16), live ? g.codes + (row0 + r) * g.ld_codes + at : g.codes, live);
+            }
+            const uint64_t tile = (row0 / 128 * g.quads + (uint64_t)(col0 / (FMT == kNvFp4 ? 64 : 128))) * 512;
+            const unsigned in_tile = (unsigned)lane * 16 + (unsigned)(chunk & 3) * 4;            // (32 rows of a chunk are 32 neighbours of a tile)
+#pragma unroll
+            for (int q = 0; q < kQuads; ++q) {
+                const bool live = row0 + lane < (uint64_t)g.D && (uint64_t)(col0 / (FMT == kNvFp4 ? 64 : 128) + q) < g.quads;
+                copy4(dst + kFewCodes + (unsigned)((((lane & 7) * 4 + (lane >> 3)) * kQuads + q) * 4), live ? g.scales + tile + q * 512 + in_tile : g.scales, live);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+
+    const int first = rank * g.chunks_per_split + warp;
+    const __nv_bfloat16 *a0 = g.dy + (uint64_t)gq * g.ld_dy, *a1 = g.dy + (uint64_t)(gq + 8) * g.ld_dy;
+    const bool live0 = gq < g.R, live1 = gq + 8 < g.R;
+    float acc[16][4];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
+#pragma unroll
+    for (int s = 0; s < kFewStages - 1; ++s) fetch(first + s * kFewWarps, s);
+    uint4 n0 = load_dy(a0, first * kFewRows + 8 * t, first < c_end ? g.D : 0, live0), n1 = load_dy(a1, first * kFewRows + 8 * t, first < c_end ? g.D : 0, live1);
+    int stage = 0;
+    for (int chunk = first; chunk < c_end; chunk += kFewWarps) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kFewStages - 2) : "memory");
+        __syncwarp();                                            // everybody's copies of this stage are there, and everybody is done with the one before
+        fetch(chunk + (kFewStages - 1) * kFewWarps, (stage + kFewStages - 1) % kFewStages);
+        const uint4 d0 = n0, d1 = n1;
+        const int next = chunk + kFewWarps;
+        n0 = load_dy(a0, next * kFewRows + 8 * t, next < c_end ? g.D : 0, live0);
+        n1 = load_dy(a1, next * kFewRows + 8 * t, next < c_end ? g.D : 0, live1);
+        const unsigned char *s = mine + (unsigned)stage * kFewStage;
+#pragma unroll
+        for (int step = 0; step < 2; ++step) {
+            const unsigned a[4] = {step ? d0.z : d0.x, step ? d1.z : d1.x, step ? d0.w : d0.y, step ? d1.w : d1.y};
+            unsigned w[2][2][2], scale[2];                       // [pair][row of the pair][8 columns]
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                unsigned h[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int place = (step * 4 + p * 2 + e) * 4 + t;
+                    const uint2 c = *reinterpret_cast<const uint2 *>(s + place * 64 + gq * 8);
+                    w[p][e][0] = c.x;
+                    w[p][e][1] = c.y;
+                    h[e] = decode_scale<FMT>(FMT == kNvFp4 ? s[kFewCodes + (place * 2 + (gq >> 2)) * 4 + (gq & 3)] : s[kFewCodes + place * 4 + (gq >> 1)]);
+                }
+                scale[p] = (h[0] & 0xffffu) | (h[1] & 0xffff0000u);
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {                        // four columns of the 16
+                const unsigned sel = q & 1 ? 0x7632u : 0x5410u;
+                const uint4 b0 = decode8<FMT>(__byte_perm(w[0][0][q >> 1], w[0][1][q >> 1], sel), scale[0]);
+                const uint4 b1 = decode8<FMT>(__byte_perm(w[1][0][q >> 1], w[1][1][q >> 1], sel), scale[1]);
+                mma_16816(acc[q * 4 + 0], a, b0.x, b1.x);
+                mma_16816(acc[q * 4 + 1], a, b0.y, b1.y);
+                mma_16816(acc[q * 4 + 2], a, b0.z, b1.z);
+                mma_16816(acc[q * 4 + 3], a, b0.w, b1.w);
+            }
+        }
+        stage = (stage + 1) % kFewStages;
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
+    // the warps' sums, 16 rows x 128 columns each (rows of 132 floats), added up into the first one's place
+    constexpr int kLd = kFewCols + 4;
+    float *part = reinterpret_cast<float *>(smem_few);
+    float *my = part + warp * 16 * kLd;
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            *reinterpret_cast<float4 *>(my + gq * kLd + 32 * t + 16 * h + i) = make_float4(acc[i][h], acc[i + 1][h], acc[i + 2][h], acc[i + 3][h]);
+            *reinterpret_cast<float4 *>(my + (gq + 8) * kLd + 32 * t + 16 * h + i) = make_float4(acc[i][2 + h], acc[i + 1][2 + h], acc[i + 2][2 + h], acc[i + 3][2 + h]);
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 16 * kFewCols / 4; i += kFewThreads) {
+        float4 *p = reinterpret_cast<float4 *>(part + (i / (kFewCols / 4)) * kLd + (i % (kFewCols / 4)) * 4);
+        float4 v = *p;
+#pragma unroll
+        for (int w = 1; w < kFewWarps; ++w) {
+            const float4 o = p[w * 16 * kLd / 4];
+            v = make_float4(v.x + o.x, v.y + o.y, v.z + o.z, v.w + o.w);
+        }
+        *p = v;
+    }
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    const auto read = [&](int i, int c) { return *reinterpret_cast<const float4 *>(cluster.map_shared_rank(reinterpret_cast<const float *>(smem_few) + i, c)); };
+    add_parts<kFewThreads>(read, rank, kLd, g.R, min(kFewCols, g.C - col0), g.splits, *g.head, FMT == kNvFp4 ? kNvHold : 1.0f, g.out, g.type, col0, g.ld);
+    cluster.sync();                                              // nobody leaves while its shared memory is being read
+}
+
+}  // namespace
+
+cudaError_t fp4_grad_few(int format, const void *dy, int R, uint64_t ld_dy, const uint8_t *packed, uint64_t D, uint64_t C, void *out, int type, uint64_t ld,
+                         int sm_count, cudaStream_t stream) {
+    Fp4Few g;
+    g.R = R; g.C = (int)C; g.D = (int)D;
+    g.chunks = (int)((D + kFewRows - 1) / kFewRows);
+    const int blocks = (int)((C + kFewCols - 1) / kFewCols);
+    if (blocks > 0x7fffffff / 8) return cudaErrorInvalidValue;
+    g.splits = 1;
+    while (g.splits < 8 && blocks * g.splits <= sm_count && g.chunks >= g.splits * 2 * kFewWarps) g.splits *= 2;
+    g.chunks_per_split = (g.chunks + g.splits - 1) / g.splits;
+    g.splits = (g.chunks + g.chunks_per_split - 1) / g.chunks_per_split;
+    g.codes = packed + kFp4Head;
+    g.scales = packed + fp4_scales_at(D, C);
+    g.ld_codes = fp4_ld(C);
+    g.quads = fp4_quads(format, C);
+    g.head = reinterpret_cast<const float *>(packed);
+    g.dy = static_cast<const __nv_bfloat16 *>(dy);
+    g.ld_dy = ld_dy;
+    g.out = out; g.ld = (long)ld; g.type = type;
+    constexpr size_t smem = (size_t)kFewWarps * kFewStages * kFewStage;
+    static_assert(smem >= (size_t)kFewWarps * 16 * (kFewCols + 4) * 4, "partial sums do not fit");
+    const auto kernel = format == kNvFp4 ? fp4_grad_few_kernel<kNvFp4> : fp4_grad_few_kernel<kMxFp4>;
+    const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (err != cudaSuccess) return err;
+    return launch_cluster(kernel, (unsigned)(blocks * g.splits), kFewThreads, g.splits, smem, stream, g);
+}
+
+}  // namespace bsq

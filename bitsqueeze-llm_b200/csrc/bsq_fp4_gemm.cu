@@ -303,9 +303,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(const __grid_
 #pragma unroll
                     for (int c = 0; c < 8; ++c) {
                         const int q = q0 + (c_first + c) * 16, have = c < c_count ? min(16, g.Q - q) : 0;
+                        if (have > 0) {
 #pragma unroll
-                        for (int j = 0; j < 16; ++j)
-                            if (j < have) store_one(g.out, g.type, (long)(q + j) * g.ld + p, __uint_as_float(r[c][j]) * f0 * f1);
+                            for (int j = 0; j < 16; ++j)
+                                if (j < have) store_one(g.out, g.type, (long)(q + j) * g.ld + p, __uint_as_float(r[c][j]) * f0 * f1);
+                        }
                     }
                 }
             }
@@ -323,7 +325,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(const __grid_
         cluster.sync();
         const int pt = first % g.p_tiles, qt = first / g.p_tiles;
         const int n_p = min(128, g.P - pt * 128), n_q = min(g.q_tile, g.Q - qt * g.q_tile);
-        const auto read = [&](int i, int c) { return *cluster.map_shared_rank(reinterpret_cast<const float *>(base) + i, c); };
+        const auto read = [&](int i, int c) { return *reinterpret_cast<const float4 *>(cluster.map_shared_rank(reinterpret_cast<const float *>(base) + i, c)); };
         if (g.lanes_contiguous)
             add_parts<kGemmThreads>(read, rank, 128, n_q, n_p, g.splits, *g.p_head, *g.q_head, g.out, g.type, (long)(qt * g.q_tile) * g.ld + pt * 128, g.ld);
         else
@@ -370,7 +372,7 @@ cudaError_t fp4_matmul(int format, const void *a, uint64_t M, const void *b, uin
                        unsigned *status, int sm_count, cudaStream_t stream) {
     if (M == 0 || N == 0) return cudaSuccess;
     const uint8_t *pa = static_cast<const uint8_t *>(a), *pb = static_cast<const uint8_t *>(b);
-    const bool swap = M <= 64;                                   // few tokens: their number is the tile's width
+    const bool swap = M <= 128;                                  // few tokens: their number is the tile's width (100 x 4096 x 4096: 17.7 us without, 8.1 with)
     const uint64_t P = swap ? N : M, Q = swap ? M : N;
     const uint8_t *pp = swap ? pb : pa, *pq = swap ? pa : pb;
     Fp4Gemm g = {};

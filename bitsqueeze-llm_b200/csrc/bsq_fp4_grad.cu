@@ -5,13 +5,15 @@
 // times its block scale has 6 significant bits and BF16's exponent covers every MXFP4 scale (NVFP4: held 2^12 smaller), so decoding is exact;
 // sums are FP32 in tensor memory, the matrix scale is multiplied in when a tile leaves, and the result is rounded once.  The tensor core
 // cuts every addition off instead of rounding it, and what is lost grows with the length of the chain: results in FP32 leave tensor memory every 1024 of D
-// and are added up rounded (4096 of D: 1.0e-6 off 64 bits in chains of 2048, %SPLITERR in chains of 1024, a rounded FP32 product 3e-7).
+// and are added up rounded (4096 of D: 1.0e-6 off 64 bits in chains of 2048, 0.6e-6 in chains of 1024, a rounded FP32 product 3e-7).
 //
 // Where there are enough tiles, a pair of CTAs on two SMs shares one of 256 x 256 (cta_group::2): each has 128 rows of dY and decodes 128 columns of B, so
 // an element is decoded once for 256 rows of the result.  Per 64 of D warp 0 brings the packed codes and scales of 64 rows of B (5 KB instead of
 // 16), warp 2 a box of dY (128-byte swizzle, in the orientation that memory has; the tensor core reads either), sixteen warps decode, four at a stage, into
 // the swizzled operand (contiguous along C), warp 1 of the leader issues the MMAs, four warps take finished tiles out while the next
 // one is computed.  Small results: one CTA per tile of 128 x 128, and clusters that share a tile along D (partial sums through distributed shared memory).
+#include "bsq_fp4_decode.cuh"
+#include "bsq_fp4_few.hpp"
 #include "bsq_fp4_tile.cuh"
 #include "bsq_internal.hpp"
 
@@ -28,7 +30,6 @@ constexpr unsigned kBoxBytes = 32 * 128;                         // 32 rows x 12
 constexpr unsigned kBoxesBytes = kEpilogueWarps * 2 * kBoxBytes;
 constexpr unsigned kABytes = 128 * kStageD * 2, kBBytes = kStageD * kTileC * 2, kOpBytes = kABytes + kBBytes;
 constexpr unsigned kCodeBytes = kStageD * kTileC / 2, kRawBytes = kCodeBytes + 1024;
-constexpr float kNvHold = 4096.0f;                               // NVFP4: decoded values are held 2^12 smaller
 constexpr int kChainStages = 1024 / kStageD;                     // FP32 results: longest chain of additions in tensor memory
 
 struct Fp4Grad {
@@ -63,42 +64,6 @@ __device__ __forceinline__ void mma_f16_pair(unsigned tmem_d, uint64_t desc_a, u
         "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5, %5, %5, %5, %5}, p;\n\t}" ::"r"(tmem_d),
         "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(acc), "r"(0u)
         : "memory");
-}
-
-__device__ __forceinline__ unsigned mul_bf16x2(unsigned a, unsigned b) {
-    unsigned r;
-    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
-}
-
-// Eight codes to BF16, times a scale.  Sign and the three magnitude bits are moved to where BF16 has its sign, the last two bits of its exponent and
-// the first of its mantissa: read as BF16 that is the element times 2^-126 (also for 0 and 0.5, which are subnormal in both), and multiplying brings it
-// back.  Word i holds elements i and i + 4: columns of a group of 8 come out in the order 0 4 1 5 2 6 3 7, which the epilogue undoes for nothing.
-template <int FMT> __device__ __forceinline__ uint4 decode8(unsigned x, unsigned scale2) {
-    // (shifts to the left, which go to the multiply pipe: the integer pipe with its half rate is what decoding is short of)
-    const unsigned y = x >> 6;
-    unsigned w[4];
-    w[0] = ((x << 12) & 0x80008000u) | ((x << 6) & 0x01C001C0u);
-    w[1] = ((x << 8) & 0x80008000u) | ((x << 2) & 0x01C001C0u);
-    w[2] = ((x << 4) & 0x80008000u) | ((y << 4) & 0x01C001C0u);
-    w[3] = (x & 0x80008000u) | (y & 0x01C001C0u);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (FMT == kMxFp4) w[i] = mul_bf16x2(w[i], 0x7E807E80u);  // 2^126: the element itself, exact; the scale's range needs a product of its own
-        w[i] = mul_bf16x2(w[i], scale2);
-    }
-    return make_uint4(w[0], w[1], w[2], w[3]);
-}
-// The factor of decode8 from a scale byte, in both halves of a word
-template <int FMT> __device__ __forceinline__ unsigned decode_scale(unsigned byte) {
-    unsigned h;
-    if (FMT == kMxFp4) {
-        h = byte == 0 ? 0x0040u : byte == 255 ? 0x7FFFu : byte << 7;
-    } else {
-        byte &= 0x7fu;                                           // s * 2^(126 - 12), exact in BF16
-        h = byte == 0x7fu ? 0x7FFFu : __float_as_uint(e4m3_decode(byte) * 2.076918743413931e34f) >> 16;
-    }
-    return h | (h << 16);
 }
 
 // 16 columns of accumulators, decode8's order of columns undone
@@ -425,7 +390,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) fp4_grad_kernel(const __grid_
         cg::cluster_group cluster = cg::this_cluster();
         cluster.sync();
         const int rt = first % g.r_tiles, ct = first / g.r_tiles;
-        const auto read = [&](int i, int c) { return *cluster.map_shared_rank(reinterpret_cast<const float *>(base) + i, c); };
+        const auto read = [&](int i, int c) { return *reinterpret_cast<const float4 *>(cluster.map_shared_rank(reinterpret_cast<const float *>(base) + i, c)); };
         add_parts<kGradThreads>(read, rank, kTileC + 4, min(128, g.R - rt * 128), min(kTileC, g.C - ct * kTileC), g.splits, *g.head, FMT == kNvFp4 ? kNvHold : 1.0f, g.out,
                                 g.type, (long)(rt * 128) * g.ld + ct * kTileC, g.ld);
         cluster.sync();                                          // nobody leaves while its shared memory is being read
@@ -475,6 +440,8 @@ cudaError_t grad_product(int format, bool a_kmajor, const void *dy, uint64_t M, 
         if (err != cudaSuccess) return err;
         dy = scratch;
     }
+    // few rows: decoded in the registers of the MMAs (16 x 4096 x 14336 in MXFP4 24 us there, 30 here; one row in NVFP4 24 / 37; 5 x 1024 x 1024 5.8 / 6.8)
+    if (a_kmajor && R <= kFewRowsMax) return fp4_grad_few(format, dy, (int)R, ld_a, b, D, C, out, type, ld, sm_count, stream);
     Fp4Grad g = {};
     g.R = (int)R; g.C = (int)C; g.D = (int)D;
     const uint64_t r128 = (R + 127) / 128, c128 = (C + kTileC - 1) / kTileC;
