@@ -28,28 +28,29 @@ template <int TYPE> __device__ unsigned absmax_span(const unsigned char *p, uint
     unsigned acc = 0;
     auto one = [&](uint64_t i) {
         const unsigned w = TYPE == kF32 ? reinterpret_cast<const unsigned *>(p)[i] : reinterpret_cast<const unsigned short *>(p)[i];
-        acc = W::max(acc, W::drop(w & W::kAbs));
+        acc = W::larger(acc, W::drop(w));
     };
     uint64_t head = ((16u - (unsigned)(reinterpret_cast<uintptr_t>(p) & 15u)) & 15u) / kSize;
     if (head > n) head = n;
     if (me < head) one(me);
     const uint4 *v = reinterpret_cast<const uint4 *>(p + head * kSize);
     const uint64_t vecs = (n - head) / kVec;
-    auto four = [&](const uint4 &a) {
-        const unsigned m[4] = {a.x & W::kAbs, a.y & W::kAbs, a.z & W::kAbs, a.w & W::kAbs};
-        if (((m[0] + W::kCarry) | (m[1] + W::kCarry) | (m[2] + W::kCarry) | (m[3] + W::kCarry)) & W::kTop) {
+    for (uint64_t i = me; i < vecs; i += 4 * threads) {          // (four loads in flight, also at the end)
+        unsigned w[16], m = 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc = W::max(acc, W::drop(m[i]));
-        } else {
-            acc = W::max(acc, W::max(W::max(m[0], m[1]), W::max(m[2], m[3])));
+        for (int j = 0; j < 4; ++j) {
+            const uint4 a = i + j * threads < vecs ? v[i + j * threads] : make_uint4(0u, 0u, 0u, 0u);
+            w[4 * j] = a.x; w[4 * j + 1] = a.y; w[4 * j + 2] = a.z; w[4 * j + 3] = a.w;
         }
-    };
-    uint64_t i = me;
-    for (; i + 3 * threads < vecs; i += 4 * threads) {
-        const uint4 a = v[i], b = v[i + threads], c = v[i + 2 * threads], d = v[i + 3 * threads];
-        four(a); four(b); four(c); four(d);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) m = W::larger(m, w[j]);
+        if (not_finite<TYPE>(m)) {                               // without what is not finite
+            m = 0;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) m = W::larger(m, W::drop(w[j]));
+        }
+        acc = W::larger(acc, m);
     }
-    for (; i < vecs; i += threads) four(v[i]);
     for (uint64_t t = head + vecs * kVec + me; t < n; t += threads) one(t);
     return acc;
 }
@@ -63,7 +64,7 @@ template <int TYPE> __device__ float absmax_share(const unsigned char *x, uint64
     } else {
         const unsigned warps = blockDim.x >> 5;
         for (uint64_t r = cta * warps + (threadIdx.x >> 5); r < rows; r += ctas * warps)
-            acc = Words<TYPE>::max(acc, absmax_span<TYPE>(x + r * ld * kSize, cols, threadIdx.x & 31, 32));
+            acc = Words<TYPE>::larger(acc, absmax_span<TYPE>(x + r * ld * kSize, cols, threadIdx.x & 31, 32));
     }
     return Words<TYPE>::top(acc);
 }
@@ -91,12 +92,21 @@ struct QuantArgs {
     uint8_t *packed;
     const float *amax;                   // given, or partial maxima
     int partials;
-    unsigned chunks, tasks;              // column chunks of 256; chunks x row blocks (32 rows: 8 by 4 that lie 32 apart)
+    unsigned chunks, blocks;             // tasks: column chunks (kUnits x unit_run units of 32), row blocks (32 rows: 8 by 4 that lie 32 apart)
 };
+// Units of 32 columns that a thread has in a task: two where a row is read straight into registers and they are 16 words, for more loads in flight and
+// less arithmetic on addresses
+__host__ __device__ constexpr int unit_run(int type, int word) { return word == 32 && type != kF32 ? 2 : 1; }
 
-// 32 columns in words -> codes and scale bytes (MXFP4: one, NVFP4: two, the first in the low byte)
-template <int FMT, int TYPE>
-__device__ __forceinline__ void quantise_unit(const unsigned *w, float g, float ginv, uint4 *codes, unsigned *bytes) {
+// x / d correctly rounded from r, 1 / d correctly rounded: the residual of x r is exact in the fma, and one step with it rounds as the quotient does
+__device__ __forceinline__ float divide_by(float x, float d, float r) {
+    const float q0 = x * r, e = __fmaf_rn(q0, d, -x);
+    return __fmaf_rn(-e, r, q0);                                 // (signs this way round: -0 stays -0)
+}
+// 32 columns in words -> codes and scale bytes (MXFP4: one, NVFP4: two, the first in the low byte).
+// table (NVFP4): the value of every E4M3 byte and its reciprocal (0 for 0), correctly rounded
+template <int FMT, int TYPE, bool CLAMP>
+__device__ __forceinline__ void quantise_unit(const unsigned *w, float g, float ginv, const float2 *table, uint4 *codes, unsigned *bytes) {
     using W = Words<TYPE>;
     constexpr int kBlocks = FMT == kMxFp4 ? 1 : 2, kElems = 32 / kBlocks, kWordsPer = kElems / W::kPer;
     unsigned out[4];
@@ -105,8 +115,8 @@ __device__ __forceinline__ void quantise_unit(const unsigned *w, float g, float 
     for (int b = 0; b < kBlocks; ++b) {
         unsigned top = 0;
 #pragma unroll
-        for (int i = 0; i < kWordsPer; ++i) top = W::max(top, w[b * kWordsPer + i] & W::kAbs);
-        const bool bad = ((top + W::kCarry) & W::kTop) != 0;
+        for (int i = 0; i < kWordsPer; ++i) top = W::larger(top, w[b * kWordsPer + i]);
+        const bool bad = not_finite<TYPE>(top);
         const float amax = W::top(top);
         unsigned byte;
         float s, inv, lim = 3.402823466e+38f;
@@ -115,12 +125,12 @@ __device__ __forceinline__ void quantise_unit(const unsigned *w, float g, float 
             s = 0.0f;
             inv = __uint_as_float((254u - byte) << 23);
         } else {
-            const float u = amax * ginv;
-            byte = ue4m3_byte(__fdiv_rn(u, 6.0f));
-            const float s8 = e4m3_decode(byte);
-            s = s8 * g;
-            inv = byte ? __fdiv_rn(1.0f, s8) * ginv : 0.0f;
-            if (u > 2688.0f) lim = 2688.0f * g;              // above the given largest magnitude: saturates (and 1/s times x may not overflow)
+            const float u = CLAMP ? fminf(amax * ginv, 65536.0f) : amax * ginv;
+            byte = ue4m3_byte(divide_by(u, 6.0f, 1.0f / 6.0f));
+            const float2 e = table[byte];
+            s = e.x * g;
+            inv = e.y * ginv;
+            if (CLAMP && u > 2688.0f) lim = 2688.0f * g;         // above the given largest magnitude: saturates (and 1/s times x may not overflow)
         }
         if (bad) {
             byte = FMT == kMxFp4 ? 255u : 127u;
@@ -137,9 +147,8 @@ __device__ __forceinline__ void quantise_unit(const unsigned *w, float g, float 
                 if (FMT == kMxFp4) {
                     v[e] = x * inv;
                 } else {
-                    x = fminf(fmaxf(x, -lim), lim);
-                    const float q0 = x * inv, r = __fmaf_rn(q0, s, -x);
-                    v[e] = __fmaf_rn(-r, inv, q0);               // (signs this way round: -0 stays -0)
+                    if (CLAMP) x = fminf(fmaxf(x, -lim), lim);
+                    v[e] = divide_by(x, s, inv);
                 }
             }
             out[b * (kElems / 8) + o] = bad ? 0u : e2m1_pack8(v);
@@ -148,7 +157,41 @@ __device__ __forceinline__ void quantise_unit(const unsigned *w, float g, float 
     *codes = make_uint4(out[0], out[1], out[2], out[3]);
 }
 
-// WORD: bytes of the pieces that rows are read in: 32 where every row starts on 32 bytes (straight into the thread's registers), else 4 or 2,
+template <int WORD> struct Piece { typedef unsigned type; };
+template <> struct Piece<8> { typedef uint2 type; };
+template <> struct Piece<2> { typedef unsigned short type; };
+// Piece p of a row, of which `live` elements from its start on are there; zeros behind them
+template <int WORD, int SIZE> __device__ __forceinline__ typename Piece<WORD>::type load_piece(const unsigned char *src, int p, int live) {
+    constexpr int kElems = WORD / SIZE;
+    typename Piece<WORD>::type v = {};
+    if (live >= kElems) return reinterpret_cast<const typename Piece<WORD>::type *>(src)[p];
+    if constexpr (kElems > 1) {
+        unsigned char *b = reinterpret_cast<unsigned char *>(&v);
+#pragma unroll
+        for (int i = 0; i < kElems; ++i)
+            if (i < live) {
+                if (SIZE == 4) *reinterpret_cast<unsigned *>(b + 4 * i) = reinterpret_cast<const unsigned *>(src + (size_t)p * WORD)[i];
+                else *reinterpret_cast<unsigned short *>(b + 2 * i) = reinterpret_cast<const unsigned short *>(src + (size_t)p * WORD)[i];
+            }
+    }
+    return v;
+}
+template <int WORD, int SIZE> __device__ __forceinline__ void store_piece(unsigned char *dst, int p, int live, const typename Piece<WORD>::type &v) {
+    constexpr int kElems = WORD / SIZE;
+    if (live >= kElems) {
+        reinterpret_cast<typename Piece<WORD>::type *>(dst)[p] = v;
+    } else if constexpr (kElems > 1) {
+        const unsigned char *b = reinterpret_cast<const unsigned char *>(&v);
+#pragma unroll
+        for (int i = 0; i < kElems; ++i)
+            if (i < live) {
+                if (SIZE == 4) reinterpret_cast<unsigned *>(dst + (size_t)p * WORD)[i] = *reinterpret_cast<const unsigned *>(b + 4 * i);
+                else reinterpret_cast<unsigned short *>(dst + (size_t)p * WORD)[i] = *reinterpret_cast<const unsigned short *>(b + 2 * i);
+            }
+    }
+}
+
+// WORD: bytes of the pieces that rows are read in: 32 where every row starts on 32 bytes (straight into the thread's registers), else 8, 4 or 2,
 // neighbouring lanes neighbouring pieces, handed out through shared memory (unit stride + 16 bytes: no bank conflicts).
 template <int FMT, int TYPE, int WORD, int AMAX>
 __global__ void __launch_bounds__(kThreads) fp4_quantize_kernel(const QuantArgs g) {
@@ -157,6 +200,14 @@ __global__ void __launch_bounds__(kThreads) fp4_quantize_kernel(const QuantArgs 
     extern __shared__ __align__(16) unsigned char stage[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane >> 3, unit = lane & 7;
     float scale = 1.0f, inv = 1.0f;
+    __shared__ float2 table[FMT == kNvFp4 ? 128 : 1];
+    if (FMT == kNvFp4) {
+        if (threadIdx.x < 128) {
+            const float s = e4m3_decode(threadIdx.x);
+            table[threadIdx.x] = make_float2(s, threadIdx.x ? __fdiv_rn(1.0f, s) : 0.0f);
+        }
+        __syncthreads();
+    }
     if (AMAX != kNoAmax) {
         float m;
         if (AMAX == kGivenAmax) {
@@ -175,69 +226,84 @@ __global__ void __launch_bounds__(kThreads) fp4_quantize_kernel(const QuantArgs 
     if (blockIdx.x == 0 && threadIdx.x < kFp4Head / 4) reinterpret_cast<float *>(g.packed)[threadIdx.x] = threadIdx.x == 0 ? scale : 0.0f;
     const uint64_t ldc = fp4_ld(g.cols), quads = fp4_quads(FMT, g.cols), units = quads * (FMT == kMxFp4 ? 4 : 2);
     uint8_t *codes = g.packed + kFp4Head, *scales = g.packed + fp4_scales_at(g.rows, g.cols);
-    for (unsigned task = blockIdx.x; task < g.tasks; task += gridDim.x) {
-        const unsigned block = task / g.chunks;
-        const uint64_t first = (uint64_t)(task - block * g.chunks) * kUnits;              // units of this tile
+    constexpr int kRun = unit_run(TYPE, WORD), kTile = kUnits * kRun;                     // units of a thread; of a row of a warp's tile
+    const unsigned by = gridDim.x / g.chunks, on = gridDim.x - by * g.chunks;            // from one task to the next: row blocks, chunks
+    unsigned nb = blockIdx.x / g.chunks, nc = blockIdx.x - nb * g.chunks;
+    for (; nb < g.blocks; nb += by, nc += on) {
+        if (nc >= g.chunks) {
+            nc -= g.chunks;
+            if (++nb >= g.blocks) break;
+        }
+        // behind a pass that has just read the matrix from its start to its end: the other way round, what was read last comes from the L2
+        const unsigned block = AMAX == kPartialAmax ? g.blocks - 1 - nb : nb;
+        const uint64_t first = (uint64_t)(AMAX == kPartialAmax ? g.chunks - 1 - nc : nc) * kTile;
         const unsigned r0 = (block & 3) * 8 + warp;                                       // row in its group, first of four
-        const uint64_t group = block >> 2, row = group * 128 + r0 + 32 * sub, u = first + unit;
-        const uint64_t col = u * 32;
-        const int have = row < g.rows && col < g.cols ? (int)min((uint64_t)32, g.cols - col) : 0;   // columns of this thread
-        unsigned w[kWords];
-        if (WORD == 32) {
-            const unsigned char *src = g.x + (row * g.ld + col) * kSize;
-            if (have == 32) {
+        const uint64_t group = block >> 2, row = group * 128 + r0 + 32 * sub;
+        unsigned w[kRun][kWords];
+        if constexpr (WORD == 32) {
+            const unsigned char *src = g.x + (row * g.ld + (first + unit) * 32) * kSize;
 #pragma unroll
-                for (int i = 0; i < kWords; i += 8) ld_words8(src + i * 4, *reinterpret_cast<unsigned(*)[8]>(&w[i]));
-            } else {
+            for (int j = 0; j < kRun; ++j, src += 256 * kSize) {
+                const uint64_t col = (first + unit + 8 * j) * 32;
+                const int have = row < g.rows && col < g.cols ? (int)min((uint64_t)32, g.cols - col) : 0;   // columns of this thread
+                if (have == 32) {
 #pragma unroll
-                for (int i = 0; i < kWords; ++i) {
-                    w[i] = 0;
-                    if (TYPE == kF32) {
-                        if (i < have) w[i] = reinterpret_cast<const unsigned *>(src)[i];
-                    } else {
-                        if (2 * i < have) w[i] = reinterpret_cast<const unsigned short *>(src)[2 * i];
-                        if (2 * i + 1 < have) w[i] |= (unsigned)reinterpret_cast<const unsigned short *>(src)[2 * i + 1] << 16;
+                    for (int i = 0; i < kWords; i += 8) ld_words8(src + i * 4, *reinterpret_cast<unsigned(*)[8]>(&w[j][i]));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kWords; ++i) {
+                        w[j][i] = 0;
+                        if (TYPE == kF32) {
+                            if (i < have) w[j][i] = reinterpret_cast<const unsigned *>(src)[i];
+                        } else {
+                            if (2 * i < have) w[j][i] = reinterpret_cast<const unsigned short *>(src)[2 * i];
+                            if (2 * i + 1 < have) w[j][i] |= (unsigned)reinterpret_cast<const unsigned short *>(src)[2 * i + 1] << 16;
+                        }
                     }
                 }
             }
         } else {
             unsigned char *mine = stage + warp * 4 * kUnits * kUnitStride;
-            constexpr int kPieces = kUnits * 32 * kSize / WORD, kPerUnit = 32 * kSize / WORD, kElems = WORD / kSize;   // pieces of a row of the tile
-            __syncwarp();
+            constexpr int kPieces = kUnits * 32 * kSize / WORD, kPerUnit = 32 * kSize / WORD, kElems = WORD / kSize, kEach = kPieces / 32;   // pieces of a row of the tile
+            typename Piece<WORD>::type piece[4][kEach];          // (all loads of the tile before the first store)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const uint64_t rq = group * 128 + r0 + 32 * q;
                 const unsigned char *src = g.x + (rq * g.ld + first * 32) * kSize;
                 const int live = rq < g.rows && first * 32 < g.cols ? (int)min((uint64_t)kUnits * 32, g.cols - first * 32) : 0;
-#pragma unroll 8
-                for (int p = lane; p < kPieces; p += 32) {
-                    unsigned char *dst = mine + (q * kUnits + p / kPerUnit) * kUnitStride + (p % kPerUnit) * WORD;
-                    if (WORD == 4) {
-                        unsigned v = 0;
-                        if ((p + 1) * kElems <= live) v = reinterpret_cast<const unsigned *>(src)[p];
-                        else if (kElems == 2 && p * kElems < live) v = reinterpret_cast<const unsigned short *>(src)[2 * p];
-                        *reinterpret_cast<unsigned *>(dst) = v;
-                    } else {
-                        *reinterpret_cast<unsigned short *>(dst) = p < live ? reinterpret_cast<const unsigned short *>(src)[p] : (unsigned short)0;
-                    }
-                }
+#pragma unroll
+                for (int i = 0; i < kEach; ++i) piece[q][i] = load_piece<WORD, kSize>(src, lane + 32 * i, live - (lane + 32 * i) * kElems);
             }
+            __syncwarp();
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+                for (int i = 0; i < kEach; ++i) {
+                    const int p = lane + 32 * i;
+                    *reinterpret_cast<typename Piece<WORD>::type *>(mine + (q * kUnits + p / kPerUnit) * kUnitStride + (p % kPerUnit) * WORD) = piece[q][i];
+                }
             __syncwarp();
             const uint4 *from = reinterpret_cast<const uint4 *>(mine + (sub * kUnits + unit) * kUnitStride);
 #pragma unroll
             for (int i = 0; i < kWords / 4; ++i) {
                 const uint4 v = from[i];
-                w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+                w[0][4 * i] = v.x; w[0][4 * i + 1] = v.y; w[0][4 * i + 2] = v.z; w[0][4 * i + 3] = v.w;
             }
         }
-        uint4 c;
-        unsigned bytes;
-        quantise_unit<FMT, TYPE>(w, scale, inv, &c, &bytes);
-        if (row < g.rows && u < units) {
-            if (u * 16 < ldc) *reinterpret_cast<uint4 *>(codes + row * ldc + u * 16) = c;
-            uint8_t *tile = scales + (group * quads + (FMT == kMxFp4 ? u >> 2 : u >> 1)) * kFp4ScaleTile + r0 * 16 + sub * 4;
-            if (FMT == kMxFp4) tile[u & 3] = (uint8_t)bytes;
-            else *reinterpret_cast<unsigned short *>(tile + 2 * (u & 1)) = (unsigned short)bytes;
+        if (row < g.rows) {
+            uint8_t *to = codes + row * ldc + (first + unit) * 16;
+            uint8_t *tile = scales + (group * quads + (FMT == kMxFp4 ? first / 4 + (unit >> 2) : first / 2 + (unit >> 1))) * kFp4ScaleTile + r0 * 16 + sub * 4;
+#pragma unroll
+            for (int j = 0; j < kRun; ++j, to += 128, tile += (FMT == kMxFp4 ? 2 : 4) * kFp4ScaleTile) {
+                const uint64_t u = first + unit + 8 * j;
+                if (u >= units) break;
+                uint4 c;
+                unsigned bytes;
+                quantise_unit<FMT, TYPE, AMAX == kGivenAmax>(w[j], scale, inv, table, &c, &bytes);
+                if (u * 16 < ldc) *reinterpret_cast<uint4 *>(to) = c;
+                if (FMT == kMxFp4) tile[unit & 3] = (uint8_t)bytes;
+                else *reinterpret_cast<unsigned short *>(tile + 2 * (unit & 1)) = (unsigned short)bytes;
+            }
         }
     }
 }
@@ -290,7 +356,7 @@ __global__ void __launch_bounds__(kThreads) fp4_dequantize_kernel(const DequantA
                 }
             }
         }
-        if (WORD == 32) {
+        if constexpr (WORD == 32) {
             unsigned char *dst = g.out + (row * g.ld + col) * kSize;
             if (have == 32) {
 #pragma unroll
@@ -321,15 +387,11 @@ __global__ void __launch_bounds__(kThreads) fp4_dequantize_kernel(const DequantA
                 const uint64_t rq = group * 128 + r0 + 32 * q;
                 unsigned char *dst = g.out + (rq * g.ld + first * 32) * kSize;
                 const int live = rq < g.rows && first * 32 < g.cols ? (int)min((uint64_t)kUnits * 32, g.cols - first * 32) : 0;
-#pragma unroll 8
-                for (int p = lane; p < kPieces; p += 32) {
-                    const unsigned char *from = mine + (q * kUnits + p / kPerUnit) * kUnitStride + (p % kPerUnit) * WORD;
-                    if (WORD == 4) {
-                        if ((p + 1) * kElems <= live) reinterpret_cast<unsigned *>(dst)[p] = *reinterpret_cast<const unsigned *>(from);
-                        else if (kElems == 2 && p * kElems < live) reinterpret_cast<unsigned short *>(dst)[2 * p] = *reinterpret_cast<const unsigned short *>(from);
-                    } else if (p < live) {
-                        reinterpret_cast<unsigned short *>(dst)[p] = *reinterpret_cast<const unsigned short *>(from);
-                    }
+#pragma unroll
+                for (int i = 0; i < kPieces / 32; ++i) {
+                    const int p = lane + 32 * i;
+                    store_piece<WORD, kSize>(dst, p, live - p * kElems,
+                                             *reinterpret_cast<const typename Piece<WORD>::type *>(mine + (q * kUnits + p / kPerUnit) * kUnitStride + (p % kPerUnit) * WORD));
                 }
             }
         }
@@ -344,7 +406,7 @@ unsigned row_blocks(uint64_t rows) {
 // the widest pieces that rows of this stride, from this address on, can be moved in
 int piece_bytes(const void *p, uint64_t row_bytes, uint64_t rows, int size) {
     const uint64_t a = reinterpret_cast<uintptr_t>(p) | (rows > 1 ? row_bytes : 0);
-    return a % 32 == 0 ? 32 : (a % 4 == 0 || size == 4) ? 4 : 2;
+    return a % 32 == 0 ? 32 : a % 8 == 0 ? 8 : (a % 4 == 0 || size == 4) ? 4 : 2;
 }
 
 template <int FMT, int TYPE, int WORD>
@@ -358,6 +420,7 @@ cudaError_t launch_quantize(const QuantArgs &g, int amax, unsigned grid, cudaStr
 template <int FMT, int TYPE>
 cudaError_t quantize_typed(const QuantArgs &g, int amax, int word, unsigned grid, cudaStream_t stream) {
     if (word == 32) return launch_quantize<FMT, TYPE, 32>(g, amax, grid, stream);
+    if (word == 8) return launch_quantize<FMT, TYPE, 8>(g, amax, grid, stream);
     if (word == 4 || TYPE == kF32) return launch_quantize<FMT, TYPE, 4>(g, amax, grid, stream);
     return launch_quantize<FMT, TYPE == kF32 ? kF16 : TYPE, 2>(g, amax, grid, stream);
 }
@@ -372,13 +435,16 @@ template <int FMT, int TYPE, int WORD> cudaError_t launch_dequantize(const Dequa
     const size_t smem = WORD == 32 ? 0 : (size_t)kThreads * (32 * (TYPE == kF32 ? 4 : 2) + 16);
     return launch_chained(fp4_dequantize_kernel<FMT, TYPE, WORD>, grid, kThreads, smem, stream, g);
 }
+template <int FMT, int TYPE> cudaError_t dequantize_typed(const DequantArgs &g, int word, unsigned grid, cudaStream_t stream) {
+    if (word == 32) return launch_dequantize<FMT, TYPE, 32>(g, grid, stream);
+    if (word == 8) return launch_dequantize<FMT, TYPE, 8>(g, grid, stream);
+    if (word == 4 || TYPE == kF32) return launch_dequantize<FMT, TYPE, 4>(g, grid, stream);
+    return launch_dequantize<FMT, TYPE == kF32 ? kF16 : TYPE, 2>(g, grid, stream);
+}
 template <int FMT> cudaError_t dequantize_format(const DequantArgs &g, int type, int word, unsigned grid, cudaStream_t stream) {
-    if (type == kF32) return word == 32 ? launch_dequantize<FMT, kF32, 32>(g, grid, stream) : launch_dequantize<FMT, kF32, 4>(g, grid, stream);
-    if (type == kF16)
-        return word == 32 ? launch_dequantize<FMT, kF16, 32>(g, grid, stream)
-             : word == 4 ? launch_dequantize<FMT, kF16, 4>(g, grid, stream) : launch_dequantize<FMT, kF16, 2>(g, grid, stream);
-    return word == 32 ? launch_dequantize<FMT, kBf16, 32>(g, grid, stream)
-         : word == 4 ? launch_dequantize<FMT, kBf16, 4>(g, grid, stream) : launch_dequantize<FMT, kBf16, 2>(g, grid, stream);
+    if (type == kF32) return dequantize_typed<FMT, kF32>(g, word, grid, stream);
+    if (type == kF16) return dequantize_typed<FMT, kF16>(g, word, grid, stream);
+    return dequantize_typed<FMT, kBf16>(g, word, grid, stream);
 }
 
 // Up to this many bytes every CTA of an NVFP4 quantiser finds the largest magnitude by itself instead of a pass of its own in front.
@@ -396,15 +462,16 @@ cudaError_t fp4_quantize(int format, const void *x, int type, uint64_t rows, uin
     g.amax = amax;
     g.partials = 0;
     const int size = op_bytes(type);
+    const int word = piece_bytes(x, ld * size, rows, size), tile = kUnits * unit_run(type, word);
     const uint64_t units = fp4_quads(format, cols) * (format == kMxFp4 ? 4 : 2);
-    g.chunks = (unsigned)((units + kUnits - 1) / kUnits);
-    const uint64_t tasks = (uint64_t)g.chunks * row_blocks(rows);
+    g.chunks = (unsigned)((units + tile - 1) / tile);
+    g.blocks = row_blocks(rows);
+    const uint64_t tasks = (uint64_t)g.chunks * g.blocks;
     if (tasks > 0xf0000000ull) return cudaErrorInvalidValue;
-    g.tasks = (unsigned)tasks;
     int mode = format == kMxFp4 ? kNoAmax : amax ? kGivenAmax : rows * cols * size <= kOwnAmaxBytes ? kOwnAmax : kPartialAmax;
     if (mode == kPartialAmax) {
         const uint64_t want = (rows * cols * size + 32767) / 32768;                      // four 16-byte loads of 512 threads each
-        const unsigned grid = (unsigned)(want < (uint64_t)sm_count * 4 ? want : (uint64_t)sm_count * 4);
+        const unsigned grid = (unsigned)(want < (uint64_t)sm_count * 2 ? want : (uint64_t)sm_count * 2);
         g.partials = (int)(grid < (unsigned)kFp4Partials ? grid : (unsigned)kFp4Partials);
         float *part = static_cast<float *>(scratch);
         g.amax = part;
@@ -413,8 +480,7 @@ cudaError_t fp4_quantize(int format, const void *x, int type, uint64_t rows, uin
                                              : launch_chained(fp4_absmax_kernel<kBf16>, g.partials, 512, 0, stream, g.x, rows, cols, ld, part);
         if (err != cudaSuccess) return err;
     }
-    const unsigned most = (unsigned)sm_count * 8, grid = g.tasks < most ? g.tasks : most;
-    const int word = piece_bytes(x, ld * size, rows, size);
+    const unsigned most = (unsigned)sm_count * 8, grid = tasks < most ? (unsigned)tasks : most;
     return format == kMxFp4 ? quantize_format<kMxFp4>(g, type, mode, word, grid, stream) : quantize_format<kNvFp4>(g, type, mode, word, grid, stream);
 }
 

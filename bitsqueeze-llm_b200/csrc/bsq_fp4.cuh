@@ -10,34 +10,48 @@
 namespace bsq {
 namespace {
 
-// Elements of a floating type as 32-bit words: what the absolute values, their maximum and the test for Inf / NaN need.
-// Magnitudes compare as integers; adding kCarry to a magnitude sets the top bit for Inf and NaN and for nothing else.
+// Elements of a floating type as 32-bit words: what the largest magnitude and the test for Inf / NaN need.  larger(a, b): the larger magnitude of each element of
+// a and b, NaN where there is one; the sign bits of its result say nothing (one instruction, where clearing the sign and comparing take two).
+// Adding kCarry to a magnitude sets the top bit for Inf and NaN and for nothing else.
 template <int TYPE> struct Words;
 template <> struct Words<kF32> {
     static constexpr int kPer = 1;
     static constexpr unsigned kAbs = 0x7fffffffu, kCarry = 0x00800000u, kTop = 0x80000000u;
-    static __device__ __forceinline__ unsigned max(unsigned a, unsigned b) { return ::max(a, b); }
-    static __device__ __forceinline__ unsigned drop(unsigned m) { return m >= 0x7f800000u ? 0u : m; }
-    static __device__ __forceinline__ float top(unsigned m) { return __uint_as_float(m); }
+    static __device__ __forceinline__ unsigned larger(unsigned a, unsigned b) {
+        float r;
+        asm("max.NaN.xorsign.abs.f32 %0, %1, %2;" : "=f"(r) : "f"(__uint_as_float(a)), "f"(__uint_as_float(b)));
+        return __float_as_uint(r);
+    }
+    static __device__ __forceinline__ unsigned drop(unsigned w) { return (w & kAbs) >= 0x7f800000u ? 0u : w & kAbs; }
+    static __device__ __forceinline__ float top(unsigned m) { return __uint_as_float(m & kAbs); }
 };
 template <> struct Words<kBf16> {
     static constexpr int kPer = 2;
     static constexpr unsigned kAbs = 0x7fff7fffu, kCarry = 0x00800080u, kTop = 0x80008000u;
-    static __device__ __forceinline__ unsigned max(unsigned a, unsigned b) { return __vmaxu2(a, b); }
-    static __device__ __forceinline__ unsigned drop(unsigned m) {
-        return ((m & 0xffffu) >= 0x7f80u ? 0u : (m & 0xffffu)) | ((m >> 16) >= 0x7f80u ? 0u : (m & 0xffff0000u));
+    static __device__ __forceinline__ unsigned larger(unsigned a, unsigned b) {
+        unsigned r;
+        asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
     }
-    static __device__ __forceinline__ float top(unsigned m) { return __uint_as_float(::max(m & 0xffffu, m >> 16) << 16); }
+    static __device__ __forceinline__ unsigned drop(unsigned w) {
+        return ((w & 0x7fffu) >= 0x7f80u ? 0u : (w & 0x7fffu)) | ((w >> 16 & 0x7fffu) >= 0x7f80u ? 0u : (w & 0x7fff0000u));
+    }
+    static __device__ __forceinline__ float top(unsigned m) { return __uint_as_float(max(m & 0x7fffu, m >> 16 & 0x7fffu) << 16); }
 };
 template <> struct Words<kF16> {
     static constexpr int kPer = 2;
     static constexpr unsigned kAbs = 0x7fff7fffu, kCarry = 0x04000400u, kTop = 0x80008000u;
-    static __device__ __forceinline__ unsigned max(unsigned a, unsigned b) { return __vmaxu2(a, b); }
-    static __device__ __forceinline__ unsigned drop(unsigned m) {
-        return ((m & 0xffffu) >= 0x7c00u ? 0u : (m & 0xffffu)) | ((m >> 16) >= 0x7c00u ? 0u : (m & 0xffff0000u));
+    static __device__ __forceinline__ unsigned larger(unsigned a, unsigned b) {
+        unsigned r;
+        asm("max.NaN.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
     }
-    static __device__ __forceinline__ float top(unsigned m) { return __half2float(__ushort_as_half((unsigned short)::max(m & 0xffffu, m >> 16))); }
+    static __device__ __forceinline__ unsigned drop(unsigned w) {
+        return ((w & 0x7fffu) >= 0x7c00u ? 0u : (w & 0x7fffu)) | ((w >> 16 & 0x7fffu) >= 0x7c00u ? 0u : (w & 0x7fff0000u));
+    }
+    static __device__ __forceinline__ float top(unsigned m) { return __half2float(__ushort_as_half((unsigned short)max(m & 0x7fffu, m >> 16 & 0x7fffu))); }
 };
+template <int TYPE> __device__ __forceinline__ bool not_finite(unsigned w) { return (((w & Words<TYPE>::kAbs) + Words<TYPE>::kCarry) & Words<TYPE>::kTop) != 0; }
 
 // The elements of a word
 template <int TYPE> __device__ __forceinline__ float word_elem(unsigned w, int i) {

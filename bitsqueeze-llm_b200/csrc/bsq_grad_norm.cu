@@ -90,7 +90,7 @@ template <int TYPE> __device__ void chunk_norm(const unsigned char *p, unsigned 
         }
         if (largest) {
 #pragma unroll
-            for (int u = 0; u < 16; ++u) *top = W::max(*top, w[u] & W::kAbs);
+            for (int u = 0; u < 16; ++u) *top = W::larger(*top, w[u]);
         } else {
             *sum += squares<TYPE>(w);
         }
@@ -99,7 +99,7 @@ template <int TYPE> __device__ void chunk_norm(const unsigned char *p, unsigned 
     const unsigned edge = me < head ? me : me - head + tail;
     if (edge < n) {
         const unsigned w[1] = {TYPE == kF32 ? reinterpret_cast<const unsigned *>(p)[edge] : (unsigned)reinterpret_cast<const unsigned short *>(p)[edge]};
-        if (largest) *top = W::max(*top, w[0] & W::kAbs);
+        if (largest) *top = W::larger(*top, w[0]);
         else *sum += squares<TYPE>(w);
     }
 }
