@@ -116,7 +116,7 @@ SIGNATURES = {
     "bsq_batch_compress": (_i, [_vp, C.POINTER(_vp), _i, _i, C.POINTER(_vp), _u64, C.POINTER(_vp), _vp, C.POINTER(_u64)]),
     "bsq_batch_decompress": (_i, [_vp, C.POINTER(_vp), _i, _i, C.POINTER(_vp), _u64]),
     "bsq_fp4_packed_bytes": (_u64, [_i, _u64, _u64]),
-    "bsq_fp4_scratch_bytes": (_sz, []),
+    "bsq_fp4_scratch_bytes": (_sz, [_i, _i, _u64, _u64]),
     "bsq_fp4_quantize": (_i, [_i, _vp, _i, _u64, _u64, _u64, _vp, _vp, _vp, _vp]),
     "bsq_fp4_dequantize": (_i, [_i, _vp, _u64, _u64, _vp, _i, _u64, _vp]),
     "bsq_fp4_matmul": (_i, [_i, _vp, _u64, _vp, _u64, _u64, _vp, _i, _u64, _vp, _vp]),
@@ -124,7 +124,7 @@ SIGNATURES = {
     "bsq_fp4_grad_input": (_i, [_i, _vp, _u64, _u64, _vp, _u64, _u64, _vp, _i, _u64, _vp, _vp, _vp]),
     "bsq_fp4_grad_weight": (_i, [_i, _vp, _u64, _u64, _u64, _vp, _u64, _vp, _i, _u64, _vp, _vp, _vp]),
     "bsq_grad_norm_scratch_bytes": (_sz, []),
-    "bsq_grad_norm_clip": (_i, [C.POINTER(_vp), C.POINTER(_u64), C.POINTER(_i), _i, C.POINTER(_vp), C.c_double, _i, _vp, _vp, _vp]),
+    "bsq_grad_norm_clip": (_i, [_vp, _vp, _vp, _i, _vp, C.c_double, _i, _vp, _vp, _vp]),
     "bsq_test_inject_status": (None, [_i, _u32]),
     "bsq_test_inject_lane_status": (None, [_vp, _i, _u32]),
     "bsq_build_info": (C.c_char_p, []),

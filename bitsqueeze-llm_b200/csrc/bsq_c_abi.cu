@@ -175,11 +175,11 @@ static inline bool op_rows_ok(const void *p, int type, uint64_t rows, uint64_t c
 }
 
 uint64_t bsq_fp4_packed_bytes(int format, uint64_t rows, uint64_t cols) { return fp4_shape_ok(format, rows, cols) ? fp4_packed_bytes(format, rows, cols) : 0; }
-size_t bsq_fp4_scratch_bytes(void) { return kFp4ScratchBytes; }
+size_t bsq_fp4_scratch_bytes(int format, int type, uint64_t rows, uint64_t cols) { return fp4_shape_ok(format, rows, cols) ? fp4_quantize_scratch(format, type, rows, cols) : 0; }
 int bsq_fp4_quantize(int format, const void *d_x, int type, uint64_t rows, uint64_t cols, uint64_t ld, const float *d_amax, void *d_packed, void *d_scratch,
                      void *stream) {
     if (!fp4_shape_ok(format, rows, cols) || !op_bytes(type) || !fp4_aligned(d_packed) || (rows && !op_rows_ok(d_x, type, rows, cols, ld))) return 1;
-    if (format == kNvFp4 && !d_amax && (!d_scratch || reinterpret_cast<uintptr_t>(d_scratch) % 4 != 0)) return 1;
+    if (!d_amax && fp4_quantize_scratch(format, type, rows, cols) && (!d_scratch || reinterpret_cast<uintptr_t>(d_scratch) % 4 != 0)) return 1;
     return rc(fp4_quantize(format, d_x, type, rows, cols, rows > 1 ? ld : cols, d_amax, d_packed, d_scratch, device_sm_count(), as_stream(stream)));
 }
 int bsq_fp4_dequantize(int format, const void *d_packed, uint64_t rows, uint64_t cols, void *d_out, int type, uint64_t ld, void *stream) {

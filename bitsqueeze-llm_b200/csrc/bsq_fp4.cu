@@ -447,9 +447,6 @@ template <int FMT> cudaError_t dequantize_format(const DequantArgs &g, int type,
     return dequantize_typed<FMT, kBf16>(g, word, grid, stream);
 }
 
-// Up to this many bytes every CTA of an NVFP4 quantiser finds the largest magnitude by itself instead of a pass of its own in front.
-constexpr uint64_t kOwnAmaxBytes = 64 << 10;
-
 }  // namespace
 
 cudaError_t fp4_quantize(int format, const void *x, int type, uint64_t rows, uint64_t cols, uint64_t ld, const float *amax, void *packed,
@@ -468,7 +465,7 @@ cudaError_t fp4_quantize(int format, const void *x, int type, uint64_t rows, uin
     g.blocks = row_blocks(rows);
     const uint64_t tasks = (uint64_t)g.chunks * g.blocks;
     if (tasks > 0xf0000000ull) return cudaErrorInvalidValue;
-    int mode = format == kMxFp4 ? kNoAmax : amax ? kGivenAmax : rows * cols * size <= kOwnAmaxBytes ? kOwnAmax : kPartialAmax;
+    int mode = format == kMxFp4 ? kNoAmax : amax ? kGivenAmax : fp4_quantize_scratch(format, type, rows, cols) == 0 ? kOwnAmax : kPartialAmax;
     if (mode == kPartialAmax) {
         const uint64_t want = (rows * cols * size + 32767) / 32768;                      // four 16-byte loads of 512 threads each
         const unsigned grid = (unsigned)(want < (uint64_t)sm_count * 2 ? want : (uint64_t)sm_count * 2);

@@ -40,7 +40,11 @@ inline int op_bytes(int type) { return type == kF32 ? 4 : (type == kF16 || type 
 
 // One float per CTA of the pass that finds the largest magnitude of an NVFP4 matrix.
 constexpr int kFp4Partials = 1024;
-constexpr size_t kFp4ScratchBytes = kFp4Partials * sizeof(float);
+// Up to this many bytes every CTA of an NVFP4 quantiser finds the largest magnitude by itself instead of a pass of its own in front.
+constexpr uint64_t kFp4OwnAmaxBytes = 64 << 10;
+inline size_t fp4_quantize_scratch(int format, int type, uint64_t rows, uint64_t cols) {
+    return format == kNvFp4 && rows * cols * (uint64_t)op_bytes(type) > kFp4OwnAmaxBytes ? kFp4Partials * sizeof(float) : 0;
+}
 
 // amax (nullable, NVFP4): a device word with the largest magnitude the caller reckons with; larger elements saturate.
 cudaError_t fp4_quantize(int format, const void *x, int type, uint64_t rows, uint64_t cols, uint64_t ld, const float *amax, void *packed,

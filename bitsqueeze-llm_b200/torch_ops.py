@@ -15,8 +15,8 @@ call to the next, and calls may be captured in a CUDA graph.  Tensors that are u
 on are the caller's to order, as with PyTorch's own operators.  A wait inside a product that ran out of tries leaves NaN in the result.
 Every result comes from the shared library; there is no fallback.
 """
-import ctypes as C
 import math
+from array import array
 
 import torch
 
@@ -25,7 +25,9 @@ from . import MXFP4, NVFP4, lib
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _BLOCK = {MXFP4: 32, NVFP4: 16}
 _HEAD = 128
+_NORM_SCRATCH = 16384                                      # bsq_grad_norm_scratch_bytes
 _stream = torch._C._cuda_getCurrentRawStream
+_device = torch._C._cuda_getDevice
 
 
 def _scales_at(rows, cols):
@@ -78,42 +80,37 @@ class Fp4Matrix:
         return tiles.permute(0, 3, 2, 1, 4).reshape(groups * 128, quads * 4)[: self.rows, :blocks].contiguous()
 
 
-class _on:
-    """Makes the tensors' device current for the call where it is not."""
-
-    __slots__ = ("index", "guard")
-
-    def __init__(self, device):
-        self.index = device.index
-        self.guard = None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return _stream(self.index)
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _call(name, index, *args):
+    """A C entry on the current stream of device `index` (its last argument), with that device current."""
+    f = getattr(lib(), name)
+    if _device() == index:
+        rc = f(*args, _stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = f(*args, _stream(index))
+    if rc != 0:
+        raise RuntimeError(name + " failed")
 
 
 def _rows(x, what):
     """(rows, cols, row stride) of a tensor whose leading dimensions lie as the rows of one matrix."""
     if not x.is_cuda or x.dtype not in _TYPES:
         raise ValueError("%s must be a float32, float16 or bfloat16 CUDA tensor" % what)
-    if x.dim() == 0 or x.size(-1) == 0:
+    dim = x.dim()
+    if dim == 0 or x.size(-1) == 0:
         raise ValueError("%s must have at least one dimension and one column" % what)
-    if x.dim() > 2:
+    if dim > 2:
         try:
             x = x.view(x.numel() // x.size(-1), x.size(-1))
         except RuntimeError:
             raise ValueError("the leading dimensions of %s do not lie as the rows of one matrix: pass a contiguous tensor" % what) from None
-    elif x.dim() == 1:
+    elif dim == 1:
         x = x.view(1, -1)
     rows, cols = x.shape
-    if cols > 1 and x.stride(1) != 1 or rows > 1 and x.stride(0) < cols:
+    ld, inner = x.stride()
+    if cols > 1 and inner != 1 or rows > 1 and ld < cols:
         raise ValueError("rows of %s must be contiguous and must not overlap" % what)
-    return rows, cols, x.stride(0)
+    return rows, cols, ld
 
 
 def _span(t):
@@ -160,7 +157,8 @@ def fp4_quantize(x, format=NVFP4, amax=None, out=None):
     if amax is not None and (format != NVFP4 or amax.dtype != torch.float32 or amax.numel() != 1 or amax.device != device):
         raise ValueError("amax is a float32 tensor of one element on x's device, for NVFP4")
     if out is None:
-        out = Fp4Matrix(torch.empty(_packed_bytes(format, rows, cols), dtype=torch.uint8, device=device), rows, cols, format)
+        out = Fp4Matrix.__new__(Fp4Matrix)
+        out.data, out.rows, out.cols, out.format = torch.empty(_packed_bytes(format, rows, cols), dtype=torch.uint8, device=device), rows, cols, format
     else:
         if _packed(out, "out").shape != (rows, cols) or out.format != format or out.data.device != device:
             raise ValueError("out must be an Fp4Matrix of %d x %d in the same format on x's device" % (rows, cols))
@@ -170,14 +168,11 @@ def fp4_quantize(x, format=NVFP4, amax=None, out=None):
             if a < d and c < b:
                 raise ValueError("out must not overlap an input")
         torch.autograd.graph.increment_version(out.data)
-    scratch = None
-    with _on(device) as stream:
-        if format == NVFP4 and amax is None:
-            scratch = torch.empty(lib().bsq_fp4_scratch_bytes(), dtype=torch.uint8, device=device)
-        rc = lib().bsq_fp4_quantize(format, x.data_ptr(), _TYPES[x.dtype], rows, cols, ld, None if amax is None else amax.data_ptr(), out.data.data_ptr(),
-                                    None if scratch is None else scratch.data_ptr(), stream)
-    if rc != 0:
-        raise RuntimeError("bsq_fp4_quantize failed")
+    type = _TYPES[x.dtype]
+    need = lib().bsq_fp4_scratch_bytes(format, type, rows, cols) if amax is None and format == NVFP4 else 0
+    scratch = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    _call("bsq_fp4_quantize", device.index, format, x.data_ptr(), type, rows, cols, ld, None if amax is None else amax.data_ptr(), out.data.data_ptr(),
+          None if scratch is None else scratch.data_ptr())
     return out
 
 
@@ -186,10 +181,7 @@ def fp4_dequantize(m, dtype=torch.float32, out=None):
     _packed(m, "m")
     device = m.data.device
     out, ld = _result(out, (m.rows, m.cols), dtype, device, m.data)
-    with _on(device) as stream:
-        rc = lib().bsq_fp4_dequantize(m.format, m.data.data_ptr(), m.rows, m.cols, out.data_ptr(), _TYPES[dtype], ld, stream)
-    if rc != 0:
-        raise RuntimeError("bsq_fp4_dequantize failed")
+    _call("bsq_fp4_dequantize", device.index, m.format, m.data.data_ptr(), m.rows, m.cols, out.data_ptr(), _TYPES[dtype], ld)
     return out
 
 
@@ -201,10 +193,7 @@ def fp4_matmul(a, b, dtype=torch.bfloat16, out=None):
     if a.format != b.format or a.cols != b.cols or b.data.device != device:
         raise ValueError("a and b must have the same format, number of columns and device")
     out, ld = _result(out, (a.rows, b.rows), dtype, device, a.data, b.data)
-    with _on(device) as stream:
-        rc = lib().bsq_fp4_matmul(a.format, a.data.data_ptr(), a.rows, b.data.data_ptr(), b.rows, a.cols, out.data_ptr(), _TYPES[dtype], ld, None, stream)
-    if rc != 0:
-        raise RuntimeError("bsq_fp4_matmul failed")
+    _call("bsq_fp4_matmul", device.index, a.format, a.data.data_ptr(), a.rows, b.data.data_ptr(), b.rows, a.cols, out.data_ptr(), _TYPES[dtype], ld, None)
     return out
 
 
@@ -223,18 +212,14 @@ def _grad(name, dy, m, packed_rows, out_rows, dtype, out):
     device = dy.device
     shape = tuple(dy.shape[:-1]) + (m.cols,) if out_rows is None else (out_rows(M, N), m.cols)
     out, ld_out = _result(out, shape, dtype, device, dy, m.data)
-    L = lib()
-    with _on(device) as stream:
-        p = dy.data_ptr()
-        need = L.bsq_fp4_grad_scratch_bytes(p, M, N, ld) if M and (p % 16 or ld % 8) else 0
-        scratch = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-        s = None if scratch is None else scratch.data_ptr()
-        if out_rows is None:
-            rc = L.bsq_fp4_grad_input(m.format, p, M, ld, m.data.data_ptr(), N, m.cols, out.data_ptr(), _TYPES[dtype], ld_out, s, None, stream)
-        else:
-            rc = L.bsq_fp4_grad_weight(m.format, p, M, N, ld, m.data.data_ptr(), m.cols, out.data_ptr(), _TYPES[dtype], ld_out, s, None, stream)
-    if rc != 0:
-        raise RuntimeError(name + " failed")
+    p = dy.data_ptr()
+    need = lib().bsq_fp4_grad_scratch_bytes(p, M, N, ld) if M and (p % 16 or ld % 8) else 0
+    scratch = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    s = None if scratch is None else scratch.data_ptr()
+    if out_rows is None:
+        _call(name, device.index, m.format, p, M, ld, m.data.data_ptr(), N, m.cols, out.data_ptr(), _TYPES[dtype], ld_out, s, None)
+    else:
+        _call(name, device.index, m.format, p, M, N, ld, m.data.data_ptr(), m.cols, out.data_ptr(), _TYPES[dtype], ld_out, s, None)
     return out
 
 
@@ -317,8 +302,8 @@ def _overlap(grads, to):
 
 def clip_grad_norm(grads, max_norm, norm_type=2.0, out=None):
     """The norm of `grads` (float32, float16 or bfloat16 CUDA tensors of one device, mixed as they come) taken as one vector, as a float32 tensor of no
-    dimensions; the gradients are multiplied by min(1, max_norm / (norm + 1e-6)), in place or into the tensors of `out` (same types, shapes and
-    strides).  norm_type 2 or math.inf.  max_norm None: the norm alone.  A NaN or Inf in any gradient makes the norm so, and goes into
+    dimensions; the gradients are multiplied by min(1, max_norm / (norm + 1e-6)), in place or into the tensors of `out` (of the same types;
+    contiguous with as many elements, or of the same shapes and strides).  norm_type 2 or math.inf.  max_norm None: the norm alone.  A NaN or Inf in any gradient makes the norm so, and goes into
     all of them, as with torch.nn.utils.clip_grad_norm_."""
     grads = list(grads)
     if norm_type not in (2, 2.0, math.inf):
@@ -329,37 +314,35 @@ def clip_grad_norm(grads, max_norm, norm_type=2.0, out=None):
         raise ValueError("out needs a max_norm")
     if max_norm is not None and not max_norm >= 0:
         raise ValueError("max_norm must not be negative or NaN")
-    device = grads[0].device
-    types, counts, ptrs = [], [], []
-    for g in grads:
-        if g.dtype not in _TYPES or not g.is_cuda or g.device != device or not _dense(g):
-            raise ValueError("gradients must be dense float32, float16 or bfloat16 CUDA tensors on one device")
-        types.append(_TYPES[g.dtype])
-        counts.append(g.numel())
-        ptrs.append(g.data_ptr())
-    n = len(grads)
+    device, n = grads[0].device, len(grads)
+    # (a list at a time: a few hundred gradients are looked at in every step)
+    index, dtypes, plain = grads[0].get_device(), [g.dtype for g in grads], [g.is_contiguous() for g in grads]
+    types = [_TYPES.get(d, -1) for d in dtypes]
+    if index < 0 or min(types) < 0 or {g.get_device() for g in grads} != {index} or not all(p or _dense(g) for p, g in zip(plain, grads)):
+        raise ValueError("gradients must be dense float32, float16 or bfloat16 CUDA tensors on one device")
     to = grads
     if out is not None:
         to = list(out)
         if len(to) != n:
             raise ValueError("out must have a tensor for each gradient")
-        for g, o in zip(grads, to):
-            if o.dtype != g.dtype or o.device != device or o.shape != g.shape or (o.stride() != g.stride() and not (g.is_contiguous() and o.is_contiguous())) or o.requires_grad:
-                raise ValueError("tensors of out must have the type, shape, strides and device of their gradients, and need no gradient")
-    c_ptrs = (C.c_void_p * n)(*ptrs)
-    c_outs = None
-    if max_norm is not None:
-        c_outs = c_ptrs if out is None else (C.c_void_p * n)(*[o.data_ptr() for o in to])
-    L = lib()
-    with _on(device) as stream:
-        norm = torch.empty((), dtype=torch.float32, device=device)
-        scratch = torch.empty(L.bsq_grad_norm_scratch_bytes(), dtype=torch.uint8, device=device)
-        rc = L.bsq_grad_norm_clip(c_ptrs, (C.c_uint64 * n)(*counts), (C.c_int * n)(*types), n, c_outs, 0.0 if max_norm is None else max_norm,
-                                  0 if norm_type == math.inf else 2, norm.data_ptr(), scratch.data_ptr(), stream)
-    if rc != 0:
-        if c_outs is not None and _overlap(grads, to):
-            raise ValueError("the tensors that are written must not overlap one another or another gradient")
-        raise RuntimeError("bsq_grad_norm_clip failed")
+        if [o.dtype for o in to] != dtypes or {o.get_device() for o in to} != {index} or any([o.requires_grad for o in to]):
+            raise ValueError("tensors of out must have the type and device of their gradients, and need no gradient")
+        if not (all(plain) and all([o.is_contiguous() for o in to])) and [(o.shape, o.stride()) for o in to] != [(g.shape, g.stride()) for g in grads]:
+            raise ValueError("tensors of out that are not contiguous must have the shape and strides of their gradients")
+    ptrs = array("Q", [g.data_ptr() for g in grads])
+    outs = None if max_norm is None else ptrs if out is None else array("Q", [o.data_ptr() for o in to])
+    counts, types = array("Q", [g.numel() for g in grads]), array("i", types)
+    if out is not None and array("Q", [o.numel() for o in to]) != counts:
+        raise ValueError("tensors of out must have as many elements as their gradients")
+    norm = torch.empty((), dtype=torch.float32, device=device)
+    scratch = torch.empty(_NORM_SCRATCH, dtype=torch.uint8, device=device)
+    try:
+        _call("bsq_grad_norm_clip", index, ptrs.buffer_info()[0], counts.buffer_info()[0], types.buffer_info()[0], n, None if outs is None else outs.buffer_info()[0],
+              0.0 if max_norm is None else max_norm, 0 if norm_type == math.inf else 2, norm.data_ptr(), scratch.data_ptr())
+    except RuntimeError:
+        if outs is not None and _overlap(grads, to):
+            raise ValueError("the tensors that are written must not overlap one another or another gradient") from None
+        raise
     if max_norm is not None:
         torch.autograd.graph.increment_version(to)
     return norm

@@ -266,11 +266,12 @@ int bsq_batch_decompress(bsq_batch_t *batch, const struct bitsqz_llm_array *cons
  * type: 0 FP32, 1 FP16, 2 BF16; ld: elements from one row to the next.  Rows may be 0.  All calls enqueue on `stream` and return; they allocate nothing and keep
  * nothing, and may be captured.  d_status (nullable): bit 0 is set when a bounded wait gave up; the results concerned are NaN then. */
 uint64_t bsq_fp4_packed_bytes(int format, uint64_t rows, uint64_t cols);
-size_t bsq_fp4_scratch_bytes(void);
+/* what bsq_fp4_quantize needs in d_scratch when it is not given d_amax: 0 for MXFP4 and for small matrices */
+size_t bsq_fp4_scratch_bytes(int format, int type, uint64_t rows, uint64_t cols);
 /* Codes are x / (block scale * matrix scale) to the nearest, ties to even, saturated at 6, with the decision made exactly.  MXFP4: the block scale is
  * 2^(floor(log2 m) - 2), at least 2^-127, m the block's largest magnitude.  NVFP4: the matrix scale is the power of two 2^t with the smallest t (-110 to 117) for
  * which the largest finite magnitude of the matrix is at most 2688 * 2^t -- of the matrix, or *d_amax where that is given (elements above it saturate) -- and the
- * block scale the nearest E4M3 to m / (6 * 2^t).  A block that holds Inf or NaN gets the scale NaN.  d_scratch: bsq_fp4_scratch_bytes, for NVFP4 without d_amax. */
+ * block scale the nearest E4M3 to m / (6 * 2^t).  A block that holds Inf or NaN gets the scale NaN. */
 int bsq_fp4_quantize(int format, const void *d_x, int type, uint64_t rows, uint64_t cols, uint64_t ld, const float *d_amax, void *d_packed, void *d_scratch,
                      void *stream);
 /* out = (element * block scale) * matrix scale, rounded once */

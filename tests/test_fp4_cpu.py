@@ -52,7 +52,7 @@ def test_c_entries_refuse(lib):
     """Every call below is turned down on the host; no pointer is looked at."""
     a, odd, f = 4096, 4097, lib
     q = f.bsq_fp4_quantize
-    ok = [9, a, 2, 4, 64, 64, None, a, a, None]
+    ok = [9, a, 2, 1024, 64, 64, None, a, a, None]
 
     def but(base, i, v):
         args = list(base)
@@ -74,6 +74,11 @@ def test_c_entries_refuse(lib):
     ok = [9, a, 4, 8, 8, a, 64, a, 2, 64, a, None, None]
     for i, v in ((0, 0), (1, None), (4, 7), (5, None), (6, 0), (7, None), (8, 4), (9, 63), (3, 1 << 31)):
         assert refused(f.bsq_fp4_grad_weight, *but(ok, i, v)), (i, v)
+
+
+def test_scratch_of_quantisation(lib):
+    f = lib.bsq_fp4_scratch_bytes
+    assert f(8, 0, 4096, 4096) == 0 and f(9, 2, 1, 4096) == 0 and f(9, 2, 8, 4096) == 0 and f(9, 2, 9, 4096) == 4096 and f(9, 0, 8, 4096) == 4096 and f(7, 0, 4096, 64) == 0
 
 
 def test_scratch_of_gradients(lib):
