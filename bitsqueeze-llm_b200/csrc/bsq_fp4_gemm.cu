@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(const __grid_
             for (int t = first; t < tiles && ok; t += step) {
                 const int p_row = ((t % g.p_tiles) * CTAS + side) * 128, q_row = (t / g.p_tiles) * g.q_tile;
                 for (int k = k0; k < k1; ++k, ++filled, r.next()) {
-                    if (r.wrapped) ok = mbar_wait_bounded(&bars.empty[r.pos], r.par ^ 1u, status);
+                    if (r.wrapped) ok = mbar_wait_asleep(&bars.empty[r.pos], r.par ^ 1u, status);
                     if (!ok) break;
                     unsigned char *s = base + (size_t)r.pos * stage_bytes;
                     uint64_t *bar = &bars.full[r.pos];
@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(const __grid_
             if (!ok) {                                           // copies in flight must have landed before this CTA's shared memory goes away
                 atomicOr(&bars.failed, 1u);
                 if (leader)
-                    for (int c = max(0, filled - g.ring); c < filled; ++c) mbar_wait_bounded(&bars.full[c % g.ring], (unsigned)(c / g.ring) & 1u, status);
+                    for (int c = max(0, filled - g.ring); c < filled; ++c) mbar_wait_asleep(&bars.full[c % g.ring], (unsigned)(c / g.ring) & 1u, status);
             }
         }
     } else if (warp == 1) {
@@ -160,11 +160,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(const __grid_
             unsigned buf = 0;
             for (int t = first; t < tiles && ok; t += step, rs.next()) {
                 const unsigned acc = tmem + (unsigned)rs.pos * acc_cols;
-                if (rs.wrapped) ok = __all_sync(kFullMask, mbar_wait_bounded(&bars.acc_empty[rs.pos], rs.par ^ 1u, status)) != 0;
+                if (rs.wrapped) ok = __all_sync(kFullMask, mbar_wait_asleep(&bars.acc_empty[rs.pos], rs.par ^ 1u, status)) != 0;
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 for (int k = k0; k < k1; ++k, r.next(), buf ^= 1u) {
-                    ok = __all_sync(kFullMask, mbar_wait_bounded(&bars.full[r.pos], r.par, status)) != 0;
+                    ok = __all_sync(kFullMask, mbar_wait_asleep(&bars.full[r.pos], r.par, status)) != 0;
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const unsigned s = smem_u32(base) + (unsigned)r.pos * stage_bytes;
@@ -203,7 +203,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(const __grid_
                 atomicOr(&bars.failed, 1u);
                 if (CTAS == 2) tc_commit_pair(&bars.drain, 1);   // MMAs under way must be done before tensor memory is given back
                 else tc_commit(&bars.drain);
-                mbar_wait_bounded(&bars.drain, 0, status);
+                mbar_wait_asleep(&bars.drain, 0, status);
             }
         }
     } else {
@@ -214,7 +214,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(const __grid_
         Ring rs(g.sets);
         for (int t = first; t < tiles; t += step, rs.next()) {
             const int p0 = ((t % g.p_tiles) * CTAS + side) * 128 + quarter * 32, q0 = (t / g.p_tiles) * g.q_tile;
-            if (ok) ok = __all_sync(kFullMask, mbar_wait_bounded(&bars.acc_full[rs.pos], rs.par, status)) != 0;
+            if (ok) ok = __all_sync(kFullMask, mbar_wait_asleep(&bars.acc_full[rs.pos], rs.par, status)) != 0;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const unsigned taddr = tmem + (unsigned)rs.pos * acc_cols + ((unsigned)(quarter * 32) << 16) + (unsigned)c_first * 16u;
             if constexpr (SPLIT) {

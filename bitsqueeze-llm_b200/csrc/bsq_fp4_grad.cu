@@ -21,16 +21,24 @@ namespace bsq {
 namespace {
 
 // warp 0: copies of B, 1: MMAs (in the other CTA of a pair: the word that a stage is ready), 2: copies of dY, 4-7: epilogue, 8-: decode
-constexpr int kDecodeWarps = 4, kDecodeGroups = 4;               // at one stage; stages that are decoded at a time
+constexpr int kDecodeWarps = 4;                                  // at one stage
 constexpr int kEpilogueWarps = 4, kFirstDecode = 4 + kEpilogueWarps;
-constexpr int kGradThreads = (kFirstDecode + kDecodeWarps * kDecodeGroups) * 32;
 constexpr int kTileC = 128, kStageD = 64;                        // a CTA's columns of B; of D per stage
-constexpr int kRing = 5, kRawRing = 6;
+constexpr int kMaxRing = 5, kRawRing = 6;
 constexpr unsigned kBoxBytes = 32 * 128;                         // 32 rows x 128 bytes of the result on their way out: two for each epilogue warp
 constexpr unsigned kBoxesBytes = kEpilogueWarps * 2 * kBoxBytes;
-constexpr unsigned kABytes = 128 * kStageD * 2, kBBytes = kStageD * kTileC * 2, kOpBytes = kABytes + kBBytes;
+constexpr unsigned kABytes = 128 * kStageD * 2, kBBytes = kStageD * kTileC * 2;
 constexpr unsigned kCodeBytes = kStageD * kTileC / 2, kRawBytes = kCodeBytes + 1024;
 constexpr int kChainStages = 1024 / kStageD;                     // FP32 results: longest chain of additions in tensor memory
+
+// A stage: MT blocks of 128 rows of dY, 128 columns of B
+__host__ __device__ constexpr unsigned op_bytes_of(int mt) { return (unsigned)mt * kABytes + kBBytes; }
+__host__ __device__ constexpr int ring_of(int mt) { return mt == 2 ? 3 : 5; }
+// Groups of decoding warps, each with a stage of its own.  Never more than there are stages in either ring: a group that waits for its stage to be emptied goes by the
+// parity of the barrier, and is at most one round ahead only because its own last stage lies no further back than a round.
+__host__ __device__ constexpr int groups_of(int mt) { return mt == 2 ? 3 : 4; }
+__host__ __device__ constexpr int grad_threads(int mt) { return (kFirstDecode + kDecodeWarps * groups_of(mt)) * 32; }
+static_assert(groups_of(1) <= ring_of(1) && groups_of(2) <= ring_of(2) && groups_of(1) <= kRawRing && groups_of(2) <= kRawRing, "a group would run two rounds ahead");
 
 struct Fp4Grad {
     int R, C, D;                     // rows and columns of the result, the dimension that is summed over
@@ -47,7 +55,7 @@ struct Fp4Grad {
 };
 
 struct GradBars {
-    uint64_t full[kRing], empty[kRing], ready[kRing], raw_full[kRawRing], raw_empty[kRawRing], acc_full[2], acc_empty[2], drain;
+    uint64_t full[kMaxRing], empty[kMaxRing], ready[kMaxRing], raw_full[kRawRing], raw_empty[kRawRing], acc_full[2], acc_empty[2], drain;
     unsigned tmem_base, failed;
 };
 
@@ -74,19 +82,21 @@ __device__ __forceinline__ void read_columns(unsigned taddr, unsigned (&r)[16], 
     for (int j = 0; j < 16; ++j) r[j] = p[(j & 8) | ((j & 3) << 1) | ((j & 4) >> 2)];
 }
 
-// CTAS: 1, or 2 for a pair.  SPLIT: the CTAs of a cluster share a tile, each with a slice of D.
-template <int FMT, int CTAS, bool SPLIT>
-__global__ void __launch_bounds__(kGradThreads, 1) fp4_grad_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+// CTAS: 1, or 2 for a pair.  MT: blocks of 128 rows of a CTA, each with accumulators of its own.  SPLIT: the CTAs of a cluster share a tile, each with a slice of D.
+template <int FMT, int CTAS, int MT, bool SPLIT>
+__global__ void __launch_bounds__(grad_threads(MT), 1) fp4_grad_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                                                                    const __grid_constant__ CUtensorMap map_c, const Fp4Grad g, unsigned *status) {
-    static_assert(CTAS == 1 || !SPLIT, "pairs do not share tiles");
+    static_assert((CTAS == 1 || !SPLIT) && (MT == 1 || CTAS == 2), "pairs do not share tiles, single CTAs have one block of rows");
     chain_begin();
+    constexpr int kRing = ring_of(MT);
+    constexpr unsigned kOpBytes = op_bytes_of(MT);
     extern __shared__ unsigned char smem_dyn[];
     unsigned char *base = smem_dyn + ((1024u - (smem_u32(smem_dyn) & 1023u)) & 1023u);
     unsigned char *raw = base + kRing * kOpBytes, *boxes = raw + kRawRing * kRawBytes;
     GradBars &bars = *reinterpret_cast<GradBars *>(boxes + kBoxesBytes);
     constexpr int kQuads = FMT == kNvFp4 ? 2 : 1;                // scale tiles across a CTA's 128 columns
     constexpr unsigned kAccCols = CTAS * kTileC;                 // columns of an accumulator
-    constexpr int kSets = SPLIT ? 4 : 2;
+    constexpr int kSets = SPLIT ? 4 : 2 / MT;                    // accumulators that follow one another (SPLIT: parts of one chain)
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int half = CTAS == 2 ? (int)(blockIdx.x & 1) : 0, unit = (int)(blockIdx.x / (SPLIT ? (unsigned)g.splits : (unsigned)CTAS));
     const int rank = SPLIT ? (int)(blockIdx.x % (unsigned)g.splits) : 0;
@@ -131,7 +141,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) fp4_grad_kernel(const __grid_
                 const int c_tile = (t / g.r_tiles) * CTAS + half;
                 const unsigned quad = (unsigned)c_tile * kQuads, sf = quad < g.quads ? min((unsigned)kQuads, g.quads - quad) * 512u : 0u;
                 for (int d = d0; d < d1; ++d, ++filled, r.next()) {
-                    if (r.wrapped) ok = mbar_wait_bounded(&bars.raw_empty[r.pos], r.par ^ 1u, status);
+                    if (r.wrapped) ok = mbar_wait_asleep(&bars.raw_empty[r.pos], r.par ^ 1u, status);
                     if (!ok) break;
                     unsigned char *s = raw + (size_t)r.pos * kRawBytes;
                     mbar_expect_tx(&bars.raw_full[r.pos], kCodeBytes + sf);
@@ -141,7 +151,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) fp4_grad_kernel(const __grid_
             }
             if (!ok) {                                           // copies in flight must have landed before this CTA's shared memory goes away
                 atomicOr(&bars.failed, 1u);
-                for (int c = max(0, filled - kRawRing); c < filled; ++c) mbar_wait_bounded(&bars.raw_full[c % kRawRing], (unsigned)(c / kRawRing) & 1u, status);
+                for (int c = max(0, filled - kRawRing); c < filled; ++c) mbar_wait_asleep(&bars.raw_full[c % kRawRing], (unsigned)(c / kRawRing) & 1u, status);
             }
         }
     } else if (warp == 1) {
@@ -150,7 +160,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) fp4_grad_kernel(const __grid_
             Ring r(kRing);
             for (int t = first; t < tiles && ok; t += step)
                 for (int d = d0; d < d1; ++d, r.next()) {
-                    ok = mbar_wait_bounded(&bars.ready[r.pos], r.par, status);
+                    ok = mbar_wait_asleep(&bars.ready[r.pos], r.par, status);
                     if (!ok) break;
                     mbar_arrive_pair(smem_u32(&bars.full[r.pos]) + lead);
                 }
@@ -160,28 +170,31 @@ __global__ void __launch_bounds__(kGradThreads, 1) fp4_grad_kernel(const __grid_
             // BF16 x BF16, FP32 sums, B contiguous along N, A along K or along M, N >> 3, M >> 4
             const unsigned idesc = (1u << 4) | (1u << 7) | (1u << 10) | (g.a_kmajor ? 0u : 1u << 15) | (1u << 16) | (kAccCols >> 3 << 17) | ((CTAS * 128u >> 4) << 24);
             const uint64_t a_step = g.a_kmajor ? 2u : 128u;
-            Ring r(kRing), rs(SPLIT ? 1 : 2);
+            Ring r(kRing), rs(SPLIT ? 1 : kSets);
             for (int t = first; t < tiles && ok; t += step) {
                 for (int c0 = d0; c0 < d1 && ok; c0 += SPLIT ? d1 - d0 : g.chain, rs.next()) {
                     const int c1 = SPLIT ? d1 : min(d1, c0 + g.chain);
-                    if (rs.wrapped) ok = __all_sync(kFullMask, mbar_wait_bounded(&bars.acc_empty[rs.pos], rs.par ^ 1u, status)) != 0;
+                    if (rs.wrapped) ok = __all_sync(kFullMask, mbar_wait_asleep(&bars.acc_empty[rs.pos], rs.par ^ 1u, status)) != 0;
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     int set = SPLIT ? 0 : rs.pos, left = g.chain;                            // (SPLIT: up to four accumulators, one behind the other)
                     bool fresh = true;
                     for (int d = c0; d < c1; ++d, r.next()) {
-                        ok = __all_sync(kFullMask, mbar_wait_bounded(&bars.full[r.pos], r.par, status)) != 0;
+                        ok = __all_sync(kFullMask, mbar_wait_asleep(&bars.full[r.pos], r.par, status)) != 0;
                         if (!ok) break;
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                         const unsigned s = smem_u32(base) + (unsigned)r.pos * kOpBytes;
-                        const uint64_t da = g.a_kmajor ? smem_desc_sw128(s) : smem_desc_mn_sw128(s), db = smem_desc_mn_sw128(s + kABytes);
+                        const uint64_t da = g.a_kmajor ? smem_desc_sw128(s) : smem_desc_mn_sw128(s), db = smem_desc_mn_sw128(s + MT * kABytes);
                         const unsigned acc = tmem + (unsigned)set * kAccCols;
                         if (elect_one()) {
 #pragma unroll
-                            for (int kk = 0; kk < kStageD / 16; ++kk) {
-                                if (CTAS == 2) mma_f16_pair(acc, da + a_step * (uint64_t)kk, db + (uint64_t)(kk * 128), idesc, !fresh || kk > 0);
-                                else mma_f16(acc, da + a_step * (uint64_t)kk, db + (uint64_t)(kk * 128), idesc, !fresh || kk > 0);
-                            }
+                            for (int kk = 0; kk < kStageD / 16; ++kk)
+#pragma unroll
+                                for (int m = 0; m < MT; ++m) {
+                                    const uint64_t dam = da + a_step * (uint64_t)kk + (uint64_t)(m * (kABytes >> 4));
+                                    if (CTAS == 2) mma_f16_pair(acc + (unsigned)m * kAccCols, dam, db + (uint64_t)(kk * 128), idesc, !fresh || kk > 0);
+                                    else mma_f16(acc, dam, db + (uint64_t)(kk * 128), idesc, !fresh || kk > 0);
+                                }
                             if (CTAS == 2) tc_commit_pair(&bars.empty[r.pos], 3);
                             else tc_commit(&bars.empty[r.pos]);
                         }
@@ -204,7 +217,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) fp4_grad_kernel(const __grid_
                 atomicOr(&bars.failed, 1u);
                 if (CTAS == 2) tc_commit_pair(&bars.drain, 1);   // MMAs under way must be done before tensor memory is given back
                 else tc_commit(&bars.drain);
-                mbar_wait_bounded(&bars.drain, 0, status);
+                mbar_wait_asleep(&bars.drain, 0, status);
             }
         }
     } else if (warp == 2) {
@@ -213,46 +226,50 @@ __global__ void __launch_bounds__(kGradThreads, 1) fp4_grad_kernel(const __grid_
             Ring r(kRing);
             int filled = 0;
             for (int t = first; t < tiles && ok; t += step) {
-                const int row = ((t % g.r_tiles) * CTAS + half) * 128;
+                const int row = ((t % g.r_tiles) * CTAS * MT + half) * 128;
                 for (int d = d0; d < d1; ++d, ++filled, r.next()) {
-                    if (r.wrapped) ok = mbar_wait_bounded(&bars.empty[r.pos], r.par ^ 1u, status);
+                    if (r.wrapped) ok = mbar_wait_asleep(&bars.empty[r.pos], r.par ^ 1u, status);
                     if (!ok) break;
                     unsigned char *s = base + (size_t)r.pos * kOpBytes;
                     uint64_t *bar = &bars.full[r.pos];
-                    if (leader) mbar_expect_tx(bar, CTAS * kABytes);
-                    if (CTAS == 2) {
-                        const unsigned lead_bar = smem_u32(bar) + lead;
-                        if (g.a_kmajor) {
-                            tma_load_2d_pair(s, &map_a, d * kStageD, row, lead_bar);
+                    if (leader) mbar_expect_tx(bar, CTAS * MT * kABytes);
+#pragma unroll
+                    for (int m = 0; m < MT; ++m, s += kABytes) {
+                        const int r0 = row + m * CTAS * 128;
+                        if (CTAS == 2) {
+                            const unsigned lead_bar = smem_u32(bar) + lead;
+                            if (g.a_kmajor) {
+                                tma_load_2d_pair(s, &map_a, d * kStageD, r0, lead_bar);
+                            } else {
+                                tma_load_2d_pair(s, &map_a, r0, d * kStageD, lead_bar);
+                                tma_load_2d_pair(s + kABytes / 2, &map_a, r0 + 64, d * kStageD, lead_bar);
+                            }
+                        } else if (g.a_kmajor) {
+                            tma_load_2d(s, &map_a, d * kStageD, r0, bar);
                         } else {
-                            tma_load_2d_pair(s, &map_a, row, d * kStageD, lead_bar);
-                            tma_load_2d_pair(s + kABytes / 2, &map_a, row + 64, d * kStageD, lead_bar);
+                            tma_load_2d(s, &map_a, r0, d * kStageD, bar);
+                            tma_load_2d(s + kABytes / 2, &map_a, r0 + 64, d * kStageD, bar);
                         }
-                    } else if (g.a_kmajor) {
-                        tma_load_2d(s, &map_a, d * kStageD, row, bar);
-                    } else {
-                        tma_load_2d(s, &map_a, row, d * kStageD, bar);
-                        tma_load_2d(s + kABytes / 2, &map_a, row + 64, d * kStageD, bar);
                     }
                 }
             }
             if (!ok) {
                 atomicOr(&bars.failed, 1u);
                 if (leader)
-                    for (int c = max(0, filled - kRing); c < filled; ++c) mbar_wait_bounded(&bars.full[c % kRing], (unsigned)(c / kRing) & 1u, status);
+                    for (int c = max(0, filled - kRing); c < filled; ++c) mbar_wait_asleep(&bars.full[c % kRing], (unsigned)(c / kRing) & 1u, status);
             }
         }
     } else if (warp >= kFirstDecode) {
-        // ---- decode: four groups of four warps take the stages in turn.  A thread has one row of B and, twice, 32 of its columns; the lanes of a warp have
+        // ---- decode: groups of four warps take the stages in turn.  A thread has one row of B and, twice, 32 of its columns; the lanes of a warp have
         // rows beside one another, so that neither the swizzled codes nor the swizzled operand see a bank conflict ----
         const int w = (warp - kFirstDecode) % kDecodeWarps, d_in = (w & 1) * 32 + lane, turn = (warp - kFirstDecode) / kDecodeWarps;
         Ring r(kRing), rr(kRawRing);
         int n = 0;
         for (int t = first; t < tiles && ok; t += step) {
-            for (int d = d0; d < d1; ++d, n = n + 1 == kDecodeGroups ? 0 : n + 1, r.next(), rr.next()) {
+            for (int d = d0; d < d1; ++d, n = n + 1 == groups_of(MT) ? 0 : n + 1, r.next(), rr.next()) {
                 if (n != turn) continue;
                 constexpr int kUnits = 8 / kDecodeWarps;         // of 32 columns for each thread
-                ok = __all_sync(kFullMask, mbar_wait_bounded(&bars.raw_full[rr.pos], rr.par, status)) != 0;
+                ok = __all_sync(kFullMask, mbar_wait_asleep(&bars.raw_full[rr.pos], rr.par, status)) != 0;
                 if (!ok) break;
                 const unsigned char *s = raw + (size_t)rr.pos * kRawBytes;
                 const int row = (d & 1) * 64 + d_in;             // in its scale tile
@@ -277,9 +294,9 @@ __global__ void __launch_bounds__(kGradThreads, 1) fp4_grad_kernel(const __grid_
                     v[j][3] = decode8<FMT>(c.w, s1);
                 }
                 // only then the operand's place is waited for: what follows is all that a free stage waits for on this side
-                if (r.wrapped) ok = __all_sync(kFullMask, mbar_wait_bounded(&bars.empty[r.pos], r.par ^ 1u, status)) != 0;
+                if (r.wrapped) ok = __all_sync(kFullMask, mbar_wait_asleep(&bars.empty[r.pos], r.par ^ 1u, status)) != 0;
                 if (!ok) break;
-                unsigned char *b = base + (size_t)r.pos * kOpBytes + kABytes + d_in * 128;
+                unsigned char *b = base + (size_t)r.pos * kOpBytes + MT * kABytes + d_in * 128;
 #pragma unroll
                 for (int j = 0; j < kUnits; ++j) {
                     const int u = (w >> 1) + j * (kDecodeWarps / 2);
@@ -300,11 +317,11 @@ __global__ void __launch_bounds__(kGradThreads, 1) fp4_grad_kernel(const __grid_
         const float f0 = *g.head, f1 = FMT == kNvFp4 ? kNvHold : 1.0f;
         const int size = g.type == kF32 ? 4 : 2;
         int which = 0;
-        Ring rs(SPLIT ? 1 : 2);
+        Ring rs(SPLIT ? 1 : kSets);
         for (int t = first; t < tiles; t += step) {
-            const int row = ((t % g.r_tiles) * CTAS + half) * 128 + quarter * 32 + lane, col = (t / g.r_tiles) * (int)kAccCols;
+            const int row = ((t % g.r_tiles) * CTAS * MT + half) * 128 + quarter * 32, col = (t / g.r_tiles) * (int)kAccCols;
             for (int c0 = d0; c0 < d1; c0 += SPLIT ? d1 - d0 : g.chain, rs.next()) {
-                if (ok) ok = __all_sync(kFullMask, mbar_wait_bounded(&bars.acc_full[rs.pos], rs.par, status)) != 0;
+                if (ok) ok = __all_sync(kFullMask, mbar_wait_asleep(&bars.acc_full[rs.pos], rs.par, status)) != 0;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const unsigned taddr = tmem + (SPLIT ? 0u : (unsigned)rs.pos * kAccCols) + ((unsigned)(quarter * 32) << 16);
                 const bool add = !SPLIT && c0 > d0;              // (FP32 only: to what this warp wrote before)
@@ -326,9 +343,10 @@ __global__ void __launch_bounds__(kGradThreads, 1) fp4_grad_kernel(const __grid_
                 } else {
                     // through boxes in shared memory, 16-byte pieces swizzled as the tensor map says, written (or added) by TMA as whole lines.  What was written to
                     // this tile before has to be there before it is added to: in that order every time, the same bits every time.
-                    const int per = 128 / size, row0 = row - lane;
+                    const int per = 128 / size;
                     if (add && lane == 0) bulk_wait_all();
-                    for (int c = 0; c < (int)kAccCols; c += per, which ^= 1) {
+                    for (int at = 0; at < MT * (int)kAccCols; at += per, which ^= 1) {
+                        const int m = at / (int)kAccCols, c = at - m * (int)kAccCols, row0 = row + m * CTAS * 128;
                         unsigned char *box = boxes + (unsigned)((warp - 4) * 2 + which) * kBoxBytes;
                         if (lane == 0) bulk_wait_read_1();       // this box's last copy has been read
                         __syncwarp();
@@ -336,7 +354,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) fp4_grad_kernel(const __grid_
 #pragma unroll 1
                         for (int h = 0; h < per; h += 16) {
                             unsigned r[16];
-                            read_columns(taddr + (unsigned)(c + h), r, ok);
+                            read_columns(taddr + (unsigned)(at + h), r, ok);
                             float v[16];
 #pragma unroll
                             for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]) * f0 * f1;
@@ -391,7 +409,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) fp4_grad_kernel(const __grid_
         cluster.sync();
         const int rt = first % g.r_tiles, ct = first / g.r_tiles;
         const auto read = [&](int i, int c) { return *reinterpret_cast<const float4 *>(cluster.map_shared_rank(reinterpret_cast<const float *>(base) + i, c)); };
-        add_parts<kGradThreads>(read, rank, kTileC + 4, min(128, g.R - rt * 128), min(kTileC, g.C - ct * kTileC), g.splits, *g.head, FMT == kNvFp4 ? kNvHold : 1.0f, g.out,
+        add_parts<grad_threads(MT)>(read, rank, kTileC + 4, min(128, g.R - rt * 128), min(kTileC, g.C - ct * kTileC), g.splits, *g.head, FMT == kNvFp4 ? kNvHold : 1.0f, g.out,
                                 g.type, (long)(rt * 128) * g.ld + ct * kTileC, g.ld);
         cluster.sync();                                          // nobody leaves while its shared memory is being read
     }
@@ -404,23 +422,24 @@ __global__ void __launch_bounds__(256) pad_rows_kernel(const unsigned short *in,
         for (uint64_t c = (uint64_t)blockIdx.x * 2048 + threadIdx.x; c < min(cols, (uint64_t)(blockIdx.x + 1) * 2048); c += 256) out[r * ld_out + c] = in[r * ld + c];
 }
 
-template <int FMT, int CTAS, bool SPLIT>
+template <int FMT, int CTAS, int MT, bool SPLIT>
 cudaError_t launch_grad(const CUtensorMap &map_a, const CUtensorMap &map_b, const CUtensorMap &map_c, const Fp4Grad &g, int sm_count, unsigned *status, cudaStream_t stream) {
-    constexpr size_t smem = 1024 + kRing * kOpBytes + kRawRing * kRawBytes + kBoxesBytes + sizeof(GradBars) + 64;
+    constexpr size_t smem = 1024 + ring_of(MT) * op_bytes_of(MT) + kRawRing * kRawBytes + kBoxesBytes + sizeof(GradBars) + 64;
     static_assert(smem <= 227 * 1024, "stages do not fit");
-    static_assert((size_t)128 * (kTileC + 4) * 4 <= (size_t)kRing * kOpBytes, "partial tile does not fit");
-    cudaError_t err = cudaFuncSetAttribute(fp4_grad_kernel<FMT, CTAS, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    static_assert((size_t)128 * (kTileC + 4) * 4 <= (size_t)ring_of(MT) * op_bytes_of(MT), "partial tile does not fit");
+    cudaError_t err = cudaFuncSetAttribute(fp4_grad_kernel<FMT, CTAS, MT, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (err != cudaSuccess) return err;
     const int tiles = g.r_tiles * g.c_tiles;
-    if (SPLIT) return launch_cluster(fp4_grad_kernel<FMT, CTAS, SPLIT>, (unsigned)(tiles * g.splits), kGradThreads, g.splits, smem, stream, map_a, map_b, map_c, g, status);
+    if (SPLIT) return launch_cluster(fp4_grad_kernel<FMT, CTAS, MT, SPLIT>, (unsigned)(tiles * g.splits), grad_threads(MT), g.splits, smem, stream, map_a, map_b, map_c, g, status);
     const int units = sm_count / CTAS, grid = (tiles < units ? tiles : units) * CTAS;
-    if (CTAS == 2) return launch_cluster(fp4_grad_kernel<FMT, CTAS, SPLIT>, (unsigned)grid, kGradThreads, CTAS, smem, stream, map_a, map_b, map_c, g, status);
-    return launch_chained(fp4_grad_kernel<FMT, CTAS, SPLIT>, (unsigned)grid, kGradThreads, smem, stream, map_a, map_b, map_c, g, status);
+    if (CTAS == 2) return launch_cluster(fp4_grad_kernel<FMT, CTAS, MT, SPLIT>, (unsigned)grid, grad_threads(MT), CTAS, smem, stream, map_a, map_b, map_c, g, status);
+    return launch_chained(fp4_grad_kernel<FMT, CTAS, MT, SPLIT>, (unsigned)grid, grad_threads(MT), smem, stream, map_a, map_b, map_c, g, status);
 }
 template <int FMT>
-cudaError_t launch_grad_format(int ctas, const CUtensorMap &map_a, const CUtensorMap &map_b, const CUtensorMap &map_c, const Fp4Grad &g, int sm_count, unsigned *status, cudaStream_t stream) {
-    if (ctas == 2) return launch_grad<FMT, 2, false>(map_a, map_b, map_c, g, sm_count, status, stream);
-    return g.splits > 1 ? launch_grad<FMT, 1, true>(map_a, map_b, map_c, g, sm_count, status, stream) : launch_grad<FMT, 1, false>(map_a, map_b, map_c, g, sm_count, status, stream);
+cudaError_t launch_grad_format(int ctas, int blocks, const CUtensorMap &map_a, const CUtensorMap &map_b, const CUtensorMap &map_c, const Fp4Grad &g, int sm_count, unsigned *status, cudaStream_t stream) {
+    if (ctas == 2 && blocks == 2) return launch_grad<FMT, 2, 2, false>(map_a, map_b, map_c, g, sm_count, status, stream);
+    if (ctas == 2) return launch_grad<FMT, 2, 1, false>(map_a, map_b, map_c, g, sm_count, status, stream);
+    return g.splits > 1 ? launch_grad<FMT, 1, 1, true>(map_a, map_b, map_c, g, sm_count, status, stream) : launch_grad<FMT, 1, 1, false>(map_a, map_b, map_c, g, sm_count, status, stream);
 }
 
 bool needs_padding(const void *dy, uint64_t rows, uint64_t ld) { return reinterpret_cast<uintptr_t>(dy) % 16 != 0 || (rows > 1 && ld % 8 != 0); }
@@ -448,7 +467,9 @@ cudaError_t grad_product(int format, bool a_kmajor, const void *dy, uint64_t M, 
     if (r128 * c128 > 0x7fffffffull / 8) return cudaErrorInvalidValue;
     // a pair per tile of 256 x 256 where that fills the device
     const int ctas = r128 > 1 && ((r128 + 1) / 2) * ((c128 + 1) / 2) * 2 >= (uint64_t)sm_count * 2 / 3 ? 2 : 1;
-    g.r_tiles = (int)((r128 + ctas - 1) / ctas); g.c_tiles = (int)((c128 + ctas - 1) / ctas);
+    // ... of 512 x 256 where that does too: an element is then decoded once for 512 rows, but no accumulators are left for the next tile while one is taken out
+    const int blocks = ctas == 2 && type != kF32 && ((r128 + 3) / 4) * ((c128 + 1) / 2) * 2 >= (uint64_t)sm_count * 2 / 3 ? 2 : 1;
+    g.r_tiles = (int)((r128 + ctas * blocks - 1) / (ctas * blocks)); g.c_tiles = (int)((c128 + ctas - 1) / ctas);
     g.d_stages = (int)((D + kStageD - 1) / kStageD);
     g.a_kmajor = a_kmajor;
     g.quads = (unsigned)fp4_quads(format, C);
@@ -481,8 +502,8 @@ cudaError_t grad_product(int format, bool a_kmajor, const void *dy, uint64_t M, 
                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
             return cudaErrorInvalidValue;
     }
-    return format == kNvFp4 ? launch_grad_format<kNvFp4>(ctas, map_a, map_b, map_c, g, sm_count, status, stream)
-                            : launch_grad_format<kMxFp4>(ctas, map_a, map_b, map_c, g, sm_count, status, stream);
+    return format == kNvFp4 ? launch_grad_format<kNvFp4>(ctas, blocks, map_a, map_b, map_c, g, sm_count, status, stream)
+                            : launch_grad_format<kMxFp4>(ctas, blocks, map_a, map_b, map_c, g, sm_count, status, stream);
 }
 
 }  // namespace

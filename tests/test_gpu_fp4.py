@@ -251,7 +251,7 @@ def test_scale_extremes(ops):
 
 
 GRAD = [(2, 33, 129), (9, 2000, 390), (15, 4090, 1000), (1, 16, 32), (1, 1031, 300), (3, 257, 1000), (16, 300, 128), (63, 640, 257), (65, 100, 31), (128, 256, 256), (129, 257, 258), (200, 1500, 640),
-        (777, 515, 1030), (1, 4096, 512), (40, 40, 4096), (2500, 72, 64), (130, 64, 9000), (2600, 2500, 520)]
+        (777, 515, 1030), (1, 4096, 512), (40, 40, 4096), (2500, 72, 64), (130, 64, 9000), (2600, 2500, 520), (4100, 200, 4100), (200, 4100, 4100)]
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
