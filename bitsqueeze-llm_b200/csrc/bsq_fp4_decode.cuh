@@ -32,16 +32,16 @@ template <int FMT> __device__ __forceinline__ uint4 decode8(unsigned x, unsigned
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
-// The factor of decode8 from a scale byte, in both halves of a word
-template <int FMT> __device__ __forceinline__ unsigned decode_scale(unsigned byte) {
-    unsigned h;
+// The factors of decode8 from two scale bytes (each in the low byte of its word): the first in the low half.  NVFP4: s * 2^(126 - 12), exact in BF16.
+template <int FMT> __device__ __forceinline__ unsigned decode_scales(unsigned b0, unsigned b1) {
     if (FMT == kMxFp4) {
-        h = byte == 0 ? 0x0040u : byte == 255 ? 0x7FFFu : byte << 7;
-    } else {
-        byte &= 0x7fu;                                           // s * 2^(126 - 12), exact in BF16
-        h = byte == 0x7fu ? 0x7FFFu : __float_as_uint(e4m3_decode(byte) * 2.076918743413931e34f) >> 16;
+        const unsigned h0 = b0 == 0 ? 0x0040u : b0 == 255 ? 0x7FFFu : b0 << 7, h1 = b1 == 0 ? 0x0040u : b1 == 255 ? 0x7FFFu : b1 << 7;
+        return h0 | (h1 << 16);
     }
-    return h | (h << 16);
+    unsigned f;
+    asm("{\n\t.reg .b16 e;\n\tcvt.u16.u32 e, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, e;\n\t}" : "=r"(f) : "r"((b0 | (b1 << 8)) & 0x7f7fu));
+    const float2 s = __half22float2(*reinterpret_cast<const __half2 *>(&f));
+    return pack_pair<kBf16>(s.x * 2.076918743413931e34f, s.y * 2.076918743413931e34f);
 }
 
 }  // namespace

@@ -68,43 +68,49 @@ template <int FMT> __global__ void __launch_bounds__(kFewThreads, 2) fp4_grad_fe
     unsigned char *mine = smem_few + (unsigned)warp * kFewStages * kFewStage;
     const unsigned mine_u = smem_u32(mine);
 
-    // row r of a chunk lies at place (r & 7) * 4 + (r >> 3): the four threads t that read rows 8 t + j at once read neighbouring places
-    const auto fetch = [&](int chunk, int stage) {
-        if (chunk < c_end) {
-            const uint64_t row0 = (uint64_t)chunk * kFewRows;
-            const unsigned dst = mine_u + (unsigned)stage * kFewStage;
+    const int first = rank * g.chunks_per_split + warp;
+    // What this lane copies of a chunk: 16 bytes of rows lane / 4, + 8, + 16, + 24, and the scales of row `lane`.  Row r lies at place (r & 7) * 4 + (r >> 3): the four
+    // threads t that read rows 8 t + j at once read neighbouring places.
+    const int quad0 = col0 / (FMT == kNvFp4 ? 64 : 128);
+    const bool col_live = (uint64_t)(col0 / 2) + (uint64_t)(lane & 3) * 16 < g.ld_codes;
+    const uint8_t *code_at = g.codes + ((uint64_t)first * kFewRows + (lane >> 2)) * g.ld_codes + col0 / 2 + (lane & 3) * 16;
+    const uint64_t row8 = 8 * g.ld_codes, code_step = (uint64_t)kFewWarps * kFewRows * g.ld_codes;
+    const unsigned code_to = mine_u + (unsigned)(lane >> 2) * 256u + (unsigned)(lane & 3) * 16u;
+    const unsigned scale_to = mine_u + kFewCodes + (unsigned)(((lane & 7) * 4 + (lane >> 3)) * kQuads * 4);
+    int ahead = first;                                           // the next chunk to be copied
+    const auto fetch = [&](int stage) {
+        if (ahead < c_end) {
+            const int row0 = ahead * kFewRows;
+            const unsigned off = (unsigned)stage * kFewStage;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int r = (lane >> 2) + 8 * i;
-                const uint64_t at = (uint64_t)(col0 / 2) + (uint64_t)(lane & 3) * 16;
-                const bool live = row0 + r < (uint64_t)g.D && at < g.ld_codes;
-                copy16(dst + (unsigned)(((r & 7) * 4 + (r >> 3)) * 64 + (lane & 3) * 16), live ? g.codes + (row0 + r) * g.ld_codes + at : g.codes, live);
+                const bool live = col_live && row0 + (lane >> 2) + 8 * i < g.D;
+                copy16(code_to + off + (unsigned)i * 64u, live ? code_at + i * row8 : g.codes, live);
             }
-            const uint64_t tile = (row0 / 128 * g.quads + (uint64_t)(col0 / (FMT == kNvFp4 ? 64 : 128))) * 512;
-            const unsigned in_tile = (unsigned)lane * 16 + (unsigned)(chunk & 3) * 4;            // (32 rows of a chunk are 32 neighbours of a tile)
+            const uint8_t *scale_at = g.scales + ((uint64_t)(ahead >> 2) * g.quads + (uint64_t)quad0) * 512 + (unsigned)lane * 16u + (unsigned)(ahead & 3) * 4u;
 #pragma unroll
             for (int q = 0; q < kQuads; ++q) {
-                const bool live = row0 + lane < (uint64_t)g.D && (uint64_t)(col0 / (FMT == kNvFp4 ? 64 : 128) + q) < g.quads;
-                copy4(dst + kFewCodes + (unsigned)((((lane & 7) * 4 + (lane >> 3)) * kQuads + q) * 4), live ? g.scales + tile + q * 512 + in_tile : g.scales, live);
+                const bool live = row0 + lane < g.D && (uint64_t)(quad0 + q) < g.quads;
+                copy4(scale_to + off + (unsigned)q * 4u, live ? scale_at + q * 512 : g.scales, live);
             }
+            code_at += code_step;
+            ahead += kFewWarps;
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-
-    const int first = rank * g.chunks_per_split + warp;
     const __nv_bfloat16 *a0 = g.dy + (uint64_t)gq * g.ld_dy, *a1 = g.dy + (uint64_t)(gq + 8) * g.ld_dy;
     const bool live0 = gq < g.R, live1 = gq + 8 < g.R;
     float acc[16][4];
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
 #pragma unroll
-    for (int s = 0; s < kFewStages - 1; ++s) fetch(first + s * kFewWarps, s);
+    for (int s = 0; s < kFewStages - 1; ++s) fetch(s);
     uint4 n0 = load_dy(a0, first * kFewRows + 8 * t, first < c_end ? g.D : 0, live0), n1 = load_dy(a1, first * kFewRows + 8 * t, first < c_end ? g.D : 0, live1);
     int stage = 0;
     for (int chunk = first; chunk < c_end; chunk += kFewWarps) {
         asm volatile("cp.async.wait_group %0;" ::"n"(kFewStages - 2) : "memory");
         __syncwarp();                                            // everybody's copies of this stage are there, and everybody is done with the one before
-        fetch(chunk + (kFewStages - 1) * kFewWarps, (stage + kFewStages - 1) % kFewStages);
+        fetch((stage + kFewStages - 1) % kFewStages);
         const uint4 d0 = n0, d1 = n1;
         const int next = chunk + kFewWarps;
         n0 = load_dy(a0, next * kFewRows + 8 * t, next < c_end ? g.D : 0, live0);
@@ -116,16 +122,16 @@ template <int FMT> __global__ void __launch_bounds__(kFewThreads, 2) fp4_grad_fe
             unsigned w[2][2][2], scale[2];                       // [pair][row of the pair][8 columns]
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
-                unsigned h[2];
+                unsigned byte[2];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const int place = (step * 4 + p * 2 + e) * 4 + t;
                     const uint2 c = *reinterpret_cast<const uint2 *>(s + place * 64 + gq * 8);
                     w[p][e][0] = c.x;
                     w[p][e][1] = c.y;
-                    h[e] = decode_scale<FMT>(FMT == kNvFp4 ? s[kFewCodes + (place * 2 + (gq >> 2)) * 4 + (gq & 3)] : s[kFewCodes + place * 4 + (gq >> 1)]);
+                    byte[e] = FMT == kNvFp4 ? s[kFewCodes + (place * 2 + (gq >> 2)) * 4 + (gq & 3)] : s[kFewCodes + place * 4 + (gq >> 1)];
                 }
-                scale[p] = (h[0] & 0xffffu) | (h[1] & 0xffff0000u);
+                scale[p] = decode_scales<FMT>(byte[0], byte[1]);
             }
 #pragma unroll
             for (int q = 0; q < 4; ++q) {                        // four columns of the 16
@@ -193,10 +199,11 @@ cudaError_t fp4_grad_few(int format, const void *dy, int R, uint64_t ld_dy, cons
     g.dy = static_cast<const __nv_bfloat16 *>(dy);
     g.ld_dy = ld_dy;
     g.out = out; g.ld = (long)ld; g.type = type;
+    static std::atomic<uint64_t> done_mx{0}, done_nv{0};
     constexpr size_t smem = (size_t)kFewWarps * kFewStages * kFewStage;
     static_assert(smem >= (size_t)kFewWarps * 16 * (kFewCols + 4) * 4, "partial sums do not fit");
     const auto kernel = format == kNvFp4 ? fp4_grad_few_kernel<kNvFp4> : fp4_grad_few_kernel<kMxFp4>;
-    const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    const cudaError_t err = allow_smem(kernel, format == kNvFp4 ? &done_nv : &done_mx);
     if (err != cudaSuccess) return err;
     return launch_cluster(kernel, (unsigned)(blocks * g.splits), kFewThreads, g.splits, smem, stream, g);
 }

@@ -352,7 +352,8 @@ cudaError_t launch_fp4_gemm(GemmMaps &maps, Fp4Gemm &g, const uint8_t *p, const 
     const size_t room = ((size_t)227 * 1024 - fixed) / stage;
     g.ring = (int)(room < (size_t)kMaxStages ? room : (size_t)kMaxStages);
     const size_t smem = fixed + g.ring * stage;
-    cudaError_t err = cudaFuncSetAttribute(fp4_gemm_kernel<FMT, CTAS, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    static std::atomic<uint64_t> done{0};
+    const cudaError_t err = allow_smem(fp4_gemm_kernel<FMT, CTAS, SPLIT>, &done);
     if (err != cudaSuccess) return err;
     const int tiles = g.p_tiles * g.q_tiles, units = sm_count / CTAS;
     if (SPLIT) return launch_cluster(fp4_gemm_kernel<FMT, CTAS, SPLIT>, (unsigned)(tiles * g.splits), kGemmThreads, g.splits, smem, stream, maps, g, status);

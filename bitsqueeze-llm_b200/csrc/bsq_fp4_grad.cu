@@ -282,11 +282,13 @@ __global__ void __launch_bounds__(grad_threads(MT), 1) fp4_grad_kernel(const __g
                     const uint4 c = *reinterpret_cast<const uint4 *>(s + d_in * 64 + ((u ^ ((d_in >> 1) & 3)) << 4));
                     unsigned s0, s1;
                     if (FMT == kMxFp4) {
-                        s0 = s1 = decode_scale<FMT>(live ? sf[u] : 0u);
+                        const unsigned one = live ? sf[u] : 0u;
+                        s0 = s1 = decode_scales<FMT>(one, one);
                     } else {
                         const unsigned two = live ? *reinterpret_cast<const unsigned short *>(sf + (u >> 1) * 512 + (u & 1) * 2) : 0u;
-                        s0 = decode_scale<FMT>(two & 0xffu);
-                        s1 = decode_scale<FMT>(two >> 8);
+                        const unsigned both = decode_scales<FMT>(two & 0xffu, two >> 8);
+                        s0 = __byte_perm(both, both, 0x1010);
+                        s1 = __byte_perm(both, both, 0x3232);
                     }
                     v[j][0] = decode8<FMT>(c.x, s0);
                     v[j][1] = decode8<FMT>(c.y, s0);
@@ -427,7 +429,8 @@ cudaError_t launch_grad(const CUtensorMap &map_a, const CUtensorMap &map_b, cons
     constexpr size_t smem = 1024 + ring_of(MT) * op_bytes_of(MT) + kRawRing * kRawBytes + kBoxesBytes + sizeof(GradBars) + 64;
     static_assert(smem <= 227 * 1024, "stages do not fit");
     static_assert((size_t)128 * (kTileC + 4) * 4 <= (size_t)ring_of(MT) * op_bytes_of(MT), "partial tile does not fit");
-    cudaError_t err = cudaFuncSetAttribute(fp4_grad_kernel<FMT, CTAS, MT, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    static std::atomic<uint64_t> done{0};
+    const cudaError_t err = allow_smem(fp4_grad_kernel<FMT, CTAS, MT, SPLIT>, &done);
     if (err != cudaSuccess) return err;
     const int tiles = g.r_tiles * g.c_tiles;
     if (SPLIT) return launch_cluster(fp4_grad_kernel<FMT, CTAS, MT, SPLIT>, (unsigned)(tiles * g.splits), grad_threads(MT), g.splits, smem, stream, map_a, map_b, map_c, g, status);

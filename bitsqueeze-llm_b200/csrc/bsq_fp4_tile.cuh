@@ -4,6 +4,8 @@
 
 #include <cooperative_groups.h>
 
+#include <atomic>
+
 #include "bsq_fp4.cuh"
 #include "bsq_gemm_tc.cuh"
 #include "bsq_tma.cuh"
@@ -113,6 +115,18 @@ inline bool map_codes(CUtensorMap *map, const uint8_t *packed, uint64_t rows, ui
     return encode_tiled() && encode_tiled()(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t *>(packed) + kFp4Head, dims, strides, box, estr,
                                             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Lets a kernel have all of an SM's shared memory, once for each device.
+template <class F> cudaError_t allow_smem(F *kernel, std::atomic<uint64_t> *done) {
+    int device = 0;
+    cudaError_t err = cudaGetDevice(&device);
+    if (err != cudaSuccess) return err;
+    const uint64_t bit = 1ull << (device & 63);
+    if (device < 64 && (done->load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+    err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+    if (err == cudaSuccess && device < 64) done->fetch_or(bit, std::memory_order_relaxed);
+    return err;
 }
 
 // A chained launch (launch_chained) in clusters of `ctas` along x
