@@ -312,6 +312,7 @@ def clip_grad_norm(grads, max_norm, norm_type=2.0, out=None):
         raise ValueError("no gradients: the device of their norm is not known")
     if max_norm is None and out is not None:
         raise ValueError("out needs a max_norm")
+    max_norm = None if max_norm is None else float(max_norm)
     if max_norm is not None and not max_norm >= 0:
         raise ValueError("max_norm must not be negative or NaN")
     device, n = grads[0].device, len(grads)

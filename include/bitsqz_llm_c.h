@@ -264,7 +264,7 @@ int bsq_batch_decompress(bsq_batch_t *batch, const struct bitsqz_llm_array *cons
  * multiple of 32 columns, scales behind the last block of a row 0 up to the end of the tile; scale bytes of rows behind the last one may hold anything.
  *
  * type: 0 FP32, 1 FP16, 2 BF16; ld: elements from one row to the next.  Rows may be 0.  All calls enqueue on `stream` and return; they allocate nothing and keep
- * nothing, and may be captured.  d_status (nullable): bit 0 is set when a bounded wait gave up; the results concerned are NaN then. */
+ * nothing, and may be captured.  What a call writes must not overlap what it reads.  d_status (nullable): bit 0 is set when a bounded wait gave up; the results concerned are NaN then. */
 uint64_t bsq_fp4_packed_bytes(int format, uint64_t rows, uint64_t cols);
 /* what bsq_fp4_quantize needs in d_scratch when it is not given d_amax: 0 for MXFP4 and for small matrices */
 size_t bsq_fp4_scratch_bytes(int format, int type, uint64_t rows, uint64_t cols);

@@ -454,3 +454,80 @@ def test_quantise_into_a_given_matrix(ops):
     x = torch.randn(20, 100, device="cuda")
     q = ops.fp4_quantize(torch.zeros(20, 100, device="cuda"))
     assert ops.fp4_quantize(x, out=q) is q and torch.equal(q.codes, ops.fp4_quantize(x).codes)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+def test_large_rows_apart(ops, fmt, dtype):
+    """Rows that are not neighbours in a matrix large enough for a pass of its own over the magnitudes, and values written to such rows."""
+    base = torch.randn(700, 310, generator=torch.Generator().manual_seed(7)).to(DTYPES[dtype])
+    base[:, 300:] = 1000.0                                        # (not part of the matrix: must not count)
+    base[699, 299] = -77.0
+    base = base.cuda()
+    for first, cols in ((0, 300), (1, 299), (5, 256)):
+        x = base[:, first: first + cols]
+        q = check_quantised(ops, x, fmt)
+        wide = torch.full((702, cols + 11), -7.0, dtype=DTYPES[dtype], device="cuda")
+        out = wide[1:701, 3: 3 + cols]
+        assert ops.fp4_dequantize(q, DTYPES[dtype], out=out) is out
+        assert torch.equal(out, ops.fp4_dequantize(q, DTYPES[dtype]))
+        assert (wide[0] == -7).all() and (wide[701] == -7).all() and (wide[:, :3] == -7).all() and (wide[:, 3 + cols:] == -7).all()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_packed_matrices_on_any_16_bytes(ops, fmt):
+    x = torch.randn(150, 200, device="cuda").to(torch.bfloat16)
+    w = torch.randn(90, 200, device="cuda").to(torch.bfloat16)
+    dy = torch.randn(150, 90, device="cuda").to(torch.bfloat16)
+    x4, w4 = ops.fp4_quantize(x, fmt), ops.fp4_quantize(w, fmt)
+
+    def moved(m, by):
+        buffer = torch.full((m.nbytes + by + 64,), 0xFF, dtype=torch.uint8, device="cuda")
+        buffer[by: by + m.nbytes] = m.data[: m.nbytes]
+        return ops.Fp4Matrix(buffer[by: by + m.nbytes], m.rows, m.cols, m.format)
+    xm, wm = moved(x4, 16), moved(w4, 48)
+    assert torch.equal(ops.fp4_matmul(xm, wm), ops.fp4_matmul(x4, w4)) and torch.equal(ops.fp4_dequantize(xm), ops.fp4_dequantize(x4))
+    assert torch.equal(ops.fp4_grad_input(dy, wm), ops.fp4_grad_input(dy, w4)) and torch.equal(ops.fp4_grad_weight(dy, xm), ops.fp4_grad_weight(dy, x4))
+    assert torch.equal(ops.fp4_grad_input(dy[:9], wm), ops.fp4_grad_input(dy[:9], w4))
+    ops.fp4_quantize(w, fmt, out=xm if xm.shape == w.shape else wm)
+    assert torch.equal(wm.codes, w4.codes)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("M", [7, 140])
+def test_non_finite_gradients_stay_where_they_belong(ops, fmt, M):
+    w, x = ops.fp4_quantize(torch.ones(90, 200, device="cuda"), fmt), ops.fp4_quantize(torch.ones(M, 200, device="cuda"), fmt)
+    dy = torch.ones(M, 90, dtype=torch.bfloat16, device="cuda")
+    dx0, dw0 = ops.fp4_grad_input(dy, w, torch.float32), ops.fp4_grad_weight(dy, x, torch.float32)
+    dy[3, 60], dy[5, 89] = float("nan"), float("inf")
+    dx, dw = ops.fp4_grad_input(dy, w, torch.float32), ops.fp4_grad_weight(dy, x, torch.float32)
+    rows, cols = [i for i in range(M) if i not in (3, 5)], [i for i in range(90) if i not in (60, 89)]
+    assert torch.isnan(dx[3]).all() and torch.isinf(dx[5]).all() and torch.equal(dx[rows], dx0[rows])
+    assert torch.isnan(dw[60]).all() and torch.isinf(dw[89]).all() and torch.equal(dw[cols], dw0[cols])
+
+
+def test_the_same_bits_every_time(ops):
+    """Shapes that take every way through the products, ten times over."""
+    torch.manual_seed(3)
+    for M, N, K in ((1, 600, 3000), (40, 4096, 2048), (300, 1000, 4096), (2100, 2200, 2050), (4100, 300, 4100)):
+        x, w = ops.fp4_quantize(torch.randn(M, K, device="cuda")), ops.fp4_quantize(torch.randn(N, K, device="cuda"))
+        dy = torch.randn(M, N, device="cuda").to(torch.bfloat16)
+        calls = [lambda: ops.fp4_matmul(x, w, torch.float32), lambda: ops.fp4_grad_input(dy, w), lambda: ops.fp4_grad_input(dy, w, torch.float32),
+                 lambda: ops.fp4_grad_weight(dy, x), lambda: ops.fp4_grad_weight(dy, x, torch.float32), lambda: ops.fp4_grad_input(dy[: min(M, 9)], w)]
+        for call in calls:
+            first = call()
+            assert not torch.isnan(first).any()
+            for _ in range(10):
+                assert torch.equal(call(), first)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_few_rows_are_the_rows_of_many(ops, fmt):
+    """The kernel for up to 16 rows against the one for more: sums of values that are exact in FP32."""
+    rng = np.random.default_rng(31)
+    for N, K in ((16, 33), (1000, 700), (4096, 300), (100, 5000)):
+        w, vw = packed(ops, rng, N, K, fmt)
+        dy = torch.from_numpy(rng.integers(-8, 9, (33, N)).astype(np.float64)).to(torch.bfloat16).cuda()
+        many = ops.fp4_grad_input(dy, w, torch.float32)
+        for a, b in ((0, 1), (1, 17), (5, 13), (16, 33)):
+            assert torch.equal(ops.fp4_grad_input(dy[a:b], w, torch.float32), many[a:b])
