@@ -8,16 +8,18 @@
 // eight rows of W make one 16-byte load of dY.  Column i of every thread's 16 is one MMA's n, so a thread ends up with 32 neighbouring
 // columns of the result.
 //
-// Codes and scales come by cp.async, four stages of 32 rows ahead for each warp on its own (18 KB a CTA and stage, no barrier in the loop).  The warps of a CTA and
+// Codes and scales come by cp.async, three chunks of 32 rows ahead for each warp on its own (no barrier in the loop).  The warps of a CTA and
 // the CTAs of a cluster share the rows; their sums are added in a fixed order.
 #include "bsq_fp4_decode.cuh"
 #include "bsq_fp4_few.hpp"
 #include "bsq_fp4_tile.cuh"
 
+#include <algorithm>
+
 namespace bsq {
 namespace {
 
-constexpr int kFewThreads = 256, kFewWarps = kFewThreads / 32, kFewStages = 4, kFewCols = 128, kFewRows = 32;
+constexpr int kFewStages = 4, kFewCols = 128, kFewRows = 32;
 constexpr unsigned kFewCodes = kFewRows * kFewCols / 2, kFewStage = kFewCodes + 256;
 
 struct Fp4Few {
@@ -58,7 +60,39 @@ __device__ __forceinline__ uint4 load_dy(const __nv_bfloat16 *row, int d, int D,
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-template <int FMT> __global__ void __launch_bounds__(kFewThreads, 2) fp4_grad_few_kernel(const Fp4Few g) {
+// 32 rows x this thread's 16 columns: decoded and multiplied.  ONE: see decode8.
+template <int FMT, bool ONE> __device__ __forceinline__ void few_chunk(const unsigned char *s, int gq, int t, const uint4 &d0, const uint4 &d1, float (&acc)[16][4]) {
+#pragma unroll
+    for (int step = 0; step < 2; ++step) {
+        const unsigned a[4] = {step ? d0.z : d0.x, step ? d1.z : d1.x, step ? d0.w : d0.y, step ? d1.w : d1.y};
+        unsigned w[2][2][2], scale[2];                           // [pair][row of the pair][8 columns]
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+            unsigned byte[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int place = (step * 4 + p * 2 + e) * 4 + t;
+                const uint2 c = *reinterpret_cast<const uint2 *>(s + place * 64 + gq * 8);
+                w[p][e][0] = c.x;
+                w[p][e][1] = c.y;
+                byte[e] = FMT == kNvFp4 ? s[kFewCodes + (place * 2 + (gq >> 2)) * 4 + (gq & 3)] : s[kFewCodes + place * 4 + (gq >> 1)];
+            }
+            scale[p] = ONE ? decode_scales_one(byte[0], byte[1]) : decode_scales<FMT>(byte[0], byte[1]);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {                            // four columns of the 16
+            const unsigned sel = q & 1 ? 0x7632u : 0x5410u;
+            const uint4 b0 = decode8<FMT, ONE>(__byte_perm(w[0][0][q >> 1], w[0][1][q >> 1], sel), scale[0]);
+            const uint4 b1 = decode8<FMT, ONE>(__byte_perm(w[1][0][q >> 1], w[1][1][q >> 1], sel), scale[1]);
+            mma_16816(acc[q * 4 + 0], a, b0.x, b1.x);
+            mma_16816(acc[q * 4 + 1], a, b0.y, b1.y);
+            mma_16816(acc[q * 4 + 2], a, b0.z, b1.z);
+            mma_16816(acc[q * 4 + 3], a, b0.w, b1.w);
+        }
+    }
+}
+
+template <int FMT, int WARPS> __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) fp4_grad_few_kernel(const Fp4Few g) {
     chain_begin();
     extern __shared__ __align__(16) unsigned char smem_few[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, t = lane & 3;
@@ -74,7 +108,7 @@ template <int FMT> __global__ void __launch_bounds__(kFewThreads, 2) fp4_grad_fe
     const int quad0 = col0 / (FMT == kNvFp4 ? 64 : 128);
     const bool col_live = (uint64_t)(col0 / 2) + (uint64_t)(lane & 3) * 16 < g.ld_codes;
     const uint8_t *code_at = g.codes + ((uint64_t)first * kFewRows + (lane >> 2)) * g.ld_codes + col0 / 2 + (lane & 3) * 16;
-    const uint64_t row8 = 8 * g.ld_codes, code_step = (uint64_t)kFewWarps * kFewRows * g.ld_codes;
+    const uint64_t row8 = 8 * g.ld_codes, code_step = (uint64_t)WARPS * kFewRows * g.ld_codes;
     const unsigned code_to = mine_u + (unsigned)(lane >> 2) * 256u + (unsigned)(lane & 3) * 16u;
     const unsigned scale_to = mine_u + kFewCodes + (unsigned)(((lane & 7) * 4 + (lane >> 3)) * kQuads * 4);
     int ahead = first;                                           // the next chunk to be copied
@@ -94,7 +128,7 @@ template <int FMT> __global__ void __launch_bounds__(kFewThreads, 2) fp4_grad_fe
                 copy4(scale_to + off + (unsigned)q * 4u, live ? scale_at + q * 512 : g.scales, live);
             }
             code_at += code_step;
-            ahead += kFewWarps;
+            ahead += WARPS;
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
@@ -107,75 +141,72 @@ template <int FMT> __global__ void __launch_bounds__(kFewThreads, 2) fp4_grad_fe
     for (int s = 0; s < kFewStages - 1; ++s) fetch(s);
     uint4 n0 = load_dy(a0, first * kFewRows + 8 * t, first < c_end ? g.D : 0, live0), n1 = load_dy(a1, first * kFewRows + 8 * t, first < c_end ? g.D : 0, live1);
     int stage = 0;
-    for (int chunk = first; chunk < c_end; chunk += kFewWarps) {
+    for (int chunk = first; chunk < c_end; chunk += WARPS) {
         asm volatile("cp.async.wait_group %0;" ::"n"(kFewStages - 2) : "memory");
         __syncwarp();                                            // everybody's copies of this stage are there, and everybody is done with the one before
         fetch((stage + kFewStages - 1) % kFewStages);
         const uint4 d0 = n0, d1 = n1;
-        const int next = chunk + kFewWarps;
+        const int next = chunk + WARPS;
         n0 = load_dy(a0, next * kFewRows + 8 * t, next < c_end ? g.D : 0, live0);
         n1 = load_dy(a1, next * kFewRows + 8 * t, next < c_end ? g.D : 0, live1);
         const unsigned char *s = mine + (unsigned)stage * kFewStage;
-#pragma unroll
-        for (int step = 0; step < 2; ++step) {
-            const unsigned a[4] = {step ? d0.z : d0.x, step ? d1.z : d1.x, step ? d0.w : d0.y, step ? d1.w : d1.y};
-            unsigned w[2][2][2], scale[2];                       // [pair][row of the pair][8 columns]
-#pragma unroll
-            for (int p = 0; p < 2; ++p) {
-                unsigned byte[2];
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int place = (step * 4 + p * 2 + e) * 4 + t;
-                    const uint2 c = *reinterpret_cast<const uint2 *>(s + place * 64 + gq * 8);
-                    w[p][e][0] = c.x;
-                    w[p][e][1] = c.y;
-                    byte[e] = FMT == kNvFp4 ? s[kFewCodes + (place * 2 + (gq >> 2)) * 4 + (gq & 3)] : s[kFewCodes + place * 4 + (gq >> 1)];
-                }
-                scale[p] = decode_scales<FMT>(byte[0], byte[1]);
-            }
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {                        // four columns of the 16
-                const unsigned sel = q & 1 ? 0x7632u : 0x5410u;
-                const uint4 b0 = decode8<FMT>(__byte_perm(w[0][0][q >> 1], w[0][1][q >> 1], sel), scale[0]);
-                const uint4 b1 = decode8<FMT>(__byte_perm(w[1][0][q >> 1], w[1][1][q >> 1], sel), scale[1]);
-                mma_16816(acc[q * 4 + 0], a, b0.x, b1.x);
-                mma_16816(acc[q * 4 + 1], a, b0.y, b1.y);
-                mma_16816(acc[q * 4 + 2], a, b0.z, b1.z);
-                mma_16816(acc[q * 4 + 3], a, b0.w, b1.w);
-            }
+        if (FMT == kMxFp4) {
+            // the words that hold this warp's 128 scale bytes, a lane one of them: none above 128?
+            const unsigned four = *reinterpret_cast<const unsigned *>(s + kFewCodes + lane * 4);
+            const bool small = __vmaxu4(four, 0x80808080u) == 0x80808080u;
+            if (__all_sync(kFullMask, small)) few_chunk<FMT, true>(s, gq, t, d0, d1, acc);
+            else few_chunk<FMT, false>(s, gq, t, d0, d1, acc);
+        } else {
+            few_chunk<FMT, false>(s, gq, t, d0, d1, acc);
         }
         stage = (stage + 1) % kFewStages;
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
-    // the warps' sums, 16 rows x 128 columns each (rows of 132 floats), added up into the first one's place
-    constexpr int kLd = kFewCols + 4;
+    // the warps' sums, 16 rows x 128 columns each, in rows of 144 floats (32 columns of a thread 36 apart: no bank conflicts), added up into rows of 132
+    constexpr int kWide = 144, kLd = kFewCols + 4, kEach = 16 * kFewCols / 4 / (WARPS * 32);
     float *part = reinterpret_cast<float *>(smem_few);
-    float *my = part + warp * 16 * kLd;
+    float *my = part + warp * 16 * kWide + 36 * t;
 #pragma unroll
     for (int i = 0; i < 16; i += 4) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            *reinterpret_cast<float4 *>(my + gq * kLd + 32 * t + 16 * h + i) = make_float4(acc[i][h], acc[i + 1][h], acc[i + 2][h], acc[i + 3][h]);
-            *reinterpret_cast<float4 *>(my + (gq + 8) * kLd + 32 * t + 16 * h + i) = make_float4(acc[i][2 + h], acc[i + 1][2 + h], acc[i + 2][2 + h], acc[i + 3][2 + h]);
+            *reinterpret_cast<float4 *>(my + gq * kWide + 16 * h + i) = make_float4(acc[i][h], acc[i + 1][h], acc[i + 2][h], acc[i + 3][h]);
+            *reinterpret_cast<float4 *>(my + (gq + 8) * kWide + 16 * h + i) = make_float4(acc[i][2 + h], acc[i + 1][2 + h], acc[i + 2][2 + h], acc[i + 3][2 + h]);
         }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < 16 * kFewCols / 4; i += kFewThreads) {
-        float4 *p = reinterpret_cast<float4 *>(part + (i / (kFewCols / 4)) * kLd + (i % (kFewCols / 4)) * 4);
-        float4 v = *p;
+    float4 v[kEach];
 #pragma unroll
-        for (int w = 1; w < kFewWarps; ++w) {
-            const float4 o = p[w * 16 * kLd / 4];
-            v = make_float4(v.x + o.x, v.y + o.y, v.z + o.z, v.w + o.w);
+    for (int j = 0; j < kEach; ++j) {
+        const int i = (int)threadIdx.x + j * WARPS * 32, row = i / 32, col = (i % 32) * 4;
+        const float4 *p = reinterpret_cast<const float4 *>(part + row * kWide + col / 32 * 36 + col % 32);
+        v[j] = *p;
+#pragma unroll
+        for (int w = 1; w < WARPS; ++w) {
+            const float4 o = p[w * 16 * kWide / 4];
+            v[j] = make_float4(v[j].x + o.x, v[j].y + o.y, v[j].z + o.z, v[j].w + o.w);
         }
-        *p = v;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+        const int i = (int)threadIdx.x + j * WARPS * 32;
+        *reinterpret_cast<float4 *>(part + i / 32 * kLd + (i % 32) * 4) = v[j];
     }
     cg::cluster_group cluster = cg::this_cluster();
     cluster.sync();
     const auto read = [&](int i, int c) { return *reinterpret_cast<const float4 *>(cluster.map_shared_rank(reinterpret_cast<const float *>(smem_few) + i, c)); };
-    add_parts<kFewThreads>(read, rank, kLd, g.R, min(kFewCols, g.C - col0), g.splits, *g.head, FMT == kNvFp4 ? kNvHold : 1.0f, g.out, g.type, col0, g.ld);
+    add_parts<WARPS * 32>(read, rank, kLd, g.R, min(kFewCols, g.C - col0), g.splits, *g.head, FMT == kNvFp4 ? kNvHold : 1.0f, g.out, g.type, col0, g.ld);
     cluster.sync();                                              // nobody leaves while its shared memory is being read
+}
+
+template <int FMT, int WARPS> cudaError_t launch_few(const Fp4Few &g, int blocks, cudaStream_t stream) {
+    constexpr size_t stages = (size_t)WARPS * kFewStages * kFewStage, sums = (size_t)WARPS * 16 * 144 * 4, smem = stages > sums ? stages : sums;
+    static std::atomic<uint64_t> done{0};
+    const cudaError_t err = allow_smem(fp4_grad_few_kernel<FMT, WARPS>, &done);
+    if (err != cudaSuccess) return err;
+    return launch_cluster(fp4_grad_few_kernel<FMT, WARPS>, (unsigned)(blocks * g.splits), WARPS * 32, g.splits, smem, stream, g);
 }
 
 }  // namespace
@@ -187,8 +218,13 @@ cudaError_t fp4_grad_few(int format, const void *dy, int R, uint64_t ld_dy, cons
     g.chunks = (int)((D + kFewRows - 1) / kFewRows);
     const int blocks = (int)((C + kFewCols - 1) / kFewCols);
     if (blocks > 0x7fffffff / 8) return cudaErrorInvalidValue;
-    g.splits = 1;
-    while (g.splits < 8 && blocks * g.splits <= sm_count && g.chunks >= g.splits * 2 * kFewWarps) g.splits *= 2;
+    // 16 warps a SM, in CTAs of 4 or 8: whichever leaves fewer of them without work, a cluster having at most 8 CTAs and a warp two chunks at least
+    const auto splits = [&](int warps) {
+        const int most = sm_count * (16 / warps) / blocks, useful = g.chunks / (2 * warps);
+        return std::max(1, std::min(8, std::min(most, useful)));
+    };
+    const int warps = splits(4) * 4 > splits(8) * 8 ? 4 : 8;
+    g.splits = splits(warps);
     g.chunks_per_split = (g.chunks + g.splits - 1) / g.splits;
     g.splits = (g.chunks + g.chunks_per_split - 1) / g.chunks_per_split;
     g.codes = packed + kFp4Head;
@@ -199,13 +235,8 @@ cudaError_t fp4_grad_few(int format, const void *dy, int R, uint64_t ld_dy, cons
     g.dy = static_cast<const __nv_bfloat16 *>(dy);
     g.ld_dy = ld_dy;
     g.out = out; g.ld = (long)ld; g.type = type;
-    static std::atomic<uint64_t> done_mx{0}, done_nv{0};
-    constexpr size_t smem = (size_t)kFewWarps * kFewStages * kFewStage;
-    static_assert(smem >= (size_t)kFewWarps * 16 * (kFewCols + 4) * 4, "partial sums do not fit");
-    const auto kernel = format == kNvFp4 ? fp4_grad_few_kernel<kNvFp4> : fp4_grad_few_kernel<kMxFp4>;
-    const cudaError_t err = allow_smem(kernel, format == kNvFp4 ? &done_nv : &done_mx);
-    if (err != cudaSuccess) return err;
-    return launch_cluster(kernel, (unsigned)(blocks * g.splits), kFewThreads, g.splits, smem, stream, g);
+    if (format == kNvFp4) return warps == 4 ? launch_few<kNvFp4, 4>(g, blocks, stream) : launch_few<kNvFp4, 8>(g, blocks, stream);
+    return warps == 4 ? launch_few<kMxFp4, 4>(g, blocks, stream) : launch_few<kMxFp4, 8>(g, blocks, stream);
 }
 
 }  // namespace bsq

@@ -462,7 +462,7 @@ cudaError_t grad_product(int format, bool a_kmajor, const void *dy, uint64_t M, 
         if (err != cudaSuccess) return err;
         dy = scratch;
     }
-    // few rows: decoded in the registers of the MMAs (16 x 4096 x 14336 in MXFP4 24 us there, 30 here; one row in NVFP4 24 / 37; 5 x 1024 x 1024 5.8 / 6.8)
+    // few rows: decoded in the registers of the MMAs (16 x 4096 x 14336 in MXFP4 18.5 us there, 30 here; one row in NVFP4 16.8 / 37; 5 x 1024 x 1024 5.6 / 6.8)
     if (a_kmajor && R <= kFewRowsMax) return fp4_grad_few(format, dy, (int)R, ld_a, b, D, C, out, type, ld, sm_count, stream);
     Fp4Grad g = {};
     g.R = (int)R; g.C = (int)C; g.D = (int)D;

@@ -531,3 +531,31 @@ def test_few_rows_are_the_rows_of_many(ops, fmt):
         many = ops.fp4_grad_input(dy, w, torch.float32)
         for a, b in ((0, 1), (1, 17), (5, 13), (16, 33)):
             assert torch.equal(ops.fp4_grad_input(dy[a:b], w, torch.float32), many[a:b])
+
+
+def test_few_rows_with_small_scales(ops):
+    """MXFP4 scales up to 2 take a shorter way; 0.25 to 1 keeps sums exact, the ends of the range (2^-127, 2) are in a matrix of their own."""
+    rng = np.random.default_rng(32)
+    for N, K, bytes_ in ((500, 300, (125, 126, 127)), (4096, 128, (126, 127, 128)), (64, 96, (0, 0, 0)), (64, 96, (128, 128, 128)), (64, 96, (129, 129, 128))):
+        codes = rng.integers(0, 16, (N, -(-K // 32) * 32)).astype(np.uint8)
+        codes[:, K:] = 0
+        byte = rng.choice(np.array(bytes_, np.uint8), (N, -(-K // 32)))
+        w = ops.Fp4Matrix(torch.from_numpy(ref.pack(codes, byte, 1.0, ref.MXFP4, K, fill=0xFF)).cuda(), N, K, ref.MXFP4)
+        dy = rng.integers(-8, 9, (16, N)).astype(np.float64)
+        want = dy @ ref.values(codes, byte, 1.0, ref.MXFP4, K)
+        got = ops.fp4_grad_input(torch.from_numpy(dy).to(torch.bfloat16).cuda(), w, torch.float32).double().cpu().numpy()
+        assert np.array_equal(got, want)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_status_word_of_the_c_entries(ops, lib, fmt):
+    x, w = ops.fp4_quantize(torch.randn(40, 64, device="cuda"), fmt), ops.fp4_quantize(torch.randn(50, 64, device="cuda"), fmt)
+    dy = torch.randn(40, 50, device="cuda").to(torch.bfloat16)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out = torch.empty(50, 64, device="cuda")
+    scratch = torch.empty(lib.bsq_fp4_grad_scratch_bytes(dy.data_ptr(), 40, 50, 50), dtype=torch.uint8, device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+    assert lib.bsq_fp4_matmul(fmt, x.data.data_ptr(), 40, w.data.data_ptr(), 50, 64, out.data_ptr(), 0, 50, status.data_ptr(), stream) == 0
+    assert torch.equal(out.view(-1)[: 2000].view(40, 50), ops.fp4_matmul(x, w, torch.float32))
+    assert lib.bsq_fp4_grad_weight(fmt, dy.data_ptr(), 40, 50, 50, x.data.data_ptr(), 64, out.data_ptr(), 0, 64, scratch.data_ptr(), status.data_ptr(), stream) == 0
+    assert torch.equal(out, ops.fp4_grad_weight(dy, x, torch.float32)) and status.item() == 0
