@@ -11,7 +11,8 @@
 //
 // Bound by memory: 4096 x 14336 in BF16 is read once for the matrix scale and once for the codes (MXFP4: once).  A thread
 // takes 32 columns (16 bytes of codes); a warp's lanes are 8 such units of 4 rows that lie 32 apart, because those are the
-// rows whose scales are neighbours in the packed form.
+// rows whose scales are neighbours in the packed form.  4096 x 14336 BF16: MXFP4 24.3 us (154 MB, 6.3 TB/s), NVFP4 43.4 (two passes over 117 MB), back to BF16
+// 27 (5.6 TB/s).  The NVFP4 quantiser executes 10 instructions an element and issues in 0.68 of the clocks, so it is not far from that bound either.
 #include "bsq_fp4.cuh"
 #include "bsq_internal.hpp"
 

@@ -10,6 +10,9 @@
 //
 // Codes and scales come by cp.async, three chunks of 32 rows ahead for each warp on its own (no barrier in the loop).  The warps of a CTA and
 // the CTAs of a cluster share the rows; their sums are added in a fixed order.
+//
+// 16 x 4096 x 14336 MXFP4 18.5 us, one row in NVFP4 16.8 (33 MB, 5 us at the memory's rate): some 5 us are launch, cluster and sums, the loads alone take 5,
+// decoding and MMAs 7 to 8 (12 instructions for 4 elements, at 0.6 of the issue rate).
 #include "bsq_fp4_decode.cuh"
 #include "bsq_fp4_few.hpp"
 #include "bsq_fp4_tile.cuh"

