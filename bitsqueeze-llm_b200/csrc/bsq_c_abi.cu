@@ -171,7 +171,7 @@ int bsq_reconstruct(const float *d_U, const float *d_S, const float *d_V, int m,
 static inline bool fp4_aligned(const void *packed) { return packed && reinterpret_cast<uintptr_t>(packed) % 16 == 0; }
 static inline bool op_rows_ok(const void *p, int type, uint64_t rows, uint64_t cols, uint64_t ld) {
     const int size = op_bytes(type);
-    return size && p && reinterpret_cast<uintptr_t>(p) % size == 0 && (rows <= 1 || ld >= cols);
+    return size && p && reinterpret_cast<uintptr_t>(p) % size == 0 && (rows <= 1 || (ld >= cols && ld < (1ull << 38)));
 }
 
 uint64_t bsq_fp4_packed_bytes(int format, uint64_t rows, uint64_t cols) { return fp4_shape_ok(format, rows, cols) ? fp4_packed_bytes(format, rows, cols) : 0; }
