@@ -99,7 +99,8 @@ struct QuantArgs {
 // less arithmetic on addresses
 __host__ __device__ constexpr int unit_run(int type, int word) { return word == 32 && type != kF32 ? 2 : 1; }
 
-// x / d correctly rounded from r, 1 / d correctly rounded: the residual of x r is exact in the fma, and one step with it rounds as the quotient does
+// x / d correctly rounded from r, 1 / d correctly rounded: the residual of x r is exact in the fma, and one step with it rounds as the quotient does (P. Markstein,
+// "Computation of elementary functions on the IBM RISC System/6000 processor", IBM J. Res. Dev. 34 (1990), theorem 8.3)
 __device__ __forceinline__ float divide_by(float x, float d, float r) {
     const float q0 = x * r, e = __fmaf_rn(q0, d, -x);
     return __fmaf_rn(-e, r, q0);                                 // (signs this way round: -0 stays -0)

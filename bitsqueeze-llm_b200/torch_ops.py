@@ -17,6 +17,7 @@ Every result comes from the shared library; there is no fallback.
 """
 import math
 from array import array
+from operator import attrgetter
 
 import torch
 
@@ -28,6 +29,8 @@ _HEAD = 128
 _NORM_SCRATCH = 16384                                      # bsq_grad_norm_scratch_bytes
 _stream = torch._C._cuda_getCurrentRawStream
 _device = torch._C._cuda_getDevice
+_dtype, _requires_grad = attrgetter("dtype"), attrgetter("requires_grad")
+_contiguous, _index, _numel, _pointer = torch.Tensor.is_contiguous, torch.Tensor.get_device, torch.Tensor.numel, torch.Tensor.data_ptr
 
 
 def _scales_at(rows, cols):
@@ -80,9 +83,19 @@ class Fp4Matrix:
         return tiles.permute(0, 3, 2, 1, 4).reshape(groups * 128, quads * 4)[: self.rows, :blocks].contiguous()
 
 
+_entries = {}                                             # C entries by name, looked up once
+
+
+def _entry(name):
+    f = _entries.get(name)
+    if f is None:
+        f = _entries[name] = getattr(lib(), name)
+    return f
+
+
 def _call(name, index, *args):
     """A C entry on the current stream of device `index` (its last argument), with that device current."""
-    f = getattr(lib(), name)
+    f = _entries.get(name) or _entry(name)
     if _device() == index:
         rc = f(*args, _stream(index))
     else:
@@ -122,7 +135,7 @@ def _result(out, shape, dtype, device, *inputs):
     if dtype not in _TYPES:
         raise ValueError("dtype must be float32, float16 or bfloat16")
     if out is None:
-        return torch.empty(shape, dtype=dtype, device=device), shape[-1]
+        return inputs[0].new_empty(shape, dtype=dtype), shape[-1]
     if out.dtype != dtype or tuple(out.shape) != tuple(shape) or out.device != device or out.requires_grad:
         raise ValueError("out must be a %s tensor of shape %s on %s that needs no gradient" % (dtype, tuple(shape), device))
     ld = shape[-1]
@@ -158,7 +171,7 @@ def fp4_quantize(x, format=NVFP4, amax=None, out=None):
         raise ValueError("amax is a float32 tensor of one element on x's device, for NVFP4")
     if out is None:
         out = Fp4Matrix.__new__(Fp4Matrix)
-        out.data, out.rows, out.cols, out.format = torch.empty(_packed_bytes(format, rows, cols), dtype=torch.uint8, device=device), rows, cols, format
+        out.data, out.rows, out.cols, out.format = x.new_empty(_packed_bytes(format, rows, cols), dtype=torch.uint8), rows, cols, format
     else:
         if _packed(out, "out").shape != (rows, cols) or out.format != format or out.data.device != device:
             raise ValueError("out must be an Fp4Matrix of %d x %d in the same format on x's device" % (rows, cols))
@@ -169,8 +182,8 @@ def fp4_quantize(x, format=NVFP4, amax=None, out=None):
                 raise ValueError("out must not overlap an input")
         torch.autograd.graph.increment_version(out.data)
     type = _TYPES[x.dtype]
-    need = lib().bsq_fp4_scratch_bytes(format, type, rows, cols) if amax is None and format == NVFP4 else 0
-    scratch = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    need = _entry("bsq_fp4_scratch_bytes")(format, type, rows, cols) if amax is None and format == NVFP4 else 0
+    scratch = x.new_empty(need, dtype=torch.uint8) if need else None
     _call("bsq_fp4_quantize", device.index, format, x.data_ptr(), type, rows, cols, ld, None if amax is None else amax.data_ptr(), out.data.data_ptr(),
           None if scratch is None else scratch.data_ptr())
     return out
@@ -213,8 +226,8 @@ def _grad(name, dy, m, packed_rows, out_rows, dtype, out):
     shape = tuple(dy.shape[:-1]) + (m.cols,) if out_rows is None else (out_rows(M, N), m.cols)
     out, ld_out = _result(out, shape, dtype, device, dy, m.data)
     p = dy.data_ptr()
-    need = lib().bsq_fp4_grad_scratch_bytes(p, M, N, ld) if M and (p % 16 or ld % 8) else 0
-    scratch = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    need = _entry("bsq_fp4_grad_scratch_bytes")(p, M, N, ld) if M and (p % 16 or ld % 8) else 0
+    scratch = m.data.new_empty(need) if need else None
     s = None if scratch is None else scratch.data_ptr()
     if out_rows is None:
         _call(name, device.index, m.format, p, M, ld, m.data.data_ptr(), N, m.cols, out.data_ptr(), _TYPES[dtype], ld_out, s, None)
@@ -316,32 +329,32 @@ def clip_grad_norm(grads, max_norm, norm_type=2.0, out=None):
     if max_norm is not None and not max_norm >= 0:
         raise ValueError("max_norm must not be negative or NaN")
     device, n = grads[0].device, len(grads)
-    # (a list at a time: a few hundred gradients are looked at in every step)
-    index, dtypes, plain = grads[0].get_device(), [g.dtype for g in grads], [g.is_contiguous() for g in grads]
+    # (an attribute of all of them at a time: a few hundred gradients are looked at in every step)
+    index, dtypes, plain = grads[0].get_device(), list(map(_dtype, grads)), list(map(_contiguous, grads))
     types = [_TYPES.get(d, -1) for d in dtypes]
-    if index < 0 or min(types) < 0 or {g.get_device() for g in grads} != {index} or not all(p or _dense(g) for p, g in zip(plain, grads)):
+    if index < 0 or min(types) < 0 or set(map(_index, grads)) != {index} or not (all(plain) or all(p or _dense(g) for p, g in zip(plain, grads))):
         raise ValueError("gradients must be dense float32, float16 or bfloat16 CUDA tensors on one device")
-    to = grads
+    counts, ptrs = array("Q", map(_numel, grads)), array("Q", map(_pointer, grads))
+    to, outs = grads, ptrs
     if out is not None:
         to = list(out)
         if len(to) != n:
             raise ValueError("out must have a tensor for each gradient")
-        if [o.dtype for o in to] != dtypes or {o.get_device() for o in to} != {index} or any([o.requires_grad for o in to]):
+        if list(map(_dtype, to)) != dtypes or set(map(_index, to)) != {index} or any(map(_requires_grad, to)):
             raise ValueError("tensors of out must have the type and device of their gradients, and need no gradient")
-        if not (all(plain) and all([o.is_contiguous() for o in to])) and [(o.shape, o.stride()) for o in to] != [(g.shape, g.stride()) for g in grads]:
+        if not (all(plain) and all(map(_contiguous, to))) and [(o.shape, o.stride()) for o in to] != [(g.shape, g.stride()) for g in grads]:
             raise ValueError("tensors of out that are not contiguous must have the shape and strides of their gradients")
-    ptrs = array("Q", [g.data_ptr() for g in grads])
-    outs = None if max_norm is None else ptrs if out is None else array("Q", [o.data_ptr() for o in to])
-    counts, types = array("Q", [g.numel() for g in grads]), array("i", types)
-    if out is not None and array("Q", [o.numel() for o in to]) != counts:
-        raise ValueError("tensors of out must have as many elements as their gradients")
+        if array("Q", map(_numel, to)) != counts:
+            raise ValueError("tensors of out must have as many elements as their gradients")
+        outs = array("Q", map(_pointer, to))
+    types = array("i", types)
     norm = torch.empty((), dtype=torch.float32, device=device)
     scratch = torch.empty(_NORM_SCRATCH, dtype=torch.uint8, device=device)
     try:
-        _call("bsq_grad_norm_clip", index, ptrs.buffer_info()[0], counts.buffer_info()[0], types.buffer_info()[0], n, None if outs is None else outs.buffer_info()[0],
+        _call("bsq_grad_norm_clip", index, ptrs.buffer_info()[0], counts.buffer_info()[0], types.buffer_info()[0], n, None if max_norm is None else outs.buffer_info()[0],
               0.0 if max_norm is None else max_norm, 0 if norm_type == math.inf else 2, norm.data_ptr(), scratch.data_ptr())
     except RuntimeError:
-        if outs is not None and _overlap(grads, to):
+        if max_norm is not None and _overlap(grads, to):
             raise ValueError("the tensors that are written must not overlap one another or another gradient") from None
         raise
     if max_norm is not None:
