@@ -353,10 +353,14 @@ __global__ void __launch_bounds__(grad_threads(MT), 1) fp4_grad_kernel(const __g
                     // this tile before has to be there before it is added to: in that order every time, the same bits every time.
                     const int per = 128 / size;
                     if (add && lane == 0) bulk_wait_all();
-                    for (int at = 0; at < MT * (int)kAccCols; at += per, which ^= 1) {
+                    for (int at = 0; at < MT * (int)kAccCols; at += per) {
                         const int m = at / (int)kAccCols, c = at - m * (int)kAccCols, row0 = row + m * CTAS * 128;
+                        if (row0 >= g.R || col + c >= g.C) continue;
+                        // The two boxes take turns with what is really copied: all copies but the newest have been read, so this box's last one has.  (A box that is
+                        // written and not copied would put the count out by one, and the next would overwrite what is still being read.)
                         unsigned char *box = boxes + (unsigned)((warp - 4) * 2 + which) * kBoxBytes;
-                        if (lane == 0) bulk_wait_read_1();       // this box's last copy has been read
+                        which ^= 1;
+                        if (lane == 0) bulk_wait_read_1();
                         __syncwarp();
                         uint4 *line = reinterpret_cast<uint4 *>(box + lane * 128);
 #pragma unroll 1
@@ -380,7 +384,6 @@ __global__ void __launch_bounds__(grad_threads(MT), 1) fp4_grad_kernel(const __g
                                 line[(h / 8 + 1) ^ (lane & 7)] = make_uint4(w[4], w[5], w[6], w[7]);
                             }
                         }
-                        if (row0 >= g.R || col + c >= g.C) continue;
                         if (g.boxes) {
                             fence_proxy_async_smem();
                             __syncwarp();
