@@ -30,7 +30,7 @@ namespace {
 constexpr int kDecodeWarps = 4;                                  // at one stage
 constexpr int kEpilogueWarps = 4, kFirstDecode = 4 + kEpilogueWarps;
 constexpr int kTileC = 128, kStageD = 64;                        // a CTA's columns of B; of D per stage
-constexpr int kMaxRing = 5, kRawRing = 6;
+constexpr int kMaxRing = 5, kMaxRawRing = 8;
 constexpr unsigned kBoxBytes = 32 * 128;                         // 32 rows x 128 bytes of the result on their way out: two for each epilogue warp
 constexpr unsigned kBoxesBytes = kEpilogueWarps * 2 * kBoxBytes;
 constexpr unsigned kABytes = 128 * kStageD * 2, kBBytes = kStageD * kTileC * 2;
@@ -39,12 +39,20 @@ constexpr int kChainStages = 1024 / kStageD;                     // FP32 results
 
 // A stage: MT blocks of 128 rows of dY, 128 columns of B
 __host__ __device__ constexpr unsigned op_bytes_of(int mt) { return (unsigned)mt * kABytes + kBBytes; }
-__host__ __device__ constexpr int ring_of(int mt) { return mt == 2 ? 3 : 5; }
-// Groups of decoding warps, each with a stage of its own.  Never more than there are stages in either ring: a group that waits for its stage to be emptied goes by the
-// parity of the barrier, and is at most one round ahead only because its own last stage lies no further back than a round.
+__host__ __device__ constexpr int ring_of(int mt) { return mt == 2 ? 3 : 4; }
+// Groups of decoding warps, each with a stage of its own.  They wait by the parity of barriers, which tells one round from the next and no more:
+//   * a stage's MMAs are done in order, so a group that has done its last stage may wait for the next one if that lies no further on than a round: never more groups
+//     than operand stages;
+//   * copies land in ANY order, so nothing that a group has seen of other places says how far the copies of its next one are: every place of the raw ring always goes
+//     to the same group, the ring a multiple of the groups.  (With six places and four groups a group could find the copy before last in a place whose last one
+//     was still under way: about one product in 100000 had a tile with a stage of old values.)
 __host__ __device__ constexpr int groups_of(int mt) { return mt == 2 ? 3 : 4; }
+__host__ __device__ constexpr int raw_ring_of(int mt) { return mt == 2 ? 6 : 8; }
 __host__ __device__ constexpr int grad_threads(int mt) { return (kFirstDecode + kDecodeWarps * groups_of(mt)) * 32; }
-static_assert(groups_of(1) <= ring_of(1) && groups_of(2) <= ring_of(2) && groups_of(1) <= kRawRing && groups_of(2) <= kRawRing, "a group would run two rounds ahead");
+template <int MT> constexpr bool rings_fit() {
+    return groups_of(MT) <= ring_of(MT) && raw_ring_of(MT) % groups_of(MT) == 0 && ring_of(MT) <= kMaxRing && raw_ring_of(MT) <= kMaxRawRing;
+}
+static_assert(rings_fit<1>() && rings_fit<2>(), "a wait could take one round for another");
 
 struct Fp4Grad {
     int R, C, D;                     // rows and columns of the result, the dimension that is summed over
@@ -61,7 +69,7 @@ struct Fp4Grad {
 };
 
 struct GradBars {
-    uint64_t full[kMaxRing], empty[kMaxRing], ready[kMaxRing], raw_full[kRawRing], raw_empty[kRawRing], acc_full[2], acc_empty[2], drain;
+    uint64_t full[kMaxRing], empty[kMaxRing], ready[kMaxRing], raw_full[kMaxRawRing], raw_empty[kMaxRawRing], acc_full[2], acc_empty[2], drain;
     unsigned tmem_base, failed;
 };
 
@@ -94,7 +102,7 @@ __global__ void __launch_bounds__(grad_threads(MT), 1) fp4_grad_kernel(const __g
                                                                    const __grid_constant__ CUtensorMap map_c, const Fp4Grad g, unsigned *status) {
     static_assert((CTAS == 1 || !SPLIT) && (MT == 1 || CTAS == 2), "pairs do not share tiles, single CTAs have one block of rows");
     chain_begin();
-    constexpr int kRing = ring_of(MT);
+    constexpr int kRing = ring_of(MT), kRawRing = raw_ring_of(MT);
     constexpr unsigned kOpBytes = op_bytes_of(MT);
     extern __shared__ unsigned char smem_dyn[];
     unsigned char *base = smem_dyn + ((1024u - (smem_u32(smem_dyn) & 1023u)) & 1023u);
@@ -435,7 +443,7 @@ __global__ void __launch_bounds__(256) pad_rows_kernel(const unsigned short *in,
 
 template <int FMT, int CTAS, int MT, bool SPLIT>
 cudaError_t launch_grad(const CUtensorMap &map_a, const CUtensorMap &map_b, const CUtensorMap &map_c, const Fp4Grad &g, int sm_count, unsigned *status, cudaStream_t stream) {
-    constexpr size_t smem = 1024 + ring_of(MT) * op_bytes_of(MT) + kRawRing * kRawBytes + kBoxesBytes + sizeof(GradBars) + 64;
+    constexpr size_t smem = 1024 + ring_of(MT) * op_bytes_of(MT) + raw_ring_of(MT) * kRawBytes + kBoxesBytes + sizeof(GradBars) + 64;
     static_assert(smem <= 227 * 1024, "stages do not fit");
     static_assert((size_t)128 * (kTileC + 4) * 4 <= (size_t)ring_of(MT) * op_bytes_of(MT), "partial tile does not fit");
     static std::atomic<uint64_t> done{0};

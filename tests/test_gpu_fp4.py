@@ -575,3 +575,25 @@ def test_partly_filled_tiles_again_and_again(ops, dtype, M, N, K):
     for _ in range(300):
         wrong += (ops.fp4_grad_input(d, w, DTYPES[dtype]) != want).any()
     assert wrong.item() == 0
+
+
+def test_copies_that_land_in_any_order(ops):
+    """Products of operands that were made just before, a library product in between: copies then land late and out of order.  A wait that took one round of a
+    ring for another let one call in a hundred decode what had not arrived."""
+    import random
+    rnd, gen = random.Random(5), torch.Generator(device="cuda").manual_seed(5)
+    wrong = []
+    for i in range(2500):
+        fmt, dtype = rnd.choice(FORMATS), rnd.choice(list(DTYPES.values()))
+        M, N, K = rnd.randint(2300, 3000), rnd.randint(2300, 3000), rnd.randint(1, 32)
+        q = ops.fp4_quantize(torch.randint(-3, 4, (N, K), generator=gen, device="cuda").float(), fmt)
+        v = ops.fp4_dequantize(q).double()
+        off, pad = rnd.choice([(0, 0), (0, 8), (1, 3), (8, 8)])
+        dy = torch.randint(-8, 9, (M, off + N + pad), generator=gen, device="cuda").to(torch.bfloat16)[:, off: off + N]
+        d = dy.double()
+        want = d @ v
+        got = ops.fp4_grad_input(dy, q, dtype).double()
+        bound = (N + 4) * 2.0 ** -23 * (d.abs() @ v.abs()) + want.abs() * (2.0 ** -22 + torch.finfo(dtype).eps / 2)   # as sum_bound, and the result's rounding
+        if bool(((got - want).abs() > bound).any()):
+            wrong.append((i, fmt, M, N, K))
+    assert not wrong
