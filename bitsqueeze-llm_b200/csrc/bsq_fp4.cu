@@ -1,13 +1,15 @@
 // Quantisation to and from microscaled 4-bit matrices (bsq_fp4.hpp has the formats and the packed form).
 //
-// quantise:  block b of a row: m = max |x|.  MXFP4: s = 2^(floor(log2 m) - 2), at least 2^-127.  NVFP4: s = e4m3(m / (6 g)) g with the
-// matrix scale g = 2^t, t from the largest magnitude of the matrix.  Codes: x / s to the nearest e2m1, ties to even, saturated at 6.
+// quantise:  block b of a row: m = max |x|.  MXFP4: s = 2^(floor(log2 m) - 2), at least 2^-127.  NVFP4: s = e4m3((m / g) fl(1/6)) g with the
+// matrix scale g = 2^t, t from the largest magnitude of the matrix, and fl(1/6) the FP32 number nearest to 1/6.  Codes: x / s to the nearest e2m1, ties to even, saturated at 6.
 // A block with an Inf or NaN gets the scale NaN and codes 0, so that whatever reads it says so; the matrix scale goes by the finite elements.
 //
 // x / s: MXFP4 multiplies by a power of two, exact.  NVFP4 takes q0 = x * (1/s), r = q0 s - x (exact in the fma), q = q0 - r * (1/s), which is
 // x / s correctly rounded; a correctly rounded quotient lies on the same side of a halfway point of e2m1 as the quotient itself
 // (halfway point times s has 7 bits: an x beside it is at least 2^-24 of itself away, more than half a step of the quotient there).
-// q0 alone is one step off for some s (15 * 0.125 against 5: 5.0000005), and a tie then goes the wrong way.
+// q0 alone is one step off for some s (15 * 0.125 against 5: 5.0000005), and a tie then goes the wrong way.  The block scale is defined by the FP32 product instead: for
+// 16-bit elements that is the nearest E4M3 to m / (6 g) all the same (a tie, m / g = 6 h with a halfway point h, gives h (1 + 2^-25), which rounds to h, and
+// the next m is 2^-11 away); an FP32 m beside a tie may go with it, to a scale that is as near to 2^-24.
 //
 // Bound by memory: 4096 x 14336 in BF16 is read once for the matrix scale and once for the codes (MXFP4: once).  A thread
 // takes 32 columns (16 bytes of codes); a warp's lanes are 8 such units of 4 rows that lie 32 apart, because those are the
@@ -128,7 +130,7 @@ __device__ __forceinline__ void quantise_unit(const unsigned *w, float g, float 
             inv = __uint_as_float((254u - byte) << 23);
         } else {
             const float u = CLAMP ? fminf(amax * ginv, 65536.0f) : amax * ginv;
-            byte = ue4m3_byte(divide_by(u, 6.0f, 1.0f / 6.0f));
+            byte = ue4m3_byte(u * (1.0f / 6.0f));
             const float2 e = table[byte];
             s = e.x * g;
             inv = e.y * ginv;

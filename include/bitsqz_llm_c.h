@@ -268,10 +268,10 @@ int bsq_batch_decompress(bsq_batch_t *batch, const struct bitsqz_llm_array *cons
 uint64_t bsq_fp4_packed_bytes(int format, uint64_t rows, uint64_t cols);
 /* what bsq_fp4_quantize needs in d_scratch when it is not given d_amax: 0 for MXFP4 and for small matrices */
 size_t bsq_fp4_scratch_bytes(int format, int type, uint64_t rows, uint64_t cols);
-/* Codes are x / (block scale * matrix scale) to the nearest, ties to even, saturated at 6, with the decision made exactly.  MXFP4: the block scale is
+/* Codes are x / (block scale * matrix scale) to the nearest, ties to even, saturated at 6; the decision is exact.  MXFP4: the block scale is
  * 2^(floor(log2 m) - 2), at least 2^-127, m the block's largest magnitude.  NVFP4: the matrix scale is the power of two 2^t with the smallest t (-110 to 117) for
  * which the largest finite magnitude of the matrix is at most 2688 * 2^t -- of the matrix, or *d_amax where that is given (elements above it saturate) -- and the
- * block scale the nearest E4M3 to m / (6 * 2^t).  A block that holds Inf or NaN gets the scale NaN. */
+ * block scale the nearest E4M3 to m / 2^t * fl(1/6), the product in FP32.  A block that holds Inf or NaN gets the scale NaN. */
 int bsq_fp4_quantize(int format, const void *d_x, int type, uint64_t rows, uint64_t cols, uint64_t ld, const float *d_amax, void *d_packed, void *d_scratch,
                      void *stream);
 /* out = (element * block scale) * matrix scale, rounded once */

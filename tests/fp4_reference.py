@@ -1,4 +1,4 @@
-"""Microscaled 4-bit matrices in 64 bits on the CPU, from the definition: the quantiser, the packed form, the values it stands for."""
+"""Microscaled 4-bit matrices on the CPU, from the definition (in 64 bits but for one FP32 product): the quantiser, the packed form, the values it stands for."""
 import numpy as np
 
 MXFP4, NVFP4 = 8, 9
@@ -56,7 +56,8 @@ def quantize(x, fmt, amax=None):
         byte = np.where(bad, 255, byte)
     else:
         g = matrix_scale((np.abs(finite).max() if finite.size else 0.0) if amax is None else float(amax))
-        byte = nearest(E4M3, m, np.full_like(m, 6.0 * g))
+        p = (m / g).astype(np.float32) * np.float32(1 / 6)             # (the definition: an FP32 product)
+        byte = nearest(E4M3, p.astype(np.float64), np.ones_like(m))
         s = E4M3[byte] * g
         byte = np.where(bad, 127, byte)
     codes = np.where(s[..., None] > 0, nearest(LEVELS, v, s[..., None]), 0).reshape(rows, -1).astype(np.uint8) | sign
