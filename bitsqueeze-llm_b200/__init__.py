@@ -127,6 +127,7 @@ SIGNATURES = {
     "bsq_grad_norm_clip": (_i, [_vp, _vp, _vp, _i, _vp, C.c_double, _i, _vp, _vp, _vp]),
     "bsq_test_inject_status": (None, [_i, _u32]),
     "bsq_test_inject_lane_status": (None, [_vp, _i, _u32]),
+    "bsq_test_limit_waits": (None, [_u32]),
     "bsq_build_info": (C.c_char_p, []),
 }
 

@@ -231,6 +231,8 @@ int bsq_grad_norm_clip(const void *const *d_grads, const uint64_t *counts, const
     }
 }
 
+void bsq_test_limit_waits(uint32_t tries) { limit_epilogue_tries(tries); }
+
 const char *bsq_build_info(void) { return "bitsqz_llm sm_100a " __DATE__; }
 
 }  // extern "C"

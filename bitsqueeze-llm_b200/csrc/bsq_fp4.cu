@@ -18,6 +18,8 @@
 #include "bsq_fp4.cuh"
 #include "bsq_internal.hpp"
 
+#include <atomic>
+
 namespace bsq {
 namespace {
 
@@ -451,7 +453,15 @@ template <int FMT> cudaError_t dequantize_format(const DequantArgs &g, int type,
     return dequantize_typed<FMT, kBf16>(g, word, grid, stream);
 }
 
+std::atomic<unsigned> g_tries{~0u};
+
 }  // namespace
+
+void limit_epilogue_tries(unsigned tries) { g_tries.store(tries, std::memory_order_relaxed); }
+unsigned epilogue_tries(unsigned usual) {
+    const unsigned tries = g_tries.load(std::memory_order_relaxed);
+    return tries < usual ? tries : usual;
+}
 
 cudaError_t fp4_quantize(int format, const void *x, int type, uint64_t rows, uint64_t cols, uint64_t ld, const float *amax, void *packed,
                          void *scratch, int sm_count, cudaStream_t stream) {

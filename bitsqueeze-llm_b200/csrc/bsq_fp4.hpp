@@ -46,6 +46,10 @@ inline size_t fp4_quantize_scratch(int format, int type, uint64_t rows, uint64_t
     return format == kNvFp4 && rows * cols * (uint64_t)op_bytes(type) > kFp4OwnAmaxBytes ? kFp4Partials * sizeof(float) : 0;
 }
 
+// Tries after which the epilogues of the products give up a wait for accumulators: `usual`, or fewer where a test has set them (bsq_test_limit_waits).
+void limit_epilogue_tries(unsigned tries);
+unsigned epilogue_tries(unsigned usual);
+
 // amax (nullable, NVFP4): a device word with the largest magnitude the caller reckons with; larger elements saturate.
 cudaError_t fp4_quantize(int format, const void *x, int type, uint64_t rows, uint64_t cols, uint64_t ld, const float *amax, void *packed,
                          void *scratch, int sm_count, cudaStream_t stream);

@@ -39,6 +39,7 @@ struct Fp4Gemm {
     int type;
     bool lanes_contiguous;           // out[q * ld + p] instead of out[p * ld + q]
     bool boxes;                      // the result can be written by TMA
+    unsigned epilogue_tries;         // of the waits for accumulators (kWaitTries but in tests)
 };
 struct GemmMaps {
     CUtensorMap p, q, p_scales, q_scales, out;
@@ -149,11 +150,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(const __grid_
                     }
                 }
             }
-            if (!ok) {                                           // copies in flight must have landed before this CTA's shared memory goes away
-                atomicOr(&bars.failed, 1u);
-                if (leader)
-                    for (int c = max(0, filled - g.ring); c < filled; ++c) mbar_wait_asleep(&bars.full[c % g.ring], (unsigned)(c / g.ring) & 1u, status);
-            }
+            // copies in flight must have landed before this CTA's shared memory goes away, also where whoever reads them has given up
+            if (leader)
+                for (int c = max(0, filled - g.ring); c < filled; ++c) mbar_wait_asleep(&bars.full[c % g.ring], (unsigned)(c / g.ring) & 1u, status, ok ? kWaitTries : kDrainTries);
         }
     } else if (warp == 1) {
         if (leader) {
@@ -203,12 +202,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(const __grid_
                 }
                 __syncwarp();
             }
-            if (!ok && lane == 0) {
-                atomicOr(&bars.failed, 1u);
-                if (CTAS == 2) tc_commit_pair(&bars.drain, 1);   // MMAs under way must be done before tensor memory is given back
+            if (elect_one()) {                                   // MMAs under way must be done before tensor memory is given back, also where the epilogue has given up
+                if (CTAS == 2) tc_commit_pair(&bars.drain, 1);
                 else tc_commit(&bars.drain);
-                mbar_wait_asleep(&bars.drain, 0, status);
             }
+            __syncwarp();
+            mbar_wait_asleep(&bars.drain, 0, status);
         }
     } else {
         const int quarter = warp & 3, half = (warp - 2) >> 2;    // the lanes this warp may read; which half of the columns
@@ -218,14 +217,14 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(const __grid_
         Ring rs(g.sets);
         for (int t = first; t < tiles; t += step, rs.next()) {
             const int p0 = ((t % g.p_tiles) * CTAS + side) * 128 + quarter * 32, q0 = (t / g.p_tiles) * g.q_tile;
-            if (ok) ok = __all_sync(kFullMask, mbar_wait_asleep(&bars.acc_full[rs.pos], rs.par, status)) != 0;
+            if (ok) ok = __all_sync(kFullMask, mbar_wait_asleep(&bars.acc_full[rs.pos], rs.par, status, g.epilogue_tries)) != 0;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const unsigned taddr = tmem + (unsigned)rs.pos * acc_cols + ((unsigned)(quarter * 32) << 16) + (unsigned)c_first * 16u;
             if constexpr (SPLIT) {
-                // stages are free: every copy has landed and every MMA has read them
+                // stages are free: every copy has landed and every MMA has read them (without the accumulators nobody knows: nothing is written then)
                 float *part = reinterpret_cast<float *>(base);
                 const int row = quarter * 32 + lane, ldp = g.q_tile + 4;
-                for (int c = 0; c < c_count; ++c) {
+                for (int c = 0; ok && c < c_count; ++c) {
                     unsigned r[16];
                     read16(taddr + (unsigned)c * 16u, r, ok);
                     if (g.lanes_contiguous) {
@@ -252,7 +251,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(const __grid_
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) {                                 // the accumulators are in registers: the next tile may begin
+                // the accumulators are in registers: the next tile may begin.  (Not where this warp has given up: it runs ahead from here on, and its arrivals would
+                // let the next tile begin while others still read.)
+                if (ok && lane == 0) {
                     if (CTAS == 2) mbar_arrive_pair(smem_u32(&bars.acc_empty[rs.pos]) + lead);
                     else mbar_arrive(&bars.acc_empty[rs.pos]);
                 }
@@ -317,7 +318,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(const __grid_
             }
         }
         if (!SPLIT && lane == 0) bulk_wait_all();
-        if (!ok && lane == 0) atomicOr(&bars.failed, 1u);
+        if (SPLIT && !ok && lane == 0) atomicOr(&bars.failed, 1u);
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
@@ -325,6 +326,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(const __grid_
     if (warp == 1) tmem_free<CTAS>(tmem, tmem_cols);
 
     if constexpr (SPLIT) {
+        // given up: NaN for the whole partial tile, now that nothing is on its way into the stages any more
+        if (bars.failed) nan_part<kGemmThreads>(reinterpret_cast<float *>(base), 128 * (g.q_tile + 4));
         cg::cluster_group cluster = cg::this_cluster();
         cluster.sync();
         const int pt = first % g.p_tiles, qt = first / g.p_tiles;
@@ -392,6 +395,7 @@ cudaError_t fp4_matmul(int format, const void *a, uint64_t M, const void *b, uin
     g.quads = (unsigned)fp4_quads(format, K);
     g.p_head = reinterpret_cast<const float *>(pp); g.q_head = reinterpret_cast<const float *>(pq);
     g.out = out; g.ld = (long)ld; g.type = type; g.lanes_contiguous = swap;
+    g.epilogue_tries = epilogue_tries(kWaitTries);
     const int tiles = g.p_tiles * g.q_tiles;
     g.splits = 1;
     if (ctas == 1)

@@ -66,6 +66,7 @@ struct Fp4Grad {
     long ld;
     int type;
     bool boxes;                      // the result can be written by TMA
+    unsigned epilogue_tries;         // of the waits for accumulators (kWaitTries but in tests)
 };
 
 struct GradBars {
@@ -163,10 +164,9 @@ __global__ void __launch_bounds__(grad_threads(MT), 1) fp4_grad_kernel(const __g
                     if (sf) bulk_g2s(s + kCodeBytes, g.scales + ((size_t)(d >> 1) * g.quads + quad) * 512, sf, &bars.raw_full[r.pos]);
                 }
             }
-            if (!ok) {                                           // copies in flight must have landed before this CTA's shared memory goes away
-                atomicOr(&bars.failed, 1u);
-                for (int c = max(0, filled - kRawRing); c < filled; ++c) mbar_wait_asleep(&bars.raw_full[c % kRawRing], (unsigned)(c / kRawRing) & 1u, status);
-            }
+            // copies in flight must have landed before this CTA's shared memory goes away, also where whoever reads them has given up
+            for (int c = max(0, filled - kRawRing); c < filled; ++c)
+                mbar_wait_asleep(&bars.raw_full[c % kRawRing], (unsigned)(c / kRawRing) & 1u, status, ok ? kWaitTries : kDrainTries);
         }
     } else if (warp == 1) {
         if (lane == 0 && !leader) {
@@ -178,7 +178,6 @@ __global__ void __launch_bounds__(grad_threads(MT), 1) fp4_grad_kernel(const __g
                     if (!ok) break;
                     mbar_arrive_pair(smem_u32(&bars.full[r.pos]) + lead);
                 }
-            if (!ok) atomicOr(&bars.failed, 1u);
         }
         if (leader) {
             // BF16 x BF16, FP32 sums, B contiguous along N, A along K or along M, N >> 3, M >> 4
@@ -227,12 +226,12 @@ __global__ void __launch_bounds__(grad_threads(MT), 1) fp4_grad_kernel(const __g
                     __syncwarp();
                 }
             }
-            if (!ok && lane == 0) {
-                atomicOr(&bars.failed, 1u);
-                if (CTAS == 2) tc_commit_pair(&bars.drain, 1);   // MMAs under way must be done before tensor memory is given back
+            if (elect_one()) {                                   // MMAs under way must be done before tensor memory is given back, also where the epilogue has given up
+                if (CTAS == 2) tc_commit_pair(&bars.drain, 1);
                 else tc_commit(&bars.drain);
-                mbar_wait_asleep(&bars.drain, 0, status);
             }
+            __syncwarp();
+            mbar_wait_asleep(&bars.drain, 0, status);
         }
     } else if (warp == 2) {
         // ---- dY ----
@@ -267,11 +266,10 @@ __global__ void __launch_bounds__(grad_threads(MT), 1) fp4_grad_kernel(const __g
                     }
                 }
             }
-            if (!ok) {
-                atomicOr(&bars.failed, 1u);
-                if (leader)
-                    for (int c = max(0, filled - kRing); c < filled; ++c) mbar_wait_asleep(&bars.full[c % kRing], (unsigned)(c / kRing) & 1u, status);
-            }
+            // (as above; a stage also waits for its decoding warps, which may have given up)
+            if (leader)
+                for (int c = max(0, filled - kRing); c < filled; ++c)
+                    mbar_wait_asleep(&bars.full[c % kRing], (unsigned)(c / kRing) & 1u, status, ok ? kWaitTries : kDrainTries);
         }
     } else if (warp >= kFirstDecode) {
         // ---- decode: groups of four warps take the stages in turn.  A thread has one row of B and, twice, 32 of its columns; the lanes of a warp have
@@ -327,7 +325,6 @@ __global__ void __launch_bounds__(grad_threads(MT), 1) fp4_grad_kernel(const __g
                 }
             }
         }
-        if (!ok && lane == 0) atomicOr(&bars.failed, 1u);
     } else if (warp >= 4) {
         const int quarter = warp & 3;                            // the lanes of tensor memory this warp may read
         const float f0 = *g.head, f1 = FMT == kNvFp4 ? kNvHold : 1.0f;
@@ -337,12 +334,13 @@ __global__ void __launch_bounds__(grad_threads(MT), 1) fp4_grad_kernel(const __g
         for (int t = first; t < tiles; t += step) {
             const int row = ((t % g.r_tiles) * CTAS * MT + half) * 128 + quarter * 32, col = (t / g.r_tiles) * (int)kAccCols;
             for (int c0 = d0; c0 < d1; c0 += SPLIT ? d1 - d0 : g.chain, rs.next()) {
-                if (ok) ok = __all_sync(kFullMask, mbar_wait_asleep(&bars.acc_full[rs.pos], rs.par, status)) != 0;
+                if (ok) ok = __all_sync(kFullMask, mbar_wait_asleep(&bars.acc_full[rs.pos], rs.par, status, g.epilogue_tries)) != 0;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const unsigned taddr = tmem + (SPLIT ? 0u : (unsigned)rs.pos * kAccCols) + ((unsigned)(quarter * 32) << 16);
                 const bool add = !SPLIT && c0 > d0;              // (FP32 only: to what this warp wrote before)
                 if constexpr (SPLIT) {
-                    for (int c = 0; c < (int)kAccCols; c += 16) {
+                    // (without the accumulators nobody knows whether the stages are free: nothing is written then)
+                    for (int c = 0; ok && c < (int)kAccCols; c += 16) {
                         unsigned r[16];
                         read_columns(taddr + (unsigned)c, r, ok);
                         for (int i = 1; i < kSets && i * g.chain < d1 - d0; ++i) {
@@ -409,14 +407,15 @@ __global__ void __launch_bounds__(grad_threads(MT), 1) fp4_grad_kernel(const __g
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) {
+                // (not where this warp has given up: it runs ahead from here on, and its arrivals would let accumulators be overwritten that others still read)
+                if (ok && lane == 0) {
                     if (CTAS == 2) mbar_arrive_pair(smem_u32(&bars.acc_empty[rs.pos]) + lead);
                     else mbar_arrive(&bars.acc_empty[rs.pos]);
                 }
             }
         }
         if (!SPLIT && lane == 0) bulk_wait_all();
-        if (!ok && lane == 0) atomicOr(&bars.failed, 1u);
+        if (SPLIT && !ok && lane == 0) atomicOr(&bars.failed, 1u);
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
@@ -424,6 +423,8 @@ __global__ void __launch_bounds__(grad_threads(MT), 1) fp4_grad_kernel(const __g
     if (warp == 1) tmem_free<CTAS>(tmem, 512u);
 
     if constexpr (SPLIT) {
+        // given up: NaN for the whole partial tile, now that nothing is on its way into the stages any more
+        if (bars.failed) nan_part<grad_threads(MT)>(reinterpret_cast<float *>(base), 128 * (kTileC + 4));
         cg::cluster_group cluster = cg::this_cluster();
         cluster.sync();
         const int rt = first % g.r_tiles, ct = first / g.r_tiles;
@@ -496,6 +497,7 @@ cudaError_t grad_product(int format, bool a_kmajor, const void *dy, uint64_t M, 
     g.scales = b + fp4_scales_at(D, C);
     g.head = reinterpret_cast<const float *>(b);
     g.out = out; g.ld = (long)ld; g.type = type;
+    g.epilogue_tries = epilogue_tries(kWaitTries);
     const int tiles = g.r_tiles * g.c_tiles;
     g.splits = 1;
     if (ctas == 1)

@@ -109,6 +109,11 @@ __device__ __forceinline__ void add_parts(const Read &read, int rank, int ld_par
     }
 }
 
+// A partial tile that was given up
+template <int THREADS> __device__ __forceinline__ void nan_part(float *part, int count) {
+    for (int i = (int)threadIdx.x; i < count; i += THREADS) part[i] = __uint_as_float(0x7fffffffu);
+}
+
 inline bool map_codes(CUtensorMap *map, const uint8_t *packed, uint64_t rows, uint64_t cols, unsigned box_rows) {
     const cuuint64_t dims[2] = {fp4_ld(cols), rows}, strides[1] = {fp4_ld(cols)};
     const cuuint32_t box[2] = {128u, box_rows}, estr[2] = {1, 1};

@@ -61,8 +61,11 @@ __device__ __forceinline__ void mbar_arrive_pair(unsigned bar) {
 // mbar_wait_bounded for the many warps of a kernel that wait most of the time: a try that finds the barrier closed sleeps up to 20 us before it answers, where the
 // default has it asked again and again.  What that costs is issue slots and, under the power limit, clock: the gradient products took 2 to 10 % longer.
 // 65536 tries of 20 us, or 1.3 s, are the bound.
-__device__ __forceinline__ bool mbar_wait_asleep(uint64_t *bar, unsigned parity, unsigned *status) {
-    for (unsigned i = 0; i < (1u << 16); ++i) {
+constexpr unsigned kWaitTries = 1u << 16;
+// ... of a role that has given up, for what it has under way itself: 82 ms
+constexpr unsigned kDrainTries = 1u << 12;
+__device__ __forceinline__ bool mbar_wait_asleep(uint64_t *bar, unsigned parity, unsigned *status, unsigned tries = kWaitTries) {
+    for (unsigned i = 0; i < tries; ++i) {
         unsigned ok;
         asm volatile(
             "{\n\t.reg .pred p;\n\t"

@@ -302,6 +302,9 @@ int bsq_grad_norm_clip(const void *const *d_grads, const uint64_t *counts, const
 void bsq_test_inject_status(int which, uint32_t bits);
 /* The same for the next compress (which = 0) or decompress (which = 1) call begun on a lane. */
 void bsq_test_inject_lane_status(bsq_lane_t *lane, int which, uint32_t bits);
+/* Until it is called again: the part of a bsq_fp4_matmul, bsq_fp4_grad_input or bsq_fp4_grad_weight kernel that takes finished tiles out gives up waiting for
+ * one after `tries` tries of some 20 us (0: at once; the usual 65536 or more: as usual).  Such a call leaves NaN and sets bit 0 of its status word. */
+void bsq_test_limit_waits(uint32_t tries);
 
 /* library build tag: "sm_100a" plus the compile date */
 const char *bsq_build_info(void);
