@@ -212,7 +212,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(const __grid_
     } else {
         const int quarter = warp & 3, half = (warp - 2) >> 2;    // the lanes this warp may read; which half of the columns
         const int chunks = g.q_tile / 16, c_first = half ? (chunks + 1) / 2 : 0, c_count = half ? chunks / 2 : (chunks + 1) / 2;
-        const float f0 = *g.p_head, f1 = *g.q_head;
+        const Factors f = join_factors(*g.p_head, *g.q_head);
         const int size = g.type == kF32 ? 4 : 2;
         Ring rs(g.sets);
         for (int t = first; t < tiles; t += step, rs.next()) {
@@ -272,7 +272,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(const __grid_
                             }
                             float v[16];
 #pragma unroll
-                            for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[c][j]) * f0 * f1;
+                            for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[c][j]) * f.first * f.second;
                             if (g.type == kF32) {
 #pragma unroll
                                 for (int j = 0; j < 4; ++j) {
@@ -311,7 +311,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(const __grid_
                         if (have > 0) {
 #pragma unroll
                             for (int j = 0; j < 16; ++j)
-                                if (j < have) store_one(g.out, g.type, (long)(q + j) * g.ld + p, __uint_as_float(r[c][j]) * f0 * f1);
+                                if (j < have) store_one(g.out, g.type, (long)(q + j) * g.ld + p, __uint_as_float(r[c][j]) * f.first * f.second);
                         }
                     }
                 }

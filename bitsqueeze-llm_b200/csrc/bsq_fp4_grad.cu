@@ -327,7 +327,7 @@ __global__ void __launch_bounds__(grad_threads(MT), 1) fp4_grad_kernel(const __g
         }
     } else if (warp >= 4) {
         const int quarter = warp & 3;                            // the lanes of tensor memory this warp may read
-        const float f0 = *g.head, f1 = FMT == kNvFp4 ? kNvHold : 1.0f;
+        const Factors f = join_factors(*g.head, FMT == kNvFp4 ? kNvHold : 1.0f);
         const int size = g.type == kF32 ? 4 : 2;
         int which = 0;
         Ring rs(SPLIT ? 1 : kSets);
@@ -375,7 +375,7 @@ __global__ void __launch_bounds__(grad_threads(MT), 1) fp4_grad_kernel(const __g
                             read_columns(taddr + (unsigned)(at + h), r, ok);
                             float v[16];
 #pragma unroll
-                            for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]) * f0 * f1;
+                            for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]) * f.first * f.second;
                             if (g.type == kF32) {
 #pragma unroll
                                 for (int j = 0; j < 4; ++j) {

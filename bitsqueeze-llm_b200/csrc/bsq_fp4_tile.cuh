@@ -40,6 +40,17 @@ __device__ __forceinline__ void read16(unsigned taddr, unsigned (&r)[16], bool o
     }
 }
 
+// The two factors of a result (matrix scales) as one where their product is a normal number; else the larger one comes first, so that a result within the range of
+// FP32 does not leave it on the way: sums up to 2^40 times 2^117 times 2^-110.
+struct Factors {
+    float first, second;
+};
+__device__ __forceinline__ Factors join_factors(float a, float b) {
+    const float c = a * b;
+    if (fabsf(c) >= 1.17549435e-38f && fabsf(c) <= 3.402823466e+38f) return {c, 1.0f};
+    return fabsf(a) >= fabsf(b) ? Factors{a, b} : Factors{b, a};
+}
+
 __device__ __forceinline__ void store_one(void *out, int type, long at, float v) {
     if (type == kF32) store_elem<kF32>(out, (uint64_t)at, v);
     else if (type == kBf16) store_elem<kBf16>(out, (uint64_t)at, v);
@@ -81,7 +92,9 @@ __device__ __forceinline__ void box_add(const unsigned char *box, int lane, floa
 // 4).  A value comes from another SM in some 1000 clocks, so a thread asks for all of four columns at once (one value at a time: 777 x 1031 x 5120 18.6 us, this way
 // 14.0).
 template <int THREADS, class Read>
-__device__ __forceinline__ void add_parts(const Read &read, int rank, int ld_part, int rows, int run, int splits, float f0, float f1, void *out, int type, long at, long ld) {
+__device__ __forceinline__ void add_parts(const Read &read, int rank, int ld_part, int rows, int run, int splits, float scale0, float scale1, void *out, int type, long at,
+                                          long ld) {
+    const Factors f = join_factors(scale0, scale1);
     const int per = (rows + splits - 1) / splits, r0 = rank * per, r1 = min(rows, r0 + per), fours = (run + 3) / 4;
     const int size = type == kF32 ? 4 : 2;
     const bool whole = ((reinterpret_cast<uintptr_t>(out) + (uintptr_t)(at * size)) | (uintptr_t)(ld * size)) % (unsigned)(4 * size) == 0;
@@ -95,7 +108,7 @@ __device__ __forceinline__ void add_parts(const Read &read, int rank, int ld_par
 #pragma unroll
         for (int c = 1; c < 8; ++c)
             if (c < splits) v = make_float4(v.x + p[c].x, v.y + p[c].y, v.z + p[c].z, v.w + p[c].w);
-        const float o[4] = {v.x * f0 * f1, v.y * f0 * f1, v.z * f0 * f1, v.w * f0 * f1};
+        const float o[4] = {v.x * f.first * f.second, v.y * f.first * f.second, v.z * f.first * f.second, v.w * f.first * f.second};
         const long to = at + (long)row * ld + col;
         if (whole && col + 4 <= run) {
             if (type == kF32) *reinterpret_cast<float4 *>(static_cast<float *>(out) + to) = make_float4(o[0], o[1], o[2], o[3]);
