@@ -325,6 +325,7 @@ __global__ void __launch_bounds__(grad_threads(MT), 1) fp4_grad_kernel(const __g
                 }
             }
         }
+        if (SPLIT && !ok && lane == 0) atomicOr(&bars.failed, 1u);                           // (as the epilogue does: this tile is not whole)
     } else if (warp >= 4) {
         const int quarter = warp & 3;                            // the lanes of tensor memory this warp may read
         const Factors f = join_factors(*g.head, FMT == kNvFp4 ? kNvHold : 1.0f);
