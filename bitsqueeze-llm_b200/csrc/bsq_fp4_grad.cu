@@ -5,7 +5,8 @@
 // times its block scale has 6 significant bits and BF16's exponent covers every MXFP4 scale (NVFP4: held 2^12 smaller), so decoding is exact;
 // sums are FP32 in tensor memory, the matrix scale is multiplied in when a tile leaves, and the result is rounded once.  The tensor core
 // cuts every addition off instead of rounding it, and what is lost grows with the length of the chain: results in FP32 leave tensor memory every 1024 of D
-// and are added up rounded (4096 of D: 1.0e-6 off 64 bits in chains of 2048, 0.4e-6 in chains of 1024, a rounded FP32 product 0.3e-6).
+// and are added up rounded (4096 of D: 1.0e-6 off 64 bits in chains of 2048, 0.4e-6 in chains of 1024, a rounded FP32 product 0.3e-6).  Where CTAs share a tile, a
+// slice of more than four such chains adds them up in tensor memory (1024 x 1024 from 65536: 0.2e-6 off, 2.6e-6 in the four chains of 8192 that it had; 199 us, 189).
 //
 // Where there are enough tiles, a pair of CTAs on two SMs shares one (cta_group::2): of 512 x 256 for 16-bit results, so that an element of B is decoded once for
 // 512 rows, of 256 x 256 for FP32 ones, which leaves a second set of accumulators for the next 1024 of D while one is taken out.  Each CTA has half of the rows of dY
@@ -22,6 +23,8 @@
 #include "bsq_fp4_few.hpp"
 #include "bsq_fp4_tile.cuh"
 #include "bsq_internal.hpp"
+
+#include <algorithm>
 
 namespace bsq {
 namespace {
@@ -98,10 +101,11 @@ __device__ __forceinline__ void read_columns(unsigned taddr, unsigned (&r)[16], 
 }
 
 // CTAS: 1, or 2 for a pair.  MT: blocks of 128 rows of a CTA, each with accumulators of its own.  SPLIT: the CTAs of a cluster share a tile, each with a slice of D.
-template <int FMT, int CTAS, int MT, bool SPLIT>
+// TOTAL: chains are added up in tensor memory, in an accumulator of their own.
+template <int FMT, int CTAS, int MT, bool SPLIT, bool TOTAL>
 __global__ void __launch_bounds__(grad_threads(MT), 1) fp4_grad_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                                                                    const __grid_constant__ CUtensorMap map_c, const Fp4Grad g, unsigned *status) {
-    static_assert((CTAS == 1 || !SPLIT) && (MT == 1 || CTAS == 2), "pairs do not share tiles, single CTAs have one block of rows");
+    static_assert((CTAS == 1 || !SPLIT) && (MT == 1 || CTAS == 2) && (SPLIT || !TOTAL), "pairs do not share tiles, single CTAs have one block of rows");
     chain_begin();
     constexpr int kRing = ring_of(MT), kRawRing = raw_ring_of(MT);
     constexpr unsigned kOpBytes = op_bytes_of(MT);
@@ -111,7 +115,10 @@ __global__ void __launch_bounds__(grad_threads(MT), 1) fp4_grad_kernel(const __g
     GradBars &bars = *reinterpret_cast<GradBars *>(boxes + kBoxesBytes);
     constexpr int kQuads = FMT == kNvFp4 ? 2 : 1;                // scale tiles across a CTA's 128 columns
     constexpr unsigned kAccCols = CTAS * kTileC;                 // columns of an accumulator
-    constexpr int kSets = SPLIT ? 4 : 2 / MT;                    // accumulators that follow one another (SPLIT: parts of one chain)
+    // Accumulators that chains take in turn.  SPLIT: a slice of up to four chains leaves them side by side, one accumulator each, and they are added once; of a longer
+    // one (TOTAL) they take two accumulators in turn, and a third holds what they have come to.
+    constexpr int kSets = SPLIT ? 4 : 2 / MT, kTurns = SPLIT ? (TOTAL ? 2 : 1) : kSets;
+    constexpr unsigned kTotal = kTurns * kAccCols;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int half = CTAS == 2 ? (int)(blockIdx.x & 1) : 0, unit = (int)(blockIdx.x / (SPLIT ? (unsigned)g.splits : (unsigned)CTAS));
     const int rank = SPLIT ? (int)(blockIdx.x % (unsigned)g.splits) : 0;
@@ -183,14 +190,14 @@ __global__ void __launch_bounds__(grad_threads(MT), 1) fp4_grad_kernel(const __g
             // BF16 x BF16, FP32 sums, B contiguous along N, A along K or along M, N >> 3, M >> 4
             const unsigned idesc = (1u << 4) | (1u << 7) | (1u << 10) | (g.a_kmajor ? 0u : 1u << 15) | (1u << 16) | (kAccCols >> 3 << 17) | ((CTAS * 128u >> 4) << 24);
             const uint64_t a_step = g.a_kmajor ? 2u : 128u;
-            Ring r(kRing), rs(SPLIT ? 1 : kSets);
+            Ring r(kRing), rs(kTurns);
             for (int t = first; t < tiles && ok; t += step) {
-                for (int c0 = d0; c0 < d1 && ok; c0 += SPLIT ? d1 - d0 : g.chain, rs.next()) {
-                    const int c1 = SPLIT ? d1 : min(d1, c0 + g.chain);
+                for (int c0 = d0; c0 < d1 && ok; c0 += SPLIT && !TOTAL ? d1 - d0 : g.chain, rs.next()) {
+                    const int c1 = SPLIT && !TOTAL ? d1 : min(d1, c0 + g.chain);
                     if (rs.wrapped) ok = __all_sync(kFullMask, mbar_wait_asleep(&bars.acc_empty[rs.pos], rs.par ^ 1u, status)) != 0;
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    int set = SPLIT ? 0 : rs.pos, left = g.chain;                            // (SPLIT: up to four accumulators, one behind the other)
+                    int set = SPLIT && !TOTAL ? 0 : rs.pos, left = g.chain;                  // (SPLIT: up to four accumulators, one behind the other)
                     bool fresh = true;
                     for (int d = c0; d < c1; ++d, r.next()) {
                         ok = __all_sync(kFullMask, mbar_wait_asleep(&bars.full[r.pos], r.par, status)) != 0;
@@ -213,7 +220,7 @@ __global__ void __launch_bounds__(grad_threads(MT), 1) fp4_grad_kernel(const __g
                         }
                         __syncwarp();
                         fresh = false;
-                        if (SPLIT && --left == 0) {
+                        if (SPLIT && !TOTAL && --left == 0) {
                             ++set;
                             left = g.chain;
                             fresh = true;
@@ -331,20 +338,34 @@ __global__ void __launch_bounds__(grad_threads(MT), 1) fp4_grad_kernel(const __g
         const Factors f = join_factors(*g.head, FMT == kNvFp4 ? kNvHold : 1.0f);
         const int size = g.type == kF32 ? 4 : 2;
         int which = 0;
-        Ring rs(SPLIT ? 1 : kSets);
+        Ring rs(kTurns);
         for (int t = first; t < tiles; t += step) {
             const int row = ((t % g.r_tiles) * CTAS * MT + half) * 128 + quarter * 32, col = (t / g.r_tiles) * (int)kAccCols;
-            for (int c0 = d0; c0 < d1; c0 += SPLIT ? d1 - d0 : g.chain, rs.next()) {
+            for (int c0 = d0; c0 < d1; c0 += SPLIT && !TOTAL ? d1 - d0 : g.chain, rs.next()) {
                 if (ok) ok = __all_sync(kFullMask, mbar_wait_asleep(&bars.acc_full[rs.pos], rs.par, status, g.epilogue_tries)) != 0;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const unsigned taddr = tmem + (SPLIT ? 0u : (unsigned)rs.pos * kAccCols) + ((unsigned)(quarter * 32) << 16);
+                const unsigned lanes = tmem + ((unsigned)(quarter * 32) << 16), taddr = lanes + (SPLIT && !TOTAL ? 0u : (unsigned)rs.pos * kAccCols);
                 const bool add = !SPLIT && c0 > d0;              // (FP32 only: to what this warp wrote before)
-                if constexpr (SPLIT) {
+                if (TOTAL && d1 - c0 > g.chain) {                // not the last chain: into the total
+                    for (int c = 0; c < (int)kAccCols; c += 16) {
+                        unsigned r[16];
+                        read16(taddr + (unsigned)c, r, ok);
+                        if (c0 > d0) add16(lanes + kTotal + (unsigned)c, r);
+                        tmem_st16(lanes + kTotal + (unsigned)c, r);
+                    }
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                } else if constexpr (SPLIT) {
                     // (without the accumulators nobody knows whether the stages are free: nothing is written then)
                     for (int c = 0; ok && c < (int)kAccCols; c += 16) {
                         unsigned r[16];
                         read_columns(taddr + (unsigned)c, r, ok);
-                        for (int i = 1; i < kSets && i * g.chain < d1 - d0; ++i) {
+                        if (TOTAL && c0 > d0) {
+                            unsigned q[16];
+                            read_columns(lanes + kTotal + (unsigned)c, q, true);
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + __uint_as_float(q[j]));
+                        }
+                        for (int i = 1; !TOTAL && i < kSets && i * g.chain < d1 - d0; ++i) {
                             unsigned q[16];
                             read_columns(taddr + (unsigned)i * kAccCols + (unsigned)c, q, ok);
 #pragma unroll
@@ -443,24 +464,26 @@ __global__ void __launch_bounds__(256) pad_rows_kernel(const unsigned short *in,
         for (uint64_t c = (uint64_t)blockIdx.x * 2048 + threadIdx.x; c < min(cols, (uint64_t)(blockIdx.x + 1) * 2048); c += 256) out[r * ld_out + c] = in[r * ld + c];
 }
 
-template <int FMT, int CTAS, int MT, bool SPLIT>
+template <int FMT, int CTAS, int MT, bool SPLIT, bool TOTAL = false>
 cudaError_t launch_grad(const CUtensorMap &map_a, const CUtensorMap &map_b, const CUtensorMap &map_c, const Fp4Grad &g, int sm_count, unsigned *status, cudaStream_t stream) {
     constexpr size_t smem = 1024 + ring_of(MT) * op_bytes_of(MT) + raw_ring_of(MT) * kRawBytes + kBoxesBytes + sizeof(GradBars) + 64;
     static_assert(smem <= 227 * 1024, "stages do not fit");
     static_assert((size_t)128 * (kTileC + 4) * 4 <= (size_t)ring_of(MT) * op_bytes_of(MT), "partial tile does not fit");
     static std::atomic<uint64_t> done{0};
-    const cudaError_t err = allow_smem(fp4_grad_kernel<FMT, CTAS, MT, SPLIT>, &done);
+    const cudaError_t err = allow_smem(fp4_grad_kernel<FMT, CTAS, MT, SPLIT, TOTAL>, &done);
     if (err != cudaSuccess) return err;
     const int tiles = g.r_tiles * g.c_tiles;
-    if (SPLIT) return launch_cluster(fp4_grad_kernel<FMT, CTAS, MT, SPLIT>, (unsigned)(tiles * g.splits), grad_threads(MT), g.splits, smem, stream, map_a, map_b, map_c, g, status);
+    if (SPLIT) return launch_cluster(fp4_grad_kernel<FMT, CTAS, MT, SPLIT, TOTAL>, (unsigned)(tiles * g.splits), grad_threads(MT), g.splits, smem, stream, map_a, map_b, map_c, g, status);
     const int units = sm_count / CTAS, grid = (tiles < units ? tiles : units) * CTAS;
-    if (CTAS == 2) return launch_cluster(fp4_grad_kernel<FMT, CTAS, MT, SPLIT>, (unsigned)grid, grad_threads(MT), CTAS, smem, stream, map_a, map_b, map_c, g, status);
-    return launch_chained(fp4_grad_kernel<FMT, CTAS, MT, SPLIT>, (unsigned)grid, grad_threads(MT), smem, stream, map_a, map_b, map_c, g, status);
+    if (CTAS == 2) return launch_cluster(fp4_grad_kernel<FMT, CTAS, MT, SPLIT, TOTAL>, (unsigned)grid, grad_threads(MT), CTAS, smem, stream, map_a, map_b, map_c, g, status);
+    return launch_chained(fp4_grad_kernel<FMT, CTAS, MT, SPLIT, TOTAL>, (unsigned)grid, grad_threads(MT), smem, stream, map_a, map_b, map_c, g, status);
 }
 template <int FMT>
 cudaError_t launch_grad_format(int ctas, int blocks, const CUtensorMap &map_a, const CUtensorMap &map_b, const CUtensorMap &map_c, const Fp4Grad &g, int sm_count, unsigned *status, cudaStream_t stream) {
     if (ctas == 2 && blocks == 2) return launch_grad<FMT, 2, 2, false>(map_a, map_b, map_c, g, sm_count, status, stream);
     if (ctas == 2) return launch_grad<FMT, 2, 1, false>(map_a, map_b, map_c, g, sm_count, status, stream);
+    // slices of more than four chains
+    if (g.splits > 1 && g.stages_per_split > 4 * g.chain) return launch_grad<FMT, 1, 1, true, true>(map_a, map_b, map_c, g, sm_count, status, stream);
     return g.splits > 1 ? launch_grad<FMT, 1, 1, true>(map_a, map_b, map_c, g, sm_count, status, stream) : launch_grad<FMT, 1, 1, false>(map_a, map_b, map_c, g, sm_count, status, stream);
 }
 
@@ -505,7 +528,7 @@ cudaError_t grad_product(int format, bool a_kmajor, const void *dy, uint64_t M, 
         while (g.splits < 8 && tiles * g.splits * 2 <= sm_count && g.d_stages >= g.splits * 4) g.splits *= 2;
     g.stages_per_split = (g.d_stages + g.splits - 1) / g.splits;
     g.splits = (g.d_stages + g.stages_per_split - 1) / g.stages_per_split;               // no slice is empty
-    g.chain = type != kF32 ? g.stages_per_split : g.splits > 1 ? (g.stages_per_split + 3) / 4 : kChainStages;
+    g.chain = type != kF32 ? g.stages_per_split : g.splits > 1 ? std::min((g.stages_per_split + 3) / 4, kChainStages) : kChainStages;
     CUtensorMap map_a, map_b, map_c;
     const cuuint64_t dims_a[2] = {N, M}, strides_a[1] = {ld_a * 2}, dims_b[2] = {fp4_ld(C), D}, strides_b[1] = {fp4_ld(C)};
     const cuuint32_t box_a[2] = {64u, a_kmajor ? 128u : 64u}, box_b[2] = {kTileC / 2, kStageD}, estr[2] = {1, 1};

@@ -40,6 +40,21 @@ __device__ __forceinline__ void read16(unsigned taddr, unsigned (&r)[16], bool o
     }
 }
 
+// 16 neighbouring accumulators of this thread's row, written (visible to reads behind a tcgen05.wait::st)
+__device__ __forceinline__ void tmem_st16(unsigned taddr, const unsigned (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};\n" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
+        "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+        : "memory");
+}
+// ... added to what is in registers, rounded
+__device__ __forceinline__ void add16(unsigned taddr, unsigned (&r)[16]) {
+    unsigned q[16];
+    read16(taddr, q, true);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + __uint_as_float(q[j]));
+}
+
 // The two factors of a result (matrix scales) as one where their product is a normal number; else the larger one comes first, so that a result within the range of
 // FP32 does not leave it on the way: sums up to 2^40 times 2^117 times 2^-110.
 struct Factors {

@@ -1,0 +1,75 @@
+"""Gradients summed over many terms, against 64 bits.
+
+The tensor core cuts an addition off instead of rounding it, so what a chain of additions in one accumulator loses grows with its length, all to one side.  FP32 results are
+summed in chains of 1024 terms, 64 additions, whose sums are added rounded.  With terms of random sign a chain is off by 1.5e-7 of itself and so is the sum of all chains
+(their errors are to the side of their signs, as their sum is); n rounded additions come to 2^-25 sqrt(n / 2) in the mean, 3.4e-7 for the 256 chains of 262144 terms.
+5e-7 holds with room; chains of 8192 terms are 2.6e-6 off."""
+import importlib
+
+import pytest
+
+import fp4_reference as ref
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+FORMATS = [ref.MXFP4, ref.NVFP4]
+SLACK = 5e-7
+
+
+@pytest.fixture(scope="module")
+def ops(pkg):
+    return importlib.import_module(pkg.__name__ + ".torch_ops")
+
+
+def product(a, b):
+    """a b in 64 bits, a piece of the sum at a time."""
+    out = torch.zeros(a.shape[0], b.shape[1], dtype=torch.float64, device="cuda")
+    for i in range(0, a.shape[1], 8192):
+        out += a[:, i: i + 8192].double() @ b[i: i + 8192].double()
+    return out
+
+
+def off(got, want):
+    return float((got.double() - want).norm() / want.norm())
+
+
+# outputs, columns, tokens: clusters with slices of up to and beyond four chains, odd lengths; one CTA a tile; pairs; both with rows off 16 bytes
+WEIGHT = [(1024, 1024, 16384), (1024, 1024, 65536), (64, 4096, 32768), (64, 300, 262144), (257, 260, 100003), (100, 100, 33000), (1036, 1040, 6001), (2304, 2304, 9000),
+          (1036, 1037, 6001), (2100, 2201, 4100)]
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("N,K,M", WEIGHT)
+def test_fp32_weight_gradient(ops, fmt, N, K, M):
+    gen = torch.Generator(device="cuda").manual_seed(M)
+    x = ops.fp4_quantize(torch.randn(M, K, generator=gen, device="cuda"), fmt)
+    dy = torch.randn(M, N, generator=gen, device="cuda").to(torch.bfloat16)
+    want = product(dy.t(), ops.fp4_dequantize(x))
+    got = ops.fp4_grad_weight(dy, x, torch.float32)
+    assert off(got, want) < SLACK
+    assert torch.equal(ops.fp4_grad_weight(dy, x, torch.float32), got)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("M,N,K", [(200, 65536, 1024), (40, 131072, 520), (128, 20000, 4096), (300, 9001, 8191)])
+def test_fp32_input_gradient(ops, fmt, M, N, K):
+    gen = torch.Generator(device="cuda").manual_seed(N)
+    w = ops.fp4_quantize(torch.randn(N, K, generator=gen, device="cuda"), fmt)
+    dy = torch.randn(M, N, generator=gen, device="cuda").to(torch.bfloat16)
+    want = product(dy, ops.fp4_dequantize(w))
+    got = ops.fp4_grad_input(dy, w, torch.float32)
+    assert off(got, want) < SLACK
+    assert torch.equal(ops.fp4_grad_input(dy, w, torch.float32), got)
+
+
+@pytest.mark.parametrize("M", [5000, 100000])
+def test_longer_slices_exact(ops, M):
+    """Sums that FP32 holds exactly, over slices that end inside a chain, inside a stage, and of every CTA of a cluster its own."""
+    gen = torch.Generator(device="cuda").manual_seed(M)
+    for N, K in ((33, 70), (300, 300), (700, 130)):
+        for extra in (0, 1, 63, 1000):
+            x = ops.fp4_quantize(torch.randint(-1, 2, (M + extra, K), generator=gen, device="cuda").float(), ref.MXFP4)
+            dy = torch.randint(-2, 3, (M + extra, N), generator=gen, device="cuda").to(torch.bfloat16)
+            want = product(dy.t(), ops.fp4_dequantize(x))
+            assert torch.equal(ops.fp4_grad_weight(dy, x, torch.float32).double(), want)
