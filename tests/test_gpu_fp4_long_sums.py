@@ -73,3 +73,26 @@ def test_longer_slices_exact(ops, M):
             dy = torch.randint(-2, 3, (M + extra, N), generator=gen, device="cuda").to(torch.bfloat16)
             want = product(dy.t(), ops.fp4_dequantize(x))
             assert torch.equal(ops.fp4_grad_weight(dy, x, torch.float32).double(), want)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("M,N,K", [(1, 131072, 520), (16, 131072, 1024), (16, 65536, 4100), (7, 30001, 14336), (16, 32769, 14336), (3, 1100, 100000),
+                                   (16, 70000, 14336), (1, 131072, 14336), (5, 9000, 70000)])
+def test_fp32_input_gradient_of_few_rows(ops, fmt, M, N, K):
+    gen = torch.Generator(device="cuda").manual_seed(N + M)
+    w = ops.fp4_quantize(torch.randn(N, K, generator=gen, device="cuda"), fmt)
+    dy = torch.randn(M, N, generator=gen, device="cuda").to(torch.bfloat16)
+    want = product(dy, ops.fp4_dequantize(w))
+    got = ops.fp4_grad_input(dy, w, torch.float32)
+    assert off(got, want) < SLACK
+    assert torch.equal(ops.fp4_grad_input(dy, w, torch.float32), got)
+
+
+def test_few_rows_of_long_sums_exact(ops):
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    for N, K in ((131072, 64), (70001, 300), (32800, 14336)):
+        w = ops.fp4_quantize(torch.randint(-1, 2, (N, K), generator=gen, device="cuda").float(), ref.MXFP4)
+        dy = torch.randint(-2, 3, (16, N), generator=gen, device="cuda").to(torch.bfloat16)
+        want = product(dy, ops.fp4_dequantize(w))
+        for M in (1, 9, 16):
+            assert torch.equal(ops.fp4_grad_input(dy[:M], w, torch.float32).double(), want[:M])
