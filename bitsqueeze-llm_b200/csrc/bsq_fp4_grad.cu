@@ -7,6 +7,7 @@
 // cuts every addition off instead of rounding it, and what is lost grows with the length of the chain: results in FP32 leave tensor memory every 1024 of D
 // and are added up rounded (4096 of D: 1.0e-6 off 64 bits in chains of 2048, 0.4e-6 in chains of 1024, a rounded FP32 product 0.3e-6).  Where CTAs share a tile, a
 // slice of more than four such chains adds them up in tensor memory (1024 x 1024 from 65536: 0.2e-6 off, 2.6e-6 in the four chains of 8192 that it had; 199 us, 189).
+// 16-bit results are one chain up to 65536 (FP16) or 524288 terms (BF16), and several that are added up in the same way beyond.
 //
 // Where there are enough tiles, a pair of CTAs on two SMs shares one (cta_group::2): of 512 x 256 for 16-bit results, so that an element of B is decoded once for
 // 512 rows, of 256 x 256 for FP32 ones, which leaves a second set of accumulators for the next 1024 of D while one is taken out.  Each CTA has half of the rows of dY
@@ -39,6 +40,9 @@ constexpr unsigned kBoxesBytes = kEpilogueWarps * 2 * kBoxBytes;
 constexpr unsigned kABytes = 128 * kStageD * 2, kBBytes = kStageD * kTileC * 2;
 constexpr unsigned kCodeBytes = kStageD * kTileC / 2, kRawBytes = kCodeBytes + 1024;
 constexpr int kChainStages = 1024 / kStageD;                     // FP32 results: longest chain of additions in tensor memory
+// ... of 16-bit results: 65536 terms lose 0.3e-4, all to one side, a sixth of what FP16's rounding takes (2.1e-4); 262144 lose 1.9e-4.  BF16 has three bits fewer.
+// (Longer chains than need be cost less: a second one rules tiles of 512 rows out, 4096 x 4096 from 65536 1360 us with them, 1700 without.)
+constexpr int kChainStagesF16 = 65536 / kStageD, kChainStagesBf16 = 8 * kChainStagesF16;
 
 // A stage: MT blocks of 128 rows of dY, 128 columns of B
 __host__ __device__ constexpr unsigned op_bytes_of(int mt) { return (unsigned)mt * kABytes + kBBytes; }
@@ -105,7 +109,7 @@ __device__ __forceinline__ void read_columns(unsigned taddr, unsigned (&r)[16], 
 template <int FMT, int CTAS, int MT, bool SPLIT, bool TOTAL>
 __global__ void __launch_bounds__(grad_threads(MT), 1) fp4_grad_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                                                                    const __grid_constant__ CUtensorMap map_c, const Fp4Grad g, unsigned *status) {
-    static_assert((CTAS == 1 || !SPLIT) && (MT == 1 || CTAS == 2) && (SPLIT || !TOTAL), "pairs do not share tiles, single CTAs have one block of rows");
+    static_assert((CTAS == 1 || !SPLIT) && (MT == 1 || CTAS == 2) && (MT == 1 || !TOTAL), "pairs do not share tiles, single CTAs have one block of rows, two blocks leave no room for a total");
     chain_begin();
     constexpr int kRing = ring_of(MT), kRawRing = raw_ring_of(MT);
     constexpr unsigned kOpBytes = op_bytes_of(MT);
@@ -117,7 +121,7 @@ __global__ void __launch_bounds__(grad_threads(MT), 1) fp4_grad_kernel(const __g
     constexpr unsigned kAccCols = CTAS * kTileC;                 // columns of an accumulator
     // Accumulators that chains take in turn.  SPLIT: a slice of up to four chains leaves them side by side, one accumulator each, and they are added once; of a longer
     // one (TOTAL) they take two accumulators in turn, and a third holds what they have come to.
-    constexpr int kSets = SPLIT ? 4 : 2 / MT, kTurns = SPLIT ? (TOTAL ? 2 : 1) : kSets;
+    constexpr int kSets = SPLIT ? 4 : 2 / MT, kTurns = SPLIT ? (TOTAL ? 2 : 1) : TOTAL ? 1 : kSets;
     constexpr unsigned kTotal = kTurns * kAccCols;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int half = CTAS == 2 ? (int)(blockIdx.x & 1) : 0, unit = (int)(blockIdx.x / (SPLIT ? (unsigned)g.splits : (unsigned)CTAS));
@@ -344,9 +348,11 @@ __global__ void __launch_bounds__(grad_threads(MT), 1) fp4_grad_kernel(const __g
             for (int c0 = d0; c0 < d1; c0 += SPLIT && !TOTAL ? d1 - d0 : g.chain, rs.next()) {
                 if (ok) ok = __all_sync(kFullMask, mbar_wait_asleep(&bars.acc_full[rs.pos], rs.par, status, g.epilogue_tries)) != 0;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const unsigned lanes = tmem + ((unsigned)(quarter * 32) << 16), taddr = lanes + (SPLIT && !TOTAL ? 0u : (unsigned)rs.pos * kAccCols);
-                const bool add = !SPLIT && c0 > d0;              // (FP32 only: to what this warp wrote before)
-                if (TOTAL && d1 - c0 > g.chain) {                // not the last chain: into the total
+                const unsigned lanes = tmem + ((unsigned)(quarter * 32) << 16);
+                unsigned taddr = lanes + (SPLIT && !TOTAL ? 0u : (unsigned)rs.pos * kAccCols);
+                const bool add = !SPLIT && !TOTAL && c0 > d0;    // (FP32 only: to what this warp wrote before)
+                const bool more = TOTAL && d1 - c0 > g.chain;    // not the last chain of this tile
+                if (TOTAL && (more || c0 > d0)) {
                     for (int c = 0; c < (int)kAccCols; c += 16) {
                         unsigned r[16];
                         read16(taddr + (unsigned)c, r, ok);
@@ -354,17 +360,14 @@ __global__ void __launch_bounds__(grad_threads(MT), 1) fp4_grad_kernel(const __g
                         tmem_st16(lanes + kTotal + (unsigned)c, r);
                     }
                     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    taddr = lanes + kTotal;
+                }
+                if (more) {
                 } else if constexpr (SPLIT) {
                     // (without the accumulators nobody knows whether the stages are free: nothing is written then)
                     for (int c = 0; ok && c < (int)kAccCols; c += 16) {
                         unsigned r[16];
                         read_columns(taddr + (unsigned)c, r, ok);
-                        if (TOTAL && c0 > d0) {
-                            unsigned q[16];
-                            read_columns(lanes + kTotal + (unsigned)c, q, true);
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + __uint_as_float(q[j]));
-                        }
                         for (int i = 1; !TOTAL && i < kSets && i * g.chain < d1 - d0; ++i) {
                             unsigned q[16];
                             read_columns(taddr + (unsigned)i * kAccCols + (unsigned)c, q, ok);
@@ -480,10 +483,13 @@ cudaError_t launch_grad(const CUtensorMap &map_a, const CUtensorMap &map_b, cons
 }
 template <int FMT>
 cudaError_t launch_grad_format(int ctas, int blocks, const CUtensorMap &map_a, const CUtensorMap &map_b, const CUtensorMap &map_c, const Fp4Grad &g, int sm_count, unsigned *status, cudaStream_t stream) {
+    // chains that can neither lie side by side (FP32 results of shared tiles: up to four) nor be added up in memory (FP32 results)
+    const bool total = g.type != kF32 ? g.stages_per_split > g.chain : g.splits > 1 && g.stages_per_split > 4 * g.chain;
     if (ctas == 2 && blocks == 2) return launch_grad<FMT, 2, 2, false>(map_a, map_b, map_c, g, sm_count, status, stream);
-    if (ctas == 2) return launch_grad<FMT, 2, 1, false>(map_a, map_b, map_c, g, sm_count, status, stream);
-    // slices of more than four chains
-    if (g.splits > 1 && g.stages_per_split > 4 * g.chain) return launch_grad<FMT, 1, 1, true, true>(map_a, map_b, map_c, g, sm_count, status, stream);
+    if (ctas == 2) return total ? launch_grad<FMT, 2, 1, false, true>(map_a, map_b, map_c, g, sm_count, status, stream)
+                                : launch_grad<FMT, 2, 1, false>(map_a, map_b, map_c, g, sm_count, status, stream);
+    if (total) return g.splits > 1 ? launch_grad<FMT, 1, 1, true, true>(map_a, map_b, map_c, g, sm_count, status, stream)
+                                   : launch_grad<FMT, 1, 1, false, true>(map_a, map_b, map_c, g, sm_count, status, stream);
     return g.splits > 1 ? launch_grad<FMT, 1, 1, true>(map_a, map_b, map_c, g, sm_count, status, stream) : launch_grad<FMT, 1, 1, false>(map_a, map_b, map_c, g, sm_count, status, stream);
 }
 
@@ -512,10 +518,12 @@ cudaError_t grad_product(int format, bool a_kmajor, const void *dy, uint64_t M, 
     if (r128 * c128 > 0x7fffffffull / 8) return cudaErrorInvalidValue;
     // a pair per tile of 256 x 256 where that fills the device
     const int ctas = r128 > 1 && ((r128 + 1) / 2) * ((c128 + 1) / 2) * 2 >= (uint64_t)sm_count * 2 / 3 ? 2 : 1;
-    // ... of 512 x 256 where that does too: an element is then decoded once for 512 rows, but no accumulators are left for the next tile while one is taken out
-    const int blocks = ctas == 2 && type != kF32 && ((r128 + 3) / 4) * ((c128 + 1) / 2) * 2 >= (uint64_t)sm_count * 2 / 3 ? 2 : 1;
-    g.r_tiles = (int)((r128 + ctas * blocks - 1) / (ctas * blocks)); g.c_tiles = (int)((c128 + ctas - 1) / ctas);
     g.d_stages = (int)((D + kStageD - 1) / kStageD);
+    const int longest = type == kF32 ? kChainStages : type == kF16 ? kChainStagesF16 : kChainStagesBf16;
+    // ... of 512 x 256 where that does too: an element is then decoded once for 512 rows, but no accumulators are left for the next tile while one is taken out, or for a
+    // second chain
+    const int blocks = ctas == 2 && type != kF32 && g.d_stages <= longest && ((r128 + 3) / 4) * ((c128 + 1) / 2) * 2 >= (uint64_t)sm_count * 2 / 3 ? 2 : 1;
+    g.r_tiles = (int)((r128 + ctas * blocks - 1) / (ctas * blocks)); g.c_tiles = (int)((c128 + ctas - 1) / ctas);
     g.a_kmajor = a_kmajor;
     g.quads = (unsigned)fp4_quads(format, C);
     g.scales = b + fp4_scales_at(D, C);
@@ -528,7 +536,7 @@ cudaError_t grad_product(int format, bool a_kmajor, const void *dy, uint64_t M, 
         while (g.splits < 8 && tiles * g.splits * 2 <= sm_count && g.d_stages >= g.splits * 4) g.splits *= 2;
     g.stages_per_split = (g.d_stages + g.splits - 1) / g.splits;
     g.splits = (g.d_stages + g.stages_per_split - 1) / g.stages_per_split;               // no slice is empty
-    g.chain = type != kF32 ? g.stages_per_split : g.splits > 1 ? std::min((g.stages_per_split + 3) / 4, kChainStages) : kChainStages;
+    g.chain = type != kF32 ? std::min(g.stages_per_split, longest) : g.splits > 1 ? std::min((g.stages_per_split + 3) / 4, longest) : longest;
     CUtensorMap map_a, map_b, map_c;
     const cuuint64_t dims_a[2] = {N, M}, strides_a[1] = {ld_a * 2}, dims_b[2] = {fp4_ld(C), D}, strides_b[1] = {fp4_ld(C)};
     const cuuint32_t box_a[2] = {64u, a_kmajor ? 128u : 64u}, box_b[2] = {kTileC / 2, kStageD}, estr[2] = {1, 1};

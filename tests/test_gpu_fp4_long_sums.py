@@ -96,3 +96,37 @@ def test_few_rows_of_long_sums_exact(ops):
         want = product(dy, ops.fp4_dequantize(w))
         for M in (1, 9, 16):
             assert torch.equal(ops.fp4_grad_input(dy[:M], w, torch.float32).double(), want[:M])
+
+
+# one CTA a tile, a second chain of one term, pairs, clusters
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("N,K,M", [(1036, 1040, 200000), (1036, 1037, 65537), (2304, 2304, 140001), (300, 300, 600000)])
+def test_fp16_weight_gradient(ops, fmt, N, K, M):
+    """Chains of FP16 results are 65536 terms long: 4096 additions, 0.33e-4 of a result, towards 0 (64 additions lose 1.5e-7; the loss grows faster than their number,
+    as larger partial sums are cut more coarsely).  FP16's own rounding goes to either side: over 90000 results 2^-12 / 300 = 8e-7.  6e-5 holds with room; 140001
+    terms in one chain lose 0.8e-4, 262144 1.9e-4."""
+    gen = torch.Generator(device="cuda").manual_seed(M)
+    x = ops.fp4_quantize(torch.randn(M, K, generator=gen, device="cuda").to(torch.bfloat16), fmt)
+    dy = torch.randn(M, N, generator=gen, device="cuda").to(torch.bfloat16)
+    want = torch.zeros(N, K, dtype=torch.float64, device="cuda")
+    v = ops.fp4_dequantize(x, torch.bfloat16)                      # (exact: 6 bits times a power of two)
+    for i in range(0, M, 8192):
+        want += dy[i: i + 8192].double().t() @ v[i: i + 8192].double()
+    got = ops.fp4_grad_weight(dy, x, torch.float16).double()
+    assert abs(float(((got - want) * want.sign()).sum() / want.abs().sum())) < 6e-5
+    bound = 2.0 ** -11 * want.abs() + 2.0 ** -25 + 1e-3 * want.abs().mean()     # a rounding, and 1e-3 of a typical result: what a chain loses, many times over
+    assert ((got - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("N,K,M", [(300, 300, 600000), (1036, 1040, 70000), (2304, 2304, 70001), (1500, 1036, 530000), (2100, 2304, 530001)])
+def test_fp16_and_bf16_exact(ops, N, K, M):
+    """As many chains as there are ways, sums that every one of them holds exactly."""
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    x = ops.fp4_quantize(torch.randint(-1, 2, (M, K), generator=gen, device="cuda", dtype=torch.int8).to(torch.bfloat16), ref.MXFP4)
+    dy = torch.randint(-2, 3, (M, N), generator=gen, device="cuda", dtype=torch.int8).to(torch.bfloat16)
+    v = ops.fp4_dequantize(x, torch.bfloat16)
+    want = torch.zeros(N, K, dtype=torch.float64, device="cuda")
+    for i in range(0, M, 8192):
+        want += dy[i: i + 8192].double().t() @ v[i: i + 8192].double()
+    for t in (torch.float16, torch.bfloat16):
+        assert torch.equal(ops.fp4_grad_weight(dy, x, t), want.float().to(t))
