@@ -91,13 +91,14 @@ __device__ __forceinline__ void box_out(const unsigned char *box, int lane, void
     }
     __syncwarp();
 }
-// ... added to what is there (FP32)
+// ... added to what is there (FP32): by the same lane as what it wrote before, so in its order, the same bits every time.  (Additions without an answer: a load, an addition
+// and a store would each wait for the one before.)
 __device__ __forceinline__ void box_add(const unsigned char *box, int lane, float *out, long at, long ld, int rows, int cols) {
     __syncwarp();
 #pragma unroll 4
     for (int r = 0; r < min(rows, 32); ++r) {
         const float v = *reinterpret_cast<const float *>(box + r * 128 + ((((lane >> 2) ^ (r & 7)) << 4) | ((lane & 3) << 2)));
-        if (lane < cols) out[at + (long)r * ld + lane] += v;
+        if (lane < cols) asm volatile("red.relaxed.gpu.global.add.f32 [%0], %1;" ::"l"(out + at + (long)r * ld + lane), "f"(v) : "memory");
     }
     __syncwarp();
 }

@@ -130,3 +130,39 @@ def test_fp16_and_bf16_exact(ops, N, K, M):
         want += dy[i: i + 8192].double().t() @ v[i: i + 8192].double()
     for t in (torch.float16, torch.bfloat16):
         assert torch.equal(ops.fp4_grad_weight(dy, x, t), want.float().to(t))
+
+
+# pairs that add in memory; tiles of 128 columns where results are off 16 bytes; clusters with tokens as columns and as rows; one CTA a tile
+LONG_PRODUCT = [(2048, 4096, 131072), (2049, 4097, 66000), (16, 4096, 131072), (777, 1031, 131072), (300, 300, 70001), (100, 20000, 20001), (1, 4096, 262144)]
+
+
+@pytest.mark.parametrize("M,N,K", LONG_PRODUCT)
+def test_fp32_product(ops, M, N, K):
+    """Of NVFP4 matrices with some columns 20 to 100 times the others', in chains of 4096 terms, 64 additions each.  A column that is large in both matrices can make up most of
+    a result: the additions behind it in its chain, 32 in the mean, are cut off at full size, 1.5e-8 (2^-26) each, 4.8e-7 at most where it makes up all of it; it does in
+    half of the results (the others are sums of many), 3.4e-7 in the mean square.  The 32 chains of 131072 terms are added up by roundings of 2^-23.5 / sqrt(12), 1.4e-7 in
+    all (64 of 262144 terms: 2.0e-7).  Together 4.0e-7.  Chains of 256 additions are 3.9e-6 off, FP32 sums that are rounded at each term 3e-7."""
+    gen = torch.Generator(device="cuda").manual_seed(K)
+
+    def matrix(rows):
+        x = torch.randn(rows, K, generator=gen, device="cuda")
+        at = torch.randperm(K, generator=gen, device="cuda")[: K // 1000]
+        x[:, at] *= 20 + 80 * torch.rand(K // 1000, generator=gen, device="cuda")
+        return ops.fp4_quantize(x)
+    a, b = matrix(M), matrix(N)
+    want = product(ops.fp4_dequantize(a), ops.fp4_dequantize(b).t())
+    got = ops.fp4_matmul(a, b, torch.float32)
+    assert off(got, want) < SLACK
+    assert torch.equal(ops.fp4_matmul(a, b, torch.float32), got)
+
+
+@pytest.mark.parametrize("M,N,K", LONG_PRODUCT + [(700, 900, 600000), (2100, 2300, 270000), (50, 130, 600000), (130, 20000, 263000)])
+def test_product_of_long_rows_exact(ops, M, N, K):
+    gen = torch.Generator(device="cuda").manual_seed(K)
+    a, b = (ops.fp4_quantize(torch.randint(-1, 2, (n, K), generator=gen, device="cuda", dtype=torch.int8).to(torch.bfloat16), ref.MXFP4) for n in (M, N))
+    va, vb = ops.fp4_dequantize(a, torch.bfloat16), ops.fp4_dequantize(b, torch.bfloat16)
+    want = torch.zeros(M, N, dtype=torch.float64, device="cuda")
+    for i in range(0, K, 8192):
+        want += va[:, i: i + 8192].double() @ vb[:, i: i + 8192].double().t()
+    for t in (torch.float32, torch.float16, torch.bfloat16):
+        assert torch.equal(ops.fp4_matmul(a, b, t), want.float().to(t))
