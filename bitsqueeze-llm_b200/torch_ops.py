@@ -316,8 +316,9 @@ def _overlap(grads, to):
 def clip_grad_norm(grads, max_norm, norm_type=2.0, out=None):
     """The norm of `grads` (float32, float16 or bfloat16 CUDA tensors of one device, mixed as they come) taken as one vector, as a float32 tensor of no
     dimensions; the gradients are multiplied by min(1, max_norm / (norm + 1e-6)), in place or into the tensors of `out` (of the same types;
-    contiguous with as many elements, or of the same shapes and strides).  norm_type 2 or math.inf.  max_norm None: the norm alone.  A NaN or Inf in any gradient makes the norm so, and goes into
-    all of them, as with torch.nn.utils.clip_grad_norm_."""
+    contiguous with as many elements, or of the same shapes and strides).  norm_type 2 or math.inf.  max_norm None: the norm alone.
+    What is scaled in place must not need a gradient itself: these are the parameters' gradients, not the parameters.
+    A NaN or Inf in any gradient makes the norm so, and goes into all of them, as with torch.nn.utils.clip_grad_norm_."""
     grads = list(grads)
     if norm_type not in (2, 2.0, math.inf):
         raise ValueError("norm_type must be 2 or infinity")
@@ -334,6 +335,8 @@ def clip_grad_norm(grads, max_norm, norm_type=2.0, out=None):
     types = [_TYPES.get(d, -1) for d in dtypes]
     if index < 0 or min(types) < 0 or set(map(_index, grads)) != {index} or not (all(plain) or all(p or _dense(g) for p, g in zip(plain, grads))):
         raise ValueError("gradients must be dense float32, float16 or bfloat16 CUDA tensors on one device")
+    if max_norm is not None and out is None and any(map(_requires_grad, grads)):
+        raise ValueError("tensors that are scaled in place must need no gradient (pass the parameters' gradients, not the parameters; detached ones if they need gradients themselves)")
     counts, ptrs = array("Q", map(_numel, grads)), array("Q", map(_pointer, grads))
     to, outs = grads, ptrs
     if out is not None:

@@ -179,3 +179,22 @@ def test_in_place_is_seen_by_autograd(ops):
     v = g._version
     ops.clip_grad_norm([g], 1.0)
     assert g._version > v
+
+
+def test_parameters_are_not_scaled_in_place(ops):
+    """Called as PyTorch's own function is, with the parameters: their values would be scaled, not their gradients."""
+    model = torch.nn.Linear(30, 20, device="cuda")
+    before = [p.detach().clone() for p in model.parameters()]
+    model(torch.randn(5, 30, device="cuda")).sum().backward()
+    params = list(model.parameters())
+    for grads in (model.parameters(), [params[0].grad, params[1]], [params[0] * 2.0]):
+        with pytest.raises(ValueError):
+            ops.clip_grad_norm(grads, 0.5)
+    with torch.no_grad(), pytest.raises(ValueError):
+        ops.clip_grad_norm(params, 0.5)
+    assert all(torch.equal(p, b) for p, b in zip(params, before))
+    assert abs(ops.clip_grad_norm(params, None).item() - exact_norm(before)) <= 1e-5 * exact_norm(before)     # the norm alone of whatever there is
+    outs = [torch.empty_like(b) for b in before]
+    ops.clip_grad_norm(params, 0.5, out=outs)                      # and into other tensors
+    assert all(torch.equal(p, b) for p, b in zip(params, before))
+    check(ops, [p.grad for p in params], 0.5)
