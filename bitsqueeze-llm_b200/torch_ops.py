@@ -318,7 +318,8 @@ def clip_grad_norm(grads, max_norm, norm_type=2.0, out=None):
     dimensions; the gradients are multiplied by min(1, max_norm / (norm + 1e-6)), in place or into the tensors of `out` (of the same types;
     contiguous with as many elements, or of the same shapes and strides).  norm_type 2 or math.inf.  max_norm None: the norm alone.
     What is scaled in place must not need a gradient itself: these are the parameters' gradients, not the parameters.
-    A NaN or Inf in any gradient makes the norm so, and goes into all of them, as with torch.nn.utils.clip_grad_norm_."""
+    As with torch.nn.utils.clip_grad_norm_ a NaN in any gradient makes the norm and all gradients NaN; an Inf makes the norm Inf, the finite gradients 0 and only the
+    infinite elements NaN.  To skip a step that went wrong look at the norm, not at a gradient."""
     grads = list(grads)
     if norm_type not in (2, 2.0, math.inf):
         raise ValueError("norm_type must be 2 or infinity")
