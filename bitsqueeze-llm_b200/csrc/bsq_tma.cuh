@@ -100,21 +100,33 @@ __device__ __forceinline__ void tc_commit_pair(uint64_t *bar, unsigned short mas
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"(mask) : "memory");
 }
 
-// cuTensorMapEncodeTiled from the driver, looked up once (the library links the runtime only).
+// cuTensorMapEncodeTiled from the driver, looked up once (the library links the runtime only).  It wants a current context, which a host thread has only after its first call of
+// the runtime that needs one: without it an operator that was the first thing a thread asked for, the thread of a backward pass say, failed.
 typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
                                   const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+typedef CUresult (*CurrentContextFn)(CUcontext *);
 inline EncodeTiledFn encode_tiled() {
     static EncodeTiledFn fn = nullptr;
+    static CurrentContextFn current = nullptr;
     static std::once_flag once;
     std::call_once(once, [] {
-        void *p = nullptr;
-        cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<EncodeTiledFn>(p);
-        else
+        const auto look_up = [](const char *name) {
+            void *p = nullptr;
+            cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
+            if (cudaGetDriverEntryPoint(name, &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess) return p;
             cudaGetLastError();
+            return (void *)nullptr;
+        };
+        current = reinterpret_cast<CurrentContextFn>(look_up("cuCtxGetCurrent"));
+        fn = reinterpret_cast<EncodeTiledFn>(look_up("cuTensorMapEncodeTiled"));
     });
+    CUcontext context = nullptr;
+    int device = 0;
+    if (fn && (!current || current(&context) != CUDA_SUCCESS || !context) && (cudaGetDevice(&device) != cudaSuccess || cudaSetDevice(device) != cudaSuccess)) {
+        cudaGetLastError();
+        return nullptr;
+    }
     return fn;
 }
 
