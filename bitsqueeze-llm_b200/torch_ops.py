@@ -13,7 +13,8 @@ include/bitsqz_llm_c.h).
 Calls enqueue on PyTorch's current stream of their tensors' device and return; nothing is synchronised, nothing is kept from one
 call to the next, and calls may be captured in a CUDA graph.  Tensors that are used on another stream than the one they were made
 on are the caller's to order, as with PyTorch's own operators.  A wait inside a product that ran out of tries leaves NaN in the result.
-Every result comes from the shared library; there is no fallback.
+Every result comes from the shared library; there is no fallback.  The operators are not registered with torch.compile: a compiled graph breaks at each call, and with
+fullgraph=True compilation fails there.
 """
 import math
 from array import array
@@ -247,6 +248,16 @@ def fp4_grad_weight(dy, x, dtype=torch.bfloat16, out=None):
     return _grad("bsq_fp4_grad_weight", dy, x, lambda M, N: M, lambda M, N: N, dtype, out)
 
 
+def _laid_out(x):
+    """x, or a copy where its elements do not lie as the rows of one matrix (a transposed or broadcast tensor)."""
+    if not x.is_contiguous():
+        try:
+            _rows(x, "x")
+        except ValueError:
+            return x.contiguous()
+    return x
+
+
 class _Fp4Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, w4, format):
@@ -277,16 +288,17 @@ class _Fp4Linear(torch.autograd.Function):
 def fp4_linear(x, weight, format=NVFP4):
     """x w^T with both operands in 4 bits, under autograd: x (bfloat16, (..., K)), weight either a tensor (N, K) that is quantised in every call and
     gets a gradient of its own type, or an Fp4Matrix that is frozen.  The backward pass treats quantisation as the identity: dx = dy q(w), dw = dy^T q(x),
-    where q(x) is kept in 4 bits between the passes."""
+    where q(x) is kept in 4 bits between the passes.  x or a weight whose elements do not lie as the rows of one matrix is copied first.  Autocast does not change what
+    is asked of x: pass it in bfloat16."""
     if x.dtype != torch.bfloat16 or not x.is_cuda:
         raise ValueError("x must be a bfloat16 CUDA tensor")
     if isinstance(weight, Fp4Matrix):
         if weight.format != format or x.dim() == 0 or x.size(-1) != weight.cols:
             raise ValueError("the weight must be packed in `format` with as many columns as x")
-        return _Fp4Linear.apply(x, None, weight, format)
+        return _Fp4Linear.apply(_laid_out(x), None, weight, format)
     if weight.dim() != 2 or x.dim() == 0 or x.size(-1) != weight.size(1) or weight.device != x.device or not weight.size(0):
         raise ValueError("the weight must be a (N, K) tensor on x's device, K the last dimension of x")
-    return _Fp4Linear.apply(x, weight, None, format)
+    return _Fp4Linear.apply(_laid_out(x), _laid_out(weight), None, format)
 
 
 def _dense(t):

@@ -597,3 +597,26 @@ def test_copies_that_land_in_any_order(ops):
         if bool(((got - want).abs() > bound).any()):
             wrong.append((i, fmt, M, N, K))
     assert not wrong
+
+
+def test_linear_of_tensors_that_do_not_lie_as_rows(ops):
+    """A transposed attention output, a broadcast one, columns of a wider matrix, a transposed weight: as contiguous copies of them."""
+    torch.manual_seed(11)
+    heads = torch.randn(2, 4, 10, 16, device="cuda").to(torch.bfloat16)
+    wide = torch.randn(2, 10, 200, device="cuda").to(torch.bfloat16)
+    w = torch.randn(48, 64, device="cuda") * 0.1
+    for make in (lambda: heads.transpose(1, 2).flatten(2), lambda: heads.permute(0, 2, 3, 1).reshape(2, 64, 10).transpose(1, 2), lambda: heads[:1, :1, :, :1].expand(2, 4, 10, 64),
+                 lambda: wide[:, :5, ::2][..., :64], lambda: wide[..., 8:72]):
+        results = []
+        for x, weight in ((make(), w), (make().contiguous(), w), (make(), w.t().contiguous().t())):
+            x, weight = x.detach(), weight.detach()
+            x.requires_grad_()
+            weight.requires_grad_()
+            y = ops.fp4_linear(x, weight)
+            y.backward(torch.arange(y.numel(), device="cuda").view(y.shape).to(torch.bfloat16) / 64)
+            results.append((y.detach(), x.grad, weight.grad))
+        for r in results[1:]:
+            assert all(torch.equal(a, b) for a, b in zip(results[0], r))
+    frozen = ops.fp4_quantize(w)
+    x = heads.permute(0, 2, 3, 1).reshape(2, 64, 10).transpose(1, 2)
+    assert torch.equal(ops.fp4_linear(x, frozen), ops.fp4_linear(x.contiguous(), frozen))
