@@ -1,7 +1,7 @@
 // Product of two microscaled 4-bit matrices (sm_100a): out[M x N] = A[M x K] B[N x K]^T with both operands packed
 // (bsq_fp4.hpp), on the block-scaled tensor-core instructions: tcgen05.mma kind::mxf4nvf4 with a scale for 16 of K (NVFP4),
 // kind::mxf4 with one for 32 (MXFP4).  Products of codes and block scales are exact, sums are FP32 in tensor memory; the
-// matrix scales are multiplied in when a tile leaves, and the result is rounded once.
+// matrix scales are multiplied in when a tile leaves, and the result is rounded once (FP32 results of more than 4096 of K: once for each chain, see kChainF32).
 //
 // Where there are tiles enough a pair of CTAs on two SMs shares one of 256 x 256 (cta_group::2): each brings 128 rows of either operand, so that shared memory
 // is read 64 bytes a clock by the MMAs and written as fast by the copies; alone, with 128 x 256, it is 96 and 96, more than the 128 it can do.
@@ -10,7 +10,8 @@
 // MMAs of 64 of K, warps 2 to 9 take the accumulators into registers, so that the next tile may begin, and then write them.  P is the operand whose rows are
 // the lanes of a tile, Q the one whose rows are its columns: P = A for training sizes; for a few tokens P = B, so that the tile's width follows the
 // number of tokens.  Where there are fewer tiles than SMs, a cluster of 2 to 8 CTAs shares a tile: each takes a slice of K, the partial tiles are
-// added through distributed shared memory in a fixed order.  Every wait is bounded; a tile whose wait ran out is written as NaN.  No multicast.
+// added through distributed shared memory in a fixed order.  Every wait is bounded; a tile whose wait ran out is written as NaN.  No load
+// is a multicast; of a pair's MMAs only the word that they are done goes to both CTAs.
 //
 // NVFP4 4096 x 14336 x 4096: 99 us, 4.9 PFLOP/s, three times the measured rate of a BF16 library product.  The tensor pipe is busy for 0.78 of a tile's time; without
 // MMAs and copies of scales the same loads take 82 us, so the rest is what shared memory is filled with (14 TB/s over all SMs), and some 600 clocks per
@@ -39,7 +40,6 @@ struct Fp4Gemm {
     int q_tile;                      // multiple of 16, up to 256; below 128 there is one tile of Q
     int p_tiles, q_tiles, ring, sets;
     int k_stages, splits, stages_per_split, chain;       // (chain: stages that are summed in one accumulator)
-    unsigned quads;                  // scale tiles along a row
     const float *p_head, *q_head;
     void *out;
     long ld;
@@ -431,11 +431,10 @@ cudaError_t fp4_matmul(int format, const void *a, uint64_t M, const void *b, uin
     Fp4Gemm g = {};
     g.P = (int)P; g.Q = (int)Q; g.K = (int)K;
     g.k_stages = (int)((K + kStageK - 1) / kStageK);
-    g.quads = (unsigned)fp4_quads(format, K);
     g.p_head = reinterpret_cast<const float *>(pp); g.q_head = reinterpret_cast<const float *>(pq);
     g.out = out; g.ld = (long)ld; g.type = type; g.lanes_contiguous = swap;
     g.epilogue_tries = epilogue_tries(kWaitTries);
-    const uint64_t row_bytes = M == 1 ? (N * op_bytes(type) + 15) / 16 * 16 : ld * op_bytes(type);
+    const uint64_t row_bytes = ld * op_bytes(type);
     const bool tma_out = !swap && reinterpret_cast<uintptr_t>(out) % 16 == 0 && row_bytes % 16 == 0;
     const int longest = type == kF32 ? kChainF32 : type == kF16 ? kChainF16 : kChainBf16;
     int ctas = 1;

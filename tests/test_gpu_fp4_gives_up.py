@@ -98,3 +98,20 @@ def test_more_tiles_than_accumulators(ops, lib, no_tries):
     assert all(torch.isnan(r).all() for r in results)
     lib.bsq_test_limit_waits(1 << 16)
     assert not any(torch.isnan(r).any() for r in (ops.fp4_matmul(a, b), ops.fp4_grad_input(dy, w), ops.fp4_grad_input(dy, w, torch.float32)))
+
+
+def test_sums_of_several_chains(ops, lib, no_tries):
+    """Accumulators that are handed back between the chains of a tile: none is, and every result is NaN."""
+    torch.manual_seed(1)
+    a, b, c = (ops.fp4_quantize(torch.randn(n, 40000, device="cuda")) for n in (300, 20, 2400))
+    dy = torch.randn(300, 40000, device="cuda").to(torch.bfloat16)
+    w = ops.fp4_quantize(torch.randn(40000, 130, device="cuda"))
+    x = ops.fp4_quantize(torch.randn(70000, 1040, device="cuda"))
+    dz = torch.randn(70000, 1040, device="cuda").to(torch.bfloat16)
+    calls = [lambda: ops.fp4_matmul(a, a, torch.float32), lambda: ops.fp4_matmul(b, a, torch.float32), lambda: ops.fp4_matmul(c, c, torch.float32),
+             lambda: ops.fp4_grad_input(dy, w, torch.float32), lambda: ops.fp4_grad_weight(dz, x, torch.float16), lambda: ops.fp4_grad_weight(dz[:, :200], x, torch.float32)]
+    for call in calls:
+        assert torch.isnan(call()).all()
+    lib.bsq_test_limit_waits(1 << 16)
+    for call in calls:
+        assert not torch.isnan(call()).any()
