@@ -435,7 +435,7 @@ cudaError_t fp4_matmul(int format, const void *a, uint64_t M, const void *b, uin
     g.out = out; g.ld = (long)ld; g.type = type; g.lanes_contiguous = swap;
     g.epilogue_tries = epilogue_tries(kWaitTries);
     const uint64_t row_bytes = ld * op_bytes(type);
-    const bool tma_out = !swap && reinterpret_cast<uintptr_t>(out) % 16 == 0 && row_bytes % 16 == 0;
+    const bool tma_out = !swap && tma_can_write(out, row_bytes, N * op_bytes(type));
     const int longest = type == kF32 ? kChainF32 : type == kF16 ? kChainF16 : kChainBf16;
     int ctas = 1;
     const auto plan = [&](int q_tile) {

@@ -547,9 +547,10 @@ cudaError_t grad_product(int format, bool a_kmajor, const void *dy, uint64_t M, 
                        CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         return cudaErrorInvalidValue;
     map_c = map_a;                                               // (not looked at without boxes)
-    g.boxes = reinterpret_cast<uintptr_t>(out) % 16 == 0 && (R == 1 || ld * op_bytes(type) % 16 == 0);
+    const uint64_t row_bytes = (R == 1 ? C : ld) * op_bytes(type);
+    g.boxes = tma_can_write(out, row_bytes, C * op_bytes(type));
     if (g.boxes) {
-        const cuuint64_t dims_c[2] = {C, R}, strides_c[1] = {R == 1 ? (C * op_bytes(type) + 15) / 16 * 16 : ld * op_bytes(type)};
+        const cuuint64_t dims_c[2] = {C, R}, strides_c[1] = {row_bytes};
         const cuuint32_t box_c[2] = {128u / (unsigned)op_bytes(type), 32u};
         if (encode_tiled()(&map_c, type == kF32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : type == kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, out,
                            dims_c, strides_c, box_c, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,

@@ -151,6 +151,12 @@ inline bool map_codes(CUtensorMap *map, const uint8_t *packed, uint64_t rows, ui
                                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Whether a result can leave by TMA: rows that start on 16 bytes and end on 16.  A tiled store leaves out what lies behind the last column only in whole pieces of 16
+// bytes; a row that ends inside one would have up to 14 bytes behind it overwritten.
+inline bool tma_can_write(const void *out, uint64_t row_stride, uint64_t row_bytes) {
+    return (reinterpret_cast<uintptr_t>(out) | row_stride | row_bytes) % 16 == 0;
+}
+
 // Lets a kernel have all of an SM's shared memory, once for each device.
 template <class F> cudaError_t allow_smem(F *kernel, std::atomic<uint64_t> *done) {
     int device = 0;
