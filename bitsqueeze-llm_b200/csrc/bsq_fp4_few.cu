@@ -23,7 +23,7 @@ namespace bsq {
 namespace {
 
 constexpr int kFewStages = 4, kFewCols = 128, kFewRows = 32;
-constexpr int kFewChain = 1024 / kFewRows;                       // FP32 results: longest chain of additions in a warp's accumulators, in chunks
+constexpr int kFewChain = 1024 / kFewRows;                       // longest chain of additions in a warp's accumulators where it has more than the result's type hides, in chunks
 constexpr unsigned kFewCodes = kFewRows * kFewCols / 2, kFewStage = kFewCodes + 256;
 
 struct Fp4Few {
@@ -271,7 +271,8 @@ cudaError_t fp4_grad_few(int format, const void *dy, int R, uint64_t ld_dy, cons
     g.dy = static_cast<const __nv_bfloat16 *>(dy);
     g.ld_dy = ld_dy;
     g.out = out; g.ld = (long)ld; g.type = type;
-    const bool longer = type == kF32 && g.chunks_per_split > kFewChain * warps;              // a warp would sum more than a chain
+    // a warp would sum more than 1024 terms of an FP32 result, 65536 of an FP16 one, 524288 of a BF16 one (as in bsq_fp4_grad.cu)
+    const bool longer = g.chunks_per_split > (type == kF32 ? 1 : type == kF16 ? 64 : 512) * kFewChain * warps;
     if (format == kNvFp4) return warps == 4 ? launch_warps<kNvFp4, 4>(longer, g, blocks, stream) : launch_warps<kNvFp4, 8>(longer, g, blocks, stream);
     return warps == 4 ? launch_warps<kMxFp4, 4>(longer, g, blocks, stream) : launch_warps<kMxFp4, 8>(longer, g, blocks, stream);
 }

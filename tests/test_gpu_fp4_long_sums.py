@@ -166,3 +166,17 @@ def test_product_of_long_rows_exact(ops, M, N, K):
         want += va[:, i: i + 8192].double() @ vb[:, i: i + 8192].double().t()
     for t in (torch.float32, torch.float16, torch.bfloat16):
         assert torch.equal(ops.fp4_matmul(a, b, t), want.float().to(t))
+
+
+def test_16_bit_results_of_few_rows_and_millions_of_terms_exact(ops):
+    """A weight of 4300001 x 100: more than 65536 rows for each of the 64 warps that share its columns."""
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    N, K = 4300001, 100
+    w = ops.fp4_quantize(torch.randint(-1, 2, (N, K), generator=gen, device="cuda", dtype=torch.int8).to(torch.bfloat16), ref.MXFP4)
+    v = ops.fp4_dequantize(w, torch.bfloat16)
+    dy = torch.randint(-2, 3, (16, N), generator=gen, device="cuda", dtype=torch.int8).to(torch.bfloat16)
+    want = torch.zeros(16, K, dtype=torch.float64, device="cuda")
+    for i in range(0, N, 1 << 16):
+        want += dy[:, i: i + (1 << 16)].double() @ v[i: i + (1 << 16)].double()
+    for t in (torch.float32, torch.float16, torch.bfloat16):
+        assert torch.equal(ops.fp4_grad_input(dy, w, t), want.float().to(t))
