@@ -200,7 +200,8 @@ def fp4_dequantize(m, dtype=torch.float32, out=None):
 
 
 def fp4_matmul(a, b, dtype=torch.bfloat16, out=None):
-    """a b^T of two Fp4Matrix of one format with the same number of columns: (a.rows, b.rows) in `dtype`, summed in FP32 and rounded once."""
+    """a b^T of two Fp4Matrix of one format with the same number of columns: (a.rows, b.rows) in `dtype`, summed in FP32 and rounded once
+    (float32 results of more than 4096 columns: at every 4096, added up in FP32)."""
     _packed(a, "a")
     _packed(b, "b")
     device = a.data.device
@@ -239,12 +240,13 @@ def _grad(name, dy, m, packed_rows, out_rows, dtype, out):
 
 def fp4_grad_input(dy, w, dtype=torch.bfloat16, out=None):
     """dy w: the gradient of the input of y = x w^T from dy (bfloat16, (..., w.rows)) and the packed weight, (..., w.cols) in `dtype`.  The weight's
-    values are exact in bfloat16; sums are FP32, rounded once."""
+    values are exact in bfloat16; sums are FP32, rounded once (float32 results: at every 1024 terms, added up in FP32)."""
     return _grad("bsq_fp4_grad_input", dy, w, lambda M, N: N, None, dtype, out)
 
 
 def fp4_grad_weight(dy, x, dtype=torch.bfloat16, out=None):
-    """dy^T x: the gradient of the weight from dy (bfloat16, (..., N) with x.rows rows in all) and the packed activations, (N, x.cols) in `dtype`."""
+    """dy^T x: the gradient of the weight from dy (bfloat16, (..., N) with x.rows rows in all) and the packed activations, (N, x.cols) in `dtype`,
+    summed as in fp4_grad_input."""
     return _grad("bsq_fp4_grad_weight", dy, x, lambda M, N: M, lambda M, N: N, dtype, out)
 
 

@@ -276,11 +276,12 @@ int bsq_fp4_quantize(int format, const void *d_x, int type, uint64_t rows, uint6
                      void *stream);
 /* out = (element * block scale) * matrix scale, rounded once */
 int bsq_fp4_dequantize(int format, const void *d_packed, uint64_t rows, uint64_t cols, void *d_out, int type, uint64_t ld, void *stream);
-/* out[M x N] = A[M x K] B[N x K]^T, both packed in the same format; FP32 sums, the result rounded once */
+/* out[M x N] = A[M x K] B[N x K]^T, both packed in the same format.  FP32 sums, the result rounded once.  The tensor core cuts additions off instead of rounding them, so sums of
+ * many terms are several chains that are added up rounded: of 4096 terms for FP32 results (each of them times the matrix scales, rounded), 262144 for FP16, 2097152 for BF16. */
 int bsq_fp4_matmul(int format, const void *d_a, uint64_t M, const void *d_b, uint64_t N, uint64_t K, void *d_out, int type, uint64_t ld, uint32_t *d_status,
                    void *stream);
 /* Gradients of y[M x N] = x[M x K] W[N x K]^T from dy (BF16) and the operands as they are packed:  dx[M x K] = dy W,  dW[N x K] = dy^T x.  FP32 sums, the result
- * rounded once.  d_scratch: bsq_fp4_grad_scratch_bytes on a 16-byte boundary (0 unless dy's rows do not all start on 16 bytes). */
+ * rounded once; in chains as above, of 1024 terms for FP32 results, 65536 for FP16, 524288 for BF16.  d_scratch: bsq_fp4_grad_scratch_bytes on a 16-byte boundary (0 unless dy's rows do not all start on 16 bytes). */
 size_t bsq_fp4_grad_scratch_bytes(const void *d_dy, uint64_t M, uint64_t N, uint64_t ld_dy);
 int bsq_fp4_grad_input(int format, const void *d_dy, uint64_t M, uint64_t ld_dy, const void *d_w, uint64_t N, uint64_t K, void *d_out, int type, uint64_t ld,
                        void *d_scratch, uint32_t *d_status, void *stream);
