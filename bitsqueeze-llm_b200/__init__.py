@@ -125,6 +125,10 @@ SIGNATURES = {
     "bsq_fp4_grad_weight": (_i, [_i, _vp, _u64, _u64, _u64, _vp, _u64, _vp, _i, _u64, _vp, _vp, _vp]),
     "bsq_grad_norm_scratch_bytes": (_sz, []),
     "bsq_grad_norm_clip": (_i, [_vp, _vp, _vp, _i, _vp, C.c_double, _i, _vp, _vp, _vp]),
+    "bsq_linear_xent_scratch_bytes": (_sz, [_i, _vp, _u64, _u64, _u64, _vp, _u64, _u64, C.c_double]),
+    "bsq_linear_xent": (_i, [_i, _vp, _u64, _u64, _u64, _vp, _u64, _u64, _vp, C.c_int64, C.c_double, _i, _vp, _vp, _vp, _vp, _vp]),
+    "bsq_linear_xent_grad_scratch_bytes": (_sz, [_i, _vp, _u64, _u64, _u64, _vp, _u64, _u64, _i]),
+    "bsq_linear_xent_grad": (_i, [_i, _vp, _u64, _u64, _u64, _vp, _u64, _u64, _vp, C.c_int64, C.c_double, _i, _vp, _vp, _vp, _u64, _vp, _u64, _vp, _vp, _vp]),
     "bsq_test_inject_status": (None, [_i, _u32]),
     "bsq_test_inject_lane_status": (None, [_vp, _i, _u32]),
     "bsq_test_limit_waits": (None, [_u32]),

@@ -6,6 +6,7 @@
 #include "bsq_fp4.hpp"
 #include "bsq_grad_norm.hpp"
 #include "bsq_internal.hpp"
+#include "bsq_xent.hpp"
 
 using namespace bsq;
 
@@ -229,6 +230,44 @@ int bsq_grad_norm_clip(const void *const *d_grads, const uint64_t *counts, const
     } catch (...) {
         return 1;
     }
+}
+
+// ---- loss over a vocabulary ----
+static inline bool xent_call(XentCall *c, int type, const void *d_x, uint64_t tokens, uint64_t cols, uint64_t ld_x, const void *d_w, uint64_t vocab, uint64_t ld_w,
+                             const int64_t *d_target, int64_t ignore, double smoothing, int reduction) {
+    if ((type != kF16 && type != kBf16) || cols < 1 || cols > kXentMaxCols || vocab < 1 || vocab > kFp4MaxDim || tokens > xent_max_tokens(type)) return false;
+    if ((tokens && !op_rows_ok(d_x, type, tokens, cols, ld_x)) || !op_rows_ok(d_w, type, vocab, cols, ld_w)) return false;
+    if (!(smoothing >= 0.0 && smoothing <= 1.0) || reduction < kXentNone || reduction > kXentMean) return false;
+    *c = {type, d_x, d_w, tokens, cols, vocab, tokens > 1 ? ld_x : cols, vocab > 1 ? ld_w : cols, reinterpret_cast<const long long *>(d_target), ignore, smoothing, reduction};
+    return true;
+}
+static inline bool on_bytes(const void *p, unsigned n) { return p && reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+size_t bsq_linear_xent_scratch_bytes(int type, const void *d_x, uint64_t tokens, uint64_t cols, uint64_t ld_x, const void *d_w, uint64_t vocab, uint64_t ld_w, double smoothing) {
+    XentCall c;
+    return xent_call(&c, type, d_x, tokens, cols, ld_x, d_w, vocab, ld_w, nullptr, 0, smoothing, kXentNone) ? xent_scratch_bytes(c, device_sm_count()) : 0;
+}
+int bsq_linear_xent(int type, const void *d_x, uint64_t tokens, uint64_t cols, uint64_t ld_x, const void *d_w, uint64_t vocab, uint64_t ld_w, const int64_t *d_target,
+                    int64_t ignore, double smoothing, int reduction, float *d_loss, float *d_stats, void *d_scratch, uint32_t *d_status, void *stream) {
+    XentCall c;
+    if (!xent_call(&c, type, d_x, tokens, cols, ld_x, d_w, vocab, ld_w, d_target, ignore, smoothing, reduction) || !on_bytes(d_stats, 4)) return 1;
+    if ((tokens || reduction != kXentNone) && !on_bytes(d_loss, 4)) return 1;
+    if (tokens && (!on_bytes(d_target, 8) || !on_bytes(d_scratch, 128))) return 1;
+    return rc(xent_loss(c, d_loss, d_stats, d_scratch, d_status, device_sm_count(), as_stream(stream)));
+}
+size_t bsq_linear_xent_grad_scratch_bytes(int type, const void *d_x, uint64_t tokens, uint64_t cols, uint64_t ld_x, const void *d_w, uint64_t vocab, uint64_t ld_w, int with_dx) {
+    XentCall c;
+    return xent_call(&c, type, d_x, tokens, cols, ld_x, d_w, vocab, ld_w, nullptr, 0, 0.0, kXentNone) ? xent_grad_scratch_bytes(c, with_dx != 0, device_sm_count()) : 0;
+}
+int bsq_linear_xent_grad(int type, const void *d_x, uint64_t tokens, uint64_t cols, uint64_t ld_x, const void *d_w, uint64_t vocab, uint64_t ld_w, const int64_t *d_target,
+                         int64_t ignore, double smoothing, int reduction, const float *d_stats, const float *d_grad, void *d_dx, uint64_t ld_dx, void *d_dw, uint64_t ld_dw,
+                         void *d_scratch, uint32_t *d_status, void *stream) {
+    XentCall c;
+    if (!xent_call(&c, type, d_x, tokens, cols, ld_x, d_w, vocab, ld_w, d_target, ignore, smoothing, reduction)) return 1;
+    if ((tokens && d_dx && !op_rows_ok(d_dx, type, tokens, cols, ld_dx)) || (d_dw && !op_rows_ok(d_dw, type, vocab, cols, ld_dw))) return 1;
+    if (tokens && (!on_bytes(d_target, 8) || !on_bytes(d_scratch, 128) || !on_bytes(d_stats, 4) || !on_bytes(d_grad, 4))) return 1;
+    if (!d_dx && !d_dw) return 0;
+    return rc(xent_grad(c, d_stats, d_grad, d_dx, tokens > 1 ? ld_dx : cols, d_dw, vocab > 1 ? ld_dw : cols, d_scratch, d_status, device_sm_count(), as_stream(stream)));
 }
 
 void bsq_test_limit_waits(uint32_t tries) { limit_epilogue_tries(tries); }

@@ -1,0 +1,589 @@
+// Softmax cross entropy of l = x W^T (x: tokens x cols, W: vocab x cols, FP16 or BF16) and its gradient, without keeping l:
+//   loss_t = lse_t - (1 - e) l_t,target - e / vocab sum_v l_tv,   lse_t = log sum_v exp l_tv
+//   dl_tv = g_t (exp(l_tv - lse_t) - (1 - e) [v = target] - e / vocab),   dx = dl W,   dW = dl^T x
+//
+// Loss: one product whose epilogue leaves, for each token and tile of 256 (128) of the vocabulary, the largest logit and the sum of exponentials against it, and the target's
+// logit; xent_join_kernel joins a token's tiles.  Nothing of size tokens x vocab is written.
+// Gradient: the vocabulary goes by in pieces of at most 128 MB of dl.  Of a piece the logits are computed again, the epilogue turns them into dl in 16 bits (the
+// rounding that a 16-bit gradient of logits has anyway: 1.7e-3 of each element, independent of one another; FP16 is scaled by a power of two so that g's smallness does not cost bits), then
+// dW of the piece is complete, and dx is summed over the pieces in FP32.
+//
+// Exponents are taken in base 2, and the reference of a tile is the rounded product of its largest logit and log2(e), so that the rounding cancels.
+#include "bsq_gemm16.cuh"
+#include "bsq_internal.hpp"
+#include "bsq_xent.hpp"
+
+namespace bsq {
+namespace {
+
+constexpr float kLog2E = 1.4426950408889634f;
+constexpr double kLn2 = 0.69314718055994530942;
+constexpr uint64_t kPieceBytes = 128ull << 20;
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// ---- loss ----
+struct XentStats {
+    int M, N;
+    const long long *target;
+    float2 *parts;                   // tiles along N x M: (largest logit) * log2 e, sum of exponentials against it
+    float *sums;                     // the same: sum of logits (nullable: no smoothing)
+    float *at_target;                // M
+
+    template <int COLS> __device__ void tile(const TileOut &o) const {
+        const int row = o.row + o.lane, n = min(COLS, N - o.col);
+        float top = __uint_as_float(0xff800000u), s = 0.0f, total = 0.0f;
+        for (int c = 0; c < n; c += 32) {
+            float v[32];
+            read32f(o.taddr + (unsigned)c, v, o.ok);
+            if (sums) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) total += c + j < n ? v[j] : 0.0f;
+            }
+            if (c + 32 > n) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                    if (c + j >= n) v[j] = __uint_as_float(0xff800000u);
+            }
+            float m = v[0];
+#pragma unroll
+            for (int j = 1; j < 32; ++j) m = fmaxf(m, v[j]);
+            m *= kLog2E;
+            if (m > top) {
+                s *= exp2_fast(top - m);
+                top = m;
+            }
+#pragma unroll
+            for (int j = 0; j < 32; ++j) s += exp2_fast(fmaf(v[j], kLog2E, -top));
+        }
+        const long long off = row < M ? target[row] - o.col : -1;
+        const bool here = off >= 0 && off < n;
+        float mine = 0.0f;
+        for (unsigned left = __ballot_sync(kFullMask, here); left; left &= left - 1) {
+            const int src = __ffs(left) - 1;
+            const float l = read_column(o.taddr + (unsigned)__shfl_sync(kFullMask, (int)off, src), o.ok);
+            if (o.lane == src) mine = l;
+        }
+        if (row >= M) return;
+        const size_t at = (size_t)(o.col / COLS) * (size_t)M + (size_t)row;
+        parts[at] = make_float2(top, s);
+        if (sums) sums[at] = total;
+        if (here) at_target[row] = mine;
+    }
+};
+
+struct XentJoin {
+    int tokens, tiles;
+    long long vocab, ignore;
+    double smoothing;
+    int reduction;
+    const long long *target;
+    const float2 *parts;
+    const float *sums, *at_target;
+    float *loss, *stats;             // stats: log2 of the sum of exponentials of each token, then the number of tokens that count
+    double2 *blocks;                 // loss and tokens of each CTA
+};
+
+// The sum over a CTA's threads, the same order every time
+__device__ __forceinline__ double2 cta_sum(double2 v, double2 *room) {
+    for (int d = 16; d; d >>= 1) {
+        v.x += __shfl_xor_sync(kFullMask, v.x, d);
+        v.y += __shfl_xor_sync(kFullMask, v.y, d);
+    }
+    if ((threadIdx.x & 31) == 0) room[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = room[0];
+    for (int i = 1; i < (int)blockDim.x / 32; ++i) {
+        v.x += room[i].x;
+        v.y += room[i].y;
+    }
+    return v;
+}
+__device__ __forceinline__ void write_total(const XentJoin &j, double2 v) {
+    j.stats[j.tokens] = (float)v.y;
+    if (j.reduction == kXentSum) *j.loss = (float)v.x;
+    else if (j.reduction == kXentMean) *j.loss = (float)(v.x / v.y);
+}
+
+// 32 tokens a CTA, one for each lane; the warps share the tiles
+__global__ void __launch_bounds__(1024) xent_join_kernel(const XentJoin j) {
+    chain_begin();
+    __shared__ float2 part[32][32];
+    __shared__ float part_sum[32][32];
+    __shared__ double2 room[32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, token = (int)blockIdx.x * 32 + lane;
+    float top = __uint_as_float(0xff800000u), s = 0.0f, total = 0.0f;
+    if (token < j.tokens) {
+#pragma unroll 4
+        for (int t = warp; t < j.tiles; t += 32) {
+            const float2 p = j.parts[(size_t)t * (size_t)j.tokens + (size_t)token];
+            const float m = fmaxf(top, p.x);
+            if (m > __uint_as_float(0xff800000u)) s = s * exp2_fast(top - m) + p.y * exp2_fast(p.x - m);
+            else s += p.y;                                       // (NaN)
+            top = m;
+            if (j.sums) total += j.sums[(size_t)t * (size_t)j.tokens + (size_t)token];
+        }
+    }
+    part[warp][lane] = make_float2(top, s);
+    part_sum[warp][lane] = total;
+    __syncthreads();
+    double2 mine = make_double2(0.0, 0.0);
+    if (warp == 0 && token < j.tokens) {
+        double sum = 0.0, all = 0.0;
+        for (int i = 0; i < 32; ++i) top = fmaxf(top, part[i][lane].x);
+        for (int i = 0; i < 32; ++i) {
+            const float2 p = part[i][lane];
+            // (a warp without a tile has nothing against -Inf)
+            if (i < j.tiles) sum += p.x == top ? (double)p.y : (double)(p.y * exp2_fast(p.x - top));
+            all += (double)part_sum[i][lane];
+        }
+        const double lse2 = (double)top + log2(sum);
+        const long long t = j.target[token];
+        const bool live = t != j.ignore, bad = live && (t < 0 || t >= j.vocab);
+        double loss = lse2 * kLn2 - (1.0 - j.smoothing) * (bad ? 0.0 : live ? (double)j.at_target[token] : 0.0);
+        if (j.sums) loss -= j.smoothing / (double)j.vocab * all;
+        if (bad) loss = __longlong_as_double(0x7ff8000000000000ll);
+        if (!live) loss = 0.0;
+        j.stats[token] = (float)lse2;
+        if (j.reduction == kXentNone) j.loss[token] = (float)loss;
+        mine = make_double2(loss, live ? 1.0 : 0.0);
+    }
+    __syncthreads();
+    const double2 v = cta_sum(mine, room);
+    if (threadIdx.x == 0) {
+        if (gridDim.x == 1) write_total(j, v);
+        else j.blocks[blockIdx.x] = v;
+    }
+}
+__global__ void __launch_bounds__(1024) xent_total_kernel(const XentJoin j, int blocks) {
+    chain_begin();
+    __shared__ double2 room[32];
+    double2 v = make_double2(0.0, 0.0);
+    for (int i = threadIdx.x; i < blocks; i += 1024) {
+        v.x += j.blocks[i].x;
+        v.y += j.blocks[i].y;
+    }
+    v = cta_sum(v, room);
+    if (threadIdx.x == 0) write_total(j, v);
+}
+
+// ---- gradient ----
+struct XentCoef {
+    int tokens;
+    long long vocab, ignore;
+    int reduction;
+    bool f16;
+    const long long *target;
+    const float *stats, *grad;
+    float *coef, *unscale;           // coefficient of each token; what the products are multiplied by
+};
+// What each token's gradient of logits is multiplied by: g_t, 0 for those that do not count, NaN for a target that is none; times a power of two that brings the
+// largest into [2^13, 2^14) where dl is FP16 (|dl| is at most that).  One CTA.
+__global__ void __launch_bounds__(1024) xent_coef_kernel(const XentCoef c) {
+    chain_begin();
+    __shared__ float room[32];
+    const float one = c.reduction == kXentNone ? 0.0f : c.reduction == kXentMean ? *c.grad / c.stats[c.tokens] : *c.grad;
+    float scale = 1.0f, back = 1.0f;
+    if (c.f16) {
+        float m = fabsf(one);
+        if (c.reduction == kXentNone) {
+            for (int i = threadIdx.x; i < c.tokens; i += 1024) {
+                const float a = fabsf(c.grad[i]);
+                if (c.target[i] != c.ignore && a < __uint_as_float(0x7f800000u)) m = fmaxf(m, a);
+            }
+            m = warp_max(m);
+            if ((threadIdx.x & 31) == 0) room[threadIdx.x >> 5] = m;
+            __syncthreads();
+            m = warp_max(room[threadIdx.x & 31]);
+        }
+        if (m > 0.0f && m < __uint_as_float(0x7f800000u)) {
+            const int e = min(max(13 - ilogbf(m), -100), 100);
+            scale = exp2f((float)e);
+            back = exp2f((float)-e);
+        }
+    }
+    if (threadIdx.x == 0) *c.unscale = back;
+    for (int i = threadIdx.x; i < c.tokens; i += 1024) {
+        const long long t = c.target[i];
+        float g = (c.reduction == kXentNone ? c.grad[i] : one) * scale;
+        if (t < 0 || t >= c.vocab) g = __uint_as_float(0x7fffffffu);
+        c.coef[i] = t == c.ignore ? 0.0f : g;
+    }
+}
+
+template <int TYPE> struct XentGrad {
+    CUtensorMap map;                 // the piece: tokens x its columns
+    int M, N;                        // N: columns of the vocabulary in the piece; the piece's others are 0
+    long long first;                 // of the vocabulary
+    long long ignore;
+    const long long *target;
+    const float *lse2, *coef;
+    float low, high;                 // e / vocab, 1 - e
+
+    template <int COLS> __device__ void tile(const TileOut &o) const {
+        const int row = o.row + o.lane;
+        const long long t = row < M ? target[row] : ignore;
+        const bool live = t != ignore;
+        const long long off = live ? t - first - o.col : -1;
+        const float lse = row < M ? lse2[row] : 0.0f, g = row < M ? coef[row] : 0.0f;
+        for (int c = 0; c < COLS; c += 64) {
+            unsigned char *box = box_next(o);
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+                float v[16];
+                read16f(o.taddr + (unsigned)(c + 16 * h), v, o.ok);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) v[j] = g * (exp2_fast(fmaf(v[j], kLog2E, -lse)) - low);
+                // (chosen, not multiplied: what an ignored token's logits are does not matter)
+                if (!live) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) v[j] = 0.0f;
+                }
+                if (o.col + c + 16 * h + 16 > N) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j)
+                        if (o.col + c + 16 * h + j >= N) v[j] = 0.0f;
+                }
+                box_put16<TYPE>(box, o.lane, h, v);
+            }
+            const bool here = off >= c && off < c + 64 && off < COLS;
+            for (unsigned left = __ballot_sync(kFullMask, here); left; left &= left - 1) {
+                const int src = __ffs(left) - 1, col = __shfl_sync(kFullMask, (int)off, src);
+                const float l = read_column(o.taddr + (unsigned)col, o.ok);
+                if (o.lane == src)
+                    store_elem<TYPE>(box + o.lane * 128 + (((((col - c) >> 3) ^ (o.lane & 7)) << 4)), (uint64_t)(col & 7), g * ((exp2_fast(fmaf(l, kLog2E, -lse)) - low) - high));
+            }
+            box_send(o, &map, o.col + c, o.row, box);
+        }
+    }
+};
+
+// A product's tiles out of tensor memory: to 16-bit rows, or into FP32 sums over several launches
+enum ProductMode : int { kProductOut = 0, kSumFirst = 1, kSumMore = 2, kSumOut = 3 };
+template <int TYPE> struct ProductOut {
+    CUtensorMap map, map_sum;
+    int M, N, mode;
+    bool boxes;                      // the result can be written by TMA
+    void *out;
+    long ld;
+    const float *sum;
+    long ld_sum;
+    const float *factor;
+
+    template <int COLS> __device__ void tile(const TileOut &o) const {
+        if (mode == kSumFirst || mode == kSumMore) {
+            for (int c = 0; c < COLS && o.col + c < N; c += 32) {
+                unsigned char *box = box_next(o);
+                uint4 *line = reinterpret_cast<uint4 *>(box + o.lane * 128);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    unsigned r[16];
+                    read16(o.taddr + (unsigned)(c + 16 * h), r, o.ok);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) line[(4 * h + j) ^ (o.lane & 7)] = make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+                }
+                box_send(o, &map_sum, o.col + c, o.row, box, mode == kSumMore);
+            }
+            return;
+        }
+        const float f = *factor;
+        const int row = o.row + o.lane;
+        for (int c = 0; c < COLS && o.col + c < N; c += 64) {
+            unsigned char *box = box_next(o);
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+                float v[16];
+                read16f(o.taddr + (unsigned)(c + 16 * h), v, o.ok);
+                if (mode == kSumOut && row < M && o.col + c + 16 * h < N) {
+                    // (rows of the sums are padded to a multiple of 16)
+                    const float4 *s = reinterpret_cast<const float4 *>(sum + (size_t)row * (size_t)ld_sum + (size_t)(o.col + c + 16 * h));
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float4 a = s[j];
+                        v[4 * j] += a.x; v[4 * j + 1] += a.y; v[4 * j + 2] += a.z; v[4 * j + 3] += a.w;
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 16; ++j) v[j] *= f;
+                box_put16<TYPE>(box, o.lane, h, v);
+            }
+            if (boxes) box_send(o, &map, o.col + c, o.row, box);
+            else box_out(box, o.lane, out, 2, (long)o.row * ld + o.col + c, ld, M - o.row, N - o.col - c);
+        }
+    }
+};
+
+// The slices of a product that was split along K, added up in their order
+template <int TYPE>
+__global__ void __launch_bounds__(256) sum_slices_kernel(const float *sum, int slices, int rows, int cols, long ld_sum, const float *factor, void *out, long ld) {
+    chain_begin();
+    const float f = *factor;
+    const long all = (long)rows * cols;
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < all; i += (long)gridDim.x * 256) {
+        const long r = i / cols, c = i - r * cols;
+        float v = 0.0f;
+#pragma unroll 4
+        for (int s = 0; s < slices; ++s) v += sum[((size_t)s * (size_t)rows + (size_t)r) * (size_t)ld_sum + (size_t)c];
+        store_elem<TYPE>(out, (uint64_t)(r * ld + c), v * f);
+    }
+}
+
+// Rows whose start or distance TMA cannot take, copied to rows on 16 bytes.  A thread writes 16 bytes.
+__global__ void __launch_bounds__(256) align_rows_kernel(const unsigned short *in, uint64_t rows, uint64_t cols, uint64_t ld, unsigned short *out, uint64_t ld_out) {
+    chain_begin();
+    const uint64_t per = ld_out / 8, all = rows * per;
+    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (uint64_t)gridDim.x * 256) {
+        const uint64_t r = i / per, c = (i - r * per) * 8;
+        const unsigned short *p = in + r * ld + c;
+        unsigned w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const unsigned lo = c + 2 * j < cols ? p[2 * j] : 0u, hi = c + 2 * j + 1 < cols ? p[2 * j + 1] : 0u;
+            w[j] = lo | hi << 16;
+        }
+        *reinterpret_cast<uint4 *>(out + r * ld_out + c) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
+// ---- host ----
+uint64_t padded(uint64_t n, uint64_t to) { return (n + to - 1) / to * to; }
+bool needs_copy(const void *p, uint64_t rows, uint64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 != 0 || (rows > 1 && ld % 8 != 0); }
+
+// Scratch, handed out piece by piece on 128 bytes
+struct Scratch {
+    unsigned char *base;
+    size_t used = 0;
+    template <class T> T *take(uint64_t count) {
+        T *p = reinterpret_cast<T *>(base + used);
+        used += padded(count * sizeof(T), 128);
+        return p;
+    }
+};
+
+struct Operands {
+    Stack x, w;
+};
+// x and W as the products read them, copied where need be
+Operands aligned_operands(const XentCall &c, Scratch *s, bool run, cudaError_t *err, int sm_count, cudaStream_t stream) {
+    Operands o = {{c.x, c.cols, c.tokens, c.ld_x, 1, 0}, {c.w, c.cols, c.vocab, c.ld_w, 1, 0}};
+    for (Stack *m : {&o.x, &o.w}) {
+        if (!needs_copy(m->at, m->rows, m->ld)) continue;
+        const uint64_t ld = padded(m->cols, 8);
+        unsigned short *to = s->take<unsigned short>(m->rows * ld);
+        if (run && *err == cudaSuccess) {
+            const uint64_t blocks = (m->rows * (ld / 8) + 255) / 256;
+            *err = launch_chained(align_rows_kernel, (unsigned)std::min<uint64_t>(blocks, (uint64_t)sm_count * 16), 256, 0, stream, static_cast<const unsigned short *>(m->at), m->rows,
+                                  m->cols, m->ld, to, ld);
+        }
+        m->at = to;
+        m->ld = ld;
+    }
+    return o;
+}
+
+struct LossPlan {
+    bool pairs;
+    uint64_t tiles;
+};
+LossPlan loss_plan(const XentCall &c, int sm_count) {
+    LossPlan p;
+    p.pairs = g16_pairs(c.tokens, c.vocab, 1, false, sm_count);
+    p.tiles = p.pairs ? (c.vocab + 255) / 256 : (c.vocab + 127) / 128;
+    return p;
+}
+struct LossRoom {
+    float2 *parts;
+    float *sums, *at_target;
+    double2 *blocks;
+};
+LossRoom loss_room(const XentCall &c, const LossPlan &p, Scratch *s) {
+    LossRoom r;
+    r.parts = s->take<float2>(p.tiles * c.tokens);
+    r.sums = c.smoothing > 0.0 ? s->take<float>(p.tiles * c.tokens) : nullptr;
+    r.at_target = s->take<float>(c.tokens);
+    r.blocks = s->take<double2>((c.tokens + 31) / 32);
+    return r;
+}
+
+struct GradPlan {
+    uint64_t piece, pieces;          // columns of the vocabulary at a time
+    bool pairs_l, pairs_w, pairs_x;
+    int splits;                      // of dx along the vocabulary
+    uint64_t ld_sum;
+};
+GradPlan grad_plan(const XentCall &c, bool dx, int sm_count) {
+    GradPlan p;
+    const uint64_t whole = padded(c.vocab, 256), most = std::min<uint64_t>(65536, std::max<uint64_t>(1024, kPieceBytes / 2 / c.tokens / 256 * 256));
+    p.pieces = (whole + most - 1) / most;
+    p.piece = padded((whole + p.pieces - 1) / p.pieces, 256);
+    p.pieces = (whole + p.piece - 1) / p.piece;
+    p.pairs_l = g16_pairs(c.tokens, p.piece, 1, false, sm_count);
+    p.pairs_w = g16_pairs(p.piece, c.cols, 1, false, sm_count);
+    p.pairs_x = g16_pairs(c.tokens, c.cols, 1, false, sm_count);
+    p.splits = 1;
+    const uint64_t tiles = ((c.tokens + 127) / 128) * ((c.cols + 127) / 128), stages = p.piece / kG16K;
+    // few tiles: slices of the vocabulary, as many as SMs take at a time, of four stages at least
+    if (dx && !p.pairs_x)
+        while (p.splits < 64 && tiles * (uint64_t)p.splits * 2 <= (uint64_t)sm_count && stages >= (uint64_t)p.splits * 8) p.splits *= 2;
+    p.ld_sum = padded(c.cols, 16);
+    return p;
+}
+struct GradRoom {
+    float *coef, *unscale, *sum;
+    unsigned short *piece;
+};
+GradRoom grad_room(const XentCall &c, const GradPlan &p, bool dx, Scratch *s) {
+    GradRoom r;
+    r.coef = s->take<float>(c.tokens);
+    r.unscale = s->take<float>(1);
+    r.piece = s->take<unsigned short>(c.tokens * p.piece);
+    r.sum = dx && (p.pieces > 1 || p.splits > 1) ? s->take<float>((uint64_t)p.splits * c.tokens * p.ld_sum) : nullptr;
+    return r;
+}
+
+Gemm16 product_of(uint64_t M, uint64_t N, bool a_kmajor, bool b_kmajor, bool bf16, int splits = 1) {
+    Gemm16 g = {};
+    g.M = (int)M;
+    g.N = (int)N;
+    g.batch = 1;
+    g.parts = 1;
+    g.splits = splits;
+    g.a_kmajor = a_kmajor;
+    g.b_kmajor = b_kmajor;
+    g.bf16 = bf16;
+    return g;
+}
+
+// out (or sums): M x N = A B^T
+template <int TYPE>
+cudaError_t product(const Stack &a, bool a_kmajor, const Stack &b, bool b_kmajor, uint64_t M, uint64_t N, uint64_t K, bool pairs, int splits, int mode, void *out, uint64_t ld,
+                    float *sum, uint64_t ld_sum, const float *factor, unsigned *status, int sm_count, cudaStream_t stream) {
+    Gemm16Maps maps;
+    ProductOut<TYPE> e;
+    if (!map_operand(&maps.a[0], a, TYPE == kBf16, a_kmajor) || !map_operand(&maps.b[0], b, TYPE == kBf16, b_kmajor)) return cudaErrorInvalidValue;
+    maps.a[1] = maps.a[0];
+    maps.b[1] = maps.b[0];
+    e.map = e.map_sum = maps.a[0];
+    e.M = (int)M;
+    e.N = (int)N;
+    e.mode = mode;
+    e.out = out;
+    e.ld = (long)ld;
+    e.sum = sum;
+    e.ld_sum = (long)ld_sum;
+    e.factor = factor;
+    e.boxes = out && tma_can_write(out, (M == 1 ? N : ld) * 2, N * 2);
+    if (e.boxes && !map_stack(&e.map, {out, N, M, ld, 1, 0}, TYPE, 64, 32)) return cudaErrorInvalidValue;
+    if (sum && !map_stack(&e.map_sum, {sum, ld_sum, M, ld_sum, (uint64_t)splits, M * ld_sum}, kF32, 32, 32)) return cudaErrorInvalidValue;
+    return launch_gemm16(maps, e, product_of(M, N, a_kmajor, b_kmajor, TYPE == kBf16, splits), K, pairs, status, sm_count, stream);
+}
+
+template <int TYPE>
+cudaError_t grad_pieces(const XentCall &c, const GradPlan &p, const GradRoom &r, const Operands &o, const float *stats, void *dx, uint64_t ld_dx, void *dw, uint64_t ld_dw,
+                        unsigned *status, int sm_count, cudaStream_t stream) {
+    cudaError_t err = cudaSuccess;
+    for (uint64_t i = 0; i < p.pieces && err == cudaSuccess; ++i) {
+        const uint64_t first = i * p.piece, n = std::min(p.piece, c.vocab - first);
+        const Stack w = {static_cast<const unsigned short *>(o.w.at) + first * o.w.ld, c.cols, n, o.w.ld, 1, 0};
+        const Stack dl = {r.piece, p.piece, c.tokens, p.piece, 1, 0}, dl_valid = {r.piece, n, c.tokens, p.piece, 1, 0};
+        Gemm16Maps maps;
+        XentGrad<TYPE> e;
+        if (!map_operand(&maps.a[0], o.x, TYPE == kBf16, true) || !map_operand(&maps.b[0], w, TYPE == kBf16, true) || !map_stack(&e.map, dl, TYPE, 64, 32)) return cudaErrorInvalidValue;
+        maps.a[1] = maps.a[0];
+        maps.b[1] = maps.b[0];
+        e.M = (int)c.tokens;
+        e.N = (int)n;
+        e.first = (long long)first;
+        e.ignore = c.ignore;
+        e.target = c.target;
+        e.lse2 = stats;
+        e.coef = r.coef;
+        e.low = (float)(c.smoothing / (double)c.vocab);
+        e.high = (float)(1.0 - c.smoothing);
+        err = launch_gemm16(maps, e, product_of(c.tokens, n, true, true, TYPE == kBf16), c.cols, p.pairs_l, status, sm_count, stream);
+        if (err != cudaSuccess) return err;
+        if (dw)
+            err = product<TYPE>(dl_valid, false, o.x, false, n, c.cols, c.tokens, p.pairs_w, 1, kProductOut, static_cast<unsigned short *>(dw) + first * ld_dw, ld_dw, nullptr, 0,
+                                r.unscale, status, sm_count, stream);
+        if (err != cudaSuccess) return err;
+        if (dx) {
+            const bool last = i + 1 == p.pieces;
+            const int mode = !r.sum ? kProductOut : p.splits == 1 && last ? kSumOut : i == 0 ? kSumFirst : kSumMore;
+            err = product<TYPE>(dl_valid, true, w, false, c.tokens, c.cols, n, p.pairs_x, p.splits, mode, dx, ld_dx, r.sum, p.ld_sum, r.unscale, status, sm_count, stream);
+        }
+    }
+    if (err == cudaSuccess && dx && p.splits > 1) {
+        const uint64_t blocks = (c.tokens * c.cols + 255) / 256;
+        err = launch_chained(sum_slices_kernel<TYPE>, (unsigned)std::min<uint64_t>(blocks, (uint64_t)sm_count * 8), 256, 0, stream, (const float *)r.sum, p.splits, (int)c.tokens, (int)c.cols,
+                             (long)p.ld_sum, (const float *)r.unscale, dx, (long)ld_dx);
+    }
+    return err;
+}
+
+}  // namespace
+
+size_t xent_scratch_bytes(const XentCall &c, int sm_count) {
+    if (c.tokens == 0) return 0;
+    Scratch s = {nullptr};
+    cudaError_t err = cudaSuccess;
+    aligned_operands(c, &s, false, &err, sm_count, nullptr);
+    loss_room(c, loss_plan(c, sm_count), &s);
+    return s.used;
+}
+
+size_t xent_grad_scratch_bytes(const XentCall &c, bool dx, int sm_count) {
+    if (c.tokens == 0) return 0;
+    Scratch s = {nullptr};
+    cudaError_t err = cudaSuccess;
+    aligned_operands(c, &s, false, &err, sm_count, nullptr);
+    grad_room(c, grad_plan(c, dx, sm_count), dx, &s);
+    return s.used;
+}
+
+cudaError_t xent_loss(const XentCall &c, float *loss, float *stats, void *scratch, unsigned *status, int sm_count, cudaStream_t stream) {
+    Scratch s = {static_cast<unsigned char *>(scratch)};
+    cudaError_t err = cudaSuccess;
+    if (c.tokens == 0) {                                         // nothing, 0 or 0 / 0
+        const XentJoin none = {0, 0, (long long)c.vocab, c.ignore, c.smoothing, c.reduction, nullptr, nullptr, nullptr, nullptr, loss, stats, nullptr};
+        return launch_chained(xent_total_kernel, 1, 1024, 0, stream, none, 0);
+    }
+    const Operands o = aligned_operands(c, &s, true, &err, sm_count, stream);
+    if (err != cudaSuccess) return err;
+    const LossPlan p = loss_plan(c, sm_count);
+    const LossRoom r = loss_room(c, p, &s);
+    Gemm16Maps maps;
+    const bool bf16 = c.type == kBf16;
+    if (!map_operand(&maps.a[0], o.x, bf16, true) || !map_operand(&maps.b[0], o.w, bf16, true)) return cudaErrorInvalidValue;
+    maps.a[1] = maps.a[0];
+    maps.b[1] = maps.b[0];
+    const XentStats e = {(int)c.tokens, (int)c.vocab, c.target, r.parts, r.sums, r.at_target};
+    err = launch_gemm16(maps, e, product_of(c.tokens, c.vocab, true, true, bf16), c.cols, p.pairs, status, sm_count, stream);
+    if (err != cudaSuccess) return err;
+    const XentJoin j = {(int)c.tokens, (int)p.tiles, (long long)c.vocab, c.ignore, c.smoothing, c.reduction, c.target, r.parts, r.sums, r.at_target, loss, stats, r.blocks};
+    const unsigned blocks = (unsigned)((c.tokens + 31) / 32);
+    err = launch_chained(xent_join_kernel, blocks, 1024, 0, stream, j);
+    if (err == cudaSuccess && blocks > 1) err = launch_chained(xent_total_kernel, 1, 1024, 0, stream, j, (int)blocks);
+    return err;
+}
+
+cudaError_t xent_grad(const XentCall &c, const float *stats, const float *grad, void *dx, uint64_t ld_dx, void *dw, uint64_t ld_dw, void *scratch, unsigned *status,
+                      int sm_count, cudaStream_t stream) {
+    Scratch s = {static_cast<unsigned char *>(scratch)};
+    cudaError_t err = cudaSuccess;
+    if (c.tokens == 0) return dw ? cudaMemset2DAsync(dw, ld_dw * 2, 0, c.cols * 2, c.vocab, stream) : cudaSuccess;
+    const Operands o = aligned_operands(c, &s, true, &err, sm_count, stream);
+    if (err != cudaSuccess) return err;
+    const GradPlan p = grad_plan(c, dx != nullptr, sm_count);
+    const GradRoom r = grad_room(c, p, dx != nullptr, &s);
+    const XentCoef k = {(int)c.tokens, (long long)c.vocab, c.ignore, c.reduction, c.type == kF16, c.target, stats, grad, r.coef, r.unscale};
+    err = launch_chained(xent_coef_kernel, 1, 1024, 0, stream, k);
+    if (err != cudaSuccess) return err;
+    return c.type == kBf16 ? grad_pieces<kBf16>(c, p, r, o, stats, dx, ld_dx, dw, ld_dw, status, sm_count, stream)
+                           : grad_pieces<kF16>(c, p, r, o, stats, dx, ld_dx, dw, ld_dw, status, sm_count, stream);
+}
+
+}  // namespace bsq

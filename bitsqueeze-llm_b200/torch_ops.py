@@ -303,6 +303,75 @@ def fp4_linear(x, weight, format=NVFP4):
     return _Fp4Linear.apply(_laid_out(x), _laid_out(weight), None, format)
 
 
+_REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
+_XENT_COLS, _XENT_TOKENS = 65536, {torch.float16: 65536, torch.bfloat16: 524288}
+
+
+def _scratch(name, device, *args):
+    """The scratch that an entry wants for `args`."""
+    f = _entries.get(name) or _entry(name)
+    if _device() == device.index:
+        need = f(*args)
+    else:
+        with torch.cuda.device(device):
+            need = f(*args)
+    return torch.empty(need, dtype=torch.uint8, device=device)
+
+
+class _LinearCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, target, ignore_index, label_smoothing, reduction):
+        rows, cols, ld = _rows(x, "x") if x.numel() else (0, x.size(-1), x.size(-1))
+        vocab, _, ld_w = _rows(weight, "weight")
+        device, type = x.device, _TYPES[x.dtype]
+        operands = (type, x.data_ptr(), rows, cols, ld, weight.data_ptr(), vocab, ld_w)
+        loss = x.new_empty(target.shape if reduction == 0 else (), dtype=torch.float32)
+        stats = x.new_empty(rows + 1, dtype=torch.float32)
+        scratch = _scratch("bsq_linear_xent_scratch_bytes", device, *operands, label_smoothing)
+        _call("bsq_linear_xent", device.index, *operands, target.data_ptr(), ignore_index, label_smoothing, reduction, loss.data_ptr(), stats.data_ptr(), scratch.data_ptr(), None)
+        ctx.save_for_backward(x, weight, target, stats)
+        ctx.operands, ctx.how = operands, (ignore_index, label_smoothing, reduction)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        x, weight, target, stats = ctx.saved_tensors
+        device, (want_x, want_w) = x.device, ctx.needs_input_grad[:2]
+        grad = grad.contiguous()                             # (one value for all tokens where the losses were added up)
+        cols = x.size(-1)
+        dx = x.new_empty(x.shape) if want_x else None
+        dw = weight.new_empty(weight.shape) if want_w else None
+        scratch = _scratch("bsq_linear_xent_grad_scratch_bytes", device, *ctx.operands, 1 if want_x else 0)
+        _call("bsq_linear_xent_grad", device.index, *ctx.operands, target.data_ptr(), *ctx.how, stats.data_ptr(), grad.data_ptr(), None if dx is None else dx.data_ptr(), cols,
+              None if dw is None else dw.data_ptr(), cols, scratch.data_ptr(), None)
+        return dx, dw, None, None, None, None
+
+
+def linear_cross_entropy(x, weight, target, ignore_index=-100, label_smoothing=0.0, reduction="mean"):
+    """Softmax cross entropy of the logits x weight^T without keeping them, under autograd: x (float16 or bfloat16, (..., D)), weight (V, D) of the same type, target int64
+    of x's leading dimensions.  A token's loss is lse - (1 - e) * logit of its target - e * mean of its logits, e = label_smoothing, in float32; tokens whose target is
+    ignore_index have 0.  reduction "none": each token's (the log probability of a given token is its negative), "sum", or "mean" over the tokens that are not ignored (none of them:
+    NaN).  A target outside 0 .. V - 1 gives NaN for its token.  Logits are FP32 sums; the backward pass computes them again, rounds their gradient to the type of x and returns the gradients of x and
+    weight in it, rounded once.  Hidden states of ignored tokens get a gradient of 0; they are multiplied by 0 on the way to the weight's and have to be finite.
+    At most 65536 columns and 65536 (float16) or 524288 (bfloat16) tokens.  Tensors that do not lie as the rows of one matrix are copied first.  Autocast does not change what is
+    asked of x: pass it and the weight in 16 bits."""
+    if x.dtype not in _XENT_TOKENS or not x.is_cuda or x.dim() == 0 or x.size(-1) == 0:
+        raise ValueError("x must be a float16 or bfloat16 CUDA tensor with at least one column")
+    if weight.dim() != 2 or weight.dtype != x.dtype or weight.device != x.device or weight.size(1) != x.size(-1) or not weight.size(0):
+        raise ValueError("the weight must be a (V, D) tensor of x's type on x's device, D the last dimension of x")
+    if target.dtype != torch.int64 or target.device != x.device or target.shape != x.shape[:-1]:
+        raise ValueError("target must be an int64 tensor of x's leading dimensions on x's device")
+    if reduction not in _REDUCTIONS:
+        raise ValueError('reduction must be "none", "sum" or "mean"')
+    label_smoothing, ignore_index = float(label_smoothing), int(ignore_index)
+    if not 0.0 <= label_smoothing <= 1.0 or not -1 << 63 <= ignore_index < 1 << 63:
+        raise ValueError("label_smoothing must be within 0 and 1, ignore_index an int64")
+    if x.size(-1) > _XENT_COLS or target.numel() > _XENT_TOKENS[x.dtype]:
+        raise ValueError("at most %d columns and %d tokens: split the batch" % (_XENT_COLS, _XENT_TOKENS[x.dtype]))
+    return _LinearCrossEntropy.apply(_laid_out(x) if x.numel() else x, _laid_out(weight), target.contiguous(), ignore_index, label_smoothing, _REDUCTIONS[reduction])
+
+
 def _dense(t):
     """Whether a tensor's elements fill one run of memory, in whatever order."""
     if t.is_contiguous():

@@ -297,6 +297,24 @@ size_t bsq_grad_norm_scratch_bytes(void);
 int bsq_grad_norm_clip(const void *const *d_grads, const uint64_t *counts, const int *types, int n, void *const *d_outs, double max_norm, int norm_kind, float *d_norm,
                        void *d_scratch, void *stream);
 
+/* ---- loss over a vocabulary (no counterpart in the reference) ------------------------------------------------------------------------------
+ * Softmax cross entropy of the logits l = x W^T, x: tokens x cols, W: vocab x cols (type 1 FP16 or 2 BF16, rows ld apart), without keeping them:
+ *   loss_t = lse_t - (1 - smoothing) l_t,target - smoothing / vocab * sum of l_t,   lse_t = log of the sum of exp(l_t)
+ * for tokens whose target is not `ignore`; those are 0.  A target outside 0 .. vocab - 1 makes its token's loss NaN.  reduction: 0 d_loss[t] = loss_t, 1 d_loss[0] = their sum,
+ * 2 the sum over the number of tokens that are not ignored (none: NaN).  d_stats: tokens + 1 floats that the gradient wants.  Sums are FP32 (of one token) and FP64 (of many).
+ * Gradient: with d_grad the gradient of d_loss (one float, or one for each token), d_dx (tokens x cols) and d_dw (vocab x cols), either nullable, in the type of x:
+ *   dx = dl W,  dW = dl^T x,  dl_tv = g_t (exp(l_tv - lse_t) - (1 - smoothing) [v = target] - smoothing / vocab)
+ * dl is rounded to the operands' type, sums are FP32, results rounded once.  Ignored tokens have a dx of 0; their x is multiplied by 0 for dW and has to be finite.
+ * At most 65536 columns, and 65536 (FP16) or 524288 (BF16) tokens.  Calls enqueue on `stream` and return; they allocate nothing, keep nothing and may be captured.  d_scratch: as many bytes as the
+ * function beside it says for the same arguments (pointers and strides included), on a 128-byte boundary.  d_status as for bsq_fp4_matmul. */
+size_t bsq_linear_xent_scratch_bytes(int type, const void *d_x, uint64_t tokens, uint64_t cols, uint64_t ld_x, const void *d_w, uint64_t vocab, uint64_t ld_w, double smoothing);
+int bsq_linear_xent(int type, const void *d_x, uint64_t tokens, uint64_t cols, uint64_t ld_x, const void *d_w, uint64_t vocab, uint64_t ld_w, const int64_t *d_target,
+                    int64_t ignore, double smoothing, int reduction, float *d_loss, float *d_stats, void *d_scratch, uint32_t *d_status, void *stream);
+size_t bsq_linear_xent_grad_scratch_bytes(int type, const void *d_x, uint64_t tokens, uint64_t cols, uint64_t ld_x, const void *d_w, uint64_t vocab, uint64_t ld_w, int with_dx);
+int bsq_linear_xent_grad(int type, const void *d_x, uint64_t tokens, uint64_t cols, uint64_t ld_x, const void *d_w, uint64_t vocab, uint64_t ld_w, const int64_t *d_target,
+                         int64_t ignore, double smoothing, int reduction, const float *d_stats, const float *d_grad, void *d_dx, uint64_t ld_dx, void *d_dw, uint64_t ld_dw,
+                         void *d_scratch, uint32_t *d_status, void *stream);
+
 /* Test hook (no counterpart in the reference): the next bsq_compress (which = 0) or bsq_decompress (which = 1) on the
  * current device starts with `bits` set in its device status word, as if a kernel had reported them; that call must
  * return 1.  Lets the error path be tested without making a kernel fail. */
