@@ -6,7 +6,12 @@
 #include "bsq_fp4.hpp"
 #include "bsq_grad_norm.hpp"
 #include "bsq_internal.hpp"
+#include "bsq_orth.hpp"
 #include "bsq_xent.hpp"
+
+#include <algorithm>
+#include <cmath>
+#include <vector>
 
 using namespace bsq;
 
@@ -268,6 +273,56 @@ int bsq_linear_xent_grad(int type, const void *d_x, uint64_t tokens, uint64_t co
     if (tokens && (!on_bytes(d_target, 8) || !on_bytes(d_scratch, 128) || !on_bytes(d_stats, 4) || !on_bytes(d_grad, 4))) return 1;
     if (!d_dx && !d_dw) return 0;
     return rc(xent_grad(c, d_stats, d_grad, d_dx, tokens > 1 ? ld_dx : cols, d_dw, vocab > 1 ? ld_dw : cols, d_scratch, d_status, device_sm_count(), as_stream(stream)));
+}
+
+// ---- orthogonalised updates ----
+size_t bsq_orthogonalize_scratch_bytes(const uint64_t *rows, const uint64_t *cols, const int *types, int n, int out_type) {
+    if (n < 1 || !rows || !cols || !types || !op_bytes(out_type)) return 0;
+    try {
+        std::vector<OrthMatrix> m((size_t)n);
+        for (int i = 0; i < n; ++i) {
+            if (!op_bytes(types[i]) || rows[i] > kOrthMaxDim || cols[i] > kOrthMaxDim) return 0;
+            m[(size_t)i] = {nullptr, nullptr, rows[i], cols[i], cols[i], cols[i], types[i]};
+        }
+        return orth_scratch_bytes({m.data(), n, out_type, 0, nullptr, 0.0, 0.0f});
+    } catch (...) {
+        return 0;
+    }
+}
+int bsq_orthogonalize(const void *const *d_in, const uint64_t *rows, const uint64_t *cols, const uint64_t *lds, const int *types, int n, void *const *d_out, const uint64_t *ld_outs,
+                      int out_type, int steps, const float *coefficients, double eps, float scale, void *d_scratch, uint32_t *d_status, void *stream) {
+    if (n < 0 || (n && (!d_in || !rows || !cols || !lds || !types || !d_out || !ld_outs)) || !op_bytes(out_type)) return 1;
+    if (steps < 1 || steps > kOrthMaxSteps || !coefficients || !(eps >= 0.0) || std::isinf(eps) || !std::isfinite(scale) || !orth_steps_ok(coefficients, steps)) return 1;
+    try {
+        struct Span {
+            uintptr_t begin, end;
+            bool out;
+        };
+        std::vector<OrthMatrix> m((size_t)n);
+        std::vector<Span> spans;
+        for (int i = 0; i < n; ++i) {
+            const uint64_t r = rows[i], c = cols[i], in = r > 1 ? lds[i] : c, out = r > 1 ? ld_outs[i] : c;
+            if (!op_bytes(types[i]) || r > kOrthMaxDim || c > kOrthMaxDim) return 1;
+            if (r && c && (!op_rows_ok(d_in[i], types[i], r, c, in) || !op_rows_ok(d_out[i], out_type, r, c, out))) return 1;
+            m[(size_t)i] = {d_in[i], d_out[i], r, c, in, out, types[i]};
+            if (!r || !c) continue;
+            const uintptr_t a = reinterpret_cast<uintptr_t>(d_in[i]), b = reinterpret_cast<uintptr_t>(d_out[i]);
+            spans.push_back({a, a + ((r - 1) * in + c) * (uint64_t)op_bytes(types[i]), false});
+            spans.push_back({b, b + ((r - 1) * out + c) * (uint64_t)op_bytes(out_type), true});
+        }
+        if (spans.empty()) return 0;
+        if (!on_bytes(d_scratch, 128)) return 1;
+        std::sort(spans.begin(), spans.end(), [](const Span &a, const Span &b) { return a.begin < b.begin; });
+        uintptr_t any = 0, written = 0;                          // where what came before ends
+        for (const Span &s : spans) {
+            if (s.begin < (s.out ? any : written)) return 1;
+            any = std::max(any, s.end);
+            if (s.out) written = std::max(written, s.end);
+        }
+        return rc(orthogonalize({m.data(), n, out_type, steps, coefficients, eps, scale}, d_scratch, d_status, device_sm_count(), as_stream(stream)));
+    } catch (...) {
+        return 1;
+    }
 }
 
 void bsq_test_limit_waits(uint32_t tries) { limit_epilogue_tries(tries); }

@@ -447,3 +447,102 @@ def clip_grad_norm(grads, max_norm, norm_type=2.0, out=None):
     if max_norm is not None:
         torch.autograd.graph.increment_version(to)
     return norm
+
+
+_QUINTIC = (3.4445, -4.7750, 2.0315)
+_ORTH_SIDE, _ORTH_STEPS = 65536, 64
+
+
+def orthogonalize(updates, steps=5, coefficients=_QUINTIC, eps=1e-7, scale=1.0, dtype=torch.bfloat16, out=None):
+    """Updates with their singular values brought near 1 by Newton-Schulz steps: X = G / (|G| + eps), then `steps` times X <- a X + (b A + c A^2) X with A = X X^T (from the
+    right with X^T X where G has more rows than columns), times `scale`.  `updates`: a tensor of at least two dimensions (the leading ones are a stack of matrices) or a list of them
+    (float32, float16 or bfloat16 CUDA tensors of one device, of any shapes); the result is of the same form, in `dtype`.  Matrices of one shape and type go through together.  coefficients: (a, b, c)
+    for all steps, or one triple for each; they must keep singular values from 0 to 1 below 1000.  `out`: tensors to write, apart from each other and from the updates.
+
+    X is held in 2 x 16 bits and products sum in FP32: bfloat16 results are off by about half their own rounding beside it.  float32 and float16 results come from products
+    of both halves of every operand, three times the work.  An Inf or NaN makes its whole matrix NaN; zeros stay zeros, and where |G| is far below eps the result may be 0.
+    Matrices whose rows are not contiguous are copied first.  The result needs no gradient and gives none to the updates.  Sides of at most 65536, 1 to 64 steps."""
+    single = isinstance(updates, torch.Tensor)
+    updates = [updates] if single else list(updates)
+    if not 1 <= steps <= _ORTH_STEPS or int(steps) != steps:
+        raise ValueError("steps must be a whole number from 1 to 64")
+    if dtype not in _TYPES:
+        raise ValueError("dtype must be float32, float16 or bfloat16")
+    table = list(coefficients)
+    table = [table] * int(steps) if len(table) == 3 and all(isinstance(v, (int, float)) for v in table) else table
+    if len(table) != steps or any(isinstance(t, (int, float)) or len(t) != 3 for t in table):
+        raise ValueError("coefficients must be (a, b, c), or one such triple for each step")
+    eps, scale = float(eps), float(scale)
+    if not 0.0 <= eps < math.inf or not math.isfinite(scale):
+        raise ValueError("eps must be finite and not negative, scale finite")
+    if not updates:
+        return []
+    device, index = updates[0].device, updates[0].get_device()
+    for g in updates:
+        if g.dtype not in _TYPES or g.get_device() != index or index < 0 or g.dim() < 2 or g.size(-1) > _ORTH_SIDE or g.size(-2) > _ORTH_SIDE:
+            raise ValueError("updates must be float32, float16 or bfloat16 CUDA tensors on one device of at least two dimensions, with sides of at most 65536")
+    if out is None:
+        outs = [torch.empty(g.shape, dtype=dtype, device=device) for g in updates]
+    else:
+        outs = [out] if isinstance(out, torch.Tensor) else list(out)
+        if len(outs) != len(updates) or isinstance(out, torch.Tensor) != single:
+            raise ValueError("out must have the form of updates")
+        for o, g in zip(outs, updates):
+            if o.dtype != dtype or o.shape != g.shape or o.device != device or o.requires_grad:
+                raise ValueError("tensors of out must have the shapes of the updates, dtype %s, their device, and need no gradient" % dtype)
+    ins, rows, cols, lds, types, tos, ld_outs, keep = array("Q"), array("Q"), array("Q"), array("Q"), array("i"), array("Q"), array("Q"), []
+    for g, o in zip(updates, outs):
+        if not g.numel():
+            continue
+        if not _stacked(g):
+            g = g.contiguous()
+            keep.append(g)                                       # (until the call has been enqueued)
+        if out is not None and not _stacked(o):
+            raise ValueError("rows of out must be contiguous and must not overlap")
+        m, n, size, to_size = g.size(-2), g.size(-1), g.element_size(), o.element_size()
+        for a, b in zip(_matrices(g), _matrices(o)):
+            ins.append(g.data_ptr() + a * size)
+            tos.append(o.data_ptr() + b * to_size)
+        count = g.numel() // (m * n)
+        rows.extend([m] * count), cols.extend([n] * count), types.extend([_TYPES[g.dtype]] * count)
+        lds.extend([g.stride(-2) if m > 1 else n] * count), ld_outs.extend([o.stride(-2) if m > 1 else n] * count)
+    if ins:
+        flat = array("f", [v for t in table for v in t])
+        arrays = [a.buffer_info()[0] for a in (ins, rows, cols, lds, types, tos, ld_outs, flat)]
+        scratch = _scratch("bsq_orthogonalize_scratch_bytes", device, arrays[1], arrays[2], arrays[4], len(ins), _TYPES[dtype])
+        try:
+            _call("bsq_orthogonalize", index, *arrays[:5], len(ins), *arrays[5:7], _TYPES[dtype], int(steps), arrays[7], eps, scale, scratch.data_ptr(), None)
+        except RuntimeError:
+            if not _steps_ok(table):
+                raise ValueError("coefficients must keep singular values from 0 to 1 below 1000") from None
+            if out is not None:
+                raise ValueError("the matrices that are written must lie apart from one another and from the updates") from None
+            raise
+    if out is not None:
+        torch.autograd.graph.increment_version(outs)
+    return outs[0] if single else outs
+
+
+def _stacked(t):
+    """Whether every matrix of a stack has contiguous rows that do not overlap."""
+    return (t.stride(-1) == 1 or t.size(-1) == 1) and (t.size(-2) == 1 or t.stride(-2) >= t.size(-1))
+
+
+def _matrices(t):
+    """Where the matrices of a stack begin, in elements from its first."""
+    at = [0]
+    for n, s in zip(t.shape[:-2], t.stride()[:-2]):
+        at = [a + i * s for a in at for i in range(n)]
+    return at
+
+
+def _steps_ok(table):
+    """As the library looks at coefficients: the largest singular value that each step may meet."""
+    most = 1.0
+    for a, b, c in table:
+        s = [most * 1.02 * i / 4096 for i in range(4097)]
+        p = [b * v * v + c * v ** 4 for v in s]
+        most = max(abs((a + q) * v) for q, v in zip(p, s))
+        if not most < 1000.0 or any(not abs(q) < 1e6 for q in p):
+            return False
+    return True

@@ -315,6 +315,18 @@ int bsq_linear_xent_grad(int type, const void *d_x, uint64_t tokens, uint64_t co
                          int64_t ignore, double smoothing, int reduction, const float *d_stats, const float *d_grad, void *d_dx, uint64_t ld_dx, void *d_dw, uint64_t ld_dw,
                          void *d_scratch, uint32_t *d_status, void *stream);
 
+/* ---- orthogonalised updates (no counterpart in the reference) ----------------------------------------------------------------------------
+ * Each of n matrices G (rows x cols, lds apart; types as above) by `steps` Newton-Schulz steps:  X = G / (|G| + eps), |G| the square root of the sum of squares;
+ * for each step's coefficients (a, b, c; 3 * steps floats)  A = X X^T,  X <- a X + (b A + c A^2) X  (with X^T X from the right where G has more rows than columns);
+ * out = scale * X in out_type.  The coefficients must keep singular values from 0 to 1 below 1000 all the way (else 1).  Products read 16 bits of each operand and sum in FP32, X is held in two
+ * times 16: results in BF16 are off by about half their own rounding; results in FP32 or FP16, and matrices with a side of up to 128, come from products of both halves (about 2^-20).
+ * An Inf or NaN makes its whole matrix NaN; a matrix of zeros stays one; where |G| is below 2^-20 * eps the result may be 0.  Sides of at most 65536, 1 to 64 steps; matrices without
+ * elements are passed over.  Results must not overlap one another or an input.  Arrays are read before the call returns.  The call enqueues on `stream`, allocates nothing on the device, keeps
+ * nothing and may be captured.  d_scratch: bsq_orthogonalize_scratch_bytes on a 128-byte boundary (matrices of one shape go together, up to 1 GB of scratch).  d_status as for bsq_fp4_matmul. */
+size_t bsq_orthogonalize_scratch_bytes(const uint64_t *rows, const uint64_t *cols, const int *types, int n, int out_type);
+int bsq_orthogonalize(const void *const *d_in, const uint64_t *rows, const uint64_t *cols, const uint64_t *lds, const int *types, int n, void *const *d_out, const uint64_t *ld_outs,
+                      int out_type, int steps, const float *coefficients, double eps, float scale, void *d_scratch, uint32_t *d_status, void *stream);
+
 /* Test hook (no counterpart in the reference): the next bsq_compress (which = 0) or bsq_decompress (which = 1) on the
  * current device starts with `bits` set in its device status word, as if a kernel had reported them; that call must
  * return 1.  Lets the error path be tested without making a kernel fail. */
