@@ -2,9 +2,12 @@
 // FP32 sums in tensor memory.  What becomes of a tile is the epilogue's: statistics of a softmax, gradients of logits, a step of an iteration.
 //
 // Where there are enough tiles, a pair of CTAs on two SMs shares one of 256 x 256 (cta_group::2): each brings 128 rows of A and 128 of B, so that an element from
-// the L2 feeds 256 multiplications.  Small results: one CTA per tile of 128 x 128.  Warp 0 brings stages of 64 of K by TMA (128-byte swizzle, six stages of 32 KB; operands that are
-// contiguous along K or along M / N, whichever they are in memory: the tensor core reads either), warp 1 of the leader issues the MMAs, warps 4 to 7 take finished
-// tiles out while the next one is summed in the other half of tensor memory.
+// the L2 feeds 256 multiplications.  Small results: one CTA per tile of 128 x 128.  Warp 0 brings stages of 64 of K by TMA (128-byte swizzle, five stages of 32 KB; operands that are
+// contiguous along K or along M / N, whichever they are in memory: the tensor core reads either), warp 1 of the leader issues the MMAs, warps 4 to 11 take finished
+// tiles out while the next one is summed in the other half of tensor memory, each 32 rows and half of the columns.  (Four warps with all columns took 20 us for a tile that read
+// and wrote two FP16 matrices, more than the 17 us of its 4096 of K.)
+//
+// The tensor core cuts additions off instead of rounding them: epilogues that want FP32's digits (kChained) get the sums every 1024 of K and add them up rounded, in registers.
 //
 // An operand may come in two parts, high + low (splits): the product is then high x high + high x low + low x high, three walks along K into the same sums.
 //
@@ -16,9 +19,10 @@
 namespace bsq {
 namespace {
 
-constexpr int kG16Stages = 6, kG16K = 64;                        // stages in flight, of K each
+constexpr int kG16Stages = 5, kG16K = 64;                        // stages in flight, of K each
 constexpr unsigned kG16Half = 128 * kG16K * 2, kG16Stage = 2 * kG16Half;
-constexpr int kG16Threads = 256, kG16Warps = 4;                  // epilogue warps, the last four
+constexpr int kG16Warps = 8, kG16Threads = 128 + 32 * kG16Warps; // epilogue warps, the last eight
+constexpr int kG16Chain = 1024 / kG16K;                          // stages of a chain of sums
 constexpr unsigned kG16Box = 32 * 128;                           // 32 rows x 128 bytes on their way out: two for each epilogue warp
 constexpr int kG16Band = 16;                                     // rows of tiles that are walked together, column after column
 
@@ -38,7 +42,7 @@ struct Gemm16Maps {
 };
 
 struct Gemm16Bars {
-    uint64_t full[kG16Stages], empty[kG16Stages], acc_full[2], acc_empty[2], drain;
+    uint64_t full[kG16Stages], empty[kG16Stages], acc_full[2], acc_empty[2], fetched[kG16Warps], drain;
     unsigned tmem_base;
 };
 
@@ -106,13 +110,16 @@ __device__ __forceinline__ TileAt tile_at(const Gemm16 &g, int t) {
     return at;
 }
 
-// What an epilogue is given: a warp has 32 rows of a tile (from `row` on; the thread's own is row + lane) and all its columns from `col` on.
+// What an epilogue is given: a warp has 32 rows of a tile (from `row` on; the thread's own is row + lane) and half of its columns, from `col` on.
 struct TileOut {
     int z, row, col, lane;
     unsigned taddr;                  // accumulators of its rows
     bool ok;                         // not: the tile was given up, everything that it would give is NaN
     unsigned char *boxes;            // two boxes of this warp
-    int *which;                      // the box that is next
+    int *which;                      // the box that is next (box_next)
+    uint64_t *fetched;               // boxes that were asked for are there
+    unsigned *fetches;               // how many times
+    unsigned *status;
 };
 // The box that is next, free to be written.  (The two take turns with what is really copied: a box that is asked for is copied out by TMA, box_send, or read by
 // the warp itself before the next one is asked for.)
@@ -132,6 +139,55 @@ __device__ __forceinline__ void box_send(const TileOut &t, const CUtensorMap *ma
         bulk_commit();
     }
 }
+// The other way to use the two boxes: both at a time, first for what comes in.  (Rows of matrices that a thread reads and writes 32 bytes at a time touch 32 lines with every
+// instruction: a tile that read and wrote two FP16 matrices took 14 us that way, more than 1024 of K; copies move whole lines.)  Asks for boxes of 64 columns x 32 rows of one or two matrices.
+__device__ __forceinline__ void boxes_ask(const TileOut &o, const CUtensorMap *first, const CUtensorMap *second, int x) {
+    fence_proxy_async_smem();                                    // this thread's reads and writes of the boxes come before the copies'
+    __syncwarp();
+    if (o.lane == 0) {
+        bulk_wait_read_all();
+        mbar_expect_tx(o.fetched, second ? 2 * kG16Box : kG16Box);
+        tma_load_3d(o.boxes, first, x, o.row, o.z, o.fetched);
+        if (second) tma_load_3d(o.boxes + kG16Box, second, x, o.row, o.z, o.fetched);
+    }
+    __syncwarp();
+}
+__device__ __forceinline__ void boxes_wait(const TileOut &o) {
+    mbar_wait_asleep(o.fetched, *o.fetches & 1u, o.status);
+    ++*o.fetches;
+    __syncwarp();
+}
+// ... free to be written without anything that came in
+__device__ __forceinline__ void boxes_free(const TileOut &o) {
+    if (o.lane == 0) bulk_wait_read_all();
+    __syncwarp();
+}
+__device__ __forceinline__ uint4 *box_piece(const TileOut &o, int which, int i) { return reinterpret_cast<uint4 *>(o.boxes + (unsigned)which * kG16Box + o.lane * 128) + (i ^ (o.lane & 7)); }
+// 16 FP16 values of the thread's row, two to a word: in, out
+__device__ __forceinline__ void box_take16(const TileOut &o, int which, int h, unsigned (&w)[8]) {
+    const uint4 a = *box_piece(o, which, 2 * h), b = *box_piece(o, which, 2 * h + 1);
+    w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w; w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
+}
+__device__ __forceinline__ void box_give16(const TileOut &o, int which, int h, const unsigned (&w)[8]) {
+    *box_piece(o, which, 2 * h) = make_uint4(w[0], w[1], w[2], w[3]);
+    *box_piece(o, which, 2 * h + 1) = make_uint4(w[4], w[5], w[6], w[7]);
+}
+// A box as box_out takes it, 16 bytes at a time where rows start on 16 bytes
+__device__ __forceinline__ void box_out_rows(const unsigned char *box, int lane, void *out, int size, long at, long ld, int rows, int cols) {
+    if ((reinterpret_cast<uintptr_t>(out) | (uintptr_t)(ld * size) | (uintptr_t)(at * size)) % 16 != 0 || cols * size < 128) {
+        box_out(box, lane, out, size, at, ld, rows, cols);
+        return;
+    }
+    __syncwarp();
+    const int piece = lane & 7;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int r = 4 * i + (lane >> 3);
+        const uint4 q = *reinterpret_cast<const uint4 *>(box + r * 128 + ((piece ^ (r & 7)) << 4));
+        if (r < rows) *reinterpret_cast<uint4 *>(static_cast<unsigned char *>(out) + (at + (long)r * ld) * size + piece * 16) = q;
+    }
+    __syncwarp();
+}
 // 16 values of the thread's row to places 16 h .. of its line of a box of 16-bit elements
 template <int TYPE> __device__ __forceinline__ void box_put16(unsigned char *box, int lane, int h, const float (&v)[16]) {
     uint4 *line = reinterpret_cast<uint4 *>(box + lane * 128);
@@ -147,21 +203,6 @@ __device__ __forceinline__ void read16f(unsigned taddr, float (&v)[16], bool ok)
 #pragma unroll
     for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
 }
-// 32 neighbouring accumulators of the thread's row
-__device__ __forceinline__ void read32f(unsigned taddr, float (&v)[32], bool ok) {
-    unsigned r[32];
-    if (ok)
-        asm volatile(
-            "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, "
-            "%26, %27, %28, %29, %30, %31}, [%32];\n"
-            : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
-              "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-              "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-            : "r"(taddr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(ok ? r[j] : 0x7fffffffu);
-}
 // One column of accumulators, of all rows of the warp
 __device__ __forceinline__ float read_column(unsigned taddr, bool ok) {
     unsigned r = 0x7fffffffu;
@@ -170,11 +211,15 @@ __device__ __forceinline__ float read_column(unsigned taddr, bool ok) {
     return ok ? __uint_as_float(r) : __uint_as_float(0x7fffffffu);
 }
 
-// EPI: a functor with `template <int COLS> void tile(const TileOut &) const`, called by whole warps.  CTAS: 1, or 2 for a pair.
+// EPI: a functor, called by whole warps:
+//   template <int COLS> void tile(const TileOut &, Ahead &) const     takes COLS columns out; kChained: tile(const TileOut &, float (&sums)[COLS])
+//   template <int COLS> void ahead(const TileOut &, Ahead &) const    what can be asked for while the tile is still being summed (not kChained)
+// CTAS: 1, or 2 for a pair.
+struct NoAhead {};
 template <class EPI, int CTAS>
 __global__ void __launch_bounds__(kG16Threads, 1) gemm16_kernel(const __grid_constant__ Gemm16Maps maps, const __grid_constant__ EPI epi, const Gemm16 g, unsigned *status) {
     chain_begin();
-    constexpr int kTile = 128 * CTAS;
+    constexpr int kTile = 128 * CTAS, kCols = kTile / 2;
     extern __shared__ unsigned char smem_dyn[];
     unsigned char *base = smem_dyn + ((1024u - (smem_u32(smem_dyn) & 1023u)) & 1023u);
     unsigned char *boxes = base + kG16Stages * kG16Stage;
@@ -182,7 +227,7 @@ __global__ void __launch_bounds__(kG16Threads, 1) gemm16_kernel(const __grid_con
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int half = CTAS == 2 ? (int)(blockIdx.x & 1) : 0, first = (int)(blockIdx.x / CTAS), step = (int)(gridDim.x / CTAS);
     const int tiles = g.batch * g.splits * (g.lower ? g.m_tiles * (g.m_tiles + 1) / 2 : g.m_tiles * g.n_tiles);
-    const int stages = g.k_stages * g.parts;
+    const int stages = g.k_stages * g.parts, chain = EPI::kChained ? kG16Chain : stages;
     const bool leader = half == 0;
 
     if (tid == 0) {
@@ -194,6 +239,7 @@ __global__ void __launch_bounds__(kG16Threads, 1) gemm16_kernel(const __grid_con
             mbar_init(&bars.acc_full[i], 1);
             mbar_init(&bars.acc_empty[i], CTAS * kG16Warps);
         }
+        for (int i = 0; i < kG16Warps; ++i) mbar_init(&bars.fetched[i], 1);
         mbar_init(&bars.drain, 1);
         mbar_fence_init();
     }
@@ -257,30 +303,33 @@ __global__ void __launch_bounds__(kG16Threads, 1) gemm16_kernel(const __grid_con
                                    ((unsigned)kTile >> 4 << 24);
             const uint64_t a_step = g.a_kmajor ? 2u : 128u, b_step = g.b_kmajor ? 2u : 128u;
             Ring r(kG16Stages), rs(2);
-            for (int t = first; t < tiles && ok; t += step, rs.next()) {
-                if (rs.wrapped) ok = __all_sync(kFullMask, mbar_wait_asleep(&bars.acc_empty[rs.pos], rs.par ^ 1u, status)) != 0;
-                if (!ok) break;
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const unsigned acc = tmem + (unsigned)rs.pos * 256u;
-                for (int d = 0; d < stages; ++d, r.next()) {
-                    ok = __all_sync(kFullMask, mbar_wait_asleep(&bars.full[r.pos], r.par, status)) != 0;
+            for (int t = first; t < tiles && ok; t += step) {
+                for (int c0 = 0; c0 < stages && ok; c0 += chain, rs.next()) {
+                    if (rs.wrapped) ok = __all_sync(kFullMask, mbar_wait_asleep(&bars.acc_empty[rs.pos], rs.par ^ 1u, status)) != 0;
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const unsigned s = smem_u32(base) + (unsigned)r.pos * kG16Stage;
-                    const uint64_t da = g.a_kmajor ? smem_desc_sw128(s) : g16_desc_mn(s), db = g.b_kmajor ? smem_desc_sw128(s + kG16Half) : g16_desc_mn(s + kG16Half);
-                    if (elect_one()) {
+                    const unsigned acc = tmem + (unsigned)rs.pos * 256u;
+                    const int c1 = min(stages, c0 + chain);
+                    for (int d = c0; d < c1; ++d, r.next()) {
+                        ok = __all_sync(kFullMask, mbar_wait_asleep(&bars.full[r.pos], r.par, status)) != 0;
+                        if (!ok) break;
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        const unsigned s = smem_u32(base) + (unsigned)r.pos * kG16Stage;
+                        const uint64_t da = g.a_kmajor ? smem_desc_sw128(s) : g16_desc_mn(s), db = g.b_kmajor ? smem_desc_sw128(s + kG16Half) : g16_desc_mn(s + kG16Half);
+                        if (elect_one()) {
 #pragma unroll
-                        for (int kk = 0; kk < kG16K / 16; ++kk) g16_mma<CTAS>(acc, da + a_step * (uint64_t)kk, db + b_step * (uint64_t)kk, idesc, d > 0 || kk > 0);
-                        if (CTAS == 2) tc_commit_pair(&bars.empty[r.pos], 3);
-                        else tc_commit(&bars.empty[r.pos]);
+                            for (int kk = 0; kk < kG16K / 16; ++kk) g16_mma<CTAS>(acc, da + a_step * (uint64_t)kk, db + b_step * (uint64_t)kk, idesc, d > c0 || kk > 0);
+                            if (CTAS == 2) tc_commit_pair(&bars.empty[r.pos], 3);
+                            else tc_commit(&bars.empty[r.pos]);
+                        }
+                        __syncwarp();
+                    }
+                    if (ok && elect_one()) {
+                        if (CTAS == 2) tc_commit_pair(&bars.acc_full[rs.pos], 3);
+                        else tc_commit(&bars.acc_full[rs.pos]);
                     }
                     __syncwarp();
                 }
-                if (ok && elect_one()) {
-                    if (CTAS == 2) tc_commit_pair(&bars.acc_full[rs.pos], 3);
-                    else tc_commit(&bars.acc_full[rs.pos]);
-                }
-                __syncwarp();
             }
             if (elect_one()) {                                   // MMAs under way must be done before tensor memory is given back, also where the epilogue has given up
                 if (CTAS == 2) tc_commit_pair(&bars.drain, 1);
@@ -289,23 +338,49 @@ __global__ void __launch_bounds__(kG16Threads, 1) gemm16_kernel(const __grid_con
             __syncwarp();
             mbar_wait_asleep(&bars.drain, 0, status);
         }
-    } else if (warp >= kG16Threads / 32 - kG16Warps) {
-        const int quarter = warp & 3;                            // the lanes of tensor memory this warp may read
+    } else if (warp >= 4) {
+        const int quarter = warp & 3, part = (warp - 4) >> 2;    // the lanes of tensor memory this warp may read, its half of the columns
         int which = 0;
+        unsigned fetches = 0;
         Ring rs(2);
-        for (int t = first; t < tiles; t += step, rs.next()) {
-            if (ok) ok = __all_sync(kFullMask, mbar_wait_asleep(&bars.acc_full[rs.pos], rs.par, status, g.tries)) != 0;
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        for (int t = first; t < tiles; t += step) {
             const TileAt at = tile_at(g, t);
-            const TileOut out = {at.z, at.i * kTile + half * 128 + quarter * 32, at.j * kTile, lane, tmem + (unsigned)rs.pos * 256u + ((unsigned)(quarter * 32) << 16), ok,
-                                 boxes + (unsigned)quarter * 2 * kG16Box, &which};
-            if (out.row < g.M) epi.template tile<kTile>(out);
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            __syncwarp();
-            // (not where this warp has given up: it runs ahead from here on, and its arrivals would let accumulators be overwritten that others still read)
-            if (ok && lane == 0) {
-                if (CTAS == 2) mbar_arrive_pair(smem_u32(&bars.acc_empty[rs.pos]) + lead);
-                else mbar_arrive(&bars.acc_empty[rs.pos]);
+            TileOut out = {at.z, at.i * kTile + half * 128 + quarter * 32, at.j * kTile + part * kCols, lane, 0, ok, boxes + (unsigned)(warp - 4) * 2 * kG16Box, &which,
+                           &bars.fetched[warp - 4], &fetches, status};
+            const bool mine = out.row < g.M && out.col < g.N;
+            float sums[EPI::kChained ? kCols : 1];
+            typename EPI::Ahead ahead;
+            if constexpr (!EPI::kChained) {
+                if (mine) epi.template ahead<kCols>(out, ahead);
+            }
+            for (int c0 = 0; c0 < stages; c0 += chain, rs.next()) {
+                if (ok) ok = __all_sync(kFullMask, mbar_wait_asleep(&bars.acc_full[rs.pos], rs.par, status, g.tries)) != 0;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                out.taddr = tmem + (unsigned)rs.pos * 256u + (unsigned)(part * kCols) + ((unsigned)(quarter * 32) << 16);
+                out.ok = ok;
+                if constexpr (EPI::kChained) {
+                    if (mine) {
+#pragma unroll
+                        for (int c = 0; c < kCols; c += 16) {
+                            float v[16];
+                            read16f(out.taddr + (unsigned)c, v, ok);
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) sums[c + j] = c0 ? sums[c + j] + v[j] : v[j];
+                        }
+                    }
+                } else {
+                    if (mine) epi.template tile<kCols>(out, ahead);
+                }
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                // (not where this warp has given up: it runs ahead from here on, and its arrivals would let accumulators be overwritten that others still read)
+                if (ok && lane == 0) {
+                    if (CTAS == 2) mbar_arrive_pair(smem_u32(&bars.acc_empty[rs.pos]) + lead);
+                    else mbar_arrive(&bars.acc_empty[rs.pos]);
+                }
+            }
+            if constexpr (EPI::kChained) {
+                if (mine) epi.template tile<kCols>(out, sums);
             }
         }
         if (lane == 0) bulk_wait_all();

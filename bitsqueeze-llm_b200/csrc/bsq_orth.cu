@@ -25,16 +25,27 @@ constexpr int kOrthMost = 64;                                    // matrices of 
 constexpr uint64_t kOrthRoom = 1ull << 30;                       // scratch that several matrices share at most
 constexpr uint64_t kSplitShort = 128;                            // short sides up to this: split operands
 constexpr int kNormThreads = 512;
-constexpr uint64_t kNormChunk = 32768;                           // elements of a CTA of the pass that finds the norms, 64 CTAs at most
-constexpr int kNormParts = 64;
+constexpr uint64_t kNormChunk = 16384;                           // elements of a CTA of the pass that finds the norms, at least
+constexpr int kNormParts = kNormThreads;
 
-__device__ __forceinline__ float half_bits(unsigned short b) { return __half2float(__ushort_as_half(b)); }
-// 16 FP16 elements on a 32-byte boundary
-__device__ __forceinline__ void load16h(const unsigned short *p, float (&v)[16]) {
-    unsigned w[8];
-    ld_words8(p, w);
+__device__ __forceinline__ float2 pair_of(unsigned w) { return __half22float2(*reinterpret_cast<const __half2 *>(&w)); }
+// 16 values in two parts of FP16, two to a word
+__device__ __forceinline__ void split16(const float (&v)[16], unsigned (&high)[8], unsigned (&low)[8]) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = half_bits((unsigned short)(w[j >> 1] >> ((j & 1) * 16)));
+    for (int j = 0; j < 8; ++j) {
+        const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+        const float2 f = __half22float2(h);
+        high[j] = *reinterpret_cast<const unsigned *>(&h);
+        low[j] = pack_pair<kF16>(v[2 * j] - f.x, v[2 * j + 1] - f.y);
+    }
+}
+// 16 floats that all rows share, on a 64-byte boundary
+__device__ __forceinline__ void load16f(const float *p, float (&v)[16]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float4 q = reinterpret_cast<const float4 *>(p)[j];
+        v[4 * j] = q.x; v[4 * j + 1] = q.y; v[4 * j + 2] = q.z; v[4 * j + 3] = q.w;
+    }
 }
 __device__ __forceinline__ float high_of(float x) { return __half2float(__float2half_rn(x)); }
 
@@ -42,33 +53,71 @@ __device__ __forceinline__ float high_of(float x) { return __half2float(__float2
 struct OrthIn {
     const void *at[kOrthMost];
     uint64_t ld[kOrthMost];
-    uint64_t rows, cols;
+    bool whole[kOrthMost];           // every row starts on 16 bytes
+    unsigned rows, cols;
     int type;
 };
-__device__ __forceinline__ float elem(const void *p, int type, uint64_t i) {
-    if (type == kF32) return static_cast<const float *>(p)[i];
-    if (type == kBf16) return __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
-    return __half2float(static_cast<const __half *>(p)[i]);
+// Eight neighbouring elements of a row; those behind its end are 0
+template <int TYPE> __device__ __forceinline__ void load8(const OrthIn &in, unsigned row, unsigned col, float (&v)[8]) {
+    constexpr int kSize = TYPE == kF32 ? 4 : 2, kWords = 8 * kSize / 4;
+    const unsigned char *p = static_cast<const unsigned char *>(in.at[blockIdx.y]) + ((size_t)row * in.ld[blockIdx.y] + col) * kSize;
+    if (in.whole[blockIdx.y] && col + 8 <= in.cols) {
+        unsigned w[kWords];
+#pragma unroll
+        for (int i = 0; i < kWords; i += 4) {
+            const uint4 q = *reinterpret_cast<const uint4 *>(p + 4 * i);
+            w[i] = q.x; w[i + 1] = q.y; w[i + 2] = q.z; w[i + 3] = q.w;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = TYPE == kF32 ? word_elem<TYPE>(w[j * kWords / 8], 0) : word_elem<TYPE>(w[j / 2], j & 1);
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        v[j] = col + j >= in.cols ? 0.0f : word_elem<TYPE>(TYPE == kF32 ? reinterpret_cast<const unsigned *>(p)[j] : (unsigned)reinterpret_cast<const unsigned short *>(p)[j], 0);
 }
 __device__ __forceinline__ double cta_total(double v, double *room) {
     for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(kFullMask, v, d);
     if ((threadIdx.x & 31) == 0) room[threadIdx.x >> 5] = v;
     __syncthreads();
     v = 0.0;
-    for (int i = 0; i < (int)blockDim.x / 32; ++i) v += room[i];
+    for (int i = 0; i < kNormThreads / 32; ++i) v += room[i];
     return v;
 }
-// Sums of squares, in FP64: blockIdx.x a part of a matrix's rows, blockIdx.y the matrix
-__global__ void __launch_bounds__(kNormThreads) orth_norm_kernel(const __grid_constant__ OrthIn in, double *parts) {
+// Squares of eight elements: in FP32 where that is good to 24 bits, else in FP64
+__device__ __forceinline__ double squares8(const float (&v)[8]) {
+    float s = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s = fmaf(v[j], v[j], s);
+    if (s == 0.0f || (s > 1e-30f && s < 1e36f)) {
+        bool any = false;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) any |= v[j] != 0.0f;
+        if (s != 0.0f || !any) return (double)s;
+    }
+    double d = 0.0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) d = fma((double)v[j], (double)v[j], d);
+    return d;
+}
+// Sums of squares: blockIdx.x a share of a matrix, blockIdx.y the matrix
+template <int TYPE> __global__ void __launch_bounds__(kNormThreads) orth_norm_kernel(const __grid_constant__ OrthIn in, double *parts) {
     chain_begin();
     __shared__ double room[kNormThreads / 32];
-    const void *p = in.at[blockIdx.y];
-    const uint64_t ld = in.ld[blockIdx.y], all = in.rows * in.cols;
+    const unsigned per = (in.cols + 7) / 8, all = in.rows * per, step = gridDim.x * kNormThreads;
     double s = 0.0;
-    for (uint64_t i = (uint64_t)blockIdx.x * kNormThreads + threadIdx.x; i < all; i += (uint64_t)gridDim.x * kNormThreads) {
-        const uint64_t r = i / in.cols;
-        const double x = (double)elem(p, in.type, r * ld + (i - r * in.cols));
-        s = fma(x, x, s);
+    for (unsigned i = blockIdx.x * kNormThreads + threadIdx.x; i < all; i += 4 * step) {
+        float v[4][8];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const unsigned k = i + u * step, r = k / per;
+            if (k < all) load8<TYPE>(in, r, (k - r * per) * 8, v[u]);
+            else
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[u][j] = 0.0f;
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) s += squares8(v[u]);
     }
     s = cta_total(s, room);
     if (threadIdx.x == 0) parts[blockIdx.y * gridDim.x + blockIdx.x] = s;
@@ -76,112 +125,105 @@ __global__ void __launch_bounds__(kNormThreads) orth_norm_kernel(const __grid_co
 
 struct OrthX {
     unsigned short *high, *low;
-    uint64_t ld, apart;
+    unsigned ld;
+    uint64_t apart;
     float *factor;                   // X = (high + low) * factor, one for each matrix
 };
-__global__ void __launch_bounds__(kNormThreads) orth_begin_kernel(const __grid_constant__ OrthIn in, const double *parts, int count, double eps, const OrthX x) {
+template <int TYPE> __global__ void __launch_bounds__(kNormThreads) orth_begin_kernel(const __grid_constant__ OrthIn in, const double *parts, int count, double eps, const OrthX x) {
     chain_begin();
     __shared__ double room[kNormThreads / 32];
-    const void *p = in.at[blockIdx.y];
     const double total = cta_total((int)threadIdx.x < count ? parts[blockIdx.y * (unsigned)count + threadIdx.x] : 0.0, room), norm = sqrt(total);
     // 2^e brings the norm, and so every element, below 2^15; a power of two, so that elements of 16 bits stay what they are
     const bool fine = norm < 3.0e38 * 65536.0 * 65536.0;         // (not: Inf or NaN)
     const int e = norm > 0.0 && fine ? min(max(14 - ilogb(norm), -160), 160) : 0;
     if (blockIdx.x == 0 && threadIdx.x == 0) x.factor[blockIdx.y] = !fine ? __uint_as_float(0x7fffffffu) : norm > 0.0 ? (float)(ldexp(1.0, -e) / (norm + eps)) : 1.0f;
     const float s0 = exp2f((float)(e / 2)), s1 = exp2f((float)(e - e / 2));
-    const uint64_t ld = in.ld[blockIdx.y], all = in.rows * x.ld;
+    const unsigned per = x.ld / 8, all = in.rows * per, step = gridDim.x * kNormThreads;
     unsigned short *high = x.high + blockIdx.y * x.apart, *low = x.low + blockIdx.y * x.apart;
-    for (uint64_t i = (uint64_t)blockIdx.x * kNormThreads + threadIdx.x; i < all; i += (uint64_t)gridDim.x * kNormThreads) {
-        const uint64_t r = i / x.ld, c = i - r * x.ld;
-        const float v = c < in.cols ? elem(p, in.type, r * ld + c) * s0 * s1 : 0.0f;
-        const float h = high_of(v);
-        high[i] = __half_as_ushort(__float2half_rn(h));
-        low[i] = __half_as_ushort(__float2half_rn(v - h));
+    for (unsigned i = blockIdx.x * kNormThreads + threadIdx.x; i < all; i += 2 * step) {
+        float v[2][8];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const unsigned k = i + u * step, r = k / per;
+            if (k < all) load8<TYPE>(in, r, (k - r * per) * 8, v[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const unsigned k = i + u * step;
+            if (k >= all) break;
+            unsigned a[4], b[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float p = v[u][2 * j] * s0 * s1, q = v[u][2 * j + 1] * s0 * s1;
+                a[j] = pack_pair<kF16>(p, q);
+                b[j] = pack_pair<kF16>(p - high_of(p), q - high_of(q));
+            }
+            *reinterpret_cast<uint4 *>(high + (size_t)k * 8) = make_uint4(a[0], a[1], a[2], a[3]);
+            *reinterpret_cast<uint4 *>(low + (size_t)k * 8) = make_uint4(b[0], b[1], b[2], b[3]);
+        }
     }
 }
 
 // ---- what the epilogues share ----
-// 16 values to a box of 16-bit elements: high parts, and low parts to another one
-__device__ __forceinline__ void put_parts(unsigned char *high, unsigned char *low, int lane, int h, const float (&v)[16]) {
-    float a[16], b[16];
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-        a[j] = high_of(v[j]);
-        b[j] = v[j] - a[j];
-    }
-    box_put16<kF16>(high, lane, h, a);
-    if (low) box_put16<kF16>(low, lane, h, b);
-}
-// A box of 32 rows x 64 columns turned into one of 64 rows x 32 (64 bytes a row, not swizzled)
-__device__ __forceinline__ void turn_box(const unsigned char *box, unsigned char *turned, int lane) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const uint4 q = *reinterpret_cast<const uint4 *>(box + lane * 128 + ((i ^ (lane & 7)) << 4));
-        const unsigned w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-        for (int j = 0; j < 8; ++j) reinterpret_cast<unsigned short *>(turned)[(i * 8 + j) * 32 + lane] = (unsigned short)(w[j >> 1] >> ((j & 1) * 16));
-    }
-}
 // The element of v on the diagonal, where the thread's row has one in these 16 columns
 __device__ __forceinline__ int diagonal_at(int row, int col) { return (unsigned)(row - col) < 16u ? row - col : -1; }
 
-struct SymmetricMaps {
-    CUtensorMap map[2], turned[2];   // high, low
+struct SymmetricOut {
+    CUtensorMap map[2], turned[2];   // boxes of 32 rows x 64 columns of the high and low parts, and of 64 rows x 32 columns (64 bytes a row, not swizzled)
+    uint64_t ld;                     // distance of the matrices' diagonals
 };
-// 64 columns of a symmetric result from `fill(h, v)`, their mirror image too where the tile is below the diagonal
-template <bool SPLIT, class Fill> __device__ __forceinline__ void put_symmetric(const TileOut &o, const SymmetricMaps &m, int c, bool mirror, const Fill &fill) {
-    float keep[SPLIT ? 64 : 1];
-    unsigned char *box = box_next(o);
+// 64 columns of a symmetric result from `fill(h, v)`, which may read what lies in the boxes, and their mirror image too where they lie below the diagonal, in a box that is
+// written column by column
+template <bool SPLIT, class Fill> __device__ __forceinline__ void put_symmetric(const TileOut &o, const SymmetricOut &m, int c, bool mirror, const Fill &fill) {
+    unsigned w[SPLIT ? 2 : 1][4][8];
+    const int col = o.col + c;
 #pragma unroll
     for (int h = 0; h < 4; ++h) {
         float v[16];
         fill(h, v);
+        unsigned low[8];
+        split16(v, w[0][h], low);
+        box_give16(o, 0, h, w[0][h]);
         if constexpr (SPLIT) {
+            box_give16(o, 1, h, low);
 #pragma unroll
-            for (int j = 0; j < 16; ++j) keep[16 * h + j] = v[j] - high_of(v[j]);
+            for (int j = 0; j < 8; ++j) w[1][h][j] = low[j];
         }
-        put_parts(box, nullptr, o.lane, h, v);
     }
-    box_send(o, &m.map[0], o.col + c, o.row, box);
-    if (mirror) {
-        unsigned char *turned = box_next(o);
-        turn_box(box, turned, o.lane);
-        box_send(o, &m.turned[0], o.row, o.col + c, turned);
-    }
-    if constexpr (SPLIT) {
-        box = box_next(o);
+    box_send(o, &m.map[0], col, o.row, o.boxes);
+    if constexpr (SPLIT) box_send(o, &m.map[1], col, o.row, o.boxes + kG16Box);
+    if (!mirror) return;
+    if constexpr (SPLIT) boxes_free(o);
 #pragma unroll
-        for (int h = 0; h < 4; ++h) {
-            float v[16];
+    for (int p = 0; p < (SPLIT ? 2 : 1); ++p) {
+        unsigned char *turned = o.boxes + (SPLIT ? (unsigned)p : 1u) * kG16Box;
 #pragma unroll
-            for (int j = 0; j < 16; ++j) v[j] = keep[16 * h + j];
-            box_put16<kF16>(box, o.lane, h, v);
-        }
-        box_send(o, &m.map[1], o.col + c, o.row, box);
-        if (mirror) {
-            unsigned char *turned = box_next(o);
-            turn_box(box, turned, o.lane);
-            box_send(o, &m.turned[1], o.row, o.col + c, turned);
-        }
+        for (int j = 0; j < 64; ++j)
+            reinterpret_cast<unsigned short *>(turned)[j * 32 + o.lane] = (unsigned short)(w[p][j >> 4][(j >> 1) & 7] >> ((j & 1) * 16));
+        box_send(o, &m.turned[p], o.row, col, turned);
     }
 }
 
 // ---- A = X X^T (or X^T X), held times 2^e ----
 template <bool SPLIT> struct GramOut {
-    SymmetricMaps maps;
+    SymmetricOut to;
     int M;
     const float *factor;             // of X, one for each matrix, or null
     float constant;                  // ... for all
     float scale;                     // 2^e
     float *rest;                     // what rounding to FP16 takes from the diagonal
 
-    template <int COLS> __device__ void tile(const TileOut &o) const {
+    static constexpr bool kChained = false;
+    using Ahead = NoAhead;
+    template <int COLS> __device__ void ahead(const TileOut &, Ahead &) const {}
+    template <int COLS> __device__ void tile(const TileOut &o, Ahead &) const {
         const float x = factor ? factor[o.z] : constant;
         const int row = o.row + o.lane;
         for (int c = 0; c < COLS && o.col + c < M; c += 64) {
             const int col = o.col + c;
             if (col > o.row + 31) continue;                      // above the diagonal: the mirror image of what another warp has
-            put_symmetric<SPLIT>(o, maps, c, col + 63 < o.row, [&](int h, float (&v)[16]) {
+            boxes_free(o);
+            put_symmetric<SPLIT>(o, to, c, col + 63 < o.row, [&](int h, float (&v)[16]) {
                 read16f(o.taddr + (unsigned)(c + 16 * h), v, o.ok);
 #pragma unroll
                 for (int j = 0; j < 16; ++j) v[j] = v[j] * x * x * scale;
@@ -190,7 +232,7 @@ template <bool SPLIT> struct GramOut {
                 if (d >= 0 && row < M) {
 #pragma unroll
                     for (int j = 0; j < 16; ++j)
-                        if (j == d) rest[(size_t)o.z * (size_t)M + (size_t)row] = v[j] - high_of(v[j]);
+                        if (j == d) rest[(size_t)o.z * to.ld + (size_t)row] = v[j] - high_of(v[j]);
                 }
             });
         }
@@ -199,51 +241,60 @@ template <bool SPLIT> struct GramOut {
 
 // ---- P = b A + c A^2, held times 2^e ----
 template <bool SPLIT> struct PolyOut {
-    SymmetricMaps maps;
+    SymmetricOut to;
     int M;
-    const unsigned short *high, *low;
-    uint64_t ld, apart;
+    CUtensorMap map[2];              // A's high and low parts
     float b, c;                      // b 2^(e - e_A), c 2^(e - 2 e_A)
-    const float *rest_a;
-    float *whole, *rest;             // the diagonal, and what rounding takes from it
+    const float *rest;               // of A
+    float a, back;                   // 2^-e
+    float *of_high, *of_low;         // what the parts of X are multiplied by beside the product: a + what rounding takes from the diagonal of P, a + the diagonal
 
-    template <int COLS> __device__ void tile(const TileOut &o) const {
+    static constexpr bool kChained = false;
+    using Ahead = NoAhead;
+    __device__ __forceinline__ bool wanted(const TileOut &o, int c) const { return o.col + c < M && o.col + c <= o.row + 31; }
+    template <int COLS> __device__ __forceinline__ void ahead(const TileOut &o, Ahead &) const {
+        if (wanted(o, 0)) boxes_ask(o, &map[0], SPLIT ? &map[1] : nullptr, o.col);
+    }
+    template <int COLS> __device__ __forceinline__ void tile(const TileOut &o, Ahead &) const {
         const int row = o.row + o.lane;
-        const float *ra = rest_a + (size_t)o.z * (size_t)M;
+        const float *ra = rest + (size_t)o.z * to.ld;
         const float mine = !SPLIT && row < M ? ra[row] : 0.0f;
-        for (int at = 0; at < COLS && o.col + at < M; at += 64) {
+        for (int at = 0; at < COLS && wanted(o, at); at += 64) {
             const int col = o.col + at;
-            if (col > o.row + 31) continue;
-            put_symmetric<SPLIT>(o, maps, at, col + 63 < o.row, [&](int h, float (&v)[16]) {
+            if (at) boxes_ask(o, &map[0], SPLIT ? &map[1] : nullptr, col);
+            boxes_wait(o);
+            put_symmetric<SPLIT>(o, to, at, col + 63 < o.row, [&](int h, float (&v)[16]) {
                 const int c0 = col + 16 * h;
-                float p[16], q[16], r[16];
+                float r[16];
+                if (!SPLIT && c0 < M) load16f(ra + c0, r);
+                else
 #pragma unroll
-                for (int j = 0; j < 16; ++j) p[j] = q[j] = r[j] = 0.0f;
-                if (row < M && c0 < M) {
-                    const size_t i = (size_t)o.z * apart + (size_t)row * ld + (size_t)c0;
-                    load16h(high + i, p);
-                    if (SPLIT) load16h(low + i, q);
-                    else {
+                    for (int j = 0; j < 16; ++j) r[j] = 0.0f;
+                unsigned wp[8], wq[8];
+                box_take16(o, 0, h, wp);
+                if (SPLIT) box_take16(o, 1, h, wq);
+                read16f(o.taddr + (unsigned)(at + 16 * h), v, o.ok);
 #pragma unroll
-                        for (int j = 0; j < 16; ++j)
-                            if (c0 + j < M) r[j] = ra[c0 + j];
+                for (int j = 0; j < 8; ++j) {
+                    // A_ij = p + [i = j] rest_i, of which the product has p only
+                    const float2 p = pair_of(wp[j]);
+                    if (SPLIT) {
+                        const float2 q = pair_of(wq[j]);
+                        v[2 * j] = fmaf(c, v[2 * j], b * (p.x + q.x));
+                        v[2 * j + 1] = fmaf(c, v[2 * j + 1], b * (p.y + q.y));
+                    } else {
+                        v[2 * j] = fmaf(c, fmaf(p.x, mine + r[2 * j], v[2 * j]), b * p.x);
+                        v[2 * j + 1] = fmaf(c, fmaf(p.y, mine + r[2 * j + 1], v[2 * j + 1]), b * p.y);
                     }
                 }
-                read16f(o.taddr + (unsigned)(at + 16 * h), v, o.ok);
                 const int d = SPLIT ? -1 : diagonal_at(row, c0);
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    // A_ij = p + [i = j] rest_i, of which the product has p only
-                    const float a = SPLIT ? p[j] + q[j] : j == d ? p[j] + mine : p[j];
-                    const float squares = SPLIT ? v[j] : fmaf(p[j], mine + r[j], v[j]) + (j == d ? mine * mine : 0.0f);
-                    v[j] = fmaf(c, squares, b * a);
-                }
                 if (d >= 0 && row < M) {
 #pragma unroll
                     for (int j = 0; j < 16; ++j)
                         if (j == d) {
-                            whole[(size_t)o.z * (size_t)M + (size_t)row] = v[j];
-                            rest[(size_t)o.z * (size_t)M + (size_t)row] = v[j] - high_of(v[j]);
+                            v[j] += mine * fmaf(c, mine, b);
+                            of_high[(size_t)o.z * to.ld + (size_t)row] = fmaf(v[j] - high_of(v[j]), back, a);
+                            of_low[(size_t)o.z * to.ld + (size_t)row] = fmaf(v[j], back, a);
                         }
                 }
             });
@@ -257,93 +308,103 @@ struct OrthOut {
     uint64_t ld[kOrthMost];
 };
 template <bool SPLIT> struct StepOut {
-    CUtensorMap map[2];              // of the next X, high and low
+    CUtensorMap map[2], next[2];     // X and the next X, high and low
     int M, N;
     bool tall;                       // the diagonal of P goes with the columns
     bool last;
     int type;                        // of the result
-    const unsigned short *high, *low;
-    uint64_t ld, apart;
     const float *factor;             // of X, one for each matrix, or null
     float constant;                  // ... for all
     float a, back, scale;            // P is held times 1 / back; the next X is held times `scale` (or the result is multiplied by it)
-    const float *whole, *rest;
-    int side;                        // of P
+    const float *of_high, *of_low;   // (SPLIT: a)
+    uint64_t ld_p;                   // of P: distance of the matrices' diagonals
     OrthOut out;                     // (last)
 
-    __device__ __forceinline__ void values(const TileOut &o, int row, int c, float x, float mine, float mine_low, float (&v)[16]) const {
-        const int c0 = o.col + c;
-        float p[16], q[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) p[j] = q[j] = 0.0f;
-        if (row < M && c0 < N) {
-            const size_t i = (size_t)o.z * apart + (size_t)row * ld + (size_t)c0;
-            load16h(high + i, p);
-            load16h(low + i, q);
+    static constexpr bool kChained = false;
+    struct Ahead {
+        float of_sum, of_p, of_q;
+    };
+    template <int COLS> __device__ __forceinline__ void ahead(const TileOut &o, Ahead &n) const {
+        boxes_ask(o, &map[0], &map[1], o.col);
+        const float x = (factor ? factor[o.z] : constant) * scale;
+        const int row = o.row + o.lane;
+        n.of_sum = x * back;
+        n.of_p = n.of_q = SPLIT ? a * x : x;
+        if (!SPLIT && !tall && row < M) {
+            n.of_p = x * of_high[(size_t)o.z * ld_p + (size_t)row];
+            n.of_q = x * of_low[(size_t)o.z * ld_p + (size_t)row];
         }
-        read16f(o.taddr + (unsigned)c, v, o.ok);
+    }
+    // 16 columns of the next X
+    __device__ __forceinline__ void values(const TileOut &o, const Ahead &n, int c, int h, float (&v)[16]) const {
+        unsigned wp[8], wq[8];
+        box_take16(o, 0, h, wp);
+        box_take16(o, 1, h, wq);
+        read16f(o.taddr + (unsigned)(c + 16 * h), v, o.ok);
+        if (!SPLIT && tall) {
+            float e[16], d[16];
+            const size_t k = (size_t)o.z * ld_p + (size_t)min(o.col + c + 16 * h, (int)ld_p - 16);
+            load16f(of_high + k, e);
+            load16f(of_low + k, d);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            float s;
-            if (SPLIT) {
-                s = fmaf(a, p[j], fmaf(a, q[j], v[j] * back));
-            } else {
-                float e = mine, d = mine_low;
-                if (tall) {
-                    const size_t k = (size_t)o.z * (size_t)side + (size_t)min(c0 + j, side - 1);
-                    e = rest[k];
-                    d = whole[k];
-                }
-                s = fmaf(fmaf(e, back, a), p[j], fmaf(fmaf(d, back, a), q[j], v[j] * back));
+            for (int j = 0; j < 8; ++j) {
+                const float2 p = pair_of(wp[j]), q = pair_of(wq[j]);
+                v[2 * j] = fmaf(n.of_p, fmaf(e[2 * j], p.x, d[2 * j] * q.x), n.of_sum * v[2 * j]);
+                v[2 * j + 1] = fmaf(n.of_p, fmaf(e[2 * j + 1], p.y, d[2 * j + 1] * q.y), n.of_sum * v[2 * j + 1]);
             }
-            v[j] = s * x * scale;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float2 p = pair_of(wp[j]), q = pair_of(wq[j]);
+                v[2 * j] = fmaf(n.of_p, p.x, fmaf(n.of_q, q.x, n.of_sum * v[2 * j]));
+                v[2 * j + 1] = fmaf(n.of_p, p.y, fmaf(n.of_q, q.y, n.of_sum * v[2 * j + 1]));
+            }
         }
     }
 
-    template <int COLS> __device__ void tile(const TileOut &o) const {
-        const int row = o.row + o.lane;
-        const float x = factor ? factor[o.z] : constant;
-        const bool wide = !SPLIT && !tall && row < M;
-        const float mine = wide ? rest[(size_t)o.z * (size_t)side + (size_t)row] : 0.0f, mine_low = wide ? whole[(size_t)o.z * (size_t)side + (size_t)row] : 0.0f;
-        if (!last) {
-            for (int c = 0; c < COLS && o.col + c < N; c += 64) {
-                unsigned char *box = box_next(o);
-                if (o.lane == 0) bulk_wait_read_all();           // (both boxes: high and low)
-                __syncwarp();
-                unsigned char *other = o.boxes + (unsigned)*o.which * kG16Box;
-#pragma unroll 1
+    template <int COLS> __device__ __forceinline__ void tile(const TileOut &o, Ahead &n) const {
+        for (int c = 0; c < COLS && o.col + c < N; c += 64) {
+            const int col = o.col + c;
+            if (c) boxes_ask(o, &map[0], &map[1], col);
+            boxes_wait(o);
+            if (!last) {
+#pragma unroll
                 for (int h = 0; h < 4; ++h) {
                     float v[16];
-                    values(o, row, c + 16 * h, x, mine, mine_low, v);
-                    put_parts(box, other, o.lane, h, v);
+                    unsigned p[8], q[8];
+                    values(o, n, c, h, v);
+                    split16(v, p, q);
+                    box_give16(o, 0, h, p);
+                    box_give16(o, 1, h, q);
                 }
-                box_send(o, &map[0], o.col + c, o.row, box);
-                *o.which ^= 1;
-                box_send(o, &map[1], o.col + c, o.row, other);
+                box_send(o, &next[0], col, o.row, o.boxes);
+                box_send(o, &next[1], col, o.row, o.boxes + kG16Box);
+                continue;
             }
-            return;
-        }
-        void *to = out.at[o.z];
-        const long ld_out = (long)out.ld[o.z];
-        const int per = type == kF32 ? 32 : 64;
-        for (int c = 0; c < COLS && o.col + c < N; c += per) {
-            unsigned char *box = box_next(o);
-#pragma unroll 1
-            for (int h = 0; h < per / 16; ++h) {
-                float v[16];
-                values(o, row, c + 16 * h, x, mine, mine_low, v);
-                if (type == kF32) {
-                    uint4 *line = reinterpret_cast<uint4 *>(box + o.lane * 128);
+            const long ld_out = (long)out.ld[o.z];
+            if (type == kF32) {
+                // (32 columns to a box: both are read before one is written)
+                float v[4][16];
+#pragma unroll
+                for (int h = 0; h < 4; ++h) values(o, n, c, h, v[h]);
+#pragma unroll
+                for (int h = 0; h < 4; ++h)
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
-                        line[(4 * h + j) ^ (o.lane & 7)] = make_uint4(__float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]), __float_as_uint(v[4 * j + 2]), __float_as_uint(v[4 * j + 3]));
-                } else if (type == kBf16) {
-                    box_put16<kBf16>(box, o.lane, h, v);
-                } else {
-                    box_put16<kF16>(box, o.lane, h, v);
-                }
+                        *box_piece(o, h >> 1, 4 * (h & 1) + j) =
+                            make_uint4(__float_as_uint(v[h][4 * j]), __float_as_uint(v[h][4 * j + 1]), __float_as_uint(v[h][4 * j + 2]), __float_as_uint(v[h][4 * j + 3]));
+                box_out_rows(o.boxes, o.lane, out.at[o.z], 4, (long)o.row * ld_out + col, ld_out, M - o.row, N - col);
+                if (col + 32 < N) box_out_rows(o.boxes + kG16Box, o.lane, out.at[o.z], 4, (long)o.row * ld_out + col + 32, ld_out, M - o.row, N - col - 32);
+                continue;
             }
-            box_out(box, o.lane, to, type == kF32 ? 4 : 2, (long)o.row * ld_out + o.col + c, ld_out, M - o.row, N - o.col - c);
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+                float v[16];
+                values(o, n, c, h, v);
+                if (type == kBf16) box_put16<kBf16>(o.boxes, o.lane, h, v);
+                else box_put16<kF16>(o.boxes, o.lane, h, v);
+            }
+            box_out_rows(o.boxes, o.lane, out.at[o.z], 2, (long)o.row * ld_out + col, ld_out, M - o.row, N - col);
         }
     }
 };
@@ -388,7 +449,7 @@ bool split_of(const OrthMatrix &m, int out_type) { return out_type != kBf16 || s
 
 struct Room {
     unsigned short *high[2], *low[2], *a[2], *p[2];
-    float *factor, *rest_a, *whole, *rest;
+    float *factor, *rest, *of_high, *of_low;
     double *parts;
     uint64_t ld_x, apart_x, ld_a, apart_a;
     size_t bytes;
@@ -415,9 +476,9 @@ Room room_of(const OrthMatrix &m, bool split, int count, void *scratch) {
         r.p[i] = reinterpret_cast<unsigned short *>(take(n * r.apart_a * 2));
     }
     r.factor = reinterpret_cast<float *>(take(n * 4));
-    r.rest_a = reinterpret_cast<float *>(take(n * s * 4));
-    r.whole = reinterpret_cast<float *>(take(n * s * 4));
-    r.rest = reinterpret_cast<float *>(take(n * s * 4));
+    r.rest = reinterpret_cast<float *>(take(n * r.ld_a * 4));
+    r.of_high = reinterpret_cast<float *>(take(n * r.ld_a * 4));
+    r.of_low = reinterpret_cast<float *>(take(n * r.ld_a * 4));
     r.parts = reinterpret_cast<double *>(take(n * kNormParts * 8));
     return r;
 }
@@ -440,13 +501,14 @@ Plan plan_of(const OrthCall &c) {
     return p;
 }
 
-bool symmetric_maps(SymmetricMaps *m, unsigned short *const (&to)[2], bool split, uint64_t s, uint64_t ld, uint64_t count, uint64_t apart) {
-    for (int i = 0; i < 2; ++i) {
-        // (whole rows of `ld`: a store never ends inside 16 bytes; what lies behind the last column is not read)
-        const Stack st = {to[split ? i : 0], ld, s, ld, count, apart};
-        if (!map_stack(&m->map[i], st, kF16, 64, 32) || !map_stack(&m->turned[i], st, kF16, 32, 64, CU_TENSOR_MAP_SWIZZLE_NONE)) return false;
-    }
-    return true;
+// (boxes are of whole rows of `ld`: a store never ends inside 16 bytes; what lies behind the last column is not read by a product)
+bool box_maps(CUtensorMap (&map)[2], unsigned short *high, unsigned short *low, uint64_t rows, uint64_t ld, uint64_t count, uint64_t apart) {
+    return map_stack(&map[0], {high, ld, rows, ld, count, apart}, kF16, 64, 32) && map_stack(&map[1], {low, ld, rows, ld, count, apart}, kF16, 64, 32);
+}
+bool symmetric_out(SymmetricOut *m, unsigned short *high, unsigned short *low, uint64_t s, uint64_t ld, uint64_t count, uint64_t apart) {
+    m->ld = ld;
+    return box_maps(m->map, high, low, s, ld, count, apart) && map_stack(&m->turned[0], {high, ld, s, ld, count, apart}, kF16, 32, 64, CU_TENSOR_MAP_SWIZZLE_NONE) &&
+           map_stack(&m->turned[1], {low, ld, s, ld, count, apart}, kF16, 32, 64, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
 template <bool SPLIT>
@@ -462,19 +524,32 @@ cudaError_t run_group(const OrthCall &c, const std::vector<StepScale> &scales, c
         out.at[i] = m[i]->out;
         out.ld[i] = m[i]->ld_out;
     }
-    in.rows = rows;
-    in.cols = cols;
+    in.rows = (unsigned)rows;
+    in.cols = (unsigned)cols;
     in.type = m[0]->type;
-    const unsigned parts = (unsigned)std::min<uint64_t>(kNormParts, (rows * cols + kNormChunk - 1) / kNormChunk);
-    cudaError_t err = launch_chained(orth_norm_kernel, dim3(parts, (unsigned)count), kNormThreads, 0, stream, in, r.parts);
-    if (err != cudaSuccess) return err;
-    const OrthX x0 = {r.high[0], r.low[0], r.ld_x, r.apart_x, r.factor};
-    const unsigned blocks = (unsigned)std::min<uint64_t>((rows * r.ld_x + kNormThreads * 4 - 1) / (kNormThreads * 4), std::max(1, sm_count * 8 / count));
-    err = launch_chained(orth_begin_kernel, dim3(blocks, (unsigned)count), kNormThreads, 0, stream, in, (const double *)r.parts, (int)parts, c.eps, x0);
+    const uint64_t size = (uint64_t)op_bytes(in.type);
+    for (int i = 0; i < count; ++i) in.whole[i] = (reinterpret_cast<uintptr_t>(in.at[i]) | (rows > 1 ? in.ld[i] * size : 0)) % 16 == 0;
+    const uint64_t share = std::max(1, sm_count * 4 / count);    // CTAs of a matrix that run at a time
+    const unsigned parts = (unsigned)std::min<uint64_t>(std::min<uint64_t>(kNormParts, share), (rows * cols + kNormChunk - 1) / kNormChunk);
+    const unsigned blocks = (unsigned)std::min<uint64_t>(share, (rows * r.ld_x / 8 + kNormThreads * 2 - 1) / (kNormThreads * 2));
+    const OrthX x0 = {r.high[0], r.low[0], (unsigned)r.ld_x, r.apart_x, r.factor};
+    const dim3 norm_grid(parts, (unsigned)count), begin_grid(blocks, (unsigned)count);
+    cudaError_t err;
+    if (in.type == kF32) {
+        err = launch_chained(orth_norm_kernel<kF32>, norm_grid, kNormThreads, 0, stream, in, r.parts);
+        if (err == cudaSuccess) err = launch_chained(orth_begin_kernel<kF32>, begin_grid, kNormThreads, 0, stream, in, (const double *)r.parts, (int)parts, c.eps, x0);
+    } else if (in.type == kBf16) {
+        err = launch_chained(orth_norm_kernel<kBf16>, norm_grid, kNormThreads, 0, stream, in, r.parts);
+        if (err == cudaSuccess) err = launch_chained(orth_begin_kernel<kBf16>, begin_grid, kNormThreads, 0, stream, in, (const double *)r.parts, (int)parts, c.eps, x0);
+    } else {
+        err = launch_chained(orth_norm_kernel<kF16>, norm_grid, kNormThreads, 0, stream, in, r.parts);
+        if (err == cudaSuccess) err = launch_chained(orth_begin_kernel<kF16>, begin_grid, kNormThreads, 0, stream, in, (const double *)r.parts, (int)parts, c.eps, x0);
+    }
     if (err != cudaSuccess) return err;
 
-    SymmetricMaps maps_a, maps_p;
-    if (!symmetric_maps(&maps_a, r.a, SPLIT, s, r.ld_a, (uint64_t)count, r.apart_a) || !symmetric_maps(&maps_p, r.p, SPLIT, s, r.ld_a, (uint64_t)count, r.apart_a)) return cudaErrorInvalidValue;
+    SymmetricOut to_a, to_p;
+    if (!symmetric_out(&to_a, r.a[0], r.a[SPLIT], s, r.ld_a, (uint64_t)count, r.apart_a) || !symmetric_out(&to_p, r.p[0], r.p[SPLIT], s, r.ld_a, (uint64_t)count, r.apart_a))
+        return cudaErrorInvalidValue;
     Gemm16 g = {};
     g.batch = count;
     g.splits = 1;
@@ -497,7 +572,7 @@ cudaError_t run_group(const OrthCall &c, const std::vector<StepScale> &scales, c
         g.M = g.N = (int)s;
         g.lower = true;
         g.a_kmajor = g.b_kmajor = !tall;
-        GramOut<SPLIT> gram = {maps_a, (int)s, factor, constant, std::ldexp(1.0f, k.a), r.rest_a};
+        GramOut<SPLIT> gram = {to_a, (int)s, factor, constant, std::ldexp(1.0f, k.a), r.rest};
         if ((err = launch_gemm16(ops, gram, g, std::max(rows, cols), pairs_s, status, sm_count, stream)) != cudaSuccess) return err;
         // P
         for (int i = 0; i < 2; ++i) {
@@ -506,7 +581,8 @@ cudaError_t run_group(const OrthCall &c, const std::vector<StepScale> &scales, c
             ops.b[i] = ops.a[i];
         }
         g.a_kmajor = g.b_kmajor = true;
-        PolyOut<SPLIT> poly = {maps_p, (int)s, r.a[0], r.a[1], r.ld_a, r.apart_a, std::ldexp(co[1], k.p - k.a), std::ldexp(co[2], k.p - 2 * k.a), r.rest_a, r.whole, r.rest};
+        PolyOut<SPLIT> poly = {to_p, (int)s, {to_a.map[0], to_a.map[1]}, std::ldexp(co[1], k.p - k.a), std::ldexp(co[2], k.p - 2 * k.a), r.rest,
+                               co[0], std::ldexp(1.0f, -k.p), r.of_high, r.of_low};
         if ((err = launch_gemm16(ops, poly, g, s, pairs_s, status, sm_count, stream)) != cudaSuccess) return err;
         // X
         for (int i = 0; i < 2; ++i) {
@@ -519,25 +595,22 @@ cudaError_t run_group(const OrthCall &c, const std::vector<StepScale> &scales, c
         g.a_kmajor = true;
         g.b_kmajor = tall;
         StepOut<SPLIT> e = {};
-        for (int i = 0; i < 2; ++i)
-            if (!map_stack(&e.map[i], {i ? r.low[now ^ 1] : r.high[now ^ 1], r.ld_x, rows, r.ld_x, (uint64_t)count, r.apart_x}, kF16, 64, 32)) return cudaErrorInvalidValue;
+        if (!box_maps(e.map, r.high[now], r.low[now], rows, r.ld_x, (uint64_t)count, r.apart_x) ||
+            !box_maps(e.next, r.high[now ^ 1], r.low[now ^ 1], rows, r.ld_x, (uint64_t)count, r.apart_x))
+            return cudaErrorInvalidValue;
         e.M = (int)rows;
         e.N = (int)cols;
         e.tall = tall;
         e.last = last;
         e.type = c.out_type;
-        e.high = r.high[now];
-        e.low = r.low[now];
-        e.ld = r.ld_x;
-        e.apart = r.apart_x;
         e.factor = factor;
         e.constant = constant;
         e.a = co[0];
         e.back = std::ldexp(1.0f, -k.p);
         e.scale = last ? c.scale : std::ldexp(1.0f, scales[(size_t)step + 1].x);
-        e.whole = r.whole;
-        e.rest = r.rest;
-        e.side = (int)s;
+        e.of_high = r.of_high;
+        e.of_low = r.of_low;
+        e.ld_p = r.ld_a;
         e.out = out;
         if ((err = launch_gemm16(ops, e, g, s, pairs_x, status, sm_count, stream)) != cudaSuccess) return err;
     }

@@ -2,10 +2,10 @@
 //   loss_t = lse_t - (1 - e) l_t,target - e / vocab sum_v l_tv,   lse_t = log sum_v exp l_tv
 //   dl_tv = g_t (exp(l_tv - lse_t) - (1 - e) [v = target] - e / vocab),   dx = dl W,   dW = dl^T x
 //
-// Loss: one product whose epilogue leaves, for each token and tile of 256 (128) of the vocabulary, the largest logit and the sum of exponentials against it, and the target's
+// Loss: one product whose epilogue leaves, for each token and 128 (64) columns of the vocabulary, the largest logit and the sum of exponentials against it, and the target's
 // logit; xent_join_kernel joins a token's tiles.  Nothing of size tokens x vocab is written.
 // Gradient: the vocabulary goes by in pieces of at most 128 MB of dl.  Of a piece the logits are computed again, the epilogue turns them into dl in 16 bits (the
-// rounding that a 16-bit gradient of logits has anyway: 1.7e-3 of each element, independent of one another; FP16 is scaled by a power of two so that g's smallness does not cost bits), then
+// rounding that a 16-bit gradient of logits has anyway; scaled, see xent_coef_kernel), then
 // dW of the piece is complete, and dx is summed over the pieces in FP32.
 //
 // Exponents are taken in base 2, and the reference of a tile is the rounded product of its largest logit and log2(e), so that the rounding cancels.
@@ -30,49 +30,44 @@ __device__ __forceinline__ float exp2_fast(float x) {
 struct XentStats {
     int M, N;
     const long long *target;
-    float2 *parts;                   // tiles along N x M: (largest logit) * log2 e, sum of exponentials against it
+    float2 *parts;                   // a warp's columns x M: (largest logit) * log2 e, sum of exponentials against it
     float *sums;                     // the same: sum of logits (nullable: no smoothing)
     float *at_target;                // M
 
-    template <int COLS> __device__ void tile(const TileOut &o) const {
-        const int row = o.row + o.lane, n = min(COLS, N - o.col);
-        float top = __uint_as_float(0xff800000u), s = 0.0f, total = 0.0f;
-        for (int c = 0; c < n; c += 32) {
-            float v[32];
-            read32f(o.taddr + (unsigned)c, v, o.ok);
-            if (sums) {
+    static constexpr bool kChained = true;
+    using Ahead = NoAhead;
+    template <int COLS> __device__ __forceinline__ void tile(const TileOut &o, float (&v)[COLS]) const {
+        const int row = o.row + o.lane, n = N - o.col;
+        const float none = __uint_as_float(0xff800000u);
+        if (n < COLS) {
 #pragma unroll
-                for (int j = 0; j < 32; ++j) total += c + j < n ? v[j] : 0.0f;
-            }
-            if (c + 32 > n) {
+            for (int j = 0; j < COLS; ++j)
+                if (j >= n) v[j] = none;
+        }
+        float top = v[0];
 #pragma unroll
-                for (int j = 0; j < 32; ++j)
-                    if (c + j >= n) v[j] = __uint_as_float(0xff800000u);
-            }
-            float m = v[0];
+        for (int j = 1; j < COLS; ++j) top = fmaxf(top, v[j]);
+        top *= kLog2E;
+        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int j = 1; j < 32; ++j) m = fmaxf(m, v[j]);
-            m *= kLog2E;
-            if (m > top) {
-                s *= exp2_fast(top - m);
-                top = m;
-            }
+        for (int j = 0; j < COLS; ++j) s[j & 3] += exp2_fast(fmaf(v[j], kLog2E, -top));
+        const size_t at = (size_t)(o.col / COLS) * (size_t)M + (size_t)row;
+        if (row < M) parts[at] = make_float2(top, (s[0] + s[1]) + (s[2] + s[3]));
+        if (sums) {
+            float total[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int j = 0; j < 32; ++j) s += exp2_fast(fmaf(v[j], kLog2E, -top));
+            for (int j = 0; j < COLS; ++j) total[j & 3] += j < n ? v[j] : 0.0f;
+            if (row < M) sums[at] = (total[0] + total[1]) + (total[2] + total[3]);
         }
         const long long off = row < M ? target[row] - o.col : -1;
-        const bool here = off >= 0 && off < n;
-        float mine = 0.0f;
-        for (unsigned left = __ballot_sync(kFullMask, here); left; left &= left - 1) {
-            const int src = __ffs(left) - 1;
-            const float l = read_column(o.taddr + (unsigned)__shfl_sync(kFullMask, (int)off, src), o.ok);
-            if (o.lane == src) mine = l;
+        const bool here = off >= 0 && off < COLS && off < n;
+        if (__any_sync(kFullMask, here)) {
+            float mine = 0.0f;
+#pragma unroll
+            for (int j = 0; j < COLS; ++j)
+                if (j == (int)off) mine = v[j];
+            if (here) at_target[row] = mine;
         }
-        if (row >= M) return;
-        const size_t at = (size_t)(o.col / COLS) * (size_t)M + (size_t)row;
-        parts[at] = make_float2(top, s);
-        if (sums) sums[at] = total;
-        if (here) at_target[row] = mine;
     }
 };
 
@@ -176,37 +171,34 @@ struct XentCoef {
     int tokens;
     long long vocab, ignore;
     int reduction;
-    bool f16;
+    float reference;                 // 1 - e + e / vocab, 1 / 4 at least
     const long long *target;
     const float *stats, *grad;
     float *coef, *unscale;           // coefficient of each token; what the products are multiplied by
 };
-// What each token's gradient of logits is multiplied by: g_t, 0 for those that do not count, NaN for a target that is none; times a power of two that brings the
-// largest into [2^13, 2^14) where dl is FP16 (|dl| is at most that).  One CTA.
+// What each token's gradient of logits is multiplied by: g_t, 0 for those that do not count, NaN for a target that is none; times what makes the largest |g| (1 - e + e / vocab) 2^13.
+// That keeps small gradients within FP16's range (|dl| stays below 2^15), and it makes the element of a target that has next to no probability, the largest of its row and the same in
+// all rows where the g are, a number that 16 bits hold: rounded, it was off by the same part of up to 2^-8 in every row, and so were dx and dW (4096 x 4096 x 32000 in BF16 up to
+// 2.9e-3 off; 1.7e-3 is what their own rounding takes).  One CTA.
 __global__ void __launch_bounds__(1024) xent_coef_kernel(const XentCoef c) {
     chain_begin();
     __shared__ float room[32];
     const float one = c.reduction == kXentNone ? 0.0f : c.reduction == kXentMean ? *c.grad / c.stats[c.tokens] : *c.grad;
-    float scale = 1.0f, back = 1.0f;
-    if (c.f16) {
-        float m = fabsf(one);
-        if (c.reduction == kXentNone) {
-            for (int i = threadIdx.x; i < c.tokens; i += 1024) {
-                const float a = fabsf(c.grad[i]);
-                if (c.target[i] != c.ignore && a < __uint_as_float(0x7f800000u)) m = fmaxf(m, a);
-            }
-            m = warp_max(m);
-            if ((threadIdx.x & 31) == 0) room[threadIdx.x >> 5] = m;
-            __syncthreads();
-            m = warp_max(room[threadIdx.x & 31]);
+    float m = fabsf(one);
+    if (c.reduction == kXentNone) {
+        for (int i = threadIdx.x; i < c.tokens; i += 1024) {
+            const float a = fabsf(c.grad[i]);
+            if (c.target[i] != c.ignore && a < __uint_as_float(0x7f800000u)) m = fmaxf(m, a);
         }
-        if (m > 0.0f && m < __uint_as_float(0x7f800000u)) {
-            const int e = min(max(13 - ilogbf(m), -100), 100);
-            scale = exp2f((float)e);
-            back = exp2f((float)-e);
-        }
+        m = warp_max(m);
+        if ((threadIdx.x & 31) == 0) room[threadIdx.x >> 5] = m;
+        __syncthreads();
+        m = warp_max(room[threadIdx.x & 31]);
     }
-    if (threadIdx.x == 0) *c.unscale = back;
+    // (a gradient of 0, Inf or NaN goes through as it is; below 2^-100 the scale stays finite)
+    const float top = m > 0.0f && m < __uint_as_float(0x7f800000u) ? fmaxf(m, 7.888609052e-31f) * c.reference : 8192.0f;
+    const float scale = 8192.0f / top;
+    if (threadIdx.x == 0) *c.unscale = top * (1.0f / 8192.0f);
     for (int i = threadIdx.x; i < c.tokens; i += 1024) {
         const long long t = c.target[i];
         float g = (c.reduction == kXentNone ? c.grad[i] : one) * scale;
@@ -224,7 +216,10 @@ template <int TYPE> struct XentGrad {
     const float *lse2, *coef;
     float low, high;                 // e / vocab, 1 - e
 
-    template <int COLS> __device__ void tile(const TileOut &o) const {
+    static constexpr bool kChained = false;
+    using Ahead = NoAhead;
+    template <int COLS> __device__ void ahead(const TileOut &, Ahead &) const {}
+    template <int COLS> __device__ void tile(const TileOut &o, Ahead &) const {
         const int row = o.row + o.lane;
         const long long t = row < M ? target[row] : ignore;
         const bool live = t != ignore;
@@ -274,7 +269,10 @@ template <int TYPE> struct ProductOut {
     long ld_sum;
     const float *factor;
 
-    template <int COLS> __device__ void tile(const TileOut &o) const {
+    static constexpr bool kChained = false;
+    using Ahead = NoAhead;
+    template <int COLS> __device__ void ahead(const TileOut &, Ahead &) const {}
+    template <int COLS> __device__ void tile(const TileOut &o, Ahead &) const {
         if (mode == kSumFirst || mode == kSumMore) {
             for (int c = 0; c < COLS && o.col + c < N; c += 32) {
                 unsigned char *box = box_next(o);
@@ -312,7 +310,7 @@ template <int TYPE> struct ProductOut {
                 box_put16<TYPE>(box, o.lane, h, v);
             }
             if (boxes) box_send(o, &map, o.col + c, o.row, box);
-            else box_out(box, o.lane, out, 2, (long)o.row * ld + o.col + c, ld, M - o.row, N - o.col - c);
+            else box_out_rows(box, o.lane, out, 2, (long)o.row * ld + o.col + c, ld, M - o.row, N - o.col - c);
         }
     }
 };
@@ -392,7 +390,7 @@ struct LossPlan {
 LossPlan loss_plan(const XentCall &c, int sm_count) {
     LossPlan p;
     p.pairs = g16_pairs(c.tokens, c.vocab, 1, false, sm_count);
-    p.tiles = p.pairs ? (c.vocab + 255) / 256 : (c.vocab + 127) / 128;
+    p.tiles = p.pairs ? (c.vocab + 127) / 128 : (c.vocab + 63) / 64;
     return p;
 }
 struct LossRoom {
@@ -579,7 +577,8 @@ cudaError_t xent_grad(const XentCall &c, const float *stats, const float *grad, 
     if (err != cudaSuccess) return err;
     const GradPlan p = grad_plan(c, dx != nullptr, sm_count);
     const GradRoom r = grad_room(c, p, dx != nullptr, &s);
-    const XentCoef k = {(int)c.tokens, (long long)c.vocab, c.ignore, c.reduction, c.type == kF16, c.target, stats, grad, r.coef, r.unscale};
+    const XentCoef k = {(int)c.tokens, (long long)c.vocab, c.ignore, c.reduction,
+                        (float)std::max(0.25, 1.0 - c.smoothing + c.smoothing / (double)c.vocab), c.target, stats, grad, r.coef, r.unscale};
     err = launch_chained(xent_coef_kernel, 1, 1024, 0, stream, k);
     if (err != cudaSuccess) return err;
     return c.type == kBf16 ? grad_pieces<kBf16>(c, p, r, o, stats, dx, ld_dx, dw, ld_dw, status, sm_count, stream)
