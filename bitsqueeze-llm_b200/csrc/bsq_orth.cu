@@ -7,11 +7,12 @@
 //     large singular values' rounding is what the small ones start from (rank-8 gradients with noise: 4e-3 off after five steps, this way 1e-4);
 //   * the diagonals of A and of P = b A + c A^2, of size 1 where everything else is small, are kept in FP32: what rounding takes from them, and what the
 //     products leave out of the low part (P_ii X_low), goes back in the epilogues (noise: 1.9e-3 off without, 0.2e-3 to 0.7e-3 with it; a rounding to BF16 is 1.7e-3).
-// Results in FP32 or FP16, and matrices with a short side of up to 128 (where launches are what a step costs), take both parts of every operand: three products of halves.
+// Results in FP32 or FP16 take both parts of every operand: three products of halves.  BF16 results of matrices with a short side of up to 128, where launches are what a step costs, are
+// bsq_orth_small.cu's.
 //
 // A and P are symmetric: tiles on and below the diagonal are computed, and written twice.  Bound by the tensor core, then by power.
 #include "bsq_gemm16.cuh"
-#include "bsq_orth.hpp"
+#include "bsq_orth_small.hpp"
 
 #include <algorithm>
 #include <cmath>
@@ -21,9 +22,7 @@
 namespace bsq {
 namespace {
 
-constexpr int kOrthMost = 64;                                    // matrices of a launch
 constexpr uint64_t kOrthRoom = 1ull << 30;                       // scratch that several matrices share at most
-constexpr uint64_t kSplitShort = 128;                            // short sides up to this: split operands
 constexpr int kNormThreads = 512;
 constexpr uint64_t kNormChunk = 16384;                           // elements of a CTA of the pass that finds the norms, at least
 constexpr int kNormParts = kNormThreads;
@@ -415,9 +414,12 @@ uint64_t up(uint64_t n, uint64_t to) { return (n + to - 1) / to * to; }
 // Powers of two that X, A and P of a step are held times: largest magnitudes below 2^15
 struct StepScale {
     int x, a, p;
+    double most;                     // the largest singular value that X may have
 };
 int below_2_15(double most) { return std::min(24, std::max(-14, most > 0.0 ? (int)std::floor(std::log2(32768.0 / most)) : 14)); }
 // Largest singular value that each step may meet, from 0 .. 1 at the start; false: it grows beyond 1000
+// (the polynomials are smooth: 256 points are within 1e-4 of their largest values, for which the scales leave a factor of two)
+constexpr int kPoints = 256;
 bool scales_of(const float *k, int steps, std::vector<StepScale> *out) {
     double most = 1.0;
     for (int i = 0; i < steps; ++i, k += 3) {
@@ -425,13 +427,13 @@ bool scales_of(const float *k, int steps, std::vector<StepScale> *out) {
         if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c)) return false;
         double next = 0.0, p = 0.0;
         const double top = most * 1.02;                          // (room for what rounding adds)
-        for (int j = 0; j <= 4096; ++j) {
-            const double s = top * j / 4096, l = s * s, y = b * l + c * l * l;
+        for (int j = 0; j <= kPoints; ++j) {
+            const double s = top * j / kPoints, l = s * s, y = b * l + c * l * l;
             p = std::max(p, std::fabs(y));
             next = std::max(next, std::fabs((a + y) * s));
         }
         if (!(next < 1000.0) || !(p < 1e6)) return false;
-        if (out) out->push_back({below_2_15(top), below_2_15(top * top), below_2_15(p)});
+        out->push_back({below_2_15(top), below_2_15(top * top), below_2_15(p), top});
         most = std::max(next, 1e-30);
     }
     return true;
@@ -445,16 +447,22 @@ struct Plan {
     std::vector<int> order;
     std::vector<Group> groups;
 };
-bool split_of(const OrthMatrix &m, int out_type) { return out_type != kBf16 || std::min(m.rows, m.cols) <= kSplitShort; }
+enum Way { kHigh, kSplit, kSmall };                              // products of the high parts, of both parts; few rows or columns
+// tame: the steps' polynomial stays within what its coefficients may grow by (small_steps)
+Way way_of(const OrthMatrix &m, int out_type, bool tame) {
+    if (out_type != kBf16) return kSplit;
+    return std::min(m.rows, m.cols) > (uint64_t)kOrthSmallSide ? kHigh : tame ? kSmall : kSplit;
+}
 
 struct Room {
     unsigned short *high[2], *low[2], *a[2], *p[2];
     float *factor, *rest, *of_high, *of_low;
     double *parts;
+    OrthSmallRoom small;
     uint64_t ld_x, apart_x, ld_a, apart_a;
     size_t bytes;
 };
-Room room_of(const OrthMatrix &m, bool split, int count, void *scratch) {
+Room room_of(const OrthMatrix &m, Way way, int count, int sm_count, void *scratch) {
     Room r = {};
     const uint64_t s = std::min(m.rows, m.cols), n = (uint64_t)count;
     unsigned char *base = static_cast<unsigned char *>(scratch);
@@ -463,6 +471,15 @@ Room room_of(const OrthMatrix &m, bool split, int count, void *scratch) {
         r.bytes += up(bytes, 128);
         return p;
     };
+    r.parts = reinterpret_cast<double *>(take(n * kNormParts * 8));
+    if (way == kSmall) {
+        r.small.slices = orth_small_slices(std::max(m.rows, m.cols), count, sm_count, &r.small.per);
+        r.small.sums = reinterpret_cast<float *>(take(n * (uint64_t)r.small.slices * s * s * 4));
+        r.small.sum = reinterpret_cast<float *>(take(n * s * s * 4));
+        r.small.q = reinterpret_cast<float *>(take(n * s * s * 4));
+        return r;
+    }
+    const bool split = way == kSplit;
     r.ld_x = up(m.cols, 16);
     r.apart_x = m.rows * r.ld_x;
     r.ld_a = up(s, 16);
@@ -479,11 +496,15 @@ Room room_of(const OrthMatrix &m, bool split, int count, void *scratch) {
     r.rest = reinterpret_cast<float *>(take(n * r.ld_a * 4));
     r.of_high = reinterpret_cast<float *>(take(n * r.ld_a * 4));
     r.of_low = reinterpret_cast<float *>(take(n * r.ld_a * 4));
-    r.parts = reinterpret_cast<double *>(take(n * kNormParts * 8));
     return r;
 }
 
-Plan plan_of(const OrthCall &c) {
+// Scratch of matrices whatever the steps are
+size_t room_for(const OrthMatrix &m, int out_type, int count, int sm_count) {
+    return std::max(room_of(m, way_of(m, out_type, true), count, sm_count, nullptr).bytes, room_of(m, way_of(m, out_type, false), count, sm_count, nullptr).bytes);
+}
+
+Plan plan_of(const OrthCall &c, int sm_count) {
     Plan p;
     for (int i = 0; i < c.n; ++i)
         if (c.m[i].rows && c.m[i].cols) p.order.push_back(i);
@@ -491,7 +512,7 @@ Plan plan_of(const OrthCall &c) {
     std::stable_sort(p.order.begin(), p.order.end(), [&](int i, int j) { return key(i) < key(j); });
     for (int i = 0; i < (int)p.order.size();) {
         const OrthMatrix &m = c.m[p.order[i]];
-        const uint64_t one = room_of(m, split_of(m, c.out_type), 1, nullptr).bytes;
+        const uint64_t one = room_for(m, c.out_type, 1, sm_count);
         const int most = (int)std::min<uint64_t>(kOrthMost, std::max<uint64_t>(1, kOrthRoom / one));
         int n = 1;
         while (n < most && i + n < (int)p.order.size() && key(p.order[i + n]) == key(p.order[i])) ++n;
@@ -511,40 +532,100 @@ bool symmetric_out(SymmetricOut *m, unsigned short *high, unsigned short *low, u
            map_stack(&m->turned[1], {low, ld, s, ld, count, apart}, kF16, 32, 64, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
+// The norms of a group's matrices, as parts of their sums of squares
+cudaError_t norms_of(const OrthMatrix *const *m, int count, OrthIn *in, double *sums, unsigned *parts, int sm_count, cudaStream_t stream) {
+    *in = {};
+    in->rows = (unsigned)m[0]->rows;
+    in->cols = (unsigned)m[0]->cols;
+    in->type = m[0]->type;
+    const uint64_t size = (uint64_t)op_bytes(in->type), share = (uint64_t)std::max(1, sm_count * 4 / count);         // CTAs of a matrix that run at a time
+    for (int i = 0; i < count; ++i) {
+        in->at[i] = m[i]->in;
+        in->ld[i] = m[i]->ld_in;
+        in->whole[i] = (reinterpret_cast<uintptr_t>(in->at[i]) | (in->rows > 1 ? in->ld[i] * size : 0)) % 16 == 0;
+    }
+    *parts = (unsigned)std::min<uint64_t>(std::min<uint64_t>(kNormParts, share), (m[0]->rows * m[0]->cols + kNormChunk - 1) / kNormChunk);
+    const dim3 grid(*parts, (unsigned)count);
+    return in->type == kF32    ? launch_chained(orth_norm_kernel<kF32>, grid, kNormThreads, 0, stream, *in, sums)
+           : in->type == kBf16 ? launch_chained(orth_norm_kernel<kBf16>, grid, kNormThreads, 0, stream, *in, sums)
+                               : launch_chained(orth_norm_kernel<kF16>, grid, kNormThreads, 0, stream, *in, sums);
+}
+
+// A step's operands and what they are held times, from bounds of A, M = a I + P and the Q that has come together; false where Q may grow beyond 1024: rounding grows with its square, and
+// where X has nothing Q still grows (five steps of the usual coefficients: 485)
+bool small_steps(const OrthCall &c, const std::vector<StepScale> &scales, OrthSmallSteps *out) {
+    out->steps = c.steps;
+    double q = 1.0;
+    int of_q = 0;                                                // Q is held times 2^of_q
+    for (int i = 0; i < c.steps; ++i) {
+        const double a = c.coefficients[3 * i], b = c.coefficients[3 * i + 1], k = c.coefficients[3 * i + 2], top = scales[(size_t)i].most;
+        double m = 0.0;
+        for (int j = 0; j <= kPoints; ++j) {
+            const double l = top * top * j / kPoints;
+            m = std::max(m, std::fabs(a + b * l + k * l * l));
+        }
+        const int at = below_2_15(top * top), am = below_2_15(m), t = below_2_15(m * top * top);
+        const int next_a = i + 1 < c.steps ? below_2_15(scales[(size_t)i + 1].most * scales[(size_t)i + 1].most) : 0;
+        q *= m;
+        if (!(q <= 1024.0)) return false;
+        const int next_q = below_2_15(q);
+        OrthSmallStep &s = out->step[i];
+        s.a = at;
+        s.square = std::ldexp((float)k, am - 2 * at);
+        s.linear = std::ldexp((float)b, am - at);
+        s.constant = std::ldexp((float)a, am);
+        s.first_q = std::ldexp(1.0f, next_q - am);
+        s.of_q = std::ldexp(1.0f, next_q - am - of_q);
+        s.of_t = std::ldexp(1.0f, t - am - at);
+        s.of_a = std::ldexp(1.0f, next_a - am - t);
+        s.out = std::ldexp(c.scale, -am - of_q);
+        of_q = next_q;
+    }
+    return true;
+}
+
+cudaError_t run_small(const OrthCall &c, const OrthSmallSteps &steps, const OrthMatrix *const *m, int count, void *scratch, unsigned *status, int sm_count, cudaStream_t stream) {
+    const uint64_t rows = m[0]->rows, cols = m[0]->cols;
+    const Room r = room_of(*m[0], kSmall, count, sm_count, scratch);
+    OrthIn in;
+    unsigned parts;
+    const cudaError_t err = norms_of(m, count, &in, r.parts, &parts, sm_count, stream);
+    if (err != cudaSuccess) return err;
+    OrthSmall g = {};
+    for (int i = 0; i < count; ++i) {
+        g.in[i] = m[i]->in;
+        g.out[i] = m[i]->out;
+        g.ld[i] = m[i]->ld_in;
+        g.ld_out[i] = m[i]->ld_out;
+    }
+    g.s = (int)std::min(rows, cols);
+    g.l = (int)std::max(rows, cols);
+    g.parts = r.parts;
+    g.part_count = (int)parts;
+    g.eps = c.eps;
+    return orth_small(g, rows > cols, in.type, steps, count, r.small, status, stream);
+}
+
 template <bool SPLIT>
 cudaError_t run_group(const OrthCall &c, const std::vector<StepScale> &scales, const OrthMatrix *const *m, int count, void *scratch, unsigned *status, int sm_count, cudaStream_t stream) {
     const uint64_t rows = m[0]->rows, cols = m[0]->cols, s = std::min(rows, cols);
     const bool tall = rows > cols;
-    const Room r = room_of(*m[0], SPLIT, count, scratch);
-    OrthIn in = {};
+    const Room r = room_of(*m[0], SPLIT ? kSplit : kHigh, count, sm_count, scratch);
+    OrthIn in;
     OrthOut out = {};
     for (int i = 0; i < count; ++i) {
-        in.at[i] = m[i]->in;
-        in.ld[i] = m[i]->ld_in;
         out.at[i] = m[i]->out;
         out.ld[i] = m[i]->ld_out;
     }
-    in.rows = (unsigned)rows;
-    in.cols = (unsigned)cols;
-    in.type = m[0]->type;
-    const uint64_t size = (uint64_t)op_bytes(in.type);
-    for (int i = 0; i < count; ++i) in.whole[i] = (reinterpret_cast<uintptr_t>(in.at[i]) | (rows > 1 ? in.ld[i] * size : 0)) % 16 == 0;
-    const uint64_t share = std::max(1, sm_count * 4 / count);    // CTAs of a matrix that run at a time
-    const unsigned parts = (unsigned)std::min<uint64_t>(std::min<uint64_t>(kNormParts, share), (rows * cols + kNormChunk - 1) / kNormChunk);
-    const unsigned blocks = (unsigned)std::min<uint64_t>(share, (rows * r.ld_x / 8 + kNormThreads * 2 - 1) / (kNormThreads * 2));
+    unsigned parts;
+    cudaError_t err = norms_of(m, count, &in, r.parts, &parts, sm_count, stream);
+    if (err != cudaSuccess) return err;
+    const unsigned blocks = (unsigned)std::min<uint64_t>((uint64_t)std::max(1, sm_count * 4 / count), (rows * r.ld_x / 8 + kNormThreads * 2 - 1) / (kNormThreads * 2));
     const OrthX x0 = {r.high[0], r.low[0], (unsigned)r.ld_x, r.apart_x, r.factor};
-    const dim3 norm_grid(parts, (unsigned)count), begin_grid(blocks, (unsigned)count);
-    cudaError_t err;
-    if (in.type == kF32) {
-        err = launch_chained(orth_norm_kernel<kF32>, norm_grid, kNormThreads, 0, stream, in, r.parts);
-        if (err == cudaSuccess) err = launch_chained(orth_begin_kernel<kF32>, begin_grid, kNormThreads, 0, stream, in, (const double *)r.parts, (int)parts, c.eps, x0);
-    } else if (in.type == kBf16) {
-        err = launch_chained(orth_norm_kernel<kBf16>, norm_grid, kNormThreads, 0, stream, in, r.parts);
-        if (err == cudaSuccess) err = launch_chained(orth_begin_kernel<kBf16>, begin_grid, kNormThreads, 0, stream, in, (const double *)r.parts, (int)parts, c.eps, x0);
-    } else {
-        err = launch_chained(orth_norm_kernel<kF16>, norm_grid, kNormThreads, 0, stream, in, r.parts);
-        if (err == cudaSuccess) err = launch_chained(orth_begin_kernel<kF16>, begin_grid, kNormThreads, 0, stream, in, (const double *)r.parts, (int)parts, c.eps, x0);
-    }
+    const dim3 grid(blocks, (unsigned)count);
+    err = in.type == kF32    ? launch_chained(orth_begin_kernel<kF32>, grid, kNormThreads, 0, stream, in, (const double *)r.parts, (int)parts, c.eps, x0)
+          : in.type == kBf16 ? launch_chained(orth_begin_kernel<kBf16>, grid, kNormThreads, 0, stream, in, (const double *)r.parts, (int)parts, c.eps, x0)
+                             : launch_chained(orth_begin_kernel<kF16>, grid, kNormThreads, 0, stream, in, (const double *)r.parts, (int)parts, c.eps, x0);
     if (err != cudaSuccess) return err;
 
     SymmetricOut to_a, to_p;
@@ -619,14 +700,12 @@ cudaError_t run_group(const OrthCall &c, const std::vector<StepScale> &scales, c
 
 }  // namespace
 
-bool orth_steps_ok(const float *coefficients, int steps) { return scales_of(coefficients, steps, nullptr); }
-
-size_t orth_scratch_bytes(const OrthCall &c) {
+size_t orth_scratch_bytes(const OrthCall &c, int sm_count) {
     size_t most = 0;
-    const Plan p = plan_of(c);
+    const Plan p = plan_of(c, sm_count);
     for (const Group &g : p.groups) {
         const OrthMatrix &m = c.m[p.order[(size_t)g.begin]];
-        most = std::max(most, room_of(m, split_of(m, c.out_type), g.count, nullptr).bytes);
+        most = std::max(most, room_for(m, c.out_type, g.count, sm_count));
     }
     return most;
 }
@@ -634,12 +713,16 @@ size_t orth_scratch_bytes(const OrthCall &c) {
 cudaError_t orthogonalize(const OrthCall &c, void *scratch, unsigned *status, int sm_count, cudaStream_t stream) {
     std::vector<StepScale> scales;
     if (!scales_of(c.coefficients, c.steps, &scales)) return cudaErrorInvalidValue;
-    const Plan p = plan_of(c);
+    OrthSmallSteps steps;
+    const bool tame = small_steps(c, scales, &steps);
+    const Plan p = plan_of(c, sm_count);
     for (const Group &g : p.groups) {
         const OrthMatrix *m[kOrthMost];
         for (int i = 0; i < g.count; ++i) m[i] = &c.m[p.order[(size_t)(g.begin + i)]];
-        const cudaError_t err = split_of(*m[0], c.out_type) ? run_group<true>(c, scales, m, g.count, scratch, status, sm_count, stream)
-                                                             : run_group<false>(c, scales, m, g.count, scratch, status, sm_count, stream);
+        const Way way = way_of(*m[0], c.out_type, tame);
+        const cudaError_t err = way == kSmall   ? run_small(c, steps, m, g.count, scratch, status, sm_count, stream)
+                                : way == kSplit ? run_group<true>(c, scales, m, g.count, scratch, status, sm_count, stream)
+                                                : run_group<false>(c, scales, m, g.count, scratch, status, sm_count, stream);
         if (err != cudaSuccess) return err;
     }
     return cudaSuccess;

@@ -1,0 +1,468 @@
+// Newton-Schulz steps of matrices with a short side of up to 128, results in BF16 (bsq_orth.hpp).
+//
+// All the steps are one polynomial in A_0 = X_0 X_0^T:  X_n = Q X_0 with Q_(k+1) = M_k Q_k, A_(k+1) = M_k A_k M_k, M_k = a I + b A_k + c A_k^2.  So the long side is walked
+// twice, for A_0 and for Q X_0, and what lies between is products of matrices of 128 x 128 at most, which one CTA does for each matrix without leaving its SM.  (Step by step, with X in memory,
+// 24 matrices of 64 x 1024 took 230 us; this way all five take 66.)
+//
+// Rounding grows with what it meets: an error of A_0 by (a^2)^(n - 1), 2 10^4 for five steps.  FP32 sums for A_0 and products of split operands (22 bits) leave 1e-4 to 2e-4 in the result
+// (singular values over a range of 1000; noise alone 1e-6), a tenth of its rounding to BF16.  FP32 and FP16 results, and long sides, are bsq_orth.cu's.
+//
+// Launches: norm (bsq_orth.cu), A_0 in slices of the long side on the FP32 pipes, their sum where there are many, the steps on the tensor core, Q X_0 on the FP32 pipes.
+#include "bsq_gemm16.cuh"
+#include "bsq_orth_small.hpp"
+
+#include <algorithm>
+#include <atomic>
+
+namespace bsq {
+namespace {
+
+constexpr int kThreads = 256, kStepThreads = 512;
+constexpr int kSliceK = 32;                                      // of the long side at a time
+constexpr int kFewSlices = 12;                                   // up to this many are added up by the CTA of the steps
+
+// Elements of a matrix as X has them: the short side is `i`, the long one `k`
+template <int TYPE, bool TALL> __device__ __forceinline__ float element(const OrthSmall &g, int z, int i, int k, float s0, float s1) {
+    const size_t at = TALL ? (size_t)k * g.ld[z] + (size_t)i : (size_t)i * g.ld[z] + (size_t)k;
+    const unsigned w = TYPE == kF32 ? static_cast<const unsigned *>(g.in[z])[at] : (unsigned)static_cast<const unsigned short *>(g.in[z])[at];
+    return word_elem<TYPE>(w, 0) * s0 * s1;
+}
+// 2^e that brings a norm below 2^15, in two factors; e
+__device__ __forceinline__ int norm_scale(double norm, float *s0, float *s1) {
+    const bool fine = norm < 3.0e38 * 65536.0 * 65536.0;         // (not: Inf or NaN)
+    const int e = norm > 0.0 && fine ? min(max(14 - ilogb(norm), -160), 160) : 0;
+    *s0 = exp2f((float)(e / 2));
+    *s1 = exp2f((float)(e - e / 2));
+    return e;
+}
+__device__ __forceinline__ double norm_of(const double *parts, int count) {
+    double s = 0.0;
+    for (int i = 0; i < count; ++i) s += parts[i];
+    return sqrt(s);
+}
+
+// Slice blockIdx.x of A_0 of matrix blockIdx.y: S x S sums over `per` of the long side, 16 x 16 threads with (S / 16)^2 each
+template <int TYPE, bool TALL, int S> __global__ void __launch_bounds__(kThreads) small_gram_kernel(const __grid_constant__ OrthSmall g, int per, float *sums) {
+    chain_begin();
+    constexpr int R = S / 16;
+    __shared__ float tile[kSliceK][S + 4];
+    const int z = blockIdx.y, tid = threadIdx.x, ty = tid / 16, tx = tid % 16, first = (int)blockIdx.x * per, last = min(g.l, first + per);
+    float s0, s1;
+    norm_scale(norm_of(g.parts + (size_t)z * g.part_count, g.part_count), &s0, &s1);
+    float acc[R][R];
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+        for (int j = 0; j < R; ++j) acc[i][j] = 0.0f;
+    constexpr int kLoads = S * kSliceK / kThreads;
+    float v[kLoads];
+    const auto ask = [&](int k0) {
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) {
+            const int n = tid + j * kThreads, k = TALL ? n / S : n % kSliceK, i = TALL ? n % S : n / kSliceK;
+            v[j] = i < g.s && k0 + k < last ? element<TYPE, TALL>(g, z, i, k0 + k, s0, s1) : 0.0f;
+        }
+    };
+    ask(first);
+    for (int k0 = first; k0 < last; k0 += kSliceK) {
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) {
+            const int n = tid + j * kThreads;
+            tile[TALL ? n / S : n % kSliceK][TALL ? n % S : n / kSliceK] = v[j];
+        }
+        __syncthreads();
+        if (k0 + kSliceK < last) ask(k0 + kSliceK);              // (on its way while these are summed)
+#pragma unroll 4
+        for (int k = 0; k < kSliceK; ++k) {
+            float a[R], b[R];
+#pragma unroll
+            for (int j = 0; j < R; j += 4) {
+                *reinterpret_cast<float4 *>(a + j) = *reinterpret_cast<const float4 *>(&tile[k][ty * R + j]);
+                *reinterpret_cast<float4 *>(b + j) = *reinterpret_cast<const float4 *>(&tile[k][j * 16 + tx * 4]);
+            }
+#pragma unroll
+            for (int i = 0; i < R; ++i)
+#pragma unroll
+                for (int j = 0; j < R; ++j) acc[i][j] = fmaf(a[i], b[j], acc[i][j]);
+        }
+    }
+    float *to = sums + ((size_t)z * gridDim.x + blockIdx.x) * (size_t)(g.s * g.s);
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            const int r = ty * R + i, c = j / 4 * 64 + tx * 4 + j % 4;
+            if (r < g.s && c < g.s) to[r * g.s + c] = acc[i][j];
+        }
+}
+__global__ void __launch_bounds__(kThreads) small_sum_kernel(const float *sums, int slices, int elements, float *to) {
+    chain_begin();
+    const int i = (int)blockIdx.x * kThreads + (int)threadIdx.x;
+    if (i >= elements) return;
+    const float *p = sums + (size_t)blockIdx.y * (size_t)slices * (size_t)elements + (size_t)i;
+    float v = 0.0f;
+#pragma unroll 8
+    for (int k = 0; k < slices; ++k) v += p[(size_t)k * (size_t)elements];
+    to[(size_t)blockIdx.y * (size_t)elements + (size_t)i] = v;
+}
+
+// A matrix of 128 x 128 as an operand: high and low parts, each two blocks of 64 columns with rows of 128 bytes (128-byte swizzle)
+constexpr unsigned kPart = 128 * 128 * 2, kMatrix = 2 * kPart;
+struct CoreBars {
+    uint64_t done, drain;
+    unsigned tmem_base;
+};
+// 16 values of the thread's row, from column `col` on (a multiple of 16)
+__device__ __forceinline__ void core_put(unsigned char *m, int row, int col, const float (&v)[16]) {
+    unsigned p[8], q[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const __half2 t = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+        const float2 f = __half22float2(t);
+        p[j] = *reinterpret_cast<const unsigned *>(&t);
+        q[j] = pack_pair<kF16>(v[2 * j] - f.x, v[2 * j + 1] - f.y);
+    }
+    unsigned char *line = m + (col >> 6) * (kPart / 2) + row * 128;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const unsigned at = (unsigned)(((((col & 63) >> 3) + i) ^ (row & 7)) << 4);
+        *reinterpret_cast<uint4 *>(line + at) = make_uint4(p[4 * i], p[4 * i + 1], p[4 * i + 2], p[4 * i + 3]);
+        *reinterpret_cast<uint4 *>(line + kPart + at) = make_uint4(q[4 * i], q[4 * i + 1], q[4 * i + 2], q[4 * i + 3]);
+    }
+}
+__device__ __forceinline__ void core_get(const unsigned char *m, int row, int col, float (&v)[16]) {
+    const unsigned char *line = m + (col >> 6) * (kPart / 2) + row * 128;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const unsigned at = (unsigned)(((((col & 63) >> 3) + i) ^ (row & 7)) << 4);
+        const uint4 a = *reinterpret_cast<const uint4 *>(line + at), b = *reinterpret_cast<const uint4 *>(line + kPart + at);
+        const unsigned p[4] = {a.x, a.y, a.z, a.w}, q[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&p[j])), e = __half22float2(*reinterpret_cast<const __half2 *>(&q[j]));
+            v[8 * i + 2 * j] = f.x + e.x;
+            v[8 * i + 2 * j + 1] = f.y + e.y;
+        }
+    }
+}
+// The product of two symmetric matrices, both parts of each: three walks along K.  One thread.
+__device__ __forceinline__ void core_product(unsigned acc, unsigned a, unsigned b, int s) {
+    const unsigned n = (unsigned)(s + 15) / 16;
+    const unsigned idesc = (1u << 4) | (n * 16 >> 3 << 17) | (128u >> 4 << 24);           // FP16 x FP16, FP32 sums, N >> 3, M >> 4
+    bool more = false;
+    for (int w = 0; w < 3; ++w)
+        for (unsigned k = 0; k < n; ++k) {
+            const unsigned at = (k >> 2) * (kPart / 2) + (k & 3u) * 32u;
+            // (the small products first)
+            mma_f16(acc, smem_desc_sw128(a + (w == 0 ? kPart : 0u) + at), smem_desc_sw128(b + (w == 1 ? kPart : 0u) + at), idesc, more);
+            more = true;
+        }
+}
+
+// The steps of matrix blockIdx.x: from A_0 (the sum of `slices`) to Q, times what X_0 is G times and the result's factor.  16 warps: a thread has a row of each result and 16 * NH
+// columns, the four warps that may read its lanes of tensor memory the others.
+template <int NH>
+__global__ void __launch_bounds__(kStepThreads, 1) small_steps_kernel(const __grid_constant__ OrthSmall g, const __grid_constant__ OrthSmallSteps t, const float *sums, int slices,
+                                                                      float *q_out, unsigned tries, unsigned *status) {
+    chain_begin();
+    extern __shared__ unsigned char smem_dyn[];
+    unsigned char *ma = smem_dyn + ((1024u - (smem_u32(smem_dyn) & 1023u)) & 1023u), *mm = ma + kMatrix, *mq = mm + kMatrix;
+    CoreBars &bars = *reinterpret_cast<CoreBars *>(mq + kMatrix);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, z = blockIdx.x, s = g.s;
+    const int row = (warp & 3) * 32 + lane, col = (warp >> 2) * 16 * NH;
+    const bool mine = (warp & 3) * 32 < s && col < s;            // (whole warps)
+    if (tid == 0) {
+        mbar_init(&bars.done, 1);
+        mbar_init(&bars.drain, 1);
+        mbar_fence_init();
+    }
+    if (warp == 0) tmem_alloc<1>(&bars.tmem_base, 512u);
+    for (unsigned i = tid; i < 3 * kMatrix / 16; i += kStepThreads) reinterpret_cast<uint4 *>(ma)[i] = make_uint4(0u, 0u, 0u, 0u);
+    const double norm = norm_of(g.parts + (size_t)z * g.part_count, g.part_count);
+    float s0, s1;
+    const int e = norm_scale(norm, &s0, &s1);
+    // X_0 = G 2^e * factor
+    const float factor = !(norm < 3.0e38 * 65536.0 * 65536.0) ? __uint_as_float(0x7fffffffu) : norm > 0.0 ? (float)(ldexp(1.0, -e) / (norm + g.eps)) : 1.0f;
+    float v[NH][16];
+    if (mine) {
+        const float x = ldexpf(factor * factor, t.step[0].a);
+#pragma unroll
+        for (int h = 0; h < NH; ++h)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[h][j] = 0.0f;
+        const float *p = sums + (size_t)z * (size_t)slices * (size_t)(s * s) + (size_t)(col * s + row);         // (symmetric: lanes along memory)
+        for (int k = 0; k < slices; ++k, p += s * s)
+#pragma unroll
+            for (int h = 0; h < NH; ++h)
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    if (row < s && col + 16 * h + j < s) v[h][j] += p[(16 * h + j) * s];
+#pragma unroll
+        for (int h = 0; h < NH; ++h)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[h][j] *= x;
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const unsigned tmem = bars.tmem_base, acc = tmem + ((unsigned)((warp & 3) * 32) << 16) + (unsigned)col;
+    unsigned parity = 0;
+    bool ok = true;
+    // Operands are written: products may read them
+    const auto meet = [&] {
+        fence_proxy_async_smem();
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncthreads();
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    };
+    const auto wait = [&] {
+        ok = mbar_wait_asleep(&bars.done, parity, status, tries) && ok;
+        parity ^= 1u;
+        __syncwarp();
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    };
+    // The thread's columns of a product times `by`; 0 outside the matrix
+    const auto take = [&](unsigned from, float by) {
+#pragma unroll
+        for (int h = 0; h < NH; ++h) {
+            read16f(acc + from + 16u * (unsigned)h, v[h], true);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[h][j] = row < s && col + 16 * h + j < s ? v[h][j] * by : 0.0f;
+        }
+    };
+    const auto put = [&](unsigned char *m) {
+#pragma unroll
+        for (int h = 0; h < NH; ++h) core_put(m, row, col + 16 * h, v[h]);
+    };
+    const auto give = [&](float by) {
+        const bool all = __syncthreads_and(ok) != 0;             // (a wait that ran out anywhere: NaN everywhere)
+        if (!mine || row >= s) return;
+#pragma unroll
+        for (int h = 0; h < NH; ++h)
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+                if (col + 16 * h + j < s) q_out[(size_t)z * (size_t)(s * s) + (size_t)((col + 16 * h + j) * s + row)] = all ? v[h][j] * by : __uint_as_float(0x7fffffffu);
+    };
+
+    if (mine) put(ma);
+    for (int k = 0; k < t.steps; ++k) {
+        const OrthSmallStep &p = t.step[k];
+        const bool last = k + 1 == t.steps;
+        // M = a I + b A + c A^2
+        meet();
+        if (warp == 0 && elect_one()) {
+            core_product(tmem, smem_u32(ma), smem_u32(ma), s);
+            tc_commit(&bars.done);
+        }
+        __syncwarp();
+        wait();
+        if (mine) {
+            take(0u, p.square);
+#pragma unroll
+            for (int h = 0; h < NH; ++h) {
+                float a[16];
+                core_get(ma, row, col + 16 * h, a);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    v[h][j] = fmaf(p.linear, a[j], v[h][j]);
+                    if (col + 16 * h + j == row && row < s) v[h][j] += p.constant;
+                }
+            }
+        }
+        if (k == 0 && last) {
+            give(p.out * factor);
+            break;
+        }
+        if (mine) {
+            put(mm);
+            if (k == 0) {
+#pragma unroll
+                for (int h = 0; h < NH; ++h)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) v[h][j] *= p.first_q;
+                put(mq);
+            }
+        }
+        // M Q, M A
+        meet();
+        if (warp == 0 && elect_one()) {
+            if (k > 0) core_product(tmem + 128u, smem_u32(mm), smem_u32(mq), s);
+            if (!last) core_product(tmem + 256u, smem_u32(mm), smem_u32(ma), s);
+            tc_commit(&bars.done);
+        }
+        __syncwarp();
+        wait();
+        if (mine && k > 0) {
+            take(128u, last ? p.out * factor : p.of_q);
+            if (!last) put(mq);
+        }
+        if (last) {
+            give(1.0f);
+            break;
+        }
+        if (mine) {
+            take(256u, p.of_t);
+            put(ma);
+        }
+        // M (M A)
+        meet();
+        if (warp == 0 && elect_one()) {
+            core_product(tmem, smem_u32(mm), smem_u32(ma), s);
+            tc_commit(&bars.done);
+        }
+        __syncwarp();
+        wait();
+        if (mine) {
+            take(0u, p.of_a);
+            put(ma);
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == 0) {
+        if (elect_one()) tc_commit(&bars.drain);                 // products under way, also behind a wait that ran out
+        __syncwarp();
+        mbar_wait_asleep(&bars.drain, 0, status);
+        tmem_free<1>(tmem, 512u);
+    }
+}
+
+// 64 of the long side of matrix blockIdx.y: out = Q G (or G Q)
+template <int TYPE, bool TALL, int S> __global__ void __launch_bounds__(kThreads) small_apply_kernel(const __grid_constant__ OrthSmall g, const float *q) {
+    chain_begin();
+    constexpr int R = S / 16;
+    extern __shared__ float smem_apply[];
+    float *mq = smem_apply, *tile = smem_apply + S * (S + 4);    // Q [k][i], G [k][64 of the long side]
+    const int z = blockIdx.y, tid = threadIdx.x, ty = tid / 16, tx = tid % 16, first = (int)blockIdx.x * 64;
+    float s0, s1;
+    norm_scale(norm_of(g.parts + (size_t)z * g.part_count, g.part_count), &s0, &s1);
+    // (asked for 16 at a time, one wait for each 16)
+#pragma unroll 1
+    for (int from = tid; from < S * S; from += 16 * kThreads) {
+        float v[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const int n = from + j * kThreads, k = n / S, i = n % S;
+            v[j] = k < g.s && i < g.s ? q[(size_t)z * (size_t)(g.s * g.s) + (size_t)(k * g.s + i)] : 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) mq[(from + j * kThreads) / S * (S + 4) + (from + j * kThreads) % S] = v[j];
+    }
+#pragma unroll 1
+    for (int from = tid; from < S * 64; from += 16 * kThreads) {
+        float v[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const int n = from + j * kThreads, k = TALL ? n % S : n / 64, i = TALL ? n / S : n % 64;
+            v[j] = k < g.s && first + i < g.l ? element<TYPE, TALL>(g, z, k, first + i, s0, s1) : 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const int n = from + j * kThreads;
+            tile[(TALL ? n % S : n / 64) * 68 + (TALL ? n / S : n % 64)] = v[j];
+        }
+    }
+    __syncthreads();
+    // wide: a thread has R rows (ty) x 4 columns (tx); tall: 4 rows (ty) x R columns (tx): neighbouring threads write neighbouring elements
+    float acc[R][4];
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
+    const int qi = TALL ? tx : ty, gj = TALL ? ty : tx;
+#pragma unroll 4
+    for (int k = 0; k < g.s; ++k) {
+        float a[R];
+#pragma unroll
+        for (int i = 0; i < R; i += 4) *reinterpret_cast<float4 *>(a + i) = *reinterpret_cast<const float4 *>(mq + k * (S + 4) + i * 16 + qi * 4);
+        const float4 b = *reinterpret_cast<const float4 *>(tile + k * 68 + gj * 4);
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            acc[i][0] = fmaf(a[i], b.x, acc[i][0]);
+            acc[i][1] = fmaf(a[i], b.y, acc[i][1]);
+            acc[i][2] = fmaf(a[i], b.z, acc[i][2]);
+            acc[i][3] = fmaf(a[i], b.w, acc[i][3]);
+        }
+    }
+    __nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(g.out[z]);
+    const size_t ld = (size_t)g.ld_out[z];
+    const bool whole = (reinterpret_cast<uintptr_t>(out) | (ld * 2)) % 8 == 0;
+    if (TALL) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int r = first + gj * 4 + j;
+            if (r >= g.l) break;
+#pragma unroll
+            for (int i = 0; i < R; i += 4) {
+                const int c = i * 16 + qi * 4;
+                __nv_bfloat16 *to = out + (size_t)r * ld + (size_t)c;
+                if (whole && c + 4 <= g.s) *reinterpret_cast<uint2 *>(to) = make_uint2(pack_pair<kBf16>(acc[i][j], acc[i + 1][j]), pack_pair<kBf16>(acc[i + 2][j], acc[i + 3][j]));
+                else
+#pragma unroll
+                    for (int u = 0; u < 4; ++u)
+                        if (c + u < g.s) to[u] = __float2bfloat16_rn(acc[i + u][j]);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int r = i / 4 * 64 + qi * 4 + i % 4, c = first + gj * 4;
+            if (r >= g.s) continue;
+            __nv_bfloat16 *to = out + (size_t)r * ld + (size_t)c;
+            if (whole && c + 4 <= g.l) *reinterpret_cast<uint2 *>(to) = make_uint2(pack_pair<kBf16>(acc[i][0], acc[i][1]), pack_pair<kBf16>(acc[i][2], acc[i][3]));
+            else
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (c + u < g.l) to[u] = __float2bfloat16_rn(acc[i][u]);
+        }
+    }
+}
+
+constexpr size_t kStepsSmem = 1024 + 3 * kMatrix + sizeof(CoreBars) + 64;
+static_assert(kStepsSmem <= 227 * 1024, "three matrices do not fit");
+constexpr size_t apply_smem(int s) { return (size_t)(s * (s + 4) + s * 68) * 4; }
+
+template <int TYPE, bool TALL, int S>
+cudaError_t run(const OrthSmall &g, const OrthSmallSteps &t, int count, const OrthSmallRoom &r, unsigned *status, cudaStream_t stream) {
+    static std::atomic<uint64_t> done_steps{0}, done_apply{0};
+    cudaError_t err = allow_smem(small_steps_kernel<S / 64>, &done_steps);
+    if (err == cudaSuccess) err = allow_smem(small_apply_kernel<TYPE, TALL, S>, &done_apply);
+    if (err != cudaSuccess) return err;
+    err = launch_chained(small_gram_kernel<TYPE, TALL, S>, dim3((unsigned)r.slices, (unsigned)count), kThreads, 0, stream, g, r.per, r.sums);
+    if (err != cudaSuccess) return err;
+    const float *sums = r.sums;
+    int slices = r.slices;
+    if (slices > kFewSlices) {
+        const int n = g.s * g.s;
+        err = launch_chained(small_sum_kernel, dim3((unsigned)((n + kThreads - 1) / kThreads), (unsigned)count), kThreads, 0, stream, (const float *)r.sums, slices, n, r.sum);
+        if (err != cudaSuccess) return err;
+        sums = r.sum;
+        slices = 1;
+    }
+    err = launch_chained(small_steps_kernel<S / 64>, (unsigned)count, kStepThreads, kStepsSmem, stream, g, t, sums, slices, r.q, epilogue_tries(kWaitTries), status);
+    if (err != cudaSuccess) return err;
+    return launch_chained(small_apply_kernel<TYPE, TALL, S>, dim3((unsigned)((g.l + 63) / 64), (unsigned)count), kThreads, apply_smem(S), stream, g, (const float *)r.q);
+}
+template <int TYPE>
+cudaError_t run_type(const OrthSmall &g, bool tall, const OrthSmallSteps &t, int count, const OrthSmallRoom &r, unsigned *status, cudaStream_t stream) {
+    if (g.s <= 64) return tall ? run<TYPE, true, 64>(g, t, count, r, status, stream) : run<TYPE, false, 64>(g, t, count, r, status, stream);
+    return tall ? run<TYPE, true, 128>(g, t, count, r, status, stream) : run<TYPE, false, 128>(g, t, count, r, status, stream);
+}
+
+}  // namespace
+
+// Slices of the long side: as many as fill the device twice, of 64 at least
+int orth_small_slices(uint64_t l, int count, int sm_count, int *per) {
+    const int most = std::max(1, 2 * sm_count / count), want = (int)std::min<uint64_t>((uint64_t)most, (l + 63) / 64);
+    *per = (int)(((l + (uint64_t)want - 1) / (uint64_t)want + kSliceK - 1) / kSliceK * kSliceK);
+    return (int)((l + (uint64_t)*per - 1) / (uint64_t)*per);
+}
+
+cudaError_t orth_small(const OrthSmall &g, bool tall, int type, const OrthSmallSteps &t, int count, const OrthSmallRoom &r, unsigned *status, cudaStream_t stream) {
+    if (type == kF32) return run_type<kF32>(g, tall, t, count, r, status, stream);
+    if (type == kBf16) return run_type<kBf16>(g, tall, t, count, r, status, stream);
+    return run_type<kF16>(g, tall, t, count, r, status, stream);
+}
+
+}  // namespace bsq

@@ -30,7 +30,7 @@ _HEAD = 128
 _NORM_SCRATCH = 16384                                      # bsq_grad_norm_scratch_bytes
 _stream = torch._C._cuda_getCurrentRawStream
 _device = torch._C._cuda_getDevice
-_dtype, _requires_grad = attrgetter("dtype"), attrgetter("requires_grad")
+_dtype, _requires_grad, _shape = attrgetter("dtype"), attrgetter("requires_grad"), attrgetter("shape")
 _contiguous, _index, _numel, _pointer = torch.Tensor.is_contiguous, torch.Tensor.get_device, torch.Tensor.numel, torch.Tensor.data_ptr
 
 
@@ -457,10 +457,11 @@ def orthogonalize(updates, steps=5, coefficients=_QUINTIC, eps=1e-7, scale=1.0, 
     """Updates with their singular values brought near 1 by Newton-Schulz steps: X = G / (|G| + eps), then `steps` times X <- a X + (b A + c A^2) X with A = X X^T (from the
     right with X^T X where G has more rows than columns), times `scale`.  `updates`: a tensor of at least two dimensions (the leading ones are a stack of matrices) or a list of them
     (float32, float16 or bfloat16 CUDA tensors of one device, of any shapes); the result is of the same form, in `dtype`.  Matrices of one shape and type go through together.  coefficients: (a, b, c)
-    for all steps, or one triple for each; they must keep singular values from 0 to 1 below 1000.  `out`: tensors to write, apart from each other and from the updates.
+    for all steps, or one triple for each; they must keep singular values from 0 to 1 below 1000.  `out`: tensors to write, apart from each other and from the updates (without it,
+    results of one shape that follow one another in a list share an allocation).
 
-    X is held in 2 x 16 bits and products sum in FP32: bfloat16 results are off by about half their own rounding beside it.  float32 and float16 results come from products
-    of both halves of every operand, three times the work.  An Inf or NaN makes its whole matrix NaN; zeros stay zeros, and where |G| is far below eps the result may be 0.
+    bfloat16 results are off by at most about half their own rounding beside it: X is held in 2 x 16 bits, products read 16 and sum in FP32 (a side of up to 128: products of 22 bits).
+    float32 and float16 results come from products of 2 x 16 bits of every operand, three times the work.  An Inf or NaN makes its whole matrix NaN; zeros stay zeros, and where |G| is far below eps the result may be 0.
     Matrices whose rows are not contiguous are copied first.  The result needs no gradient and gives none to the updates.  Sides of at most 65536, 1 to 64 steps."""
     single = isinstance(updates, torch.Tensor)
     updates = [updates] if single else list(updates)
@@ -477,35 +478,47 @@ def orthogonalize(updates, steps=5, coefficients=_QUINTIC, eps=1e-7, scale=1.0, 
         raise ValueError("eps must be finite and not negative, scale finite")
     if not updates:
         return []
-    device, index = updates[0].device, updates[0].get_device()
-    for g in updates:
-        if g.dtype not in _TYPES or g.get_device() != index or index < 0 or g.dim() < 2 or g.size(-1) > _ORTH_SIDE or g.size(-2) > _ORTH_SIDE:
-            raise ValueError("updates must be float32, float16 or bfloat16 CUDA tensors on one device of at least two dimensions, with sides of at most 65536")
+    # (an attribute of all of them at a time: a step has a few hundred matrices)
+    device, index, n = updates[0].device, updates[0].get_device(), len(updates)
+    dtypes, shapes = list(map(_dtype, updates)), list(map(_shape, updates))
+    if index < 0 or set(map(_index, updates)) != {index} or not _TYPES.keys() >= set(dtypes) or any(len(s) < 2 or s[-1] > _ORTH_SIDE or s[-2] > _ORTH_SIDE for s in shapes):
+        raise ValueError("updates must be float32, float16 or bfloat16 CUDA tensors on one device of at least two dimensions, with sides of at most 65536")
     if out is None:
-        outs = [torch.empty(g.shape, dtype=dtype, device=device) for g in updates]
+        outs, at = [], 0
+        while at < n:                                            # (neighbours of one shape from one allocation: a call of the allocator costs more than a matrix's other arguments)
+            end = at + 1
+            while end < n and shapes[end] == shapes[at]:
+                end += 1
+            outs += [torch.empty(shapes[at], dtype=dtype, device=device)] if end == at + 1 else torch.empty((end - at,) + shapes[at], dtype=dtype, device=device).unbind(0)
+            at = end
     else:
         outs = [out] if isinstance(out, torch.Tensor) else list(out)
-        if len(outs) != len(updates) or isinstance(out, torch.Tensor) != single:
+        if len(outs) != n or isinstance(out, torch.Tensor) != single:
             raise ValueError("out must have the form of updates")
-        for o, g in zip(outs, updates):
-            if o.dtype != dtype or o.shape != g.shape or o.device != device or o.requires_grad:
-                raise ValueError("tensors of out must have the shapes of the updates, dtype %s, their device, and need no gradient" % dtype)
-    ins, rows, cols, lds, types, tos, ld_outs, keep = array("Q"), array("Q"), array("Q"), array("Q"), array("i"), array("Q"), array("Q"), []
-    for g, o in zip(updates, outs):
-        if not g.numel():
-            continue
-        if not _stacked(g):
-            g = g.contiguous()
-            keep.append(g)                                       # (until the call has been enqueued)
-        if out is not None and not _stacked(o):
-            raise ValueError("rows of out must be contiguous and must not overlap")
-        m, n, size, to_size = g.size(-2), g.size(-1), g.element_size(), o.element_size()
-        for a, b in zip(_matrices(g), _matrices(o)):
-            ins.append(g.data_ptr() + a * size)
-            tos.append(o.data_ptr() + b * to_size)
-        count = g.numel() // (m * n)
-        rows.extend([m] * count), cols.extend([n] * count), types.extend([_TYPES[g.dtype]] * count)
-        lds.extend([g.stride(-2) if m > 1 else n] * count), ld_outs.extend([o.stride(-2) if m > 1 else n] * count)
+        if set(map(_dtype, outs)) != {dtype} or list(map(_shape, outs)) != shapes or set(map(_index, outs)) != {index} or any(map(_requires_grad, outs)):
+            raise ValueError("tensors of out must have the shapes of the updates, dtype %s, their device, and need no gradient" % dtype)
+    keep = updates                                               # (until the call has been enqueued)
+    if all(map(_contiguous, updates)) and all(map(_contiguous, outs)) and all(len(s) == 2 and s[0] and s[1] for s in shapes):
+        ins, tos = array("Q", map(_pointer, updates)), array("Q", map(_pointer, outs))
+        rows, cols, types = array("Q", [s[0] for s in shapes]), array("Q", [s[1] for s in shapes]), array("i", [_TYPES[d] for d in dtypes])
+        lds = ld_outs = cols
+    else:
+        ins, rows, cols, lds, types, tos, ld_outs, keep = array("Q"), array("Q"), array("Q"), array("Q"), array("i"), array("Q"), array("Q"), []
+        for g, o in zip(updates, outs):
+            if not g.numel():
+                continue
+            if not _stacked(g):
+                g = g.contiguous()
+                keep.append(g)
+            if not _stacked(o):
+                raise ValueError("rows of out must be contiguous and must not overlap")
+            m, k, size, to_size = g.size(-2), g.size(-1), g.element_size(), o.element_size()
+            for a, b in zip(_matrices(g), _matrices(o)):
+                ins.append(g.data_ptr() + a * size)
+                tos.append(o.data_ptr() + b * to_size)
+            count = g.numel() // (m * k)
+            rows.extend([m] * count), cols.extend([k] * count), types.extend([_TYPES[g.dtype]] * count)
+            lds.extend([g.stride(-2) if m > 1 else k] * count), ld_outs.extend([o.stride(-2) if m > 1 else k] * count)
     if ins:
         flat = array("f", [v for t in table for v in t])
         arrays = [a.buffer_info()[0] for a in (ins, rows, cols, lds, types, tos, ld_outs, flat)]
@@ -540,7 +553,7 @@ def _steps_ok(table):
     """As the library looks at coefficients: the largest singular value that each step may meet."""
     most = 1.0
     for a, b, c in table:
-        s = [most * 1.02 * i / 4096 for i in range(4097)]
+        s = [most * 1.02 * i / 256 for i in range(257)]
         p = [b * v * v + c * v ** 4 for v in s]
         most = max(abs((a + q) * v) for q, v in zip(p, s))
         if not most < 1000.0 or any(not abs(q) < 1e6 for q in p):
