@@ -157,14 +157,14 @@ inline bool tma_can_write(const void *out, uint64_t row_stride, uint64_t row_byt
     return (reinterpret_cast<uintptr_t>(out) | row_stride | row_bytes) % 16 == 0;
 }
 
-// Lets a kernel have all of an SM's shared memory, once for each device.
-template <class F> cudaError_t allow_smem(F *kernel, std::atomic<uint64_t> *done) {
+// Lets a kernel have all of an SM's shared memory, or `bytes` of it, once for each device.
+template <class F> cudaError_t allow_smem(F *kernel, std::atomic<uint64_t> *done, int bytes = 227 * 1024) {
     int device = 0;
     cudaError_t err = cudaGetDevice(&device);
     if (err != cudaSuccess) return err;
     const uint64_t bit = 1ull << (device & 63);
     if (device < 64 && (done->load(std::memory_order_relaxed) & bit)) return cudaSuccess;
-    err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+    err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (err == cudaSuccess && device < 64) done->fetch_or(bit, std::memory_order_relaxed);
     return err;
 }

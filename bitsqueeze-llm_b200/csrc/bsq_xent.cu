@@ -18,6 +18,7 @@ namespace {
 
 constexpr float kLog2E = 1.4426950408889634f;
 constexpr double kLn2 = 0.69314718055994530942;
+constexpr float kLowest = -3.0e38f;                              // below every logit but -Inf, whose exponential is 0 against it
 constexpr uint64_t kPieceBytes = 128ull << 20;
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -47,7 +48,7 @@ struct XentStats {
         float top = v[0];
 #pragma unroll
         for (int j = 1; j < COLS; ++j) top = fmaxf(top, v[j]);
-        top *= kLog2E;
+        top = fmaxf(top * kLog2E, kLowest);                      // (NaN shows in the sum)
         float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int j = 0; j < COLS; ++j) s[j & 3] += exp2_fast(fmaf(v[j], kLog2E, -top));
@@ -70,6 +71,126 @@ struct XentStats {
         }
     }
 };
+
+// Up to four tokens: the weight's bytes are all there is, and every multiplication fits beside them on the FP32 pipes, with rounded sums.  A warp has a row or two of the weight at a time,
+// x lies in shared memory; a CTA leaves one part for each token.  VEC elements to a load, what the rows' alignment allows: 8, 2 or 1, so that nothing is copied first.
+// 1 x 4096 x 32000 43 us for 262 MB (6.1 TB/s; on the tensor core, a tile of 128 x 128 with one row, 70); rows off 16 bytes would take three times that with their copy.
+constexpr int kFewTokens = 4, kFewThreads = 512;
+// Rows that a warp has at a time: two share what is read and unpacked of x; of one token that is little, and the finer division leaves fewer warps without work at the end
+__host__ __device__ constexpr int few_rows(int tokens) { return tokens == 1 ? 1 : 2; }
+constexpr size_t kFewSmem = 96 << 10;                            // of x: two CTAs to an SM
+struct XentFew {
+    const unsigned short *x, *w;
+    uint64_t ld_x, ld_w;
+    int cols;
+    long long vocab;
+    const long long *target;
+    float2 *parts;                   // CTAs x tokens
+    float *sums, *at_target;         // (sums nullable)
+};
+template <int VEC> struct FewWords;
+template <> struct FewWords<8> { typedef uint4 type; };
+template <> struct FewWords<2> { typedef unsigned type; };
+template <> struct FewWords<1> { typedef unsigned short type; };
+template <int TYPE, int VEC> __device__ __forceinline__ void few_unpack(const typename FewWords<VEC>::type &w, float (&v)[VEC]) {
+    if constexpr (VEC == 8) {
+        const unsigned a[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = word_elem<TYPE>(a[j / 2], j & 1);
+    } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[j] = word_elem<TYPE>((unsigned)w, j);
+    }
+}
+template <int TYPE, int VEC, int TOKENS> __global__ void __launch_bounds__(kFewThreads, 2) xent_few_kernel(const XentFew f) {
+    chain_begin();
+    typedef typename FewWords<VEC>::type Word;
+    constexpr int kFewRows = few_rows(TOKENS), kUnroll = VEC == 8 ? 4 / kFewRows : 8;
+    extern __shared__ uint4 smem_x[];
+    unsigned short *sx = reinterpret_cast<unsigned short *>(smem_x);
+    __shared__ float part[3][kFewThreads / 32][TOKENS];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, words = f.cols / VEC, ld = (f.cols + 7) / 8 * 8;
+    for (int t = 0; t < TOKENS; ++t)
+        for (int i = tid; i < f.cols; i += kFewThreads) sx[t * ld + i] = f.x[(uint64_t)t * f.ld_x + i];
+    long long target[TOKENS];
+    float top[TOKENS], s[TOKENS], total[TOKENS];
+#pragma unroll
+    for (int t = 0; t < TOKENS; ++t) {
+        target[t] = f.target[t];
+        top[t] = kLowest;
+        s[t] = total[t] = 0.0f;
+    }
+    __syncthreads();
+    for (long long r0 = ((long long)blockIdx.x * (kFewThreads / 32) + warp) * kFewRows; r0 < f.vocab; r0 += (long long)gridDim.x * (kFewThreads / 32) * kFewRows) {
+        const Word *p[kFewRows];
+        float acc[kFewRows][TOKENS];
+#pragma unroll
+        for (int r = 0; r < kFewRows; ++r) {
+            p[r] = reinterpret_cast<const Word *>(f.w + (uint64_t)min(r0 + r, f.vocab - 1) * f.ld_w);
+#pragma unroll
+            for (int t = 0; t < TOKENS; ++t) acc[r][t] = 0.0f;
+        }
+        for (int i = lane; i < words; i += 32 * kUnroll) {
+            Word w[kUnroll][kFewRows];
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+                for (int r = 0; r < kFewRows; ++r)
+                    if (i + 32 * u < words) w[u][r] = p[r][i + 32 * u];
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) {
+                if (i + 32 * u >= words) break;
+                float a[kFewRows][VEC];
+#pragma unroll
+                for (int r = 0; r < kFewRows; ++r) few_unpack<TYPE, VEC>(w[u][r], a[r]);
+#pragma unroll
+                for (int t = 0; t < TOKENS; ++t) {
+                    float b[VEC];
+                    few_unpack<TYPE, VEC>(reinterpret_cast<const Word *>(sx + t * ld)[i + 32 * u], b);
+#pragma unroll
+                    for (int r = 0; r < kFewRows; ++r)
+#pragma unroll
+                        for (int j = 0; j < VEC; ++j) acc[r][t] = fmaf(a[r][j], b[j], acc[r][t]);
+                }
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < TOKENS; ++t)
+#pragma unroll
+            for (int r = 0; r < kFewRows; ++r) {
+                float l = acc[r][t];
+                for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(kFullMask, l, d);
+                if (r0 + r >= f.vocab) break;
+                total[t] += l;
+                if (r0 + r == target[t] && lane == 0) f.at_target[t] = l;
+                const float m = l * kLog2E;
+                if (m > top[t]) {
+                    s[t] *= exp2_fast(top[t] - m);
+                    top[t] = m;
+                }
+                s[t] += exp2_fast(fmaf(l, kLog2E, -top[t]));
+            }
+    }
+#pragma unroll
+    for (int t = 0; t < TOKENS; ++t)
+        if (lane == t) {
+            part[0][warp][t] = top[t];
+            part[1][warp][t] = s[t];
+            part[2][warp][t] = total[t];
+        }
+    __syncthreads();
+    if (tid < TOKENS) {
+        float m = part[0][0][tid], sum = 0.0f, all = 0.0f;
+        for (int i = 1; i < kFewThreads / 32; ++i) m = fmaxf(m, part[0][i][tid]);
+        for (int i = 0; i < kFewThreads / 32; ++i) {
+            sum += part[1][i][tid] * exp2_fast(part[0][i][tid] - m);
+            all += part[2][i][tid];
+        }
+        const size_t at = (size_t)blockIdx.x * TOKENS + (size_t)tid;
+        f.parts[at] = make_float2(m, sum);
+        if (f.sums) f.sums[at] = all;
+    }
+}
 
 struct XentJoin {
     int tokens, tiles;
@@ -111,14 +232,13 @@ __global__ void __launch_bounds__(1024) xent_join_kernel(const XentJoin j) {
     __shared__ float part_sum[32][32];
     __shared__ double2 room[32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, token = (int)blockIdx.x * 32 + lane;
-    float top = __uint_as_float(0xff800000u), s = 0.0f, total = 0.0f;
+    float top = kLowest, s = 0.0f, total = 0.0f;
     if (token < j.tokens) {
 #pragma unroll 4
         for (int t = warp; t < j.tiles; t += 32) {
             const float2 p = j.parts[(size_t)t * (size_t)j.tokens + (size_t)token];
             const float m = fmaxf(top, p.x);
-            if (m > __uint_as_float(0xff800000u)) s = s * exp2_fast(top - m) + p.y * exp2_fast(p.x - m);
-            else s += p.y;                                       // (NaN)
+            s = s * exp2_fast(top - m) + p.y * exp2_fast(p.x - m);
             top = m;
             if (j.sums) total += j.sums[(size_t)t * (size_t)j.tokens + (size_t)token];
         }
@@ -132,8 +252,7 @@ __global__ void __launch_bounds__(1024) xent_join_kernel(const XentJoin j) {
         for (int i = 0; i < 32; ++i) top = fmaxf(top, part[i][lane].x);
         for (int i = 0; i < 32; ++i) {
             const float2 p = part[i][lane];
-            // (a warp without a tile has nothing against -Inf)
-            if (i < j.tiles) sum += p.x == top ? (double)p.y : (double)(p.y * exp2_fast(p.x - top));
+            sum += (double)(p.y * exp2_fast(p.x - top));
             all += (double)part_sum[i][lane];
         }
         const double lse2 = (double)top + log2(sum);
@@ -385,10 +504,21 @@ Operands aligned_operands(const XentCall &c, Scratch *s, bool run, cudaError_t *
 
 struct LossPlan {
     bool pairs;
-    uint64_t tiles;
+    int few;                         // elements to a load of the kernel for up to four tokens, 0: the product
+    uint64_t tiles;                  // parts of a token
 };
 LossPlan loss_plan(const XentCall &c, int sm_count) {
     LossPlan p;
+    p.pairs = false;
+    p.few = 0;
+    if (c.tokens <= (uint64_t)kFewTokens && c.tokens * ((c.cols + 7) / 8 * 8) * 2 <= kFewSmem) {
+        const uintptr_t start = reinterpret_cast<uintptr_t>(c.w);
+        const uint64_t ld = c.vocab > 1 ? c.ld_w : 0;
+        p.few = start % 16 == 0 && (ld | c.cols) % 8 == 0 ? 8 : start % 4 == 0 && (ld | c.cols) % 2 == 0 ? 2 : 1;
+        const uint64_t rows = kFewThreads / 32 * (uint64_t)few_rows((int)c.tokens);
+        p.tiles = std::min<uint64_t>((uint64_t)std::max(1, 2 * sm_count), (c.vocab + rows - 1) / rows);
+        return p;
+    }
     p.pairs = g16_pairs(c.tokens, c.vocab, 1, false, sm_count);
     p.tiles = p.pairs ? (c.vocab + 127) / 128 : (c.vocab + 63) / 64;
     return p;
@@ -405,6 +535,19 @@ LossRoom loss_room(const XentCall &c, const LossPlan &p, Scratch *s) {
     r.at_target = s->take<float>(c.tokens);
     r.blocks = s->take<double2>((c.tokens + 31) / 32);
     return r;
+}
+
+template <int TYPE, int VEC, int TOKENS> cudaError_t launch_few_as(const XentFew &f, const LossPlan &p, cudaStream_t stream) {
+    static std::atomic<uint64_t> done{0};
+    const cudaError_t err = allow_smem(xent_few_kernel<TYPE, VEC, TOKENS>, &done, (int)kFewSmem);
+    if (err != cudaSuccess) return err;
+    return launch_chained(xent_few_kernel<TYPE, VEC, TOKENS>, (unsigned)p.tiles, kFewThreads, (size_t)TOKENS * (size_t)((f.cols + 7) / 8 * 16), stream, f);
+}
+template <int TYPE, int TOKENS> cudaError_t launch_few_of(const XentFew &f, const LossPlan &p, cudaStream_t stream) {
+    return p.few == 8 ? launch_few_as<TYPE, 8, TOKENS>(f, p, stream) : p.few == 2 ? launch_few_as<TYPE, 2, TOKENS>(f, p, stream) : launch_few_as<TYPE, 1, TOKENS>(f, p, stream);
+}
+template <int TYPE> cudaError_t launch_few(const XentFew &f, const LossPlan &p, int tokens, cudaStream_t stream) {
+    return tokens == 1 ? launch_few_of<TYPE, 1>(f, p, stream) : tokens == 2 ? launch_few_of<TYPE, 2>(f, p, stream) : tokens == 3 ? launch_few_of<TYPE, 3>(f, p, stream) : launch_few_of<TYPE, 4>(f, p, stream);
 }
 
 struct GradPlan {
@@ -528,8 +671,9 @@ size_t xent_scratch_bytes(const XentCall &c, int sm_count) {
     if (c.tokens == 0) return 0;
     Scratch s = {nullptr};
     cudaError_t err = cudaSuccess;
-    aligned_operands(c, &s, false, &err, sm_count, nullptr);
-    loss_room(c, loss_plan(c, sm_count), &s);
+    const LossPlan p = loss_plan(c, sm_count);
+    loss_room(c, p, &s);
+    if (!p.few) aligned_operands(c, &s, false, &err, sm_count, nullptr);
     return s.used;
 }
 
@@ -549,17 +693,22 @@ cudaError_t xent_loss(const XentCall &c, float *loss, float *stats, void *scratc
         const XentJoin none = {0, 0, (long long)c.vocab, c.ignore, c.smoothing, c.reduction, nullptr, nullptr, nullptr, nullptr, loss, stats, nullptr};
         return launch_chained(xent_total_kernel, 1, 1024, 0, stream, none, 0);
     }
-    const Operands o = aligned_operands(c, &s, true, &err, sm_count, stream);
-    if (err != cudaSuccess) return err;
     const LossPlan p = loss_plan(c, sm_count);
     const LossRoom r = loss_room(c, p, &s);
-    Gemm16Maps maps;
-    const bool bf16 = c.type == kBf16;
-    if (!map_operand(&maps.a[0], o.x, bf16, true) || !map_operand(&maps.b[0], o.w, bf16, true)) return cudaErrorInvalidValue;
-    maps.a[1] = maps.a[0];
-    maps.b[1] = maps.b[0];
-    const XentStats e = {(int)c.tokens, (int)c.vocab, c.target, r.parts, r.sums, r.at_target};
-    err = launch_gemm16(maps, e, product_of(c.tokens, c.vocab, true, true, bf16), c.cols, p.pairs, status, sm_count, stream);
+    if (p.few) {
+        const XentFew f = {static_cast<const unsigned short *>(c.x), static_cast<const unsigned short *>(c.w), c.ld_x, c.ld_w, (int)c.cols, (long long)c.vocab, c.target, r.parts, r.sums, r.at_target};
+        err = c.type == kBf16 ? launch_few<kBf16>(f, p, (int)c.tokens, stream) : launch_few<kF16>(f, p, (int)c.tokens, stream);
+    } else {
+        const Operands o = aligned_operands(c, &s, true, &err, sm_count, stream);
+        if (err != cudaSuccess) return err;
+        Gemm16Maps maps;
+        const bool bf16 = c.type == kBf16;
+        if (!map_operand(&maps.a[0], o.x, bf16, true) || !map_operand(&maps.b[0], o.w, bf16, true)) return cudaErrorInvalidValue;
+        maps.a[1] = maps.a[0];
+        maps.b[1] = maps.b[0];
+        const XentStats e = {(int)c.tokens, (int)c.vocab, c.target, r.parts, r.sums, r.at_target};
+        err = launch_gemm16(maps, e, product_of(c.tokens, c.vocab, true, true, bf16), c.cols, p.pairs, status, sm_count, stream);
+    }
     if (err != cudaSuccess) return err;
     const XentJoin j = {(int)c.tokens, (int)p.tiles, (long long)c.vocab, c.ignore, c.smoothing, c.reduction, c.target, r.parts, r.sums, r.at_target, loss, stats, r.blocks};
     const unsigned blocks = (unsigned)((c.tokens + 31) / 32);

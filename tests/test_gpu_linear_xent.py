@@ -93,6 +93,36 @@ def test_sizes(ops, dtype, tokens, cols, vocab):
     check(ops, *make(tokens, cols, vocab, DTYPES[dtype], seed=tokens + cols + vocab))
 
 
+@pytest.mark.parametrize("tokens", [1, 2, 3, 4, 5])
+@pytest.mark.parametrize("cols,vocab", [(1, 1), (7, 3), (8, 33), (66, 5000), (1000, 9473), (1031, 20001), (4104, 700), (2, 40000)])
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+def test_few_tokens(ops, dtype, cols, vocab, tokens):
+    """Around the kernel that takes up to four: its three widths of loads, rows and CTAs that have nothing."""
+    check(ops, *make(tokens, cols, vocab, DTYPES[dtype], seed=tokens + vocab, ignored=0.3), e=0.1 * (vocab % 2))
+
+
+def test_few_tokens_of_many_columns(ops):
+    """More than fit into shared memory."""
+    check(ops, *make(1, 50000, 300, torch.bfloat16))
+    check(ops, *make(4, 12296, 300, torch.bfloat16))
+    check(ops, *make(4, 12288, 300, torch.float16))
+
+
+@pytest.mark.parametrize("tokens", [2, 40, 300])
+def test_infinite_weights(ops, tokens):
+    """A logit of -Inf has no probability; one of +Inf leaves nothing to compute with."""
+    x, w, t = make(tokens, 64, 7000, torch.bfloat16, ignored=0.0)
+    x = x.abs()
+    t.clamp_(min=300)
+    want = ops.linear_cross_entropy(x, torch.cat([w[300:]]), t - 300, reduction="none")
+    low = w.clone()
+    low[:300, 3] = float("-inf")
+    got = ops.linear_cross_entropy(x, low, t, reduction="none")
+    assert torch.isfinite(got).all() and (got - want).abs().max() <= 1e-5
+    low[5000, 3] = float("inf")
+    assert torch.isnan(ops.linear_cross_entropy(x, low, t, reduction="none")).all()
+
+
 @pytest.mark.parametrize("tokens,cols,vocab", [(1, 8, 2), (7, 65, 129), (300, 96, 6529), (40, 256, 3001)])
 @pytest.mark.parametrize("e", [0.1, 0.5, 1.0])
 def test_label_smoothing(ops, e, tokens, cols, vocab):
