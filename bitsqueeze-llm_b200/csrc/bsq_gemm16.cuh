@@ -3,11 +3,11 @@
 //
 // Where there are enough tiles, a pair of CTAs on two SMs shares one of 256 x 256 (cta_group::2): each brings 128 rows of A and 128 of B, so that an element from
 // the L2 feeds 256 multiplications.  Small results: one CTA per tile of 128 x 128.  Warp 0 brings stages of 64 of K by TMA (128-byte swizzle, five stages of 32 KB; operands that are
-// contiguous along K or along M / N, whichever they are in memory: the tensor core reads either), warp 1 of the leader issues the MMAs, warps 4 to 11 take finished
+// contiguous along K or along M / N, whichever they are in memory: the tensor core reads either), warp 1 of the leader issues the MMAs, warps 2 to 9 take finished
 // tiles out while the next one is summed in the other half of tensor memory, each 32 rows and half of the columns.  (Four warps with all columns took 20 us for a tile that read
 // and wrote two FP16 matrices, more than the 17 us of its 4096 of K.)
 //
-// The tensor core cuts additions off instead of rounding them: epilogues that want FP32's digits (kChained) get the sums every 1024 of K and add them up rounded, in registers.
+// The tensor core cuts additions off instead of rounding them: epilogues that want FP32's digits (kChained) get the sums every 1024 of K or so and add them up rounded, in registers.
 //
 // An operand may come in two parts, high + low (splits): the product is then high x high + high x low + low x high, three walks along K into the same sums.
 //
@@ -21,8 +21,8 @@ namespace {
 
 constexpr int kG16Stages = 5, kG16K = 64;                        // stages in flight, of K each
 constexpr unsigned kG16Half = 128 * kG16K * 2, kG16Stage = 2 * kG16Half;
-constexpr int kG16Warps = 8, kG16Threads = 128 + 32 * kG16Warps; // epilogue warps, the last eight
-constexpr int kG16Chain = 1024 / kG16K;                          // stages of a chain of sums
+constexpr int kG16Warps = 8, kG16First = 2, kG16Threads = 32 * (kG16First + kG16Warps);       // epilogue warps, the last eight (ten in all: 200 registers a thread)
+constexpr int kG16Chain = 1024 / kG16K;                          // stages of a chain of sums, about
 constexpr unsigned kG16Box = 32 * 128;                           // 32 rows x 128 bytes on their way out: two for each epilogue warp
 constexpr int kG16Band = 16;                                     // rows of tiles that are walked together, column after column
 
@@ -85,6 +85,9 @@ template <int CTAS> __device__ __forceinline__ void g16_mma(unsigned tmem_d, uin
 __device__ __forceinline__ void pair_meet() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+
+// Chains of sums, 1024 of K each, the last one 512 to 1472 (one stage behind one of 16 kept the epilogue's warps as busy as a whole chain)
+__device__ __forceinline__ int chains_of(int stages) { return max(1, (stages + kG16Chain / 2) / kG16Chain); }
 
 // Where a tile lies
 struct TileAt {
@@ -227,7 +230,7 @@ __global__ void __launch_bounds__(kG16Threads, 1) gemm16_kernel(const __grid_con
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int half = CTAS == 2 ? (int)(blockIdx.x & 1) : 0, first = (int)(blockIdx.x / CTAS), step = (int)(gridDim.x / CTAS);
     const int tiles = g.batch * g.splits * (g.lower ? g.m_tiles * (g.m_tiles + 1) / 2 : g.m_tiles * g.n_tiles);
-    const int stages = g.k_stages * g.parts, chain = EPI::kChained ? kG16Chain : stages;
+    const int stages = g.k_stages * g.parts, chains = EPI::kChained ? chains_of(stages) : 1;
     const bool leader = half == 0;
 
     if (tid == 0) {
@@ -304,12 +307,12 @@ __global__ void __launch_bounds__(kG16Threads, 1) gemm16_kernel(const __grid_con
             const uint64_t a_step = g.a_kmajor ? 2u : 128u, b_step = g.b_kmajor ? 2u : 128u;
             Ring r(kG16Stages), rs(2);
             for (int t = first; t < tiles && ok; t += step) {
-                for (int c0 = 0; c0 < stages && ok; c0 += chain, rs.next()) {
+                for (int n = 0, c0 = 0; n < chains && ok; ++n, c0 += kG16Chain, rs.next()) {
                     if (rs.wrapped) ok = __all_sync(kFullMask, mbar_wait_asleep(&bars.acc_empty[rs.pos], rs.par ^ 1u, status)) != 0;
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const unsigned acc = tmem + (unsigned)rs.pos * 256u;
-                    const int c1 = min(stages, c0 + chain);
+                    const int c1 = n + 1 == chains ? stages : c0 + kG16Chain;
                     for (int d = c0; d < c1; ++d, r.next()) {
                         ok = __all_sync(kFullMask, mbar_wait_asleep(&bars.full[r.pos], r.par, status)) != 0;
                         if (!ok) break;
@@ -338,22 +341,22 @@ __global__ void __launch_bounds__(kG16Threads, 1) gemm16_kernel(const __grid_con
             __syncwarp();
             mbar_wait_asleep(&bars.drain, 0, status);
         }
-    } else if (warp >= 4) {
-        const int quarter = warp & 3, part = (warp - 4) >> 2;    // the lanes of tensor memory this warp may read, its half of the columns
+    } else {
+        const int quarter = warp & 3, part = (warp - kG16First) >> 2;    // the lanes of tensor memory this warp may read, its half of the columns
         int which = 0;
         unsigned fetches = 0;
         Ring rs(2);
         for (int t = first; t < tiles; t += step) {
             const TileAt at = tile_at(g, t);
-            TileOut out = {at.z, at.i * kTile + half * 128 + quarter * 32, at.j * kTile + part * kCols, lane, 0, ok, boxes + (unsigned)(warp - 4) * 2 * kG16Box, &which,
-                           &bars.fetched[warp - 4], &fetches, status};
+            TileOut out = {at.z, at.i * kTile + half * 128 + quarter * 32, at.j * kTile + part * kCols, lane, 0, ok, boxes + (unsigned)(warp - kG16First) * 2 * kG16Box, &which,
+                           &bars.fetched[warp - kG16First], &fetches, status};
             const bool mine = out.row < g.M && out.col < g.N;
             float sums[EPI::kChained ? kCols : 1];
             typename EPI::Ahead ahead;
             if constexpr (!EPI::kChained) {
                 if (mine) epi.template ahead<kCols>(out, ahead);
             }
-            for (int c0 = 0; c0 < stages; c0 += chain, rs.next()) {
+            for (int n = 0; n < chains; ++n, rs.next()) {
                 if (ok) ok = __all_sync(kFullMask, mbar_wait_asleep(&bars.acc_full[rs.pos], rs.par, status, g.tries)) != 0;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 out.taddr = tmem + (unsigned)rs.pos * 256u + (unsigned)(part * kCols) + ((unsigned)(quarter * 32) << 16);
@@ -362,10 +365,10 @@ __global__ void __launch_bounds__(kG16Threads, 1) gemm16_kernel(const __grid_con
                     if (mine) {
 #pragma unroll
                         for (int c = 0; c < kCols; c += 16) {
-                            float v[16];
+                            float v[16];                         // (32 at a time spill: 1264 -> 1634 us for 8192 x 4096 x 32000)
                             read16f(out.taddr + (unsigned)c, v, ok);
 #pragma unroll
-                            for (int j = 0; j < 16; ++j) sums[c + j] = c0 ? sums[c + j] + v[j] : v[j];
+                            for (int j = 0; j < 16; ++j) sums[c + j] = n ? sums[c + j] + v[j] : v[j];
                         }
                     }
                 } else {

@@ -489,7 +489,7 @@ Operands aligned_operands(const XentCall &c, Scratch *s, bool run, cudaError_t *
     Operands o = {{c.x, c.cols, c.tokens, c.ld_x, 1, 0}, {c.w, c.cols, c.vocab, c.ld_w, 1, 0}};
     for (Stack *m : {&o.x, &o.w}) {
         if (!needs_copy(m->at, m->rows, m->ld)) continue;
-        const uint64_t ld = padded(m->cols, 8);
+        const uint64_t ld = padded(m->cols, 64);                  // (rows of whole lines: boxes of 128 bytes then are a line each, not parts of two)
         unsigned short *to = s->take<unsigned short>(m->rows * ld);
         if (run && *err == cudaSuccess) {
             const uint64_t blocks = (m->rows * (ld / 8) + 255) / 256;
@@ -564,12 +564,23 @@ GradPlan grad_plan(const XentCall &c, bool dx, int sm_count) {
     p.pieces = (whole + p.piece - 1) / p.piece;
     p.pairs_l = g16_pairs(c.tokens, p.piece, 1, false, sm_count);
     p.pairs_w = g16_pairs(p.piece, c.cols, 1, false, sm_count);
-    p.pairs_x = g16_pairs(c.tokens, c.cols, 1, false, sm_count);
+    p.pairs_x = false;
     p.splits = 1;
-    const uint64_t tiles = ((c.tokens + 127) / 128) * ((c.cols + 127) / 128), stages = p.piece / kG16K;
-    // few tiles: slices of the vocabulary, as many as SMs take at a time, of four stages at least
-    if (dx && !p.pairs_x)
-        while (p.splits < 64 && tiles * (uint64_t)p.splits * 2 <= (uint64_t)sm_count && stages >= (uint64_t)p.splits * 8) p.splits *= 2;
+    const uint64_t stages = p.piece / kG16K;
+    // Few tiles of dx: slices of the vocabulary, added up afterwards.  What takes least by rounds of tiles times their stages (0.35 us for a pair's, 0.3 us for a single CTA's) and some
+    // 8 us that a round begins and ends with.  777 x 1031 from 50001: 63 tiles of 128 x 128 in two slices 127 us, 20 of 256 x 256 in seven 84.
+    double best = 0.0;
+    for (int pairs = c.tokens > 128 ? 1 : 0; dx && pairs >= 0; --pairs) {
+        const uint64_t side = pairs ? 256 : 128, tiles = ((c.tokens + side - 1) / side) * ((c.cols + side - 1) / side), units = std::max<uint64_t>(1, (uint64_t)sm_count / (pairs ? 2 : 1));
+        for (uint64_t n = 1; n <= 64 && n * 4 <= stages + 3; ++n) {
+            const double sums = n > 1 ? 6.0 + (double)(n * c.tokens * c.cols) * (4.0 + 4.0 * (double)p.pieces) / 5e6 : 0.0;                  // (written piece by piece, read once: 5 TB/s)
+            const double time = (double)p.pieces * (double)((tiles * n + units - 1) / units) * ((double)((stages + n - 1) / n) * (pairs ? 0.35 : 0.3) + 8.0) + sums;
+            if (best != 0.0 && time >= best) continue;
+            best = time;
+            p.pairs_x = pairs != 0;
+            p.splits = (int)n;
+        }
+    }
     p.ld_sum = padded(c.cols, 16);
     return p;
 }
