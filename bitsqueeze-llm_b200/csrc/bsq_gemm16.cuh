@@ -2,7 +2,7 @@
 // FP32 sums in tensor memory.  What becomes of a tile is the epilogue's: statistics of a softmax, gradients of logits, a step of an iteration.
 //
 // Where there are enough tiles, a pair of CTAs on two SMs shares one of 256 x 256 (cta_group::2): each brings 128 rows of A and 128 of B, so that an element from
-// the L2 feeds 256 multiplications.  Small results: one CTA per tile of 128 x 128.  Warp 0 brings stages of 64 of K by TMA (128-byte swizzle, five stages of 32 KB; operands that are
+// the L2 feeds 256 multiplications.  Small results: one CTA per tile of 128 x 128.  Warp 0 brings stages of 64 of K by TMA (128-byte swizzle, five stages of 32 KB or seven; operands that are
 // contiguous along K or along M / N, whichever they are in memory: the tensor core reads either), warp 1 of the leader issues the MMAs, warps 2 to 9 take finished
 // tiles out while the next one is summed in the other half of tensor memory, each 32 rows and half of the columns.  (Four warps with all columns took 20 us for a tile that read
 // and wrote two FP16 matrices, more than the 17 us of its 4096 of K.)
@@ -19,11 +19,11 @@
 namespace bsq {
 namespace {
 
-constexpr int kG16Stages = 5, kG16K = 64;                        // stages in flight, of K each
+constexpr int kG16MaxStages = 7, kG16K = 64;                     // stages in flight at most, of K each
 constexpr unsigned kG16Half = 128 * kG16K * 2, kG16Stage = 2 * kG16Half;
 constexpr int kG16Warps = 8, kG16First = 2, kG16Threads = 32 * (kG16First + kG16Warps);       // epilogue warps, the last eight (ten in all: 200 registers a thread)
 constexpr int kG16Chain = 1024 / kG16K;                          // stages of a chain of sums, about
-constexpr unsigned kG16Box = 32 * 128;                           // 32 rows x 128 bytes on their way out: two for each epilogue warp
+constexpr unsigned kG16Box = 32 * 128;                           // 32 rows x 128 bytes on their way in or out: two for each epilogue warp, or none (EPI::kBoxes)
 constexpr int kG16Band = 16;                                     // rows of tiles that are walked together, column after column
 
 struct Gemm16 {
@@ -42,7 +42,7 @@ struct Gemm16Maps {
 };
 
 struct Gemm16Bars {
-    uint64_t full[kG16Stages], empty[kG16Stages], acc_full[2], acc_empty[2], fetched[kG16Warps], drain;
+    uint64_t full[kG16MaxStages], empty[kG16MaxStages], acc_full[2], acc_empty[2], fetched[kG16Warps], drain;
     unsigned tmem_base;
 };
 
@@ -214,6 +214,7 @@ __device__ __forceinline__ float read_column(unsigned taddr, bool ok) {
     return ok ? __uint_as_float(r) : __uint_as_float(0x7fffffffu);
 }
 
+template <class EPI> __host__ __device__ constexpr int g16_stages() { return EPI::kBoxes ? 5 : kG16MaxStages; }
 // EPI: a functor, called by whole warps:
 //   template <int COLS> void tile(const TileOut &, Ahead &) const     takes COLS columns out; kChained: tile(const TileOut &, float (&sums)[COLS])
 //   template <int COLS> void ahead(const TileOut &, Ahead &) const    what can be asked for while the tile is still being summed (not kChained)
@@ -222,11 +223,11 @@ struct NoAhead {};
 template <class EPI, int CTAS>
 __global__ void __launch_bounds__(kG16Threads, 1) gemm16_kernel(const __grid_constant__ Gemm16Maps maps, const __grid_constant__ EPI epi, const Gemm16 g, unsigned *status) {
     chain_begin();
-    constexpr int kTile = 128 * CTAS, kCols = kTile / 2;
+    constexpr int kTile = 128 * CTAS, kCols = kTile / 2, kStages = g16_stages<EPI>();
     extern __shared__ unsigned char smem_dyn[];
     unsigned char *base = smem_dyn + ((1024u - (smem_u32(smem_dyn) & 1023u)) & 1023u);
-    unsigned char *boxes = base + kG16Stages * kG16Stage;
-    Gemm16Bars &bars = *reinterpret_cast<Gemm16Bars *>(boxes + kG16Warps * 2 * kG16Box);
+    unsigned char *boxes = base + kStages * kG16Stage;
+    Gemm16Bars &bars = *reinterpret_cast<Gemm16Bars *>(boxes + (EPI::kBoxes ? kG16Warps * 2 * kG16Box : 0));
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int half = CTAS == 2 ? (int)(blockIdx.x & 1) : 0, first = (int)(blockIdx.x / CTAS), step = (int)(gridDim.x / CTAS);
     const int tiles = g.batch * g.splits * (g.lower ? g.m_tiles * (g.m_tiles + 1) / 2 : g.m_tiles * g.n_tiles);
@@ -234,7 +235,7 @@ __global__ void __launch_bounds__(kG16Threads, 1) gemm16_kernel(const __grid_con
     const bool leader = half == 0;
 
     if (tid == 0) {
-        for (int i = 0; i < kG16Stages; ++i) {
+        for (int i = 0; i < kStages; ++i) {
             mbar_init(&bars.full[i], 1);
             mbar_init(&bars.empty[i], 1);
         }
@@ -258,7 +259,7 @@ __global__ void __launch_bounds__(kG16Threads, 1) gemm16_kernel(const __grid_con
     if (warp == 0) {
         // ---- operands: this CTA's 128 rows of A and 128 of B ----
         if (lane == 0) {
-            Ring r(kG16Stages);
+            Ring r(kStages);
             int filled = 0;
             for (int t = first; t < tiles && ok; t += step) {
                 const TileAt at = tile_at(g, t);
@@ -295,8 +296,8 @@ __global__ void __launch_bounds__(kG16Threads, 1) gemm16_kernel(const __grid_con
             // copies in flight must have landed before shared memory goes away, also where whoever reads them has given up.  (Those of the other CTA count here too:
             // it does not leave before this one has been here.)
             if (leader)
-                for (int c = max(0, filled - kG16Stages); c < filled; ++c)
-                    mbar_wait_asleep(&bars.full[c % kG16Stages], (unsigned)(c / kG16Stages) & 1u, status, ok ? kWaitTries : kDrainTries);
+                for (int c = max(0, filled - kStages); c < filled; ++c)
+                    mbar_wait_asleep(&bars.full[c % kStages], (unsigned)(c / kStages) & 1u, status, ok ? kWaitTries : kDrainTries);
         }
     } else if (warp == 1) {
         if (leader) {
@@ -305,7 +306,7 @@ __global__ void __launch_bounds__(kG16Threads, 1) gemm16_kernel(const __grid_con
             const unsigned idesc = (1u << 4) | (type << 7) | (type << 10) | (g.a_kmajor ? 0u : 1u << 15) | (g.b_kmajor ? 0u : 1u << 16) | ((unsigned)kTile >> 3 << 17) |
                                    ((unsigned)kTile >> 4 << 24);
             const uint64_t a_step = g.a_kmajor ? 2u : 128u, b_step = g.b_kmajor ? 2u : 128u;
-            Ring r(kG16Stages), rs(2);
+            Ring r(kStages), rs(2);
             for (int t = first; t < tiles && ok; t += step) {
                 for (int n = 0, c0 = 0; n < chains && ok; ++n, c0 += kG16Chain, rs.next()) {
                     if (rs.wrapped) ok = __all_sync(kFullMask, mbar_wait_asleep(&bars.acc_empty[rs.pos], rs.par ^ 1u, status)) != 0;
@@ -395,8 +396,7 @@ __global__ void __launch_bounds__(kG16Threads, 1) gemm16_kernel(const __grid_con
 }
 
 // ---- host ----
-constexpr size_t kG16Smem = 1024 + kG16Stages * kG16Stage + kG16Warps * 2 * kG16Box + sizeof(Gemm16Bars) + 64;
-static_assert(kG16Smem <= 227 * 1024, "stages do not fit");
+template <class EPI> constexpr size_t g16_smem() { return 1024 + g16_stages<EPI>() * kG16Stage + (EPI::kBoxes ? kG16Warps * 2 * kG16Box : 0) + sizeof(Gemm16Bars) + 64; }
 
 // A stack of matrices of 16- or 32-bit elements in memory: `rows` rows of `cols` elements, `ld` apart, matrices `apart` elements apart
 struct Stack {
@@ -423,14 +423,15 @@ inline bool g16_pairs(uint64_t M, uint64_t N, uint64_t batch, bool lower, int sm
 
 template <class EPI, int CTAS>
 cudaError_t launch_gemm16_ctas(const Gemm16Maps &maps, const EPI &epi, const Gemm16 &g, unsigned *status, int sm_count, cudaStream_t stream) {
+    static_assert(g16_smem<EPI>() <= 227 * 1024, "stages do not fit");
     static std::atomic<uint64_t> done{0};
     const cudaError_t err = allow_smem(gemm16_kernel<EPI, CTAS>, &done);
     if (err != cudaSuccess) return err;
     const long tiles = (long)g.batch * g.splits * (g.lower ? (long)g.m_tiles * (g.m_tiles + 1) / 2 : (long)g.m_tiles * g.n_tiles);
     if (tiles > 0x7fffffff / 2 || g.k_stages < 1) return cudaErrorInvalidValue;
     const unsigned grid = (unsigned)std::min<long>(tiles, sm_count / CTAS) * CTAS;
-    if (CTAS == 2) return launch_cluster(gemm16_kernel<EPI, CTAS>, grid, kG16Threads, CTAS, kG16Smem, stream, maps, epi, g, status);
-    return launch_chained(gemm16_kernel<EPI, CTAS>, grid, kG16Threads, kG16Smem, stream, maps, epi, g, status);
+    if (CTAS == 2) return launch_cluster(gemm16_kernel<EPI, CTAS>, grid, kG16Threads, CTAS, g16_smem<EPI>(), stream, maps, epi, g, status);
+    return launch_chained(gemm16_kernel<EPI, CTAS>, grid, kG16Threads, g16_smem<EPI>(), stream, maps, epi, g, status);
 }
 // M, N, batch, parts, splits and the flags of `g` are set; pairs: g16_pairs
 template <class EPI>

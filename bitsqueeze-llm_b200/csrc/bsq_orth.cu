@@ -212,7 +212,7 @@ template <bool SPLIT> struct GramOut {
     float scale;                     // 2^e
     float *rest;                     // what rounding to FP16 takes from the diagonal
 
-    static constexpr bool kChained = false;
+    static constexpr bool kChained = false, kBoxes = true;
     using Ahead = NoAhead;
     template <int COLS> __device__ void ahead(const TileOut &, Ahead &) const {}
     template <int COLS> __device__ void tile(const TileOut &o, Ahead &) const {
@@ -248,7 +248,7 @@ template <bool SPLIT> struct PolyOut {
     float a, back;                   // 2^-e
     float *of_high, *of_low;         // what the parts of X are multiplied by beside the product: a + what rounding takes from the diagonal of P, a + the diagonal
 
-    static constexpr bool kChained = false;
+    static constexpr bool kChained = false, kBoxes = true;
     using Ahead = NoAhead;
     __device__ __forceinline__ bool wanted(const TileOut &o, int c) const { return o.col + c < M && o.col + c <= o.row + 31; }
     template <int COLS> __device__ __forceinline__ void ahead(const TileOut &o, Ahead &) const {
@@ -319,7 +319,7 @@ template <bool SPLIT> struct StepOut {
     uint64_t ld_p;                   // of P: distance of the matrices' diagonals
     OrthOut out;                     // (last)
 
-    static constexpr bool kChained = false;
+    static constexpr bool kChained = false, kBoxes = true;
     struct Ahead {
         float of_sum, of_p, of_q;
     };

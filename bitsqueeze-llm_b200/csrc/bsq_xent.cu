@@ -35,7 +35,7 @@ struct XentStats {
     float *sums;                     // the same: sum of logits (nullable: no smoothing)
     float *at_target;                // M
 
-    static constexpr bool kChained = true;
+    static constexpr bool kChained = true, kBoxes = false;
     using Ahead = NoAhead;
     template <int COLS> __device__ __forceinline__ void tile(const TileOut &o, float (&v)[COLS]) const {
         const int row = o.row + o.lane, n = N - o.col;
@@ -335,7 +335,7 @@ template <int TYPE> struct XentGrad {
     const float *lse2, *coef;
     float low, high;                 // e / vocab, 1 - e
 
-    static constexpr bool kChained = false;
+    static constexpr bool kChained = false, kBoxes = true;
     using Ahead = NoAhead;
     template <int COLS> __device__ void ahead(const TileOut &, Ahead &) const {}
     template <int COLS> __device__ void tile(const TileOut &o, Ahead &) const {
@@ -388,7 +388,7 @@ template <int TYPE> struct ProductOut {
     long ld_sum;
     const float *factor;
 
-    static constexpr bool kChained = false;
+    static constexpr bool kChained = false, kBoxes = true;
     using Ahead = NoAhead;
     template <int COLS> __device__ void ahead(const TileOut &, Ahead &) const {}
     template <int COLS> __device__ void tile(const TileOut &o, Ahead &) const {

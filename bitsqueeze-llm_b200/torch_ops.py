@@ -318,19 +318,25 @@ def _scratch(name, device, *args):
     return torch.empty(need, dtype=torch.uint8, device=device)
 
 
+def _xent_loss(x, weight, target, ignore_index, label_smoothing, reduction):
+    """The loss, what the gradient wants beside it, and the operands as the entries take them."""
+    rows, cols, ld = _rows(x, "x") if x.numel() else (0, x.size(-1), x.size(-1))
+    vocab, _, ld_w = _rows(weight, "weight")
+    device = x.device
+    operands = (_TYPES[x.dtype], x.data_ptr(), rows, cols, ld, weight.data_ptr(), vocab, ld_w)
+    loss = torch.empty(target.shape if reduction == 0 else (), dtype=torch.float32, device=device)
+    stats = torch.empty(rows + 1, dtype=torch.float32, device=device)
+    scratch = _scratch("bsq_linear_xent_scratch_bytes", device, *operands, label_smoothing)
+    _call("bsq_linear_xent", device.index, *operands, target.data_ptr(), ignore_index, label_smoothing, reduction, loss.data_ptr(), stats.data_ptr(), scratch.data_ptr(), None)
+    return loss, stats, operands
+
+
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, target, ignore_index, label_smoothing, reduction):
-        rows, cols, ld = _rows(x, "x") if x.numel() else (0, x.size(-1), x.size(-1))
-        vocab, _, ld_w = _rows(weight, "weight")
-        device, type = x.device, _TYPES[x.dtype]
-        operands = (type, x.data_ptr(), rows, cols, ld, weight.data_ptr(), vocab, ld_w)
-        loss = x.new_empty(target.shape if reduction == 0 else (), dtype=torch.float32)
-        stats = x.new_empty(rows + 1, dtype=torch.float32)
-        scratch = _scratch("bsq_linear_xent_scratch_bytes", device, *operands, label_smoothing)
-        _call("bsq_linear_xent", device.index, *operands, target.data_ptr(), ignore_index, label_smoothing, reduction, loss.data_ptr(), stats.data_ptr(), scratch.data_ptr(), None)
+        loss, stats, ctx.operands = _xent_loss(x, weight, target, ignore_index, label_smoothing, reduction)
         ctx.save_for_backward(x, weight, target, stats)
-        ctx.operands, ctx.how = operands, (ignore_index, label_smoothing, reduction)
+        ctx.how = ignore_index, label_smoothing, reduction
         return loss
 
     @staticmethod
@@ -369,7 +375,10 @@ def linear_cross_entropy(x, weight, target, ignore_index=-100, label_smoothing=0
         raise ValueError("label_smoothing must be within 0 and 1, ignore_index an int64")
     if x.size(-1) > _XENT_COLS or target.numel() > _XENT_TOKENS[x.dtype]:
         raise ValueError("at most %d columns and %d tokens: split the batch" % (_XENT_COLS, _XENT_TOKENS[x.dtype]))
-    return _LinearCrossEntropy.apply(_laid_out(x) if x.numel() else x, _laid_out(weight), target.contiguous(), ignore_index, label_smoothing, _REDUCTIONS[reduction])
+    call = _laid_out(x) if x.numel() else x, _laid_out(weight), target.contiguous(), ignore_index, label_smoothing, _REDUCTIONS[reduction]
+    if (x.requires_grad or weight.requires_grad) and torch.is_grad_enabled():
+        return _LinearCrossEntropy.apply(*call)
+    return _xent_loss(*call)[0]
 
 
 def _dense(t):
