@@ -218,6 +218,7 @@ template <class EPI> __host__ __device__ constexpr int g16_stages() { return EPI
 // EPI: a functor, called by whole warps:
 //   template <int COLS> void tile(const TileOut &, Ahead &) const     takes COLS columns out; kChained: tile(const TileOut &, float (&sums)[COLS])
 //   template <int COLS> void ahead(const TileOut &, Ahead &) const    what can be asked for while the tile is still being summed (not kChained)
+//   void begin() const                                                by one thread of the launch (kChained)
 // CTAS: 1, or 2 for a pair.
 struct NoAhead {};
 template <class EPI, int CTAS>
@@ -246,6 +247,9 @@ __global__ void __launch_bounds__(kG16Threads, 1) gemm16_kernel(const __grid_con
         for (int i = 0; i < kG16Warps; ++i) mbar_init(&bars.fetched[i], 1);
         mbar_init(&bars.drain, 1);
         mbar_fence_init();
+        if constexpr (EPI::kChained) {
+            if (blockIdx.x == 0) epi.begin();
+        }
     }
     if (warp == 1) tmem_alloc<CTAS>(&bars.tmem_base, 512u);
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");

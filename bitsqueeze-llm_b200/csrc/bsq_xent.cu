@@ -5,7 +5,7 @@
 // Loss: one product whose epilogue leaves, for each token and 128 (64) columns of the vocabulary, the largest logit and the sum of exponentials against it, and the target's
 // logit; xent_join_kernel joins a token's tiles.  Nothing of size tokens x vocab is written.
 // Gradient: the vocabulary goes by in pieces of at most 128 MB of dl.  Of a piece the logits are computed again, the epilogue turns them into dl in 16 bits (the
-// rounding that a 16-bit gradient of logits has anyway; scaled, see xent_coef_kernel), then
+// rounding that a 16-bit gradient of logits has anyway; scaled, see XentScale), then
 // dW of the piece is complete, and dx is summed over the pieces in FP32.
 //
 // Exponents are taken in base 2, and the reference of a tile is the rounded product of its largest logit and log2(e), so that the rounding cancels.
@@ -34,9 +34,11 @@ struct XentStats {
     float2 *parts;                   // a warp's columns x M: (largest logit) * log2 e, sum of exponentials against it
     float *sums;                     // the same: sum of logits (nullable: no smoothing)
     float *at_target;                // M
+    unsigned *joined;                // of XentJoin
 
     static constexpr bool kChained = true, kBoxes = false;
     using Ahead = NoAhead;
+    __device__ __forceinline__ void begin() const { *joined = 0u; }
     template <int COLS> __device__ __forceinline__ void tile(const TileOut &o, float (&v)[COLS]) const {
         const int row = o.row + o.lane, n = N - o.col;
         const float none = __uint_as_float(0xff800000u);
@@ -87,6 +89,7 @@ struct XentFew {
     const long long *target;
     float2 *parts;                   // CTAs x tokens
     float *sums, *at_target;         // (sums nullable)
+    unsigned *joined;                // of XentJoin
 };
 template <int VEC> struct FewWords;
 template <> struct FewWords<8> { typedef uint4 type; };
@@ -110,6 +113,7 @@ template <int TYPE, int VEC, int TOKENS> __global__ void __launch_bounds__(kFewT
     unsigned short *sx = reinterpret_cast<unsigned short *>(smem_x);
     __shared__ float part[3][kFewThreads / 32][TOKENS];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, words = f.cols / VEC, ld = (f.cols + 7) / 8 * 8;
+    if (blockIdx.x == 0 && tid == 0) *f.joined = 0u;
     for (int t = 0; t < TOKENS; ++t)
         for (int i = tid; i < f.cols; i += kFewThreads) sx[t * ld + i] = f.x[(uint64_t)t * f.ld_x + i];
     long long target[TOKENS];
@@ -202,6 +206,7 @@ struct XentJoin {
     const float *sums, *at_target;
     float *loss, *stats;             // stats: log2 of the sum of exponentials of each token, then the number of tokens that count
     double2 *blocks;                 // loss and tokens of each CTA
+    unsigned *joined;                // CTAs that have left theirs; 0 at the start (the kernel in front sees to it)
 };
 
 // The sum over a CTA's threads, the same order every time
@@ -267,72 +272,84 @@ __global__ void __launch_bounds__(1024) xent_join_kernel(const XentJoin j) {
         mine = make_double2(loss, live ? 1.0 : 0.0);
     }
     __syncthreads();
-    const double2 v = cta_sum(mine, room);
-    if (threadIdx.x == 0) {
-        if (gridDim.x == 1) write_total(j, v);
-        else j.blocks[blockIdx.x] = v;
+    double2 v = cta_sum(mine, room);
+    if (gridDim.x == 1) {
+        if (threadIdx.x == 0) write_total(j, v);
+        return;
     }
-}
-__global__ void __launch_bounds__(1024) xent_total_kernel(const XentJoin j, int blocks) {
-    chain_begin();
-    __shared__ double2 room[32];
-    double2 v = make_double2(0.0, 0.0);
-    for (int i = threadIdx.x; i < blocks; i += 1024) {
-        v.x += j.blocks[i].x;
-        v.y += j.blocks[i].y;
+    // the CTA that comes last adds them all up, in their order
+    __shared__ bool last;
+    if (threadIdx.x == 0) {
+        j.blocks[blockIdx.x] = v;
+        __threadfence();
+        last = atomicAdd(j.joined, 1u) + 1u == gridDim.x;
+    }
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    v = make_double2(0.0, 0.0);
+    for (unsigned i = threadIdx.x; i < gridDim.x; i += 1024) {
+        const double2 b = __ldcg(&j.blocks[i]);
+        v.x += b.x;
+        v.y += b.y;
     }
     v = cta_sum(v, room);
     if (threadIdx.x == 0) write_total(j, v);
 }
+// No tokens: nothing, 0 or 0 / 0
+__global__ void xent_none_kernel(const XentJoin j) {
+    chain_begin();
+    if (threadIdx.x == 0) write_total(j, make_double2(0.0, 0.0));
+}
 
 // ---- gradient ----
-struct XentCoef {
-    int tokens;
-    long long vocab, ignore;
-    int reduction;
-    float reference;                 // 1 - e + e / vocab, 1 / 4 at least
-    const long long *target;
-    const float *stats, *grad;
-    float *coef, *unscale;           // coefficient of each token; what the products are multiplied by
-};
-// What each token's gradient of logits is multiplied by: g_t, 0 for those that do not count, NaN for a target that is none; times what makes the largest |g| (1 - e + e / vocab) 2^13.
+// What gradients of logits are multiplied by on the way to 16 bits, and the products by on the way back: what makes the largest |g| (1 - e + e / vocab) 2^13.
 // That keeps small gradients within FP16's range (|dl| stays below 2^15), and it makes the element of a target that has next to no probability, the largest of its row and the same in
 // all rows where the g are, a number that 16 bits hold: rounded, it was off by the same part of up to 2^-8 in every row, and so were dx and dW (4096 x 4096 x 32000 in BF16 up to
-// 2.9e-3 off; 1.7e-3 is what their own rounding takes).  One CTA.
-__global__ void __launch_bounds__(1024) xent_coef_kernel(const XentCoef c) {
+// 2.9e-3 off; 1.7e-3 is what their own rounding takes).
+struct XentScale {
+    const float *grad, *stats;       // one gradient for all tokens: of the loss, and (the mean's) the number of tokens behind their statistics
+    int tokens, reduction;
+    float reference;                 // 1 - e + e / vocab, 1 / 4 at least
+    const float *coef, *unscale;     // or one for each token: g_t times the scale, and the way back (xent_coef_kernel)
+
+    // (a gradient of 0, Inf or NaN goes through as it is; below 2^-100 the scale stays finite)
+    __device__ __forceinline__ float top(float m) const { return m > 0.0f && m < __uint_as_float(0x7f800000u) ? fmaxf(m, 7.888609052e-31f) * reference : 8192.0f; }
+    __device__ __forceinline__ float one() const { return reduction == kXentMean ? *grad / stats[tokens] : *grad; }
+    __device__ __forceinline__ float back() const { return coef ? *unscale : top(fabsf(one())) * (1.0f / 8192.0f); }
+    // ... of a token that counts; NaN for a target that is none
+    __device__ __forceinline__ float of(int row, long long target, long long vocab) const {
+        if (target < 0 || target >= vocab) return __uint_as_float(0x7fffffffu);
+        if (coef) return coef[row];
+        const float g = one();
+        return g * (8192.0f / top(fabsf(g)));
+    }
+};
+// Each token's own g: the largest of them, and all of them scaled.  One CTA.
+__global__ void __launch_bounds__(1024) xent_coef_kernel(const XentScale s, const long long *target, long long ignore, float *coef, float *unscale) {
     chain_begin();
     __shared__ float room[32];
-    const float one = c.reduction == kXentNone ? 0.0f : c.reduction == kXentMean ? *c.grad / c.stats[c.tokens] : *c.grad;
-    float m = fabsf(one);
-    if (c.reduction == kXentNone) {
-        for (int i = threadIdx.x; i < c.tokens; i += 1024) {
-            const float a = fabsf(c.grad[i]);
-            if (c.target[i] != c.ignore && a < __uint_as_float(0x7f800000u)) m = fmaxf(m, a);
-        }
-        m = warp_max(m);
-        if ((threadIdx.x & 31) == 0) room[threadIdx.x >> 5] = m;
-        __syncthreads();
-        m = warp_max(room[threadIdx.x & 31]);
+    float m = 0.0f;
+    for (int i = threadIdx.x; i < s.tokens; i += 1024) {
+        const float a = fabsf(s.grad[i]);
+        if (target[i] != ignore && a < __uint_as_float(0x7f800000u)) m = fmaxf(m, a);
     }
-    // (a gradient of 0, Inf or NaN goes through as it is; below 2^-100 the scale stays finite)
-    const float top = m > 0.0f && m < __uint_as_float(0x7f800000u) ? fmaxf(m, 7.888609052e-31f) * c.reference : 8192.0f;
-    const float scale = 8192.0f / top;
-    if (threadIdx.x == 0) *c.unscale = top * (1.0f / 8192.0f);
-    for (int i = threadIdx.x; i < c.tokens; i += 1024) {
-        const long long t = c.target[i];
-        float g = (c.reduction == kXentNone ? c.grad[i] : one) * scale;
-        if (t < 0 || t >= c.vocab) g = __uint_as_float(0x7fffffffu);
-        c.coef[i] = t == c.ignore ? 0.0f : g;
-    }
+    m = warp_max(m);
+    if ((threadIdx.x & 31) == 0) room[threadIdx.x >> 5] = m;
+    __syncthreads();
+    const float top = s.top(warp_max(room[threadIdx.x & 31]));
+    if (threadIdx.x == 0) *unscale = top * (1.0f / 8192.0f);
+    for (int i = threadIdx.x; i < s.tokens; i += 1024) coef[i] = s.grad[i] * (8192.0f / top);
 }
 
 template <int TYPE> struct XentGrad {
     CUtensorMap map;                 // the piece: tokens x its columns
     int M, N;                        // N: columns of the vocabulary in the piece; the piece's others are 0
     long long first;                 // of the vocabulary
-    long long ignore;
+    long long vocab, ignore;
     const long long *target;
-    const float *lse2, *coef;
+    const float *lse2;
+    XentScale scale;
     float low, high;                 // e / vocab, 1 - e
 
     static constexpr bool kChained = false, kBoxes = true;
@@ -343,7 +360,7 @@ template <int TYPE> struct XentGrad {
         const long long t = row < M ? target[row] : ignore;
         const bool live = t != ignore;
         const long long off = live ? t - first - o.col : -1;
-        const float lse = row < M ? lse2[row] : 0.0f, g = row < M ? coef[row] : 0.0f;
+        const float lse = row < M ? lse2[row] : 0.0f, g = live ? scale.of(row, t, vocab) : 0.0f;
         for (int c = 0; c < COLS; c += 64) {
             unsigned char *box = box_next(o);
 #pragma unroll
@@ -386,7 +403,7 @@ template <int TYPE> struct ProductOut {
     long ld;
     const float *sum;
     long ld_sum;
-    const float *factor;
+    XentScale scale;
 
     static constexpr bool kChained = false, kBoxes = true;
     using Ahead = NoAhead;
@@ -407,7 +424,7 @@ template <int TYPE> struct ProductOut {
             }
             return;
         }
-        const float f = *factor;
+        const float f = scale.back();
         const int row = o.row + o.lane;
         for (int c = 0; c < COLS && o.col + c < N; c += 64) {
             unsigned char *box = box_next(o);
@@ -436,9 +453,9 @@ template <int TYPE> struct ProductOut {
 
 // The slices of a product that was split along K, added up in their order
 template <int TYPE>
-__global__ void __launch_bounds__(256) sum_slices_kernel(const float *sum, int slices, int rows, int cols, long ld_sum, const float *factor, void *out, long ld) {
+__global__ void __launch_bounds__(256) sum_slices_kernel(const float *sum, int slices, int rows, int cols, long ld_sum, const XentScale scale, void *out, long ld) {
     chain_begin();
-    const float f = *factor;
+    const float f = scale.back();
     const long all = (long)rows * cols;
     for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < all; i += (long)gridDim.x * 256) {
         const long r = i / cols, c = i - r * cols;
@@ -527,6 +544,7 @@ struct LossRoom {
     float2 *parts;
     float *sums, *at_target;
     double2 *blocks;
+    unsigned *joined;
 };
 LossRoom loss_room(const XentCall &c, const LossPlan &p, Scratch *s) {
     LossRoom r;
@@ -534,6 +552,7 @@ LossRoom loss_room(const XentCall &c, const LossPlan &p, Scratch *s) {
     r.sums = c.smoothing > 0.0 ? s->take<float>(p.tiles * c.tokens) : nullptr;
     r.at_target = s->take<float>(c.tokens);
     r.blocks = s->take<double2>((c.tokens + 31) / 32);
+    r.joined = s->take<unsigned>(1);
     return r;
 }
 
@@ -613,7 +632,7 @@ Gemm16 product_of(uint64_t M, uint64_t N, bool a_kmajor, bool b_kmajor, bool bf1
 // out (or sums): M x N = A B^T
 template <int TYPE>
 cudaError_t product(const Stack &a, bool a_kmajor, const Stack &b, bool b_kmajor, uint64_t M, uint64_t N, uint64_t K, bool pairs, int splits, int mode, void *out, uint64_t ld,
-                    float *sum, uint64_t ld_sum, const float *factor, unsigned *status, int sm_count, cudaStream_t stream) {
+                    float *sum, uint64_t ld_sum, const XentScale &scale, unsigned *status, int sm_count, cudaStream_t stream) {
     Gemm16Maps maps;
     ProductOut<TYPE> e;
     if (!map_operand(&maps.a[0], a, TYPE == kBf16, a_kmajor) || !map_operand(&maps.b[0], b, TYPE == kBf16, b_kmajor)) return cudaErrorInvalidValue;
@@ -627,7 +646,7 @@ cudaError_t product(const Stack &a, bool a_kmajor, const Stack &b, bool b_kmajor
     e.ld = (long)ld;
     e.sum = sum;
     e.ld_sum = (long)ld_sum;
-    e.factor = factor;
+    e.scale = scale;
     e.boxes = out && tma_can_write(out, (M == 1 ? N : ld) * 2, N * 2);
     if (e.boxes && !map_stack(&e.map, {out, N, M, ld, 1, 0}, TYPE, 64, 32)) return cudaErrorInvalidValue;
     if (sum && !map_stack(&e.map_sum, {sum, ld_sum, M, ld_sum, (uint64_t)splits, M * ld_sum}, kF32, 32, 32)) return cudaErrorInvalidValue;
@@ -635,7 +654,7 @@ cudaError_t product(const Stack &a, bool a_kmajor, const Stack &b, bool b_kmajor
 }
 
 template <int TYPE>
-cudaError_t grad_pieces(const XentCall &c, const GradPlan &p, const GradRoom &r, const Operands &o, const float *stats, void *dx, uint64_t ld_dx, void *dw, uint64_t ld_dw,
+cudaError_t grad_pieces(const XentCall &c, const GradPlan &p, const GradRoom &r, const Operands &o, const float *stats, const XentScale &scale, void *dx, uint64_t ld_dx, void *dw, uint64_t ld_dw,
                         unsigned *status, int sm_count, cudaStream_t stream) {
     cudaError_t err = cudaSuccess;
     for (uint64_t i = 0; i < p.pieces && err == cudaSuccess; ++i) {
@@ -650,28 +669,29 @@ cudaError_t grad_pieces(const XentCall &c, const GradPlan &p, const GradRoom &r,
         e.M = (int)c.tokens;
         e.N = (int)n;
         e.first = (long long)first;
+        e.vocab = (long long)c.vocab;
         e.ignore = c.ignore;
         e.target = c.target;
         e.lse2 = stats;
-        e.coef = r.coef;
+        e.scale = scale;
         e.low = (float)(c.smoothing / (double)c.vocab);
         e.high = (float)(1.0 - c.smoothing);
         err = launch_gemm16(maps, e, product_of(c.tokens, n, true, true, TYPE == kBf16), c.cols, p.pairs_l, status, sm_count, stream);
         if (err != cudaSuccess) return err;
         if (dw)
             err = product<TYPE>(dl_valid, false, o.x, false, n, c.cols, c.tokens, p.pairs_w, 1, kProductOut, static_cast<unsigned short *>(dw) + first * ld_dw, ld_dw, nullptr, 0,
-                                r.unscale, status, sm_count, stream);
+                                scale, status, sm_count, stream);
         if (err != cudaSuccess) return err;
         if (dx) {
             const bool last = i + 1 == p.pieces;
             const int mode = !r.sum ? kProductOut : p.splits == 1 && last ? kSumOut : i == 0 ? kSumFirst : kSumMore;
-            err = product<TYPE>(dl_valid, true, w, false, c.tokens, c.cols, n, p.pairs_x, p.splits, mode, dx, ld_dx, r.sum, p.ld_sum, r.unscale, status, sm_count, stream);
+            err = product<TYPE>(dl_valid, true, w, false, c.tokens, c.cols, n, p.pairs_x, p.splits, mode, dx, ld_dx, r.sum, p.ld_sum, scale, status, sm_count, stream);
         }
     }
     if (err == cudaSuccess && dx && p.splits > 1) {
         const uint64_t blocks = (c.tokens * c.cols + 255) / 256;
         err = launch_chained(sum_slices_kernel<TYPE>, (unsigned)std::min<uint64_t>(blocks, (uint64_t)sm_count * 8), 256, 0, stream, (const float *)r.sum, p.splits, (int)c.tokens, (int)c.cols,
-                             (long)p.ld_sum, (const float *)r.unscale, dx, (long)ld_dx);
+                             (long)p.ld_sum, scale, dx, (long)ld_dx);
     }
     return err;
 }
@@ -700,14 +720,14 @@ size_t xent_grad_scratch_bytes(const XentCall &c, bool dx, int sm_count) {
 cudaError_t xent_loss(const XentCall &c, float *loss, float *stats, void *scratch, unsigned *status, int sm_count, cudaStream_t stream) {
     Scratch s = {static_cast<unsigned char *>(scratch)};
     cudaError_t err = cudaSuccess;
-    if (c.tokens == 0) {                                         // nothing, 0 or 0 / 0
-        const XentJoin none = {0, 0, (long long)c.vocab, c.ignore, c.smoothing, c.reduction, nullptr, nullptr, nullptr, nullptr, loss, stats, nullptr};
-        return launch_chained(xent_total_kernel, 1, 1024, 0, stream, none, 0);
+    if (c.tokens == 0) {
+        const XentJoin none = {0, 0, (long long)c.vocab, c.ignore, c.smoothing, c.reduction, nullptr, nullptr, nullptr, nullptr, loss, stats, nullptr, nullptr};
+        return launch_chained(xent_none_kernel, 1, 32, 0, stream, none);
     }
     const LossPlan p = loss_plan(c, sm_count);
     const LossRoom r = loss_room(c, p, &s);
     if (p.few) {
-        const XentFew f = {static_cast<const unsigned short *>(c.x), static_cast<const unsigned short *>(c.w), c.ld_x, c.ld_w, (int)c.cols, (long long)c.vocab, c.target, r.parts, r.sums, r.at_target};
+        const XentFew f = {static_cast<const unsigned short *>(c.x), static_cast<const unsigned short *>(c.w), c.ld_x, c.ld_w, (int)c.cols, (long long)c.vocab, c.target, r.parts, r.sums, r.at_target, r.joined};
         err = c.type == kBf16 ? launch_few<kBf16>(f, p, (int)c.tokens, stream) : launch_few<kF16>(f, p, (int)c.tokens, stream);
     } else {
         const Operands o = aligned_operands(c, &s, true, &err, sm_count, stream);
@@ -717,15 +737,13 @@ cudaError_t xent_loss(const XentCall &c, float *loss, float *stats, void *scratc
         if (!map_operand(&maps.a[0], o.x, bf16, true) || !map_operand(&maps.b[0], o.w, bf16, true)) return cudaErrorInvalidValue;
         maps.a[1] = maps.a[0];
         maps.b[1] = maps.b[0];
-        const XentStats e = {(int)c.tokens, (int)c.vocab, c.target, r.parts, r.sums, r.at_target};
+        const XentStats e = {(int)c.tokens, (int)c.vocab, c.target, r.parts, r.sums, r.at_target, r.joined};
         err = launch_gemm16(maps, e, product_of(c.tokens, c.vocab, true, true, bf16), c.cols, p.pairs, status, sm_count, stream);
     }
     if (err != cudaSuccess) return err;
-    const XentJoin j = {(int)c.tokens, (int)p.tiles, (long long)c.vocab, c.ignore, c.smoothing, c.reduction, c.target, r.parts, r.sums, r.at_target, loss, stats, r.blocks};
+    const XentJoin j = {(int)c.tokens, (int)p.tiles, (long long)c.vocab, c.ignore, c.smoothing, c.reduction, c.target, r.parts, r.sums, r.at_target, loss, stats, r.blocks, r.joined};
     const unsigned blocks = (unsigned)((c.tokens + 31) / 32);
-    err = launch_chained(xent_join_kernel, blocks, 1024, 0, stream, j);
-    if (err == cudaSuccess && blocks > 1) err = launch_chained(xent_total_kernel, 1, 1024, 0, stream, j, (int)blocks);
-    return err;
+    return launch_chained(xent_join_kernel, blocks, 1024, 0, stream, j);
 }
 
 cudaError_t xent_grad(const XentCall &c, const float *stats, const float *grad, void *dx, uint64_t ld_dx, void *dw, uint64_t ld_dw, void *scratch, unsigned *status,
@@ -737,12 +755,12 @@ cudaError_t xent_grad(const XentCall &c, const float *stats, const float *grad, 
     if (err != cudaSuccess) return err;
     const GradPlan p = grad_plan(c, dx != nullptr, sm_count);
     const GradRoom r = grad_room(c, p, dx != nullptr, &s);
-    const XentCoef k = {(int)c.tokens, (long long)c.vocab, c.ignore, c.reduction,
-                        (float)std::max(0.25, 1.0 - c.smoothing + c.smoothing / (double)c.vocab), c.target, stats, grad, r.coef, r.unscale};
-    err = launch_chained(xent_coef_kernel, 1, 1024, 0, stream, k);
+    const bool each = c.reduction == kXentNone;
+    const XentScale scale = {grad, stats, (int)c.tokens, c.reduction, (float)std::max(0.25, 1.0 - c.smoothing + c.smoothing / (double)c.vocab), each ? r.coef : nullptr, each ? r.unscale : nullptr};
+    if (each) err = launch_chained(xent_coef_kernel, 1, 1024, 0, stream, scale, c.target, c.ignore, r.coef, r.unscale);
     if (err != cudaSuccess) return err;
-    return c.type == kBf16 ? grad_pieces<kBf16>(c, p, r, o, stats, dx, ld_dx, dw, ld_dw, status, sm_count, stream)
-                           : grad_pieces<kF16>(c, p, r, o, stats, dx, ld_dx, dw, ld_dw, status, sm_count, stream);
+    return c.type == kBf16 ? grad_pieces<kBf16>(c, p, r, o, stats, scale, dx, ld_dx, dw, ld_dw, status, sm_count, stream)
+                           : grad_pieces<kF16>(c, p, r, o, stats, scale, dx, ld_dx, dw, ld_dw, status, sm_count, stream);
 }
 
 }  // namespace bsq
