@@ -22,33 +22,38 @@ constexpr int kSliceK = 32;                                      // of the long 
 constexpr int kFewSlices = 12;                                   // up to this many are added up by the CTA of the steps
 
 // Elements of a matrix as X has them: the short side is `i`, the long one `k`
-template <int TYPE, bool TALL> __device__ __forceinline__ float element(const OrthSmall &g, int z, int i, int k, float s0, float s1) {
+template <int TYPE, bool TALL> __device__ __forceinline__ float element(const OrthSmall &g, int z, int i, int k) {
     const size_t at = TALL ? (size_t)k * g.ld[z] + (size_t)i : (size_t)i * g.ld[z] + (size_t)k;
     const unsigned w = TYPE == kF32 ? static_cast<const unsigned *>(g.in[z])[at] : (unsigned)static_cast<const unsigned short *>(g.in[z])[at];
-    return word_elem<TYPE>(w, 0) * s0 * s1;
+    return word_elem<TYPE>(w, 0);
 }
-// 2^e that brings a norm below 2^15, in two factors; e
-__device__ __forceinline__ int norm_scale(double norm, float *s0, float *s1) {
-    const bool fine = norm < 3.0e38 * 65536.0 * 65536.0;         // (not: Inf or NaN)
-    const int e = norm > 0.0 && fine ? min(max(14 - ilogb(norm), -160), 160) : 0;
-    *s0 = exp2f((float)(e / 2));
-    *s1 = exp2f((float)(e - e / 2));
+// The sum of squares of a matrix
+__device__ __forceinline__ double squares_of(const OrthSmall &g, int z) {
+    double s = 0.0;
+#pragma unroll 4
+    for (int i = 0; i < g.part_count; ++i) s += g.parts[(size_t)z * (size_t)g.part_count + (size_t)i];
+    return s;
+}
+// 2^e that brings the norm, the square root of `squares`, below 2^15, in two factors; e
+__device__ __forceinline__ int norm_scale(double squares, float *s0, float *s1) {
+    const int of = (int)(((unsigned)__double2hiint(squares) >> 20) & 0x7ffu) - 1023;       // (zero, Inf and NaN: outside of what a sum of FP32's squares has)
+    const int e = of < -320 || of > 320 ? 0 : min(max(14 - (of >> 1), -160), 160);
+    *s0 = exp2f((float)(e >> 1));
+    *s1 = exp2f((float)(e - (e >> 1)));
     return e;
 }
-__device__ __forceinline__ double norm_of(const double *parts, int count) {
-    double s = 0.0;
-    for (int i = 0; i < count; ++i) s += parts[i];
-    return sqrt(s);
+// W (2 or 4) neighbouring floats of shared memory
+template <int W> __device__ __forceinline__ void load_some(const float *p, float *v) {
+    if constexpr (W == 4) *reinterpret_cast<float4 *>(v) = *reinterpret_cast<const float4 *>(p);
+    else *reinterpret_cast<float2 *>(v) = *reinterpret_cast<const float2 *>(p);
 }
 
 // Slice blockIdx.x of A_0 of matrix blockIdx.y: S x S sums over `per` of the long side, 16 x 16 threads with (S / 16)^2 each
 template <int TYPE, bool TALL, int S> __global__ void __launch_bounds__(kThreads) small_gram_kernel(const __grid_constant__ OrthSmall g, int per, float *sums) {
     chain_begin();
-    constexpr int R = S / 16;
+    constexpr int R = S / 16, W = R % 4 ? 2 : 4;                 // sums of a thread: R rows, R columns in runs of W
     __shared__ float tile[kSliceK][S + 4];
     const int z = blockIdx.y, tid = threadIdx.x, ty = tid / 16, tx = tid % 16, first = (int)blockIdx.x * per, last = min(g.l, first + per);
-    float s0, s1;
-    norm_scale(norm_of(g.parts + (size_t)z * g.part_count, g.part_count), &s0, &s1);
     float acc[R][R];
 #pragma unroll
     for (int i = 0; i < R; ++i)
@@ -60,26 +65,28 @@ template <int TYPE, bool TALL, int S> __global__ void __launch_bounds__(kThreads
 #pragma unroll
         for (int j = 0; j < kLoads; ++j) {
             const int n = tid + j * kThreads, k = TALL ? n / S : n % kSliceK, i = TALL ? n % S : n / kSliceK;
-            v[j] = i < g.s && k0 + k < last ? element<TYPE, TALL>(g, z, i, k0 + k, s0, s1) : 0.0f;
+            v[j] = i < g.s && k0 + k < last ? element<TYPE, TALL>(g, z, i, k0 + k) : 0.0f;
         }
     };
-    ask(first);
+    ask(first);                                                  // (before the norm, which is on its way for as long)
+    float s0, s1;
+    norm_scale(squares_of(g, z), &s0, &s1);
     for (int k0 = first; k0 < last; k0 += kSliceK) {
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < kLoads; ++j) {
             const int n = tid + j * kThreads;
-            tile[TALL ? n / S : n % kSliceK][TALL ? n % S : n / kSliceK] = v[j];
+            tile[TALL ? n / S : n % kSliceK][TALL ? n % S : n / kSliceK] = v[j] * s0 * s1;
         }
         __syncthreads();
         if (k0 + kSliceK < last) ask(k0 + kSliceK);              // (on its way while these are summed)
 #pragma unroll 4
         for (int k = 0; k < kSliceK; ++k) {
-            float a[R], b[R];
+            alignas(16) float a[R], b[R];
 #pragma unroll
-            for (int j = 0; j < R; j += 4) {
-                *reinterpret_cast<float4 *>(a + j) = *reinterpret_cast<const float4 *>(&tile[k][ty * R + j]);
-                *reinterpret_cast<float4 *>(b + j) = *reinterpret_cast<const float4 *>(&tile[k][j * 16 + tx * 4]);
+            for (int j = 0; j < R; j += W) {
+                load_some<W>(&tile[k][ty * R + j], a + j);
+                load_some<W>(&tile[k][j * 16 + tx * W], b + j);
             }
 #pragma unroll
             for (int i = 0; i < R; ++i)
@@ -92,7 +99,7 @@ template <int TYPE, bool TALL, int S> __global__ void __launch_bounds__(kThreads
     for (int i = 0; i < R; ++i)
 #pragma unroll
         for (int j = 0; j < R; ++j) {
-            const int r = ty * R + i, c = j / 4 * 64 + tx * 4 + j % 4;
+            const int r = ty * R + i, c = j / W * 16 * W + tx * W + j % W;
             if (r < g.s && c < g.s) to[r * g.s + c] = acc[i][j];
         }
 }
@@ -179,9 +186,9 @@ __global__ void __launch_bounds__(kStepThreads, 1) small_steps_kernel(const __gr
     }
     if (warp == 0) tmem_alloc<1>(&bars.tmem_base, 512u);
     for (unsigned i = tid; i < 3 * kMatrix / 16; i += kStepThreads) reinterpret_cast<uint4 *>(ma)[i] = make_uint4(0u, 0u, 0u, 0u);
-    const double norm = norm_of(g.parts + (size_t)z * g.part_count, g.part_count);
+    const double squares = squares_of(g, z), norm = sqrt(squares);
     float s0, s1;
-    const int e = norm_scale(norm, &s0, &s1);
+    const int e = norm_scale(squares, &s0, &s1);
     // X_0 = G 2^e * factor
     const float factor = !(norm < 3.0e38 * 65536.0 * 65536.0) ? __uint_as_float(0x7fffffffu) : norm > 0.0 ? (float)(ldexp(1.0, -e) / (norm + g.eps)) : 1.0f;
     float v[NH][16];
@@ -331,37 +338,37 @@ __global__ void __launch_bounds__(kStepThreads, 1) small_steps_kernel(const __gr
 // 64 of the long side of matrix blockIdx.y: out = Q G (or G Q)
 template <int TYPE, bool TALL, int S> __global__ void __launch_bounds__(kThreads) small_apply_kernel(const __grid_constant__ OrthSmall g, const float *q) {
     chain_begin();
-    constexpr int R = S / 16;
+    constexpr int R = S / 16, W = R % 4 ? 2 : 4;
     extern __shared__ float smem_apply[];
     float *mq = smem_apply, *tile = smem_apply + S * (S + 4);    // Q [k][i], G [k][64 of the long side]
     const int z = blockIdx.y, tid = threadIdx.x, ty = tid / 16, tx = tid % 16, first = (int)blockIdx.x * 64;
-    float s0, s1;
-    norm_scale(norm_of(g.parts + (size_t)z * g.part_count, g.part_count), &s0, &s1);
-    // (asked for 16 at a time, one wait for each 16)
-#pragma unroll 1
-    for (int from = tid; from < S * S; from += 16 * kThreads) {
-        float v[16];
+    // (all of G and the first 16 of Q are asked for before anything is waited for)
+    constexpr int kLoads = S * 64 / kThreads;
+    float v[kLoads];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            const int n = from + j * kThreads, k = n / S, i = n % S;
-            v[j] = k < g.s && i < g.s ? q[(size_t)z * (size_t)(g.s * g.s) + (size_t)(k * g.s + i)] : 0.0f;
-        }
-#pragma unroll
-        for (int j = 0; j < 16; ++j) mq[(from + j * kThreads) / S * (S + 4) + (from + j * kThreads) % S] = v[j];
+    for (int j = 0; j < kLoads; ++j) {
+        const int n = tid + j * kThreads, k = TALL ? n % S : n / 64, i = TALL ? n / S : n % 64;
+        v[j] = k < g.s && first + i < g.l ? element<TYPE, TALL>(g, z, k, first + i) : 0.0f;
     }
+    constexpr int kBatch = S * S / kThreads < 16 ? S * S / kThreads : 16;
 #pragma unroll 1
-    for (int from = tid; from < S * 64; from += 16 * kThreads) {
-        float v[16];
+    for (int from = tid; from < S * S; from += kBatch * kThreads) {
+        float w[kBatch];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            const int n = from + j * kThreads, k = TALL ? n % S : n / 64, i = TALL ? n / S : n % 64;
-            v[j] = k < g.s && first + i < g.l ? element<TYPE, TALL>(g, z, k, first + i, s0, s1) : 0.0f;
+        for (int j = 0; j < kBatch; ++j) {
+            const int n = from + j * kThreads, k = n / S, i = n % S;
+            w[j] = k < g.s && i < g.s ? q[(size_t)z * (size_t)(g.s * g.s) + (size_t)(k * g.s + i)] : 0.0f;
         }
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            const int n = from + j * kThreads;
-            tile[(TALL ? n % S : n / 64) * 68 + (TALL ? n / S : n % 64)] = v[j];
-        }
+        for (int j = 0; j < kBatch; ++j)
+            if (from + j * kThreads < S * S) mq[(from + j * kThreads) / S * (S + 4) + (from + j * kThreads) % S] = w[j];
+    }
+    float s0, s1;
+    norm_scale(squares_of(g, z), &s0, &s1);
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {
+        const int n = tid + j * kThreads;
+        tile[(TALL ? n % S : n / 64) * 68 + (TALL ? n / S : n % 64)] = v[j] * s0 * s1;
     }
     __syncthreads();
     // wide: a thread has R rows (ty) x 4 columns (tx); tall: 4 rows (ty) x R columns (tx): neighbouring threads write neighbouring elements
@@ -373,9 +380,9 @@ template <int TYPE, bool TALL, int S> __global__ void __launch_bounds__(kThreads
     const int qi = TALL ? tx : ty, gj = TALL ? ty : tx;
 #pragma unroll 4
     for (int k = 0; k < g.s; ++k) {
-        float a[R];
+        alignas(16) float a[R];
 #pragma unroll
-        for (int i = 0; i < R; i += 4) *reinterpret_cast<float4 *>(a + i) = *reinterpret_cast<const float4 *>(mq + k * (S + 4) + i * 16 + qi * 4);
+        for (int i = 0; i < R; i += W) load_some<W>(mq + k * (S + 4) + i * 16 + qi * W, a + i);
         const float4 b = *reinterpret_cast<const float4 *>(tile + k * 68 + gj * 4);
 #pragma unroll
         for (int i = 0; i < R; ++i) {
@@ -385,36 +392,35 @@ template <int TYPE, bool TALL, int S> __global__ void __launch_bounds__(kThreads
             acc[i][3] = fmaf(a[i], b.w, acc[i][3]);
         }
     }
-    __nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(g.out[z]);
+    // through shared memory, so that neighbouring threads write neighbouring elements whatever the rows' alignment: [S][64], or [64][S] where tall
+    __syncthreads();
+    unsigned short *box = reinterpret_cast<unsigned short *>(tile);
+    const auto bits = [](float x) { return __bfloat16_as_ushort(__float2bfloat16_rn(x)); };
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const int r = i / W * 16 * W + qi * W + i % W;
+        if (TALL) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) box[(gj * 4 + j) * S + r] = bits(acc[i][j]);
+        } else {
+            *reinterpret_cast<uint2 *>(box + r * 64 + gj * 4) = make_uint2(pack_pair<kBf16>(acc[i][0], acc[i][1]), pack_pair<kBf16>(acc[i][2], acc[i][3]));
+        }
+    }
+    __syncthreads();
+    unsigned short *out = static_cast<unsigned short *>(g.out[z]);
     const size_t ld = (size_t)g.ld_out[z];
-    const bool whole = (reinterpret_cast<uintptr_t>(out) | (ld * 2)) % 8 == 0;
-    if (TALL) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int r = first + gj * 4 + j;
-            if (r >= g.l) break;
-#pragma unroll
-            for (int i = 0; i < R; i += 4) {
-                const int c = i * 16 + qi * 4;
-                __nv_bfloat16 *to = out + (size_t)r * ld + (size_t)c;
-                if (whole && c + 4 <= g.s) *reinterpret_cast<uint2 *>(to) = make_uint2(pack_pair<kBf16>(acc[i][j], acc[i + 1][j]), pack_pair<kBf16>(acc[i + 2][j], acc[i + 3][j]));
-                else
-#pragma unroll
-                    for (int u = 0; u < 4; ++u)
-                        if (c + u < g.s) to[u] = __float2bfloat16_rn(acc[i + u][j]);
-            }
+    const int rows = TALL ? min(64, g.l - first) : g.s, cols = TALL ? g.s : min(64, g.l - first), width = TALL ? S : 64, at = TALL ? 0 : first, row0 = TALL ? first : 0;
+    if ((reinterpret_cast<uintptr_t>(out) | (ld * 2)) % 8 == 0 && cols % 4 == 0) {
+        const int per = cols / 4;
+        for (int n = tid; n < rows * per; n += kThreads) {
+            const int r = n / per, c = (n - r * per) * 4;
+            *reinterpret_cast<uint2 *>(out + (size_t)(row0 + r) * ld + (size_t)(at + c)) = *reinterpret_cast<const uint2 *>(box + r * width + c);
         }
     } else {
-#pragma unroll
-        for (int i = 0; i < R; ++i) {
-            const int r = i / 4 * 64 + qi * 4 + i % 4, c = first + gj * 4;
-            if (r >= g.s) continue;
-            __nv_bfloat16 *to = out + (size_t)r * ld + (size_t)c;
-            if (whole && c + 4 <= g.l) *reinterpret_cast<uint2 *>(to) = make_uint2(pack_pair<kBf16>(acc[i][0], acc[i][1]), pack_pair<kBf16>(acc[i][2], acc[i][3]));
-            else
-#pragma unroll
-                for (int u = 0; u < 4; ++u)
-                    if (c + u < g.l) to[u] = __float2bfloat16_rn(acc[i][u]);
+#pragma unroll 4
+        for (int n = tid; n < rows * width; n += kThreads) {
+            const int r = n / width, c = n - r * width;
+            if (c < cols) out[(size_t)(row0 + r) * ld + (size_t)(at + c)] = box[n];
         }
     }
 }
@@ -426,7 +432,7 @@ constexpr size_t apply_smem(int s) { return (size_t)(s * (s + 4) + s * 68) * 4; 
 template <int TYPE, bool TALL, int S>
 cudaError_t run(const OrthSmall &g, const OrthSmallSteps &t, int count, const OrthSmallRoom &r, unsigned *status, cudaStream_t stream) {
     static std::atomic<uint64_t> done_steps{0}, done_apply{0};
-    cudaError_t err = allow_smem(small_steps_kernel<S / 64>, &done_steps);
+    cudaError_t err = allow_smem(small_steps_kernel<(S + 63) / 64>, &done_steps);
     if (err == cudaSuccess) err = allow_smem(small_apply_kernel<TYPE, TALL, S>, &done_apply);
     if (err != cudaSuccess) return err;
     err = launch_chained(small_gram_kernel<TYPE, TALL, S>, dim3((unsigned)r.slices, (unsigned)count), kThreads, 0, stream, g, r.per, r.sums);
@@ -440,14 +446,19 @@ cudaError_t run(const OrthSmall &g, const OrthSmallSteps &t, int count, const Or
         sums = r.sum;
         slices = 1;
     }
-    err = launch_chained(small_steps_kernel<S / 64>, (unsigned)count, kStepThreads, kStepsSmem, stream, g, t, sums, slices, r.q, epilogue_tries(kWaitTries), status);
+    err = launch_chained(small_steps_kernel<(S + 63) / 64>, (unsigned)count, kStepThreads, kStepsSmem, stream, g, t, sums, slices, r.q, epilogue_tries(kWaitTries), status);
     if (err != cudaSuccess) return err;
     return launch_chained(small_apply_kernel<TYPE, TALL, S>, dim3((unsigned)((g.l + 63) / 64), (unsigned)count), kThreads, apply_smem(S), stream, g, (const float *)r.q);
 }
+template <int TYPE, bool TALL>
+cudaError_t run_side(const OrthSmall &g, const OrthSmallSteps &t, int count, const OrthSmallRoom &r, unsigned *status, cudaStream_t stream) {
+    if (g.s <= 32) return run<TYPE, TALL, 32>(g, t, count, r, status, stream);
+    if (g.s <= 64) return run<TYPE, TALL, 64>(g, t, count, r, status, stream);
+    return g.s <= 96 ? run<TYPE, TALL, 96>(g, t, count, r, status, stream) : run<TYPE, TALL, 128>(g, t, count, r, status, stream);
+}
 template <int TYPE>
 cudaError_t run_type(const OrthSmall &g, bool tall, const OrthSmallSteps &t, int count, const OrthSmallRoom &r, unsigned *status, cudaStream_t stream) {
-    if (g.s <= 64) return tall ? run<TYPE, true, 64>(g, t, count, r, status, stream) : run<TYPE, false, 64>(g, t, count, r, status, stream);
-    return tall ? run<TYPE, true, 128>(g, t, count, r, status, stream) : run<TYPE, false, 128>(g, t, count, r, status, stream);
+    return tall ? run_side<TYPE, true>(g, t, count, r, status, stream) : run_side<TYPE, false>(g, t, count, r, status, stream);
 }
 
 }  // namespace
