@@ -1,5 +1,5 @@
-"""PyTorch door onto the operators on microscaled 4-bit matrices and on gradients (bsq_fp4_*, bsq_grad_norm_clip in
-include/bitsqz_llm_c.h).
+"""PyTorch door onto the operators on microscaled 4-bit matrices, on gradients, and of the two ends of a training step (bsq_fp4_*, bsq_grad_norm_clip, bsq_linear_xent*,
+bsq_orthogonalize in include/bitsqz_llm_c.h).
 
     x4 = fp4_quantize(x, NVFP4)                 # activations, parked in 4 bits: 0.5625 bytes an element
     w4 = fp4_quantize(w, NVFP4)
@@ -9,6 +9,8 @@ include/bitsqz_llm_c.h).
     x_again = fp4_dequantize(x4, torch.bfloat16)
     norm = clip_grad_norm([dw, ...], 1.0)
     y = fp4_linear(x, w)                        # the first five under autograd
+    loss = linear_cross_entropy(y, head, t)     # over a vocabulary, without its logits, under autograd
+    updates = orthogonalize([dw, ...])          # Newton-Schulz steps
 
 Calls enqueue on PyTorch's current stream of their tensors' device and return; nothing is synchronised, nothing is kept from one
 call to the next, and calls may be captured in a CUDA graph.  Tensors that are used on another stream than the one they were made
