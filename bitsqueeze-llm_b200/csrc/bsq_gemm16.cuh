@@ -155,10 +155,12 @@ __device__ __forceinline__ void boxes_ask(const TileOut &o, const CUtensorMap *f
     }
     __syncwarp();
 }
-__device__ __forceinline__ void boxes_wait(const TileOut &o) {
-    mbar_wait_asleep(o.fetched, *o.fetches & 1u, o.status);
+// The tile with boxes that are there (one that is given up where they do not come)
+__device__ __forceinline__ TileOut boxes_wait(const TileOut &o) {
+    TileOut t = o;
+    t.ok = __all_sync(kFullMask, mbar_wait_asleep(o.fetched, *o.fetches & 1u, o.status)) != 0 && o.ok;
     ++*o.fetches;
-    __syncwarp();
+    return t;
 }
 // ... free to be written without anything that came in
 __device__ __forceinline__ void boxes_free(const TileOut &o) {

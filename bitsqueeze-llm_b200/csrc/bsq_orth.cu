@@ -261,7 +261,7 @@ template <bool SPLIT> struct PolyOut {
         for (int at = 0; at < COLS && wanted(o, at); at += 64) {
             const int col = o.col + at;
             if (at) boxes_ask(o, &map[0], SPLIT ? &map[1] : nullptr, col);
-            boxes_wait(o);
+            const TileOut t = boxes_wait(o);
             put_symmetric<SPLIT>(o, to, at, col + 63 < o.row, [&](int h, float (&v)[16]) {
                 const int c0 = col + 16 * h;
                 float r[16];
@@ -272,7 +272,7 @@ template <bool SPLIT> struct PolyOut {
                 unsigned wp[8], wq[8];
                 box_take16(o, 0, h, wp);
                 if (SPLIT) box_take16(o, 1, h, wq);
-                read16f(o.taddr + (unsigned)(at + 16 * h), v, o.ok);
+                read16f(o.taddr + (unsigned)(at + 16 * h), v, t.ok);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     // A_ij = p + [i = j] rest_i, of which the product has p only
@@ -365,13 +365,13 @@ template <bool SPLIT> struct StepOut {
         for (int c = 0; c < COLS && o.col + c < N; c += 64) {
             const int col = o.col + c;
             if (c) boxes_ask(o, &map[0], &map[1], col);
-            boxes_wait(o);
+            const TileOut t = boxes_wait(o);
             if (!last) {
 #pragma unroll
                 for (int h = 0; h < 4; ++h) {
                     float v[16];
                     unsigned p[8], q[8];
-                    values(o, n, c, h, v);
+                    values(t, n, c, h, v);
                     split16(v, p, q);
                     box_give16(o, 0, h, p);
                     box_give16(o, 1, h, q);
@@ -385,7 +385,7 @@ template <bool SPLIT> struct StepOut {
                 // (32 columns to a box: both are read before one is written)
                 float v[4][16];
 #pragma unroll
-                for (int h = 0; h < 4; ++h) values(o, n, c, h, v[h]);
+                for (int h = 0; h < 4; ++h) values(t, n, c, h, v[h]);
 #pragma unroll
                 for (int h = 0; h < 4; ++h)
 #pragma unroll
@@ -399,7 +399,7 @@ template <bool SPLIT> struct StepOut {
 #pragma unroll
             for (int h = 0; h < 4; ++h) {
                 float v[16];
-                values(o, n, c, h, v);
+                values(t, n, c, h, v);
                 if (type == kBf16) box_put16<kBf16>(o.boxes, o.lane, h, v);
                 else box_put16<kF16>(o.boxes, o.lane, h, v);
             }

@@ -320,23 +320,26 @@ def _scratch(name, device, *args):
     return torch.empty(need, dtype=torch.uint8, device=device)
 
 
-def _xent_loss(x, weight, target, ignore_index, label_smoothing, reduction):
-    """The loss, what the gradient wants beside it, and the operands as the entries take them."""
+def _xent_operands(x, weight):
     rows, cols, ld = _rows(x, "x") if x.numel() else (0, x.size(-1), x.size(-1))
     vocab, _, ld_w = _rows(weight, "weight")
-    device = x.device
-    operands = (_TYPES[x.dtype], x.data_ptr(), rows, cols, ld, weight.data_ptr(), vocab, ld_w)
+    return _TYPES[x.dtype], x.data_ptr(), rows, cols, ld, weight.data_ptr(), vocab, ld_w
+
+
+def _xent_loss(x, weight, target, ignore_index, label_smoothing, reduction):
+    """The loss, and what the gradient wants beside it."""
+    device, operands = x.device, _xent_operands(x, weight)
     loss = torch.empty(target.shape if reduction == 0 else (), dtype=torch.float32, device=device)
-    stats = torch.empty(rows + 1, dtype=torch.float32, device=device)
+    stats = torch.empty(operands[2] + 1, dtype=torch.float32, device=device)
     scratch = _scratch("bsq_linear_xent_scratch_bytes", device, *operands, label_smoothing)
     _call("bsq_linear_xent", device.index, *operands, target.data_ptr(), ignore_index, label_smoothing, reduction, loss.data_ptr(), stats.data_ptr(), scratch.data_ptr(), None)
-    return loss, stats, operands
+    return loss, stats
 
 
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, target, ignore_index, label_smoothing, reduction):
-        loss, stats, ctx.operands = _xent_loss(x, weight, target, ignore_index, label_smoothing, reduction)
+        loss, stats = _xent_loss(x, weight, target, ignore_index, label_smoothing, reduction)
         ctx.save_for_backward(x, weight, target, stats)
         ctx.how = ignore_index, label_smoothing, reduction
         return loss
@@ -346,12 +349,12 @@ class _LinearCrossEntropy(torch.autograd.Function):
     def backward(ctx, grad):
         x, weight, target, stats = ctx.saved_tensors
         device, (want_x, want_w) = x.device, ctx.needs_input_grad[:2]
-        grad = grad.contiguous()                             # (one value for all tokens where the losses were added up)
-        cols = x.size(-1)
+        x, weight = _laid_out(x) if x.numel() else x, _laid_out(weight)      # (hooks may bring back other tensors than were saved)
+        operands, grad, cols = _xent_operands(x, weight), grad.contiguous(), x.size(-1)          # (grad: one value for all tokens where the losses were added up)
         dx = x.new_empty(x.shape) if want_x else None
         dw = weight.new_empty(weight.shape) if want_w else None
-        scratch = _scratch("bsq_linear_xent_grad_scratch_bytes", device, *ctx.operands, 1 if want_x else 0)
-        _call("bsq_linear_xent_grad", device.index, *ctx.operands, target.data_ptr(), *ctx.how, stats.data_ptr(), grad.data_ptr(), None if dx is None else dx.data_ptr(), cols,
+        scratch = _scratch("bsq_linear_xent_grad_scratch_bytes", device, *operands, 1 if want_x else 0)
+        _call("bsq_linear_xent_grad", device.index, *operands, target.data_ptr(), *ctx.how, stats.data_ptr(), grad.data_ptr(), None if dx is None else dx.data_ptr(), cols,
               None if dw is None else dw.data_ptr(), cols, scratch.data_ptr(), None)
         return dx, dw, None, None, None, None
 

@@ -288,6 +288,29 @@ def test_only_what_is_asked_for(ops, need):
         assert not ops.linear_cross_entropy(x, w, t).requires_grad
 
 
+def test_saved_tensors_that_move(ops):
+    """Hooks that put what is kept for the backward pass elsewhere and bring back other tensors, with other strides."""
+    x, w, t = make(70, 64, 900, torch.bfloat16)
+    xa, wa = x.clone().requires_grad_(), w.clone().requires_grad_()
+    want = torch.autograd.grad(ops.linear_cross_entropy(xa, wa, t), (xa, wa))
+    for unpack in (lambda v: v.cuda(), lambda v: v.cuda().t().contiguous().t() if v.dim() == 2 else v.cuda()):
+        with torch.autograd.graph.saved_tensors_hooks(lambda v: v.cpu(), unpack):
+            xb, wb = x.clone().requires_grad_(), w.clone().requires_grad_()
+            loss = ops.linear_cross_entropy(xb * 1, wb * 1, t)
+        filler = [torch.full_like(v, float("nan")) for v in (x, w) for _ in range(4)]            # (over what the products with 1 had)
+        got = torch.autograd.grad(loss, (xb, wb))
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and len(filler) == 8
+
+
+def test_what_was_kept_and_changed(ops):
+    x, w, t = make(70, 64, 900, torch.bfloat16)
+    w.requires_grad_()
+    loss = ops.linear_cross_entropy(x, w, t)
+    x.add_(1)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(loss, w)
+
+
 @pytest.mark.parametrize("tokens,cols,vocab", [(5, 64, 20000), (300, 72, 70001), (2000, 512, 9000)])
 def test_same_bits_every_time(ops, tokens, cols, vocab):
     x, w, t = make(tokens, cols, vocab, torch.bfloat16)
