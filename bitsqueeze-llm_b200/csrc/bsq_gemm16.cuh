@@ -208,14 +208,6 @@ __device__ __forceinline__ void read16f(unsigned taddr, float (&v)[16], bool ok)
 #pragma unroll
     for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
 }
-// One column of accumulators, of all rows of the warp
-__device__ __forceinline__ float read_column(unsigned taddr, bool ok) {
-    unsigned r = 0x7fffffffu;
-    if (ok) asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-    return ok ? __uint_as_float(r) : __uint_as_float(0x7fffffffu);
-}
-
 template <class EPI> __host__ __device__ constexpr int g16_stages() { return EPI::kBoxes ? 5 : kG16MaxStages; }
 // EPI: a functor, called by whole warps:
 //   template <int COLS> void tile(const TileOut &, Ahead &) const     takes COLS columns out; kChained: tile(const TileOut &, float (&sums)[COLS])

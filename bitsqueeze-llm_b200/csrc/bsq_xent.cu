@@ -17,7 +17,7 @@ namespace bsq {
 namespace {
 
 constexpr float kLog2E = 1.4426950408889634f;
-constexpr double kLn2 = 0.69314718055994530942;
+constexpr double kLn2 = 1.0 / (double)kLog2E;                    // the way back from exponents that were taken with the rounded log2(e)
 constexpr float kLowest = -3.0e38f;                              // below every logit but -Inf, whose exponential is 0 against it
 constexpr uint64_t kPieceBytes = 128ull << 20;
 
@@ -204,7 +204,7 @@ struct XentJoin {
     const long long *target;
     const float2 *parts;
     const float *sums, *at_target;
-    float *loss, *stats;             // stats: log2 of the sum of exponentials of each token, then the number of tokens that count
+    float *loss, *stats;             // stats: log2 of the sum of exponentials of each token, the number of tokens that count, then lse - (logit of the target) of each
     double2 *blocks;                 // loss and tokens of each CTA
     unsigned *joined;                // CTAs that have left theirs; 0 at the start (the kernel in front sees to it)
 };
@@ -263,11 +263,13 @@ __global__ void __launch_bounds__(1024) xent_join_kernel(const XentJoin j) {
         const double lse2 = (double)top + log2(sum);
         const long long t = j.target[token];
         const bool live = t != j.ignore, bad = live && (t < 0 || t >= j.vocab);
-        double loss = lse2 * kLn2 - (1.0 - j.smoothing) * (bad ? 0.0 : live ? (double)j.at_target[token] : 0.0);
+        const double at_target = live && !bad ? (double)j.at_target[token] : 0.0;
+        double loss = lse2 * kLn2 - (1.0 - j.smoothing) * at_target;
         if (j.sums) loss -= j.smoothing / (double)j.vocab * all;
         if (bad) loss = __longlong_as_double(0x7ff8000000000000ll);
         if (!live) loss = 0.0;
         j.stats[token] = (float)lse2;
+        j.stats[j.tokens + 1 + token] = (float)(lse2 * kLn2 - at_target);
         if (j.reduction == kXentNone) j.loss[token] = (float)loss;
         mine = make_double2(loss, live ? 1.0 : 0.0);
     }
@@ -348,9 +350,9 @@ template <int TYPE> struct XentGrad {
     long long first;                 // of the vocabulary
     long long vocab, ignore;
     const long long *target;
-    const float *lse2;
+    const float *lse2, *apart;       // apart: lse - (logit of the target)
     XentScale scale;
-    float low, high;                 // e / vocab, 1 - e
+    float low, rest;                 // e / vocab, e - e / vocab
 
     static constexpr bool kChained = false, kBoxes = true;
     using Ahead = NoAhead;
@@ -361,6 +363,8 @@ template <int TYPE> struct XentGrad {
         const bool live = t != ignore;
         const long long off = live ? t - first - o.col : -1;
         const float lse = row < M ? lse2[row] : 0.0f, g = live ? scale.of(row, t, vocab) : 0.0f;
+        // The target's element, from the loss: where p is near 1, p - 1 from the logits would be what their last digits leave of it (1 - p = 1e-3: 2 % off)
+        const float of_target = !o.ok ? __uint_as_float(0x7fffffffu) : live ? g * (expm1f(-apart[row]) + rest) : 0.0f;
         for (int c = 0; c < COLS; c += 64) {
             unsigned char *box = box_next(o);
 #pragma unroll
@@ -381,12 +385,9 @@ template <int TYPE> struct XentGrad {
                 }
                 box_put16<TYPE>(box, o.lane, h, v);
             }
-            const bool here = off >= c && off < c + 64 && off < COLS;
-            for (unsigned left = __ballot_sync(kFullMask, here); left; left &= left - 1) {
-                const int src = __ffs(left) - 1, col = __shfl_sync(kFullMask, (int)off, src);
-                const float l = read_column(o.taddr + (unsigned)col, o.ok);
-                if (o.lane == src)
-                    store_elem<TYPE>(box + o.lane * 128 + (((((col - c) >> 3) ^ (o.lane & 7)) << 4)), (uint64_t)(col & 7), g * ((exp2_fast(fmaf(l, kLog2E, -lse)) - low) - high));
+            if (off >= c && off < c + 64 && off < COLS) {
+                const int col = (int)off - c;
+                store_elem<TYPE>(box + o.lane * 128 + (((col >> 3) ^ (o.lane & 7)) << 4), (uint64_t)(col & 7), of_target);
             }
             box_send(o, &map, o.col + c, o.row, box);
         }
@@ -673,9 +674,10 @@ cudaError_t grad_pieces(const XentCall &c, const GradPlan &p, const GradRoom &r,
         e.ignore = c.ignore;
         e.target = c.target;
         e.lse2 = stats;
+        e.apart = stats + c.tokens + 1;
         e.scale = scale;
         e.low = (float)(c.smoothing / (double)c.vocab);
-        e.high = (float)(1.0 - c.smoothing);
+        e.rest = (float)(c.smoothing - c.smoothing / (double)c.vocab);
         err = launch_gemm16(maps, e, product_of(c.tokens, n, true, true, TYPE == kBf16), c.cols, p.pairs_l, status, sm_count, stream);
         if (err != cudaSuccess) return err;
         if (dw)

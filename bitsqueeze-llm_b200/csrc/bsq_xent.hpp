@@ -25,7 +25,7 @@ struct XentCall {
 
 size_t xent_scratch_bytes(const XentCall &c, int sm_count);
 size_t xent_grad_scratch_bytes(const XentCall &c, bool dx, int sm_count);
-// loss: one float, or one for each token (kXentNone).  stats: tokens + 1 floats for the gradient.
+// loss: one float, or one for each token (kXentNone).  stats: 2 * tokens + 1 floats for the gradient.
 cudaError_t xent_loss(const XentCall &c, float *loss, float *stats, void *scratch, unsigned *status, int sm_count, cudaStream_t stream);
 // grad: of the loss, one float or one for each token.  dx, dw nullable.
 cudaError_t xent_grad(const XentCall &c, const float *stats, const float *grad, void *dx, uint64_t ld_dx, void *dw, uint64_t ld_dw, void *scratch, unsigned *status,

@@ -330,7 +330,7 @@ def _xent_loss(x, weight, target, ignore_index, label_smoothing, reduction):
     """The loss, and what the gradient wants beside it."""
     device, operands = x.device, _xent_operands(x, weight)
     loss = torch.empty(target.shape if reduction == 0 else (), dtype=torch.float32, device=device)
-    stats = torch.empty(operands[2] + 1, dtype=torch.float32, device=device)
+    stats = torch.empty(2 * operands[2] + 1, dtype=torch.float32, device=device)
     scratch = _scratch("bsq_linear_xent_scratch_bytes", device, *operands, label_smoothing)
     _call("bsq_linear_xent", device.index, *operands, target.data_ptr(), ignore_index, label_smoothing, reduction, loss.data_ptr(), stats.data_ptr(), scratch.data_ptr(), None)
     return loss, stats

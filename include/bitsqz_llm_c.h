@@ -301,7 +301,7 @@ int bsq_grad_norm_clip(const void *const *d_grads, const uint64_t *counts, const
  * Softmax cross entropy of the logits l = x W^T, x: tokens x cols, W: vocab x cols (type 1 FP16 or 2 BF16, rows ld apart), without keeping them:
  *   loss_t = lse_t - (1 - smoothing) l_t,target - smoothing / vocab * sum of l_t,   lse_t = log of the sum of exp(l_t)
  * for tokens whose target is not `ignore`; those are 0.  A target outside 0 .. vocab - 1 makes its token's loss NaN.  reduction: 0 d_loss[t] = loss_t, 1 d_loss[0] = their sum,
- * 2 the sum over the number of tokens that are not ignored (none: NaN).  d_stats: tokens + 1 floats that the gradient wants.  Sums are FP32 (of one token) and FP64 (of many).
+ * 2 the sum over the number of tokens that are not ignored (none: NaN).  d_stats: 2 * tokens + 1 floats that the gradient wants.  Sums are FP32 (of one token) and FP64 (of many).
  * Gradient: with d_grad the gradient of d_loss (one float, or one for each token), d_dx (tokens x cols) and d_dw (vocab x cols), either nullable, in the type of x:
  *   dx = dl W,  dW = dl^T x,  dl_tv = g_t (exp(l_tv - lse_t) - (1 - smoothing) [v = target] - smoothing / vocab)
  * dl is rounded to the operands' type, sums are FP32, results rounded once.  Ignored tokens have a dx of 0; their x is multiplied by 0 for dW and has to be finite.

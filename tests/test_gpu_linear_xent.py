@@ -244,6 +244,37 @@ def test_far_logits(ops, dtype):
     check(ops, x * 0, w, t)
 
 
+@pytest.mark.parametrize("tokens", [1, 30, 300])
+@pytest.mark.parametrize("cols,vocab", [(64, 200), (1600, 3000)])
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+def test_sure_tokens(ops, dtype, cols, vocab, tokens):
+    """Targets of a probability of 0.99 to 0.99999: the loss and the gradient are what is left of 1, and as good as any other.  Losses: the rounding of sums near 1 (2^-24 a few
+    times over) against 1e-5 and more; gradients: two roundings of 2^-12 or 2^-9, each row for itself."""
+    gen = torch.Generator(device="cuda").manual_seed(tokens)
+    w = torch.randn(vocab, cols, generator=gen, device="cuda") * (1.5 / cols ** 0.5)
+    t = torch.randint(0, vocab, (tokens,), generator=gen, device="cuda")
+    p = 1 - 10 ** (-2 - 3 * torch.rand(tokens, 1, generator=gen, device="cuda", dtype=torch.float64))
+    x = torch.randn(tokens, cols, generator=gen, device="cuda").double()
+    for _ in range(30):                                            # (moved along the target's row until it has that probability)
+        l = x @ w.double().t()
+        left = torch.log(p / (1 - p)) - (l.gather(1, t[:, None]) - torch.logsumexp(l.scatter(1, t[:, None], float("-inf")), 1, keepdim=True))
+        x = x + left * w[t].double() / w[t].double().square().sum(1, keepdim=True)
+    x, w = x.to(DTYPES[dtype]), w.to(DTYPES[dtype])
+    l = x.double() @ w.double().t()
+    loss = torch.nn.functional.cross_entropy(l, t, reduction="none")
+    dl = torch.softmax(l, 1)
+    dl[torch.arange(tokens), t] = torch.expm1(-loss)
+    dx = dl @ w.double()
+    x.requires_grad_()
+    got = ops.linear_cross_entropy(x, w, t, reduction="none")
+    # (a logit's own error, of the products and their chains, moves the loss by its part of 1 - p)
+    off_l = ((cols / 16 + 2) * 2.0 ** -23) * (x.detach().double().abs() @ w.double().abs().t()).amax(dim=1)
+    assert ((got - loss).abs() <= 8 * 2.0 ** -24 + loss * (2 * off_l + 2.0 ** -18)).all()
+    a, = torch.autograd.grad(got.sum(), x)
+    row = (a.double() - dx).norm(dim=1) / dx.norm(dim=1)
+    assert (row <= 2.5 * torch.finfo(x.dtype).eps / 2 + 8 * 2.0 ** -24 / loss + 2 * off_l).all(), row.max()
+
+
 @pytest.mark.parametrize("scale", [2.0 ** -30, 2.0 ** -15, 1.0, 2.0 ** 16, -3.0])
 @pytest.mark.parametrize("dtype", sorted(DTYPES))
 def test_small_and_large_gradients(ops, dtype, scale):
@@ -375,7 +406,7 @@ def test_beside_the_results(ops, lib, dtype, tokens, cols, vocab):
     xa, wa = x.clone().requires_grad_(), w.clone().requires_grad_()
     dx, dw = torch.autograd.grad(ops.linear_cross_entropy(xa, wa, t, reduction="sum"), (xa, wa))
     type, stream = {"f16": 1, "bf16": 2}[dtype], torch.cuda.current_stream().cuda_stream
-    loss, stats, one = torch.empty(1, device="cuda"), torch.empty(tokens + 1, device="cuda"), torch.ones(1, device="cuda")
+    loss, stats, one = torch.empty(1, device="cuda"), torch.empty(2 * tokens + 1, device="cuda"), torch.ones(1, device="cuda")
     base = (type, x.data_ptr(), tokens, cols, cols, w.data_ptr(), vocab, cols)
     room = torch.empty(lib.bsq_linear_xent_scratch_bytes(*base, 0.0), dtype=torch.uint8, device="cuda")
     assert lib.bsq_linear_xent(*base, t.data_ptr(), IGNORE, 0.0, 1, loss.data_ptr(), stats.data_ptr(), room.data_ptr(), None, stream) == 0
