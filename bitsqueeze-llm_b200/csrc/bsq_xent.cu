@@ -47,30 +47,30 @@ struct XentStats {
             for (int j = 0; j < COLS; ++j)
                 if (j >= n) v[j] = none;
         }
-        float top = v[0];
-#pragma unroll
-        for (int j = 1; j < COLS; ++j) top = fmaxf(top, v[j]);
-        top = fmaxf(top * kLog2E, kLowest);                      // (NaN shows in the sum)
-        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int j = 0; j < COLS; ++j) s[j & 3] += exp2_fast(fmaf(v[j], kLog2E, -top));
         const size_t at = (size_t)(o.col / COLS) * (size_t)M + (size_t)row;
-        if (row < M) parts[at] = make_float2(top, (s[0] + s[1]) + (s[2] + s[3]));
         if (sums) {
             float total[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int j = 0; j < COLS; ++j) total[j & 3] += j < n ? v[j] : 0.0f;
             if (row < M) sums[at] = (total[0] + total[1]) + (total[2] + total[3]);
         }
+        float top = v[0];
+#pragma unroll
+        for (int j = 1; j < COLS; ++j) top = fmaxf(top, v[j]);
+        top = fmaxf(top * kLog2E, kLowest);                      // (NaN shows in the sum)
+        // The target's logit goes by itself, and out of the sum (XentJoin).  (Chosen for every element: taken out in its place it puts the whole array into memory, and sums taken
+        // again in the few warps that have a target spill; 1264 -> 1600 us for 8192 x 4096 x 32000 either way.)
         const long long off = row < M ? target[row] - o.col : -1;
         const bool here = off >= 0 && off < COLS && off < n;
-        if (__any_sync(kFullMask, here)) {
-            float mine = 0.0f;
+        const int at_j = here ? (int)off : -1;
+        float mine = 0.0f, s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int j = 0; j < COLS; ++j)
-                if (j == (int)off) mine = v[j];
-            if (here) at_target[row] = mine;
+        for (int j = 0; j < COLS; ++j) {
+            mine = j == at_j ? v[j] : mine;
+            s[j & 3] += exp2_fast(fmaf(j == at_j ? none : v[j], kLog2E, -top));
         }
+        if (here) at_target[row] = mine;
+        if (row < M) parts[at] = make_float2(top, (s[0] + s[1]) + (s[2] + s[3]));
     }
 };
 
@@ -164,9 +164,12 @@ template <int TYPE, int VEC, int TOKENS> __global__ void __launch_bounds__(kFewT
             for (int r = 0; r < kFewRows; ++r) {
                 float l = acc[r][t];
                 for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(kFullMask, l, d);
-                if (r0 + r >= f.vocab) break;
+                if (r0 + r >= f.vocab) continue;
                 total[t] += l;
-                if (r0 + r == target[t] && lane == 0) f.at_target[t] = l;
+                if (r0 + r == target[t]) {                       // (by itself, and out of the sum)
+                    if (lane == 0) f.at_target[t] = l;
+                    continue;
+                }
                 const float m = l * kLog2E;
                 if (m > top[t]) {
                     s[t] *= exp2_fast(top[t] - m);
@@ -230,7 +233,8 @@ __device__ __forceinline__ void write_total(const XentJoin &j, double2 v) {
     else if (j.reduction == kXentMean) *j.loss = (float)(v.x / v.y);
 }
 
-// 32 tokens a CTA, one for each lane; the warps share the tiles
+// 32 tokens a CTA, one for each lane; the warps share the tiles.  The parts are without the target's logit t: the loss is log(1 + sum exp(l_v - t)), and as good where the sum is
+// 10^-6 as where it is 10 (with exp(t - t) among the terms, a loss of 10^-3 was 5e-5 off).
 __global__ void __launch_bounds__(1024) xent_join_kernel(const XentJoin j) {
     chain_begin();
     __shared__ float2 part[32][32];
@@ -253,23 +257,29 @@ __global__ void __launch_bounds__(1024) xent_join_kernel(const XentJoin j) {
     __syncthreads();
     double2 mine = make_double2(0.0, 0.0);
     if (warp == 0 && token < j.tokens) {
-        double sum = 0.0, all = 0.0;
+        float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};                // (FP64 additions one behind the other took 3 us)
+#pragma unroll
         for (int i = 0; i < 32; ++i) top = fmaxf(top, part[i][lane].x);
-        for (int i = 0; i < 32; ++i) {
-            const float2 p = part[i][lane];
-            sum += (double)(p.y * exp2_fast(p.x - top));
-            all += (double)part_sum[i][lane];
-        }
-        const double lse2 = (double)top + log2(sum);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) sums[i & 3] += part[i][lane].y * exp2_fast(part[i][lane].x - top);
+        const double sum = (double)((sums[0] + sums[1]) + (sums[2] + sums[3]));
+        double all = 0.0;
+        if (j.sums)
+            for (int i = 0; i < 32; ++i) all += (double)part_sum[i][lane];
         const long long t = j.target[token];
-        const bool live = t != j.ignore, bad = live && (t < 0 || t >= j.vocab);
-        const double at_target = live && !bad ? (double)j.at_target[token] : 0.0;
-        double loss = lse2 * kLn2 - (1.0 - j.smoothing) * at_target;
-        if (j.sums) loss -= j.smoothing / (double)j.vocab * all;
-        if (bad) loss = __longlong_as_double(0x7ff8000000000000ll);
+        const bool live = t != j.ignore, in = t >= 0 && t < j.vocab;
+        double lse2 = (double)top + log2(sum), apart = 0.0;      // (without its target nobody wants it)
+        if (in) {
+            const double at = (double)j.at_target[token], at2 = at * (double)kLog2E, other = lse2 - at2;        // (log2 of the others against the target)
+            apart = isinf(at) && at > 0.0 ? __longlong_as_double(0x7ff8000000000000ll) : other > 60.0 ? other * kLn2 : log1p(exp2(other));
+            lse2 = at2 > (double)top ? at2 + apart / kLn2 : (double)top + log2(sum + exp2(at2 - (double)top));
+        }
+        double loss = apart;
+        if (j.sums) loss += j.smoothing * ((in ? (double)j.at_target[token] : 0.0) - all / (double)j.vocab);
+        if (!in) loss = __longlong_as_double(0x7ff8000000000000ll);
         if (!live) loss = 0.0;
         j.stats[token] = (float)lse2;
-        j.stats[j.tokens + 1 + token] = (float)(lse2 * kLn2 - at_target);
+        j.stats[j.tokens + 1 + token] = (float)apart;
         if (j.reduction == kXentNone) j.loss[token] = (float)loss;
         mine = make_double2(loss, live ? 1.0 : 0.0);
     }
