@@ -8,6 +8,7 @@
 // and wrote two FP16 matrices, more than the 17 us of its 4096 of K.)
 //
 // The tensor core cuts additions off instead of rounding them: epilogues that want FP32's digits (kChained) get the sums every 1024 of K or so and add them up rounded, in registers.
+// Others (kTotals, chains of Gemm16::chain) have them added up, rounded, in the other half of tensor memory, from which the tile is then taken: 128 sums beside what those epilogues hold spill.
 //
 // An operand may come in two parts, high + low (splits): the product is then high x high + high x low + low x high, three walks along K into the same sums.
 //
@@ -30,6 +31,7 @@ struct Gemm16 {
     int M, N;                        // of one matrix of the stack
     int m_tiles, n_tiles, batch;
     int k_stages, parts;             // stages along K of a tile, walks along K (1, or 3 of split operands)
+    int chain;                       // stages of a chain of sums, about; 0: one chain (kTotals)
     int splits;                      // a matrix's tiles are this many, each with k_stages of K, one behind the other: z = matrix * splits + slice
     bool a_kmajor, b_kmajor;         // contiguous along K, or along M / N
     bool lower;                      // the result is symmetric: tiles on and below the diagonal only
@@ -86,8 +88,8 @@ __device__ __forceinline__ void pair_meet() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// Chains of sums, 1024 of K each, the last one 512 to 1472 (one stage behind one of 16 kept the epilogue's warps as busy as a whole chain)
-__device__ __forceinline__ int chains_of(int stages) { return max(1, (stages + kG16Chain / 2) / kG16Chain); }
+// Chains of sums, the last one half to one and a half of the others' length (one stage behind one of 16 kept the epilogue's warps as busy as a whole chain)
+__device__ __forceinline__ int chains_of(int stages, int chain) { return chain ? max(1, (stages + chain / 2) / chain) : 1; }
 
 // Where a tile lies
 struct TileAt {
@@ -226,7 +228,8 @@ __global__ void __launch_bounds__(kG16Threads, 1) gemm16_kernel(const __grid_con
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int half = CTAS == 2 ? (int)(blockIdx.x & 1) : 0, first = (int)(blockIdx.x / CTAS), step = (int)(gridDim.x / CTAS);
     const int tiles = g.batch * g.splits * (g.lower ? g.m_tiles * (g.m_tiles + 1) / 2 : g.m_tiles * g.n_tiles);
-    const int stages = g.k_stages * g.parts, chains = EPI::kChained ? chains_of(stages) : 1;
+    const int stages = g.k_stages * g.parts, chain = EPI::kChained ? kG16Chain : EPI::kTotals ? g.chain : 0, chains = chains_of(stages, chain);
+    const bool totals = EPI::kTotals && chains > 1;              // the MMAs write one half of tensor memory, the other one has the tile's total; else they write both by turns
     const bool leader = half == 0;
 
     if (tid == 0) {
@@ -304,14 +307,14 @@ __global__ void __launch_bounds__(kG16Threads, 1) gemm16_kernel(const __grid_con
             const unsigned idesc = (1u << 4) | (type << 7) | (type << 10) | (g.a_kmajor ? 0u : 1u << 15) | (g.b_kmajor ? 0u : 1u << 16) | ((unsigned)kTile >> 3 << 17) |
                                    ((unsigned)kTile >> 4 << 24);
             const uint64_t a_step = g.a_kmajor ? 2u : 128u, b_step = g.b_kmajor ? 2u : 128u;
-            Ring r(kStages), rs(2);
+            Ring r(kStages), rs(totals ? 1 : 2);
             for (int t = first; t < tiles && ok; t += step) {
-                for (int n = 0, c0 = 0; n < chains && ok; ++n, c0 += kG16Chain, rs.next()) {
+                for (int n = 0, c0 = 0; n < chains && ok; ++n, c0 += chain, rs.next()) {
                     if (rs.wrapped) ok = __all_sync(kFullMask, mbar_wait_asleep(&bars.acc_empty[rs.pos], rs.par ^ 1u, status)) != 0;
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const unsigned acc = tmem + (unsigned)rs.pos * 256u;
-                    const int c1 = n + 1 == chains ? stages : c0 + kG16Chain;
+                    const int c1 = n + 1 == chains ? stages : c0 + chain;
                     for (int d = c0; d < c1; ++d, r.next()) {
                         ok = __all_sync(kFullMask, mbar_wait_asleep(&bars.full[r.pos], r.par, status)) != 0;
                         if (!ok) break;
@@ -344,7 +347,7 @@ __global__ void __launch_bounds__(kG16Threads, 1) gemm16_kernel(const __grid_con
         const int quarter = warp & 3, part = (warp - kG16First) >> 2;    // the lanes of tensor memory this warp may read, its half of the columns
         int which = 0;
         unsigned fetches = 0;
-        Ring rs(2);
+        Ring rs(totals ? 1 : 2);
         for (int t = first; t < tiles; t += step) {
             const TileAt at = tile_at(g, t);
             TileOut out = {at.z, at.i * kTile + half * 128 + quarter * 32, at.j * kTile + part * kCols, lane, 0, ok, boxes + (unsigned)(warp - kG16First) * 2 * kG16Box, &which,
@@ -355,6 +358,15 @@ __global__ void __launch_bounds__(kG16Threads, 1) gemm16_kernel(const __grid_con
             if constexpr (!EPI::kChained) {
                 if (mine) epi.template ahead<kCols>(out, ahead);
             }
+            const auto empty = [&] {
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                // (not where this warp has given up: it runs ahead from here on, and its arrivals would let accumulators be overwritten that others still read)
+                if (ok && lane == 0) {
+                    if (CTAS == 2) mbar_arrive_pair(smem_u32(&bars.acc_empty[rs.pos]) + lead);
+                    else mbar_arrive(&bars.acc_empty[rs.pos]);
+                }
+            };
             for (int n = 0; n < chains; ++n, rs.next()) {
                 if (ok) ok = __all_sync(kFullMask, mbar_wait_asleep(&bars.acc_full[rs.pos], rs.par, status, g.tries)) != 0;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -370,19 +382,29 @@ __global__ void __launch_bounds__(kG16Threads, 1) gemm16_kernel(const __grid_con
                             for (int j = 0; j < 16; ++j) sums[c + j] = n ? sums[c + j] + v[j] : v[j];
                         }
                     }
-                } else {
-                    if (mine) epi.template tile<kCols>(out, ahead);
+                } else if (totals && mine && ok) {
+                    const unsigned total = out.taddr + 256u;
+#pragma unroll 2
+                    for (unsigned c = 0; c < (unsigned)kCols; c += 16) {
+                        unsigned v[16];
+                        read16(out.taddr + c, v, true);
+                        if (n) add16(total + c, v);
+                        tmem_st16(total + c, v);
+                    }
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 }
-                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                __syncwarp();
-                // (not where this warp has given up: it runs ahead from here on, and its arrivals would let accumulators be overwritten that others still read)
-                if (ok && lane == 0) {
-                    if (CTAS == 2) mbar_arrive_pair(smem_u32(&bars.acc_empty[rs.pos]) + lead);
-                    else mbar_arrive(&bars.acc_empty[rs.pos]);
-                }
+                if (!EPI::kChained && !totals) break;
+                empty();
             }
             if constexpr (EPI::kChained) {
                 if (mine) epi.template tile<kCols>(out, sums);
+            } else {
+                if (totals) out.taddr += 256u;
+                if (mine) epi.template tile<kCols>(out, ahead);
+                if (!totals) {
+                    empty();
+                    rs.next();
+                }
             }
         }
         if (lane == 0) bulk_wait_all();

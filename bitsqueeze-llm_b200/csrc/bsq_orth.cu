@@ -25,6 +25,9 @@ namespace bsq {
 namespace {
 
 constexpr uint64_t kOrthRoom = 1ull << 30;                       // scratch that several matrices share at most
+// Stages of a chain of sums (4096 of K, of split operands 1024).  What the tensor core cuts off where a sum's terms have one sign is not of X's rank, and each step pulls it up by 3.4: rank one,
+// 65536 x 33000, was 8.8e-3 off in BF16 and 3.1e-2 in FP32 with one chain for all of K, and is 2.8e-3 (its rounding to BF16 is 2e-3 of that) and 1.7e-4.  Up to 6100 of K BF16 has one chain still
+template <bool SPLIT> constexpr int kOrthChain = (SPLIT ? 1024 : 4096) / kG16K;
 constexpr int kNormThreads = 512;
 constexpr uint64_t kNormChunk = 16384;                           // elements of a CTA of the pass that finds the norms, at least
 constexpr int kNormParts = kNormThreads;
@@ -216,7 +219,7 @@ template <bool SPLIT> struct GramOut {
     float scale;                     // 2^e
     float *rest;                     // what rounding to FP16 takes from the diagonal
 
-    static constexpr bool kChained = false, kBoxes = true;
+    static constexpr bool kChained = false, kTotals = true, kBoxes = true;
     using Ahead = NoAhead;
     template <int COLS> __device__ void ahead(const TileOut &, Ahead &) const {}
     template <int COLS> __device__ void tile(const TileOut &o, Ahead &) const {
@@ -252,7 +255,7 @@ template <bool SPLIT> struct PolyOut {
     float a, back;                   // 2^-e
     float *of_high, *of_low;         // what the parts of X are multiplied by beside the product: a + what rounding takes from the diagonal of P, a + the diagonal
 
-    static constexpr bool kChained = false, kBoxes = true;
+    static constexpr bool kChained = false, kTotals = true, kBoxes = true;
     struct Ahead {
         float mine;                  // of A's diagonal: the row's, the columns'
         Shared64 theirs;
@@ -326,7 +329,7 @@ template <bool SPLIT> struct StepOut {
     uint64_t ld_p;                   // of P: distance of the matrices' diagonals
     OrthOut out;                     // (last)
 
-    static constexpr bool kChained = false, kBoxes = true;
+    static constexpr bool kChained = false, kTotals = true, kBoxes = true;
     struct Ahead {
         float of_sum, of_p, of_q;
         Shared64 e, d;               // (tall: the columns')
@@ -647,6 +650,7 @@ cudaError_t run_group(const OrthCall &c, const std::vector<StepScale> &scales, c
     g.batch = count;
     g.splits = 1;
     g.parts = SPLIT ? 3 : 1;
+    g.chain = kOrthChain<SPLIT>;
     const bool pairs_s = g16_pairs(s, s, (uint64_t)count, true, sm_count), pairs_x = g16_pairs(rows, cols, (uint64_t)count, false, sm_count);
     for (int step = 0; step < c.steps; ++step) {
         const int now = step & 1;

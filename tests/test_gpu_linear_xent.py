@@ -144,6 +144,33 @@ def test_many_tokens(ops):
     check(ops, *make(40000, 16, 513, torch.float16))
 
 
+@pytest.mark.parametrize("tokens", [2, 9])
+def test_weights_beyond_32_bits(ops, tokens):
+    """2.2 10^9 elements, rows off 16 bytes; targets and the rows that are looked at on both sides of 2^31."""
+    cols, vocab = 4100, 530000
+    gen = torch.Generator(device="cuda").manual_seed(tokens)
+    w = torch.empty(vocab, cols, dtype=torch.bfloat16, device="cuda").normal_(0, 1.5 / cols ** 0.5, generator=gen)
+    x = torch.randn(tokens, cols, generator=gen, device="cuda").bfloat16()
+    t = torch.tensor([vocab - 1 - 3000 * i for i in range(tokens)], device="cuda")
+    l = torch.cat([x.double() @ w[i: i + 50000].double().t() for i in range(0, vocab, 50000)], dim=1)
+    loss = torch.nn.functional.cross_entropy(l, t, reduction="none")
+    dl = torch.softmax(l, 1)
+    dl[torch.arange(tokens), t] -= 1
+    x.requires_grad_(), w.requires_grad_()
+    got = ops.linear_cross_entropy(x, w, t, reduction="none")
+    assert ((got - loss).abs() <= 1e-4).all()                      # (cols / 16 steps of 2^-23 of sums of magnitudes of some 80, and more)
+    dx, dw = torch.autograd.grad(got.sum(), (x, w))
+    with torch.no_grad():
+        want = sum(dl[:, i: i + 50000] @ w[i: i + 50000].double() for i in range(0, vocab, 50000))
+        assert ((dx.double() - want).norm(dim=1) <= 2.0 ** -7 * want.norm(dim=1)).all()
+        for first in (0, 500, (1 << 31) // cols - 50, vocab - 100):
+            part = dl[:, first: first + 100].t() @ x.double()
+            assert ((dw[first: first + 100].double() - part).norm() <= 2.0 ** -7 * part.norm())
+        for v in t.tolist():
+            part = dl[:, v] @ x.double()
+            assert ((dw[v].double() - part).norm() <= 2.0 ** -7 * part.norm())
+
+
 @pytest.mark.parametrize("dtype", sorted(DTYPES))
 def test_strides(ops, dtype):
     x, w, t = make(150, 100, 1000, DTYPES[dtype])

@@ -97,6 +97,38 @@ def test_magnitudes(ops, scale):
         check(ops, make(300, 150, scale=scale).half())
 
 
+@pytest.mark.parametrize("m,n", [(33000, 65536), (65536, 33000)])
+def test_beyond_32_bits(ops, m, n):
+    """2.2 10^9 elements of rank one, u v^T: the one singular value goes the way of a number, the rest stays what it is, nothing."""
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    u, v = torch.randint(1, 9, (m, 1), generator=gen, device="cuda").bfloat16(), torch.randint(1, 9, (1, n), generator=gen, device="cuda").bfloat16()
+    g = u * v                                                      # (whole numbers up to 64: exact)
+    got = ops.orthogonalize(g)
+    s, (a, b, c) = 1.0, QUINTIC
+    for _ in range(5):
+        s = a * s + b * s ** 3 + c * s ** 5
+    scale = s / (u.double().norm() * v.double().norm()).item()
+    for rows in (slice(0, 300), slice(m // 2, m // 2 + 300), slice(m - 300, m)):
+        want = u[rows].double() @ v.double() * scale
+        assert off(got[rows], want) <= 2.0 ** -8
+
+
+@pytest.mark.parametrize("m,n", [(16384, 32768), (32768, 16384)])
+def test_long_sums_of_one_sign(ops, m, n):
+    """Rank one in FP32.  What the sums of P X lose need not be of X's rank: each later step pulls it up by a = 3.4445.  A chain has 92 additions of 16 products at most (23 stages of 64); each cuts
+    off up to 2^-23 of what it has by then, so the sum loses up to (92 + 1) / 2 * 2^-23 = 5.5e-6 of |P| s.  With s = 1, 0.701, 1.114, 0.721, 1.090 and |P| = 2.74, 1.86, 2.80, 1.93, 2.81, and 3.4445^4
+    ... 1 for the steps that follow: 2.8e-3 of s = 0.696 at the end, 4.1e-3 of it; roundings to 22 bits are in that, and A and P, whose errors share u or v with X and grow by 1.6 a step at most, add 2.5e-4."""
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    u, v = torch.randint(1, 9, (m, 1), generator=gen, device="cuda").bfloat16(), torch.randint(1, 9, (1, n), generator=gen, device="cuda").bfloat16()
+    got = ops.orthogonalize(u * v, dtype=torch.float32)
+    s, (a, b, c) = 1.0, QUINTIC
+    for _ in range(5):
+        s = a * s + b * s ** 3 + c * s ** 5
+    scale = s / (u.double().norm() * v.double().norm()).item()
+    for rows in (slice(0, 300), slice(m // 2, m // 2 + 300), slice(m - 300, m)):
+        assert off(got[rows], u[rows].double() @ v.double() * scale) <= 4.5e-3
+
+
 def test_eps(ops):
     g = make(150, 300, scale=1e-9)                                 # |G| about 2e-7
     for eps in (0.0, 1e-7, 1e-6):
