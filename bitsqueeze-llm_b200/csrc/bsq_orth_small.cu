@@ -5,7 +5,9 @@
 // 24 matrices of 64 x 1024 took 230 us; this way all five take 66.)
 //
 // Rounding grows with what it meets: an error of A_0 by (a^2)^(n - 1), 2 10^4 for five steps.  FP32 sums for A_0 and products of split operands (22 bits) leave 1e-4 to 2e-4 in the result
-// (singular values over a range of 1000; noise alone 1e-6), a tenth of its rounding to BF16.  FP32 and FP16 results, and long sides, are bsq_orth.cu's.
+// (singular values over a range of 1000; noise alone 1e-6), a tenth of its rounding to BF16.
+// Of rank one there is nothing beside the one direction but A_0's roundings: Gaussian factors 2.4e-3 to 3.1e-3 with the rounding to BF16 (1.7e-3), whole numbers from 1 to 8, whose few products
+// are all rounded alike, up to 9e-3 (128 x 65536); with rank 8 or noise 1.7e-3 again.  FP32 and FP16 results, and long sides, are bsq_orth.cu's.
 //
 // Launches: norm (bsq_orth.cu), A_0 in slices of the long side on the FP32 pipes, their sum where there are many, the steps on the tensor core, Q X_0 on the FP32 pipes.
 #include "bsq_gemm16.cuh"
