@@ -284,7 +284,7 @@ size_t bsq_orthogonalize_scratch_bytes(const uint64_t *rows, const uint64_t *col
             if (!op_bytes(types[i]) || rows[i] > kOrthMaxDim || cols[i] > kOrthMaxDim) return 0;
             m[(size_t)i] = {nullptr, nullptr, rows[i], cols[i], cols[i], cols[i], types[i]};
         }
-        return orth_scratch_bytes({m.data(), n, out_type, 0, nullptr, 0.0, 0.0f}, device_sm_count());
+        return orth_scratch_bytes({m.data(), n, out_type, 0, nullptr, 0.0, 0.0f});
     } catch (...) {
         return 0;
     }

@@ -477,7 +477,7 @@ struct Room {
     uint64_t ld_x, apart_x, ld_a, apart_a;
     size_t bytes;
 };
-Room room_of(const OrthMatrix &m, Way way, int count, int sm_count, void *scratch) {
+Room room_of(const OrthMatrix &m, Way way, int count, void *scratch) {
     Room r = {};
     const uint64_t s = std::min(m.rows, m.cols), n = (uint64_t)count;
     unsigned char *base = static_cast<unsigned char *>(scratch);
@@ -488,7 +488,7 @@ Room room_of(const OrthMatrix &m, Way way, int count, int sm_count, void *scratc
     };
     r.parts = reinterpret_cast<double *>(take(n * kNormParts * 8));
     if (way == kSmall) {
-        r.small.slices = orth_small_slices(std::max(m.rows, m.cols), count, sm_count, &r.small.per);
+        r.small.slices = orth_small_slices(std::max(m.rows, m.cols), &r.small.per);
         r.small.sums = reinterpret_cast<float *>(take(n * (uint64_t)r.small.slices * s * s * 4));
         r.small.sum = reinterpret_cast<float *>(take(n * s * s * 4));
         r.small.q = reinterpret_cast<float *>(take(n * s * s * 4));
@@ -515,11 +515,11 @@ Room room_of(const OrthMatrix &m, Way way, int count, int sm_count, void *scratc
 }
 
 // Scratch of matrices whatever the steps are
-size_t room_for(const OrthMatrix &m, int out_type, int count, int sm_count) {
-    return std::max(room_of(m, way_of(m, out_type, true), count, sm_count, nullptr).bytes, room_of(m, way_of(m, out_type, false), count, sm_count, nullptr).bytes);
+size_t room_for(const OrthMatrix &m, int out_type, int count) {
+    return std::max(room_of(m, way_of(m, out_type, true), count, nullptr).bytes, room_of(m, way_of(m, out_type, false), count, nullptr).bytes);
 }
 
-Plan plan_of(const OrthCall &c, int sm_count) {
+Plan plan_of(const OrthCall &c) {
     Plan p;
     for (int i = 0; i < c.n; ++i)
         if (c.m[i].rows && c.m[i].cols) p.order.push_back(i);
@@ -527,7 +527,7 @@ Plan plan_of(const OrthCall &c, int sm_count) {
     std::stable_sort(p.order.begin(), p.order.end(), [&](int i, int j) { return key(i) < key(j); });
     for (int i = 0; i < (int)p.order.size();) {
         const OrthMatrix &m = c.m[p.order[i]];
-        const uint64_t one = room_for(m, c.out_type, 1, sm_count);
+        const uint64_t one = room_for(m, c.out_type, 1);
         const int most = (int)std::min<uint64_t>(kOrthMost, std::max<uint64_t>(1, kOrthRoom / one));
         int n = 1;
         while (n < most && i + n < (int)p.order.size() && key(p.order[i + n]) == key(p.order[i])) ++n;
@@ -548,18 +548,18 @@ bool symmetric_out(SymmetricOut *m, unsigned short *high, unsigned short *low, u
 }
 
 // The norms of a group's matrices, as parts of their sums of squares
-cudaError_t norms_of(const OrthMatrix *const *m, int count, OrthIn *in, double *sums, unsigned *parts, int sm_count, cudaStream_t stream) {
+cudaError_t norms_of(const OrthMatrix *const *m, int count, OrthIn *in, double *sums, unsigned *parts, cudaStream_t stream) {
     *in = {};
     in->rows = (unsigned)m[0]->rows;
     in->cols = (unsigned)m[0]->cols;
     in->type = m[0]->type;
-    const uint64_t size = (uint64_t)op_bytes(in->type), share = (uint64_t)std::max(1, sm_count * 4 / count);         // CTAs of a matrix that run at a time
+    const uint64_t size = (uint64_t)op_bytes(in->type);
     for (int i = 0; i < count; ++i) {
         in->at[i] = m[i]->in;
         in->ld[i] = m[i]->ld_in;
         in->whole[i] = (reinterpret_cast<uintptr_t>(in->at[i]) | (in->rows > 1 ? in->ld[i] * size : 0)) % 16 == 0;
     }
-    *parts = (unsigned)std::min<uint64_t>(std::min<uint64_t>(kNormParts, share), (m[0]->rows * m[0]->cols + kNormChunk - 1) / kNormChunk);
+    *parts = (unsigned)std::min<uint64_t>(kNormParts, (m[0]->rows * m[0]->cols + kNormChunk - 1) / kNormChunk);      // (by the matrix alone: its sum is the same whatever goes with it)
     const dim3 grid(*parts, (unsigned)count);
     return in->type == kF32    ? launch_chained(orth_norm_kernel<kF32>, grid, kNormThreads, 0, stream, *in, sums)
            : in->type == kBf16 ? launch_chained(orth_norm_kernel<kBf16>, grid, kNormThreads, 0, stream, *in, sums)
@@ -599,12 +599,12 @@ bool small_steps(const OrthCall &c, const std::vector<StepScale> &scales, OrthSm
     return true;
 }
 
-cudaError_t run_small(const OrthCall &c, const OrthSmallSteps &steps, const OrthMatrix *const *m, int count, void *scratch, unsigned *status, int sm_count, cudaStream_t stream) {
+cudaError_t run_small(const OrthCall &c, const OrthSmallSteps &steps, const OrthMatrix *const *m, int count, void *scratch, unsigned *status, cudaStream_t stream) {
     const uint64_t rows = m[0]->rows, cols = m[0]->cols;
-    const Room r = room_of(*m[0], kSmall, count, sm_count, scratch);
+    const Room r = room_of(*m[0], kSmall, count, scratch);
     OrthIn in;
     unsigned parts;
-    const cudaError_t err = norms_of(m, count, &in, r.parts, &parts, sm_count, stream);
+    const cudaError_t err = norms_of(m, count, &in, r.parts, &parts, stream);
     if (err != cudaSuccess) return err;
     OrthSmall g = {};
     for (int i = 0; i < count; ++i) {
@@ -625,7 +625,7 @@ template <bool SPLIT>
 cudaError_t run_group(const OrthCall &c, const std::vector<StepScale> &scales, const OrthMatrix *const *m, int count, void *scratch, unsigned *status, int sm_count, cudaStream_t stream) {
     const uint64_t rows = m[0]->rows, cols = m[0]->cols, s = std::min(rows, cols);
     const bool tall = rows > cols;
-    const Room r = room_of(*m[0], SPLIT ? kSplit : kHigh, count, sm_count, scratch);
+    const Room r = room_of(*m[0], SPLIT ? kSplit : kHigh, count, scratch);
     OrthIn in;
     OrthOut out = {};
     for (int i = 0; i < count; ++i) {
@@ -633,7 +633,7 @@ cudaError_t run_group(const OrthCall &c, const std::vector<StepScale> &scales, c
         out.ld[i] = m[i]->ld_out;
     }
     unsigned parts;
-    cudaError_t err = norms_of(m, count, &in, r.parts, &parts, sm_count, stream);
+    cudaError_t err = norms_of(m, count, &in, r.parts, &parts, stream);
     if (err != cudaSuccess) return err;
     const unsigned blocks = (unsigned)std::min<uint64_t>((uint64_t)std::max(1, sm_count * 4 / count), (rows * r.ld_x / 8 + kNormThreads * 2 - 1) / (kNormThreads * 2));
     const OrthX x0 = {r.high[0], r.low[0], (unsigned)r.ld_x, r.apart_x, r.factor};
@@ -716,12 +716,12 @@ cudaError_t run_group(const OrthCall &c, const std::vector<StepScale> &scales, c
 
 }  // namespace
 
-size_t orth_scratch_bytes(const OrthCall &c, int sm_count) {
+size_t orth_scratch_bytes(const OrthCall &c) {
     size_t most = 0;
-    const Plan p = plan_of(c, sm_count);
+    const Plan p = plan_of(c);
     for (const Group &g : p.groups) {
         const OrthMatrix &m = c.m[p.order[(size_t)g.begin]];
-        most = std::max(most, room_for(m, c.out_type, g.count, sm_count));
+        most = std::max(most, room_for(m, c.out_type, g.count));
     }
     return most;
 }
@@ -731,12 +731,12 @@ cudaError_t orthogonalize(const OrthCall &c, void *scratch, unsigned *status, in
     if (!scales_of(c.coefficients, c.steps, &scales)) return cudaErrorInvalidValue;
     OrthSmallSteps steps;
     const bool tame = small_steps(c, scales, &steps);
-    const Plan p = plan_of(c, sm_count);
+    const Plan p = plan_of(c);
     for (const Group &g : p.groups) {
         const OrthMatrix *m[kOrthMost];
         for (int i = 0; i < g.count; ++i) m[i] = &c.m[p.order[(size_t)(g.begin + i)]];
         const Way way = way_of(*m[0], c.out_type, tame);
-        const cudaError_t err = way == kSmall   ? run_small(c, steps, m, g.count, scratch, status, sm_count, stream)
+        const cudaError_t err = way == kSmall   ? run_small(c, steps, m, g.count, scratch, status, stream)
                                 : way == kSplit ? run_group<true>(c, scales, m, g.count, scratch, status, sm_count, stream)
                                                 : run_group<false>(c, scales, m, g.count, scratch, status, sm_count, stream);
         if (err != cudaSuccess) return err;

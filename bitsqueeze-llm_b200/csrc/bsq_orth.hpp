@@ -25,7 +25,7 @@ struct OrthCall {
     float scale;
 };
 
-size_t orth_scratch_bytes(const OrthCall &c, int sm_count);
+size_t orth_scratch_bytes(const OrthCall &c);
 // cudaErrorInvalidValue where the steps do not keep singular values that start within 0 and 1 below 1000: nothing is launched then
 cudaError_t orthogonalize(const OrthCall &c, void *scratch, unsigned *status, int sm_count, cudaStream_t stream);
 

@@ -29,11 +29,12 @@ template <int TYPE, bool TALL> __device__ __forceinline__ float element(const Or
     const unsigned w = TYPE == kF32 ? static_cast<const unsigned *>(g.in[z])[at] : (unsigned)static_cast<const unsigned short *>(g.in[z])[at];
     return word_elem<TYPE>(w, 0);
 }
-// The sum of squares of a matrix
+// The sum of squares of a matrix, by each warp for itself
 __device__ __forceinline__ double squares_of(const OrthSmall &g, int z) {
     double s = 0.0;
 #pragma unroll 4
-    for (int i = 0; i < g.part_count; ++i) s += g.parts[(size_t)z * (size_t)g.part_count + (size_t)i];
+    for (int i = (int)threadIdx.x & 31; i < g.part_count; i += 32) s += g.parts[(size_t)z * (size_t)g.part_count + (size_t)i];
+    for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(kFullMask, s, d);
     return s;
 }
 // 2^e that brings the norm, the square root of `squares`, below 2^15, in two factors; e
@@ -110,10 +111,10 @@ __global__ void __launch_bounds__(kThreads) small_sum_kernel(const float *sums, 
     const int i = (int)blockIdx.x * kThreads + (int)threadIdx.x;
     if (i >= elements) return;
     const float *p = sums + (size_t)blockIdx.y * (size_t)slices * (size_t)elements + (size_t)i;
-    float v = 0.0f;
+    double v = 0.0;
 #pragma unroll 8
-    for (int k = 0; k < slices; ++k) v += p[(size_t)k * (size_t)elements];
-    to[(size_t)blockIdx.y * (size_t)elements + (size_t)i] = v;
+    for (int k = 0; k < slices; ++k) v += (double)p[(size_t)k * (size_t)elements];
+    to[(size_t)blockIdx.y * (size_t)elements + (size_t)i] = (float)v;
 }
 
 // A matrix of 128 x 128 as an operand: high and low parts, each two blocks of 64 columns with rows of 128 bytes (128-byte swizzle)
@@ -465,10 +466,11 @@ cudaError_t run_type(const OrthSmall &g, bool tall, const OrthSmallSteps &t, int
 
 }  // namespace
 
-// Slices of the long side: as many as fill the device twice, of 64 at least
-int orth_small_slices(uint64_t l, int count, int sm_count, int *per) {
-    const int most = std::max(1, 2 * sm_count / count), want = (int)std::min<uint64_t>((uint64_t)most, (l + 63) / 64);
-    *per = (int)(((l + (uint64_t)want - 1) / (uint64_t)want + kSliceK - 1) / kSliceK * kSliceK);
+// Slices of the long side, which are chains of FP32 sums: of 96 to 256, by the length alone.  (As few as fill the device, they were longer the more matrices went together, and a matrix's result
+// was another one: 16384 in a chain left rank one 1.4e-1 off among 64.)
+int orth_small_slices(uint64_t l, int *per) {
+    const uint64_t want = std::min<uint64_t>(kOrthMaxDim / 256, (l + 95) / 96);
+    *per = (int)(((l + want - 1) / want + kSliceK - 1) / kSliceK * kSliceK);
     return (int)((l + (uint64_t)*per - 1) / (uint64_t)*per);
 }
 

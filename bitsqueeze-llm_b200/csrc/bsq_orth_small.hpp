@@ -39,7 +39,7 @@ struct OrthSmallRoom {
     float *sums, *sum, *q;                                       // count x slices x s x s, count x s x s each
 };
 
-int orth_small_slices(uint64_t l, int count, int sm_count, int *per);
+int orth_small_slices(uint64_t l, int *per);
 cudaError_t orth_small(const OrthSmall &g, bool tall, int type, const OrthSmallSteps &t, int count, const OrthSmallRoom &r, unsigned *status, cudaStream_t stream);
 
 }  // namespace bsq
