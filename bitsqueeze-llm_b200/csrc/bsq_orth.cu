@@ -491,7 +491,8 @@ Room room_of(const OrthMatrix &m, Way way, int count, void *scratch) {
         r.small.slices = orth_small_slices(std::max(m.rows, m.cols), &r.small.per);
         r.small.sums = reinterpret_cast<float *>(take(n * (uint64_t)r.small.slices * s * s * 4));
         r.small.sum = reinterpret_cast<float *>(take(n * s * s * 4));
-        r.small.q = reinterpret_cast<float *>(take(n * s * s * 4));
+        r.small.r = reinterpret_cast<float *>(take(n * s * s * 4));
+        r.small.identity = reinterpret_cast<float *>(take(n * 4));
         return r;
     }
     const bool split = way == kSplit;
@@ -566,36 +567,43 @@ cudaError_t norms_of(const OrthMatrix *const *m, int count, OrthIn *in, double *
                                : launch_chained(orth_norm_kernel<kF16>, grid, kNormThreads, 0, stream, *in, sums);
 }
 
-// A step's operands and what they are held times, from bounds of A, M = a I + P and the Q that has come together; false where Q may grow beyond 1024: rounding grows with its square, and
-// where X has nothing Q still grows (five steps of the usual coefficients: 485)
+// A step's operands and what they are held times, from bounds of A, N, M = a I + N and the Q = q I + R that has come together; false where Q may grow beyond 1024: rounding grows with its
+// square, and where X has nothing Q still grows (five steps of the usual coefficients: 485)
 bool small_steps(const OrthCall &c, const std::vector<StepScale> &scales, OrthSmallSteps *out) {
     out->steps = c.steps;
-    double q = 1.0;
-    int of_q = 0;                                                // Q is held times 2^of_q
+    double most = 1.0, q = 1.0;                                  // of Q
+    int of_r = 0;                                                // R is held times 2^of_r
     for (int i = 0; i < c.steps; ++i) {
         const double a = c.coefficients[3 * i], b = c.coefficients[3 * i + 1], k = c.coefficients[3 * i + 2], top = scales[(size_t)i].most;
-        double m = 0.0;
+        const bool last = i + 1 == c.steps;
+        double m = 0.0, n = 0.0;
         for (int j = 0; j <= kPoints; ++j) {
-            const double l = top * top * j / kPoints;
-            m = std::max(m, std::fabs(a + b * l + k * l * l));
+            const double l = top * top * j / kPoints, y = b * l + k * l * l;
+            m = std::max(m, std::fabs(a + y));
+            n = std::max(n, std::fabs(y));
         }
-        const int at = below_2_15(top * top), am = below_2_15(m), t = below_2_15(m * top * top);
-        const int next_a = i + 1 < c.steps ? below_2_15(scales[(size_t)i + 1].most * scales[(size_t)i + 1].most) : 0;
-        q *= m;
-        if (!(q <= 1024.0)) return false;
-        const int next_q = below_2_15(q);
+        const int at = below_2_15(top * top), an = below_2_15(n), t = below_2_15(m * top * top);
+        const int next_a = last ? 0 : below_2_15(scales[(size_t)i + 1].most * scales[(size_t)i + 1].most);
+        most *= m;
+        if (!(most <= 1024.0)) return false;
+        const int next_r = last ? 0 : below_2_15(most + std::fabs(q * a));
+        const float scale = last ? c.scale : 1.0f;
         OrthSmallStep &s = out->step[i];
         s.a = at;
-        s.square = std::ldexp((float)k, am - 2 * at);
-        s.linear = std::ldexp((float)b, am - at);
-        s.constant = std::ldexp((float)a, am);
-        s.first_q = std::ldexp(1.0f, next_q - am);
-        s.of_q = std::ldexp(1.0f, next_q - am - of_q);
-        s.of_t = std::ldexp(1.0f, t - am - at);
-        s.of_a = std::ldexp(1.0f, next_a - am - t);
-        s.out = std::ldexp(c.scale, -am - of_q);
-        of_q = next_q;
+        s.square = std::ldexp((float)k, an - 2 * at);
+        s.linear = std::ldexp((float)b, an - at);
+        s.first_r = std::ldexp(scale, next_r - an);
+        s.r_product = std::ldexp(scale, next_r - an - of_r);
+        s.r_self = std::ldexp(scale * (float)a, next_r - of_r);
+        s.r_n = std::ldexp(scale * (float)q, next_r - an);
+        s.t_product = std::ldexp(1.0f, t - an - at);
+        s.t_self = std::ldexp((float)a, t - at);
+        s.a_product = std::ldexp(1.0f, next_a - an - t);
+        s.a_self = std::ldexp((float)a, next_a - t);
+        of_r = next_r;
+        q *= a;
     }
+    out->identity = (float)(c.scale * q);
     return true;
 }
 

@@ -2,12 +2,13 @@
 //
 // All the steps are one polynomial in A_0 = X_0 X_0^T:  X_n = Q X_0 with Q_(k+1) = M_k Q_k, A_(k+1) = M_k A_k M_k, M_k = a I + b A_k + c A_k^2.  So the long side is walked
 // twice, for A_0 and for Q X_0, and what lies between is products of matrices of 128 x 128 at most, which one CTA does for each matrix without leaving its SM.  (Step by step, with X in memory,
-// 24 matrices of 64 x 1024 took 230 us; this way all five take 66.)
+// 24 matrices of 64 x 1024 took 230 us; this way all five take 70.)
 //
-// Rounding grows with what it meets: an error of A_0 by (a^2)^(n - 1), 2 10^4 for five steps.  FP32 sums for A_0 and products of split operands (22 bits) leave 1e-4 to 2e-4 in the result
-// (singular values over a range of 1000; noise alone 1e-6), a tenth of its rounding to BF16.
-// Of rank one there is nothing beside the one direction but A_0's roundings: Gaussian factors 2.4e-3 to 3.1e-3 with the rounding to BF16 (1.7e-3), whole numbers from 1 to 8, whose few products
-// are all rounded alike, up to 9e-3 (128 x 65536); with rank 8 or noise 1.7e-3 again.  FP32 and FP16 results, and long sides, are bsq_orth.cu's.
+// Rounding grows with what it meets: an error of A_0 by (a^2)^(n - 1), 2 10^4 for five steps, and where X has one direction Q has 485 for all others and 0.7 there.  So A_0's sums are FP32 in chains of
+// at most 256, products are of split operands (22 bits), and the identity's shares stay out of them: M = a I + N, Q = q I + R,  R <- N R + a R + q N,  T = N A + a A,  A <- N T + a T.  (In the products
+// a and q are terms of 3.4 and 485 beside others of 1 / s, which the tensor core aligns with them and cuts off: rank one was 2.4e-3 to 3.1e-3 off and up to 2.1e-2 where elements take few values, all
+// rounded alike.)  Results are within 4e-4 of those of 64 bits but for their rounding to BF16, 1.7e-3 (where elements take few values one that lies next to the middle of two BF16 numbers may go the
+// other way: up to 3.1e-3 in all).  FP32 and FP16 results, and long sides, are bsq_orth.cu's.
 //
 // Launches: norm (bsq_orth.cu), A_0 in slices of the long side on the FP32 pipes, their sum where there are many, the steps on the tensor core, Q X_0 on the FP32 pipes.
 #include "bsq_gemm16.cuh"
@@ -156,29 +157,34 @@ __device__ __forceinline__ void core_get(const unsigned char *m, int row, int co
         }
     }
 }
-// The product of two symmetric matrices, both parts of each: three walks along K.  One thread.
+// ... as the second operand: row k of it is k of the product, columns are contiguous: groups of 64 columns kPart / 2 apart (leading byte offset), of 8 rows 1024 bytes apart
+__device__ __forceinline__ uint64_t core_desc_mn(unsigned addr) {
+    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(kPart / 2 >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// The product a b of two matrices, both parts of each: three walks along K.  The sum comes in two accumulators, the second one 128 columns behind: half of the additions of its size, and with them what
+// they cut off.  (The operands are symmetric but for their rounding, and b could be read turned; then what is not symmetric in A grows by a^2 each step and shows at once in the last one: rank one of
+// the values 3, 5 and 7, 128 x 1024, 1.1e-2 off.)  One thread.
 __device__ __forceinline__ void core_product(unsigned acc, unsigned a, unsigned b, int s) {
-    const unsigned n = (unsigned)(s + 15) / 16;
-    const unsigned idesc = (1u << 4) | (n * 16 >> 3 << 17) | (128u >> 4 << 24);           // FP16 x FP16, FP32 sums, N >> 3, M >> 4
-    bool more = false;
-    for (int w = 0; w < 3; ++w)
+    const unsigned n = (unsigned)(s + 15) / 16, half = n / 2;         // (both accumulators are written whatever n is)
+    const unsigned idesc = (1u << 4) | (1u << 16) | (n * 16 >> 3 << 17) | (128u >> 4 << 24);          // FP16 x FP16, FP32 sums, b contiguous along N, N >> 3, M >> 4
+    for (unsigned w = 0; w < 3; ++w)
         for (unsigned k = 0; k < n; ++k) {
-            const unsigned at = (k >> 2) * (kPart / 2) + (k & 3u) * 32u;
             // (the small products first)
-            mma_f16(acc, smem_desc_sw128(a + (w == 0 ? kPart : 0u) + at), smem_desc_sw128(b + (w == 1 ? kPart : 0u) + at), idesc, more);
-            more = true;
+            const unsigned at = a + (w == 0 ? kPart : 0u) + (k >> 2) * (kPart / 2) + (k & 3u) * 32u, bt = b + (w == 1 ? kPart : 0u) + k * 2048u;
+            const bool second = w == 2 && k >= half;
+            mma_f16(acc + (second ? 128u : 0u), smem_desc_sw128(at), core_desc_mn(bt), idesc, second ? k > half : w + k > 0);
         }
 }
 
-// The steps of matrix blockIdx.x: from A_0 (the sum of `slices`) to Q, times what X_0 is G times and the result's factor.  16 warps: a thread has a row of each result and 16 * NH
+// The steps of matrix blockIdx.x: from A_0 (the sum of `slices`) to R and q, times what X_0 is G times and the result's factor.  16 warps: a thread has a row of each result and 16 * NH
 // columns, the four warps that may read its lanes of tensor memory the others.
 template <int NH>
 __global__ void __launch_bounds__(kStepThreads, 1) small_steps_kernel(const __grid_constant__ OrthSmall g, const __grid_constant__ OrthSmallSteps t, const float *sums, int slices,
-                                                                      float *q_out, unsigned tries, unsigned *status) {
+                                                                      float *r_out, float *identity, unsigned tries, unsigned *status) {
     chain_begin();
     extern __shared__ unsigned char smem_dyn[];
-    unsigned char *ma = smem_dyn + ((1024u - (smem_u32(smem_dyn) & 1023u)) & 1023u), *mm = ma + kMatrix, *mq = mm + kMatrix;
-    CoreBars &bars = *reinterpret_cast<CoreBars *>(mq + kMatrix);
+    unsigned char *ma = smem_dyn + ((1024u - (smem_u32(smem_dyn) & 1023u)) & 1023u), *mn = ma + kMatrix, *mr = mn + kMatrix;
+    CoreBars &bars = *reinterpret_cast<CoreBars *>(mr + kMatrix);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, z = blockIdx.x, s = g.s;
     const int row = (warp & 3) * 32 + lane, col = (warp >> 2) * 16 * NH;
     const bool mine = (warp & 3) * 32 < s && col < s;            // (whole warps)
@@ -236,9 +242,21 @@ __global__ void __launch_bounds__(kStepThreads, 1) small_steps_kernel(const __gr
     const auto take = [&](unsigned from, float by) {
 #pragma unroll
         for (int h = 0; h < NH; ++h) {
+            float second[16];
             read16f(acc + from + 16u * (unsigned)h, v[h], true);
+            read16f(acc + from + 128u + 16u * (unsigned)h, second, true);
 #pragma unroll
-            for (int j = 0; j < 16; ++j) v[h][j] = row < s && col + 16 * h + j < s ? v[h][j] * by : 0.0f;
+            for (int j = 0; j < 16; ++j) v[h][j] = row < s && col + 16 * h + j < s ? (v[h][j] + second[j]) * by : 0.0f;
+        }
+    };
+    // ... and an operand times `by`
+    const auto add = [&](const unsigned char *m, float by) {
+#pragma unroll
+        for (int h = 0; h < NH; ++h) {
+            float a[16];
+            core_get(m, row, col + 16 * h, a);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[h][j] = fmaf(by, a[j], v[h][j]);
         }
     };
     const auto put = [&](unsigned char *m) {
@@ -247,19 +265,20 @@ __global__ void __launch_bounds__(kStepThreads, 1) small_steps_kernel(const __gr
     };
     const auto give = [&](float by) {
         const bool all = __syncthreads_and(ok) != 0;             // (a wait that ran out anywhere: NaN everywhere)
+        if (tid == 0) identity[z] = t.identity * factor;
         if (!mine || row >= s) return;
 #pragma unroll
         for (int h = 0; h < NH; ++h)
 #pragma unroll
             for (int j = 0; j < 16; ++j)
-                if (col + 16 * h + j < s) q_out[(size_t)z * (size_t)(s * s) + (size_t)((col + 16 * h + j) * s + row)] = all ? v[h][j] * by : __uint_as_float(0x7fffffffu);
+                if (col + 16 * h + j < s) r_out[(size_t)z * (size_t)(s * s) + (size_t)((col + 16 * h + j) * s + row)] = all ? v[h][j] * by : __uint_as_float(0x7fffffffu);
     };
 
     if (mine) put(ma);
     for (int k = 0; k < t.steps; ++k) {
         const OrthSmallStep &p = t.step[k];
         const bool last = k + 1 == t.steps;
-        // M = a I + b A + c A^2
+        // N = b A + c A^2
         meet();
         if (warp == 0 && elect_one()) {
             core_product(tmem, smem_u32(ma), smem_u32(ma), s);
@@ -269,62 +288,57 @@ __global__ void __launch_bounds__(kStepThreads, 1) small_steps_kernel(const __gr
         wait();
         if (mine) {
             take(0u, p.square);
-#pragma unroll
-            for (int h = 0; h < NH; ++h) {
-                float a[16];
-                core_get(ma, row, col + 16 * h, a);
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    v[h][j] = fmaf(p.linear, a[j], v[h][j]);
-                    if (col + 16 * h + j == row && row < s) v[h][j] += p.constant;
-                }
-            }
+            add(ma, p.linear);
         }
         if (k == 0 && last) {
-            give(p.out * factor);
+            give(p.first_r * factor);
             break;
         }
         if (mine) {
-            put(mm);
+            put(mn);
             if (k == 0) {
 #pragma unroll
                 for (int h = 0; h < NH; ++h)
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) v[h][j] *= p.first_q;
-                put(mq);
+                    for (int j = 0; j < 16; ++j) v[h][j] *= p.first_r;
+                put(mr);
             }
         }
-        // M Q, M A
+        // R <- N R + a R + q N, T = N A + a A
         meet();
         if (warp == 0 && elect_one()) {
-            if (k > 0) core_product(tmem + 128u, smem_u32(mm), smem_u32(mq), s);
-            if (!last) core_product(tmem + 256u, smem_u32(mm), smem_u32(ma), s);
+            if (k > 0) core_product(tmem, smem_u32(mn), smem_u32(mr), s);
+            if (!last) core_product(tmem + 256u, smem_u32(mn), smem_u32(ma), s);
             tc_commit(&bars.done);
         }
         __syncwarp();
         wait();
         if (mine && k > 0) {
-            take(128u, last ? p.out * factor : p.of_q);
-            if (!last) put(mq);
+            take(0u, p.r_product);
+            add(mr, p.r_self);
+            add(mn, p.r_n);
+            if (!last) put(mr);
         }
         if (last) {
-            give(1.0f);
+            give(factor);
             break;
         }
         if (mine) {
-            take(256u, p.of_t);
+            take(256u, p.t_product);
+            add(ma, p.t_self);
             put(ma);
         }
-        // M (M A)
+        // A <- N T + a T
         meet();
         if (warp == 0 && elect_one()) {
-            core_product(tmem, smem_u32(mm), smem_u32(ma), s);
+            core_product(tmem, smem_u32(mn), smem_u32(ma), s);
             tc_commit(&bars.done);
         }
         __syncwarp();
         wait();
         if (mine) {
-            take(0u, p.of_a);
+            take(0u, p.a_product);
+            add(ma, p.a_self);
             put(ma);
         }
     }
@@ -338,14 +352,14 @@ __global__ void __launch_bounds__(kStepThreads, 1) small_steps_kernel(const __gr
     }
 }
 
-// 64 of the long side of matrix blockIdx.y: out = Q G (or G Q)
-template <int TYPE, bool TALL, int S> __global__ void __launch_bounds__(kThreads) small_apply_kernel(const __grid_constant__ OrthSmall g, const float *q) {
+// 64 of the long side of matrix blockIdx.y: out = R G + q G (or G R + q G)
+template <int TYPE, bool TALL, int S> __global__ void __launch_bounds__(kThreads) small_apply_kernel(const __grid_constant__ OrthSmall g, const float *r_in, const float *identity) {
     chain_begin();
     constexpr int R = S / 16, W = R % 4 ? 2 : 4;
     extern __shared__ float smem_apply[];
-    float *mq = smem_apply, *tile = smem_apply + S * (S + 4);    // Q [k][i], G [k][64 of the long side]
+    float *mr = smem_apply, *tile = smem_apply + S * (S + 4);    // R [k][i], G [k][64 of the long side]
     const int z = blockIdx.y, tid = threadIdx.x, ty = tid / 16, tx = tid % 16, first = (int)blockIdx.x * 64;
-    // (all of G and the first 16 of Q are asked for before anything is waited for)
+    // (all of G and the first 16 of R are asked for before anything is waited for)
     constexpr int kLoads = S * 64 / kThreads;
     float v[kLoads];
 #pragma unroll
@@ -360,12 +374,13 @@ template <int TYPE, bool TALL, int S> __global__ void __launch_bounds__(kThreads
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
             const int n = from + j * kThreads, k = n / S, i = n % S;
-            w[j] = k < g.s && i < g.s ? q[(size_t)z * (size_t)(g.s * g.s) + (size_t)(k * g.s + i)] : 0.0f;
+            w[j] = k < g.s && i < g.s ? r_in[(size_t)z * (size_t)(g.s * g.s) + (size_t)(k * g.s + i)] : 0.0f;
         }
 #pragma unroll
         for (int j = 0; j < kBatch; ++j)
-            if (from + j * kThreads < S * S) mq[(from + j * kThreads) / S * (S + 4) + (from + j * kThreads) % S] = w[j];
+            if (from + j * kThreads < S * S) mr[(from + j * kThreads) / S * (S + 4) + (from + j * kThreads) % S] = w[j];
     }
+    const float q = identity[z];
     float s0, s1;
     norm_scale(squares_of(g, z), &s0, &s1);
 #pragma unroll
@@ -380,12 +395,12 @@ template <int TYPE, bool TALL, int S> __global__ void __launch_bounds__(kThreads
     for (int i = 0; i < R; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
-    const int qi = TALL ? tx : ty, gj = TALL ? ty : tx;
+    const int ri = TALL ? tx : ty, gj = TALL ? ty : tx;
 #pragma unroll 4
     for (int k = 0; k < g.s; ++k) {
         alignas(16) float a[R];
 #pragma unroll
-        for (int i = 0; i < R; i += W) load_some<W>(mq + k * (S + 4) + i * 16 + qi * W, a + i);
+        for (int i = 0; i < R; i += W) load_some<W>(mr + k * (S + 4) + i * 16 + ri * W, a + i);
         const float4 b = *reinterpret_cast<const float4 *>(tile + k * 68 + gj * 4);
 #pragma unroll
         for (int i = 0; i < R; ++i) {
@@ -395,13 +410,21 @@ template <int TYPE, bool TALL, int S> __global__ void __launch_bounds__(kThreads
             acc[i][3] = fmaf(a[i], b.w, acc[i][3]);
         }
     }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const float4 b = *reinterpret_cast<const float4 *>(tile + (i / W * 16 * W + ri * W + i % W) * 68 + gj * 4);
+        acc[i][0] = fmaf(q, b.x, acc[i][0]);
+        acc[i][1] = fmaf(q, b.y, acc[i][1]);
+        acc[i][2] = fmaf(q, b.z, acc[i][2]);
+        acc[i][3] = fmaf(q, b.w, acc[i][3]);
+    }
     // through shared memory, so that neighbouring threads write neighbouring elements whatever the rows' alignment: [S][64], or [64][S] where tall
     __syncthreads();
     unsigned short *box = reinterpret_cast<unsigned short *>(tile);
     const auto bits = [](float x) { return __bfloat16_as_ushort(__float2bfloat16_rn(x)); };
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-        const int r = i / W * 16 * W + qi * W + i % W;
+        const int r = i / W * 16 * W + ri * W + i % W;
         if (TALL) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) box[(gj * 4 + j) * S + r] = bits(acc[i][j]);
@@ -449,9 +472,9 @@ cudaError_t run(const OrthSmall &g, const OrthSmallSteps &t, int count, const Or
         sums = r.sum;
         slices = 1;
     }
-    err = launch_chained(small_steps_kernel<(S + 63) / 64>, (unsigned)count, kStepThreads, kStepsSmem, stream, g, t, sums, slices, r.q, epilogue_tries(kWaitTries), status);
+    err = launch_chained(small_steps_kernel<(S + 63) / 64>, (unsigned)count, kStepThreads, kStepsSmem, stream, g, t, sums, slices, r.r, r.identity, epilogue_tries(kWaitTries), status);
     if (err != cudaSuccess) return err;
-    return launch_chained(small_apply_kernel<TYPE, TALL, S>, dim3((unsigned)((g.l + 63) / 64), (unsigned)count), kThreads, apply_smem(S), stream, g, (const float *)r.q);
+    return launch_chained(small_apply_kernel<TYPE, TALL, S>, dim3((unsigned)((g.l + 63) / 64), (unsigned)count), kThreads, apply_smem(S), stream, g, (const float *)r.r, (const float *)r.identity);
 }
 template <int TYPE, bool TALL>
 cudaError_t run_side(const OrthSmall &g, const OrthSmallSteps &t, int count, const OrthSmallRoom &r, unsigned *status, cudaStream_t stream) {

@@ -25,18 +25,20 @@ struct OrthSmall {
 // A step as products of operands that are held times powers of two: factors of the accumulators and operands
 struct OrthSmallStep {
     int a;                                                       // A is held times 2^a
-    float square, linear, constant;                              // of A A, A and I in M
-    float first_q;                                               // Q = M of the first step
-    float of_q, of_t, of_a;                                      // M Q, M A, M (M A)
-    float out;                                                   // Q of the last step
+    float square, linear;                                        // of A A and A in N
+    float first_r;                                               // R = N of the first step
+    float r_product, r_self, r_n;                                // of N R, R and N in the next R, or in the result's
+    float t_product, t_self;                                     // of N A and A in T
+    float a_product, a_self;                                     // of N T and T in the next A
 };
 struct OrthSmallSteps {
     OrthSmallStep step[kOrthMaxSteps];
+    float identity;                                              // q of the result
     int steps;
 };
 struct OrthSmallRoom {
     int slices, per;                                             // of the long side, and how long each is
-    float *sums, *sum, *q;                                       // count x slices x s x s, count x s x s each
+    float *sums, *sum, *r, *identity;                            // count x slices x s x s, count x s x s each, count
 };
 
 int orth_small_slices(uint64_t l, int *per);

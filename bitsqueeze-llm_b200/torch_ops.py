@@ -474,9 +474,9 @@ def orthogonalize(updates, steps=5, coefficients=_QUINTIC, eps=1e-7, scale=1.0, 
     for all steps, or one triple for each; they must keep singular values from 0 to 1 below 1000.  `out`: tensors to write, apart from each other and from the updates (without it,
     results of one shape that follow one another in a list share an allocation).
 
-    bfloat16 results are off by at most about half their own rounding beside it: X is held in 2 x 16 bits, products read 16 and sum in FP32 (a side of up to 128: products of 22 bits; of exactly
-    rank one these are up to 3e-3 off in all, 9e-3 where the elements take few values: `dtype=torch.float32` keeps 1e-4).
-    float32 and float16 results come from products of 2 x 16 bits of every operand, three times the work (1e-6 to 1e-4 off, more the further singular values lie apart; 4e-4 for rank one of elements of one sign).  An Inf or NaN makes its whole matrix NaN; zeros stay zeros, and where |G| is far below eps the result may be 0.
+    bfloat16 results are off by at most about half their own rounding beside it: X is held in 2 x 16 bits, products read 16 and sum in FP32 (a side of up to 128: products of 22 bits); of exactly
+    rank one up to 3.5e-3 in all, 5e-3 where the elements take few values, whose roundings do not average out.
+    float32 and float16 results come from products of 2 x 16 bits of every operand, three times the work (1e-6 to 2e-4 off, more the further singular values lie apart; up to 6e-4 for rank one of few values).  An Inf or NaN makes its whole matrix NaN; zeros stay zeros, and where |G| is far below eps the result may be 0.
     Matrices whose rows are not contiguous are copied first.  The result needs no gradient and gives none to the updates.  Sides of at most 65536, 1 to 64 steps."""
     single = isinstance(updates, torch.Tensor)
     updates = [updates] if single else list(updates)

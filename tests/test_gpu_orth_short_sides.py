@@ -83,3 +83,28 @@ def test_slices_of_one_length(ops):
         g = make(kind, s, l, False)
         alone, among = ops.orthogonalize(g), ops.orthogonalize([g] * count)[count // 2]
         assert torch.equal(alone, among)
+
+
+@pytest.mark.parametrize("tall", [False, True])
+@pytest.mark.parametrize("s,l", SIDES + [(40, 300), (64, 200), (128, 200), (128, 1024)])
+def test_rank_one(ops, s, l, tall):
+    """The gradient of one token.  A rounding to BF16 is 2^-8 of an element at most.  Beside it: the result is R u v^T + q u v^T, -484 and 485 of u v^T for 0.7.  Each of the four products that make R adds
+    up to h = s / 32 times in either accumulator what is of its size, and each time cuts 16 terms off at 2^-25 of the sum so far, by half a step on average: (h + 1) / 2 * 16 * 2^-26 * 484 / 0.7
+    where all elements lose alike, 1.7e-4 up to 32 and 4.1e-4 at 128; what is lost stays in proportion, so four times that.  The FP32 additions of R's rounding and R G, (s + 1) / 2 * 2^-24 * 484 / 0.7:
+    6.8e-4 and 2.7e-3.  1.4e-3 and 4.3e-3 in all.  Elements of many values do not lose alike: 1.3e-3 whatever the side."""
+    for kind in ("gaussian", "1 to 8", "3, 5, 7", "11, 13"):
+        g = make(kind, s, l, tall)
+        beside = 1.3e-3 if kind == "gaussian" else 1.4e-3 if s <= 32 else 4.3e-3
+        assert off(ops.orthogonalize(g), exact(g)) <= 2.0 ** -8 + beside, kind
+
+
+@pytest.mark.parametrize("m,n", [(8, 300), (300, 8), (16, 65536), (5, 7), (32, 32), (32, 100), (31, 5000), (33, 40), (128, 200)])
+def test_few_rows_of_far_singular_values(ops, m, n):
+    """Noise beside a mean thirty times as large, singular values from 1 to 1 / 1000, one far above the others.  A_0 in 22 bits is 2^-23 off; a direction of singular value x then |Q'(x^2)| x 2^-23, at
+    most 3.6e4 * 2^-23 = 4.3e-3 (at x = 0.004), of some 0.7 to 1.1, if all of it fell into that direction; it is spread over as many as there are rows.  A rounding to BF16 is 2^-8 / sqrt(3) of the norm."""
+    gen = torch.Generator(device="cuda").manual_seed(m + n)
+    noise = torch.randn(m, n, generator=gen, device="cuda")
+    u, v = (torch.linalg.qr(torch.randn(k, min(m, n), generator=gen, device="cuda"))[0] for k in (m, n))
+    one = torch.randn(m, 1, generator=gen, device="cuda") * torch.randn(1, n, generator=gen, device="cuda")
+    for g in (noise + 30, noise + 300, u * torch.logspace(0, -3, min(m, n), device="cuda") @ v.t(), one + 1e-2 * noise, one + 1e-3 * noise):
+        assert off(ops.orthogonalize(g), exact(g)) <= 2.0 ** -8 / math.sqrt(3) + 4.3e-3 / 0.69 / math.sqrt(min(m, n))
