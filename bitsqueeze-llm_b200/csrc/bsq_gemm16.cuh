@@ -8,7 +8,8 @@
 // and wrote two FP16 matrices, more than the 17 us of its 4096 of K.)
 //
 // The tensor core cuts additions off instead of rounding them: epilogues that want FP32's digits (kChained) get the sums every 1024 of K or so and add them up rounded, in registers.
-// Others (kTotals, chains of Gemm16::chain) have them added up, rounded, in the other half of tensor memory, from which the tile is then taken: 128 sums beside what those epilogues hold spill.
+// Others have no room for 128 sums beside what they hold (up to 4 KB a thread spill).  kBack: a function of its own adds them up and writes them back to where the last chain lies; the tile is taken from
+// there while the next one's first chain is summed.  kTotals (chains of Gemm16::chain): they are added up, rounded, in the other half of tensor memory, where the tile is then taken from.
 //
 // An operand may come in two parts, high + low (splits): the product is then high x high + high x low + low x high, three walks along K into the same sums.
 //
@@ -23,7 +24,10 @@ namespace {
 constexpr int kG16MaxStages = 7, kG16K = 64;                     // stages in flight at most, of K each
 constexpr unsigned kG16Half = 128 * kG16K * 2, kG16Stage = 2 * kG16Half;
 constexpr int kG16Warps = 8, kG16First = 2, kG16Threads = 32 * (kG16First + kG16Warps);       // epilogue warps, the last eight (ten in all: 200 registers a thread)
-constexpr int kG16Chain = 1024 / kG16K;                          // stages of a chain of sums, about
+constexpr int kG16Chain = 1024 / kG16K;                          // stages of a chain of sums, about (kChained)
+// ... (kBack).  A tile that is taken out holds the half that the next tile's second chain wants: loss and gradients of 4096 x 4096 x 32000 took 3270 us with one chain, 3310 this way, 3610 with chains of
+// 2048, 4500 with 1024.  What is lost of sums of one sign, 2e-5 of them in FP16, is a tenth of a rounding to it.
+constexpr int kG16BackChain = 4096 / kG16K;
 constexpr unsigned kG16Box = 32 * 128;                           // 32 rows x 128 bytes on their way in or out: two for each epilogue warp, or none (EPI::kBoxes)
 constexpr int kG16Band = 16;                                     // rows of tiles that are walked together, column after column
 
@@ -210,8 +214,48 @@ __device__ __forceinline__ void read16f(unsigned taddr, float (&v)[16], bool ok)
 #pragma unroll
     for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
 }
+// What a warp of the epilogue does before it takes a tile of several chains (kBack): all but the last one are added up in registers and given back, the last one's place gets the total.
+// The ring is at the tile's first chain; the last one is still to be given back.  False: a wait has run out.
+template <int COLS, int CTAS>
+__device__ __noinline__ bool sum_chains(Gemm16Bars *bars, Ring rs, int chains, unsigned taddr, unsigned lead, bool mine, unsigned *status, unsigned tries, bool ok) {
+    float sums[COLS];
+    for (int n = 0;; ++n, rs.next()) {
+        if (ok) ok = __all_sync(kFullMask, mbar_wait_asleep(&bars->acc_full[rs.pos], rs.par, status, tries)) != 0;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (!ok || n + 1 == chains) break;
+        if (mine) {
+#pragma unroll
+            for (int c = 0; c < COLS; c += 16) {
+                float v[16];
+                read16f(taddr + (unsigned)rs.pos * 256u + (unsigned)c, v, true);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) sums[c + j] = n ? sums[c + j] + v[j] : v[j];
+            }
+        }
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) {
+            if (CTAS == 2) mbar_arrive_pair(smem_u32(&bars->acc_empty[rs.pos]) + lead);
+            else mbar_arrive(&bars->acc_empty[rs.pos]);
+        }
+    }
+    if (mine && ok) {
+#pragma unroll
+        for (int c = 0; c < COLS; c += 16) {
+            const unsigned at = taddr + (unsigned)rs.pos * 256u + (unsigned)c;
+            unsigned w[16];
+            read16(at, w, true);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(sums[c + j] + __uint_as_float(w[j]));
+            tmem_st16(at, w);
+        }
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+    }
+    return ok;
+}
 template <class EPI> __host__ __device__ constexpr int g16_stages() { return EPI::kBoxes ? 5 : kG16MaxStages; }
 // EPI: a functor, called by whole warps:
+//   kChained, kBack, kTotals                                          how chains of sums come together (one of them, or none: one chain)
 //   template <int COLS> void tile(const TileOut &, Ahead &) const     takes COLS columns out; kChained: tile(const TileOut &, float (&sums)[COLS])
 //   template <int COLS> void ahead(const TileOut &, Ahead &) const    what can be asked for while the tile is still being summed (not kChained)
 //   void begin() const                                                by one thread of the launch (kChained)
@@ -228,7 +272,7 @@ __global__ void __launch_bounds__(kG16Threads, 1) gemm16_kernel(const __grid_con
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int half = CTAS == 2 ? (int)(blockIdx.x & 1) : 0, first = (int)(blockIdx.x / CTAS), step = (int)(gridDim.x / CTAS);
     const int tiles = g.batch * g.splits * (g.lower ? g.m_tiles * (g.m_tiles + 1) / 2 : g.m_tiles * g.n_tiles);
-    const int stages = g.k_stages * g.parts, chain = EPI::kChained ? kG16Chain : EPI::kTotals ? g.chain : 0, chains = chains_of(stages, chain);
+    const int stages = g.k_stages * g.parts, chain = EPI::kChained ? kG16Chain : EPI::kBack ? kG16BackChain : EPI::kTotals ? g.chain : 0, chains = chains_of(stages, chain);
     const bool totals = EPI::kTotals && chains > 1;              // the MMAs write one half of tensor memory, the other one has the tile's total; else they write both by turns
     const bool leader = half == 0;
 
@@ -367,8 +411,14 @@ __global__ void __launch_bounds__(kG16Threads, 1) gemm16_kernel(const __grid_con
                     else mbar_arrive(&bars.acc_empty[rs.pos]);
                 }
             };
+            if constexpr (EPI::kBack) {
+                if (chains > 1) {
+                    ok = sum_chains<kCols, CTAS>(&bars, rs, chains, tmem + (unsigned)(part * kCols) + ((unsigned)(quarter * 32) << 16), lead, mine, status, g.tries, ok);
+                    for (int n = 1; n < chains; ++n) rs.next();
+                }
+            }
             for (int n = 0; n < chains; ++n, rs.next()) {
-                if (ok) ok = __all_sync(kFullMask, mbar_wait_asleep(&bars.acc_full[rs.pos], rs.par, status, g.tries)) != 0;
+                if (ok && !(EPI::kBack && chains > 1)) ok = __all_sync(kFullMask, mbar_wait_asleep(&bars.acc_full[rs.pos], rs.par, status, g.tries)) != 0;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 out.taddr = tmem + (unsigned)rs.pos * 256u + (unsigned)(part * kCols) + ((unsigned)(quarter * 32) << 16);
                 out.ok = ok;

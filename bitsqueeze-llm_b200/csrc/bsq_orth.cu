@@ -219,7 +219,7 @@ template <bool SPLIT> struct GramOut {
     float scale;                     // 2^e
     float *rest;                     // what rounding to FP16 takes from the diagonal
 
-    static constexpr bool kChained = false, kTotals = true, kBoxes = true;
+    static constexpr bool kChained = false, kBack = false, kTotals = true, kBoxes = true;
     using Ahead = NoAhead;
     template <int COLS> __device__ void ahead(const TileOut &, Ahead &) const {}
     template <int COLS> __device__ void tile(const TileOut &o, Ahead &) const {
@@ -255,7 +255,7 @@ template <bool SPLIT> struct PolyOut {
     float a, back;                   // 2^-e
     float *of_high, *of_low;         // what the parts of X are multiplied by beside the product: a + what rounding takes from the diagonal of P, a + the diagonal
 
-    static constexpr bool kChained = false, kTotals = true, kBoxes = true;
+    static constexpr bool kChained = false, kBack = false, kTotals = true, kBoxes = true;
     struct Ahead {
         float mine;                  // of A's diagonal: the row's, the columns'
         Shared64 theirs;
@@ -329,7 +329,7 @@ template <bool SPLIT> struct StepOut {
     uint64_t ld_p;                   // of P: distance of the matrices' diagonals
     OrthOut out;                     // (last)
 
-    static constexpr bool kChained = false, kTotals = true, kBoxes = true;
+    static constexpr bool kChained = false, kBack = false, kTotals = true, kBoxes = true;
     struct Ahead {
         float of_sum, of_p, of_q;
         Shared64 e, d;               // (tall: the columns')

@@ -39,7 +39,7 @@ struct XentStats {
     float *at_target;                // M
     unsigned *joined;                // of XentJoin
 
-    static constexpr bool kChained = true, kTotals = false, kBoxes = false;
+    static constexpr bool kChained = true, kBack = false, kTotals = false, kBoxes = false;
     using Ahead = NoAhead;
     __device__ __forceinline__ void begin() const { *joined = 0u; }
     template <int COLS> __device__ __forceinline__ void tile(const TileOut &o, float (&v)[COLS]) const {
@@ -367,7 +367,7 @@ template <int TYPE> struct XentGrad {
     XentScale scale;
     float low, rest;                 // e / vocab, e - e / vocab
 
-    static constexpr bool kChained = false, kTotals = false, kBoxes = true;
+    static constexpr bool kChained = false, kBack = true, kTotals = false, kBoxes = true;          // (p is exp of these logits less the loss's lse: with 65536 columns in one chain 1.7e-2 too small)
     using Ahead = NoAhead;
     template <int COLS> __device__ void ahead(const TileOut &, Ahead &) const {}
     template <int COLS> __device__ void tile(const TileOut &o, Ahead &) const {
@@ -419,7 +419,7 @@ template <int TYPE> struct ProductOut {
     long ld_sum;
     XentScale scale;
 
-    static constexpr bool kChained = false, kTotals = false, kBoxes = true;
+    static constexpr bool kChained = false, kBack = true, kTotals = false, kBoxes = true;          // (524288 tokens of one sign in one chain: 3.2e-3 too small)
     using Ahead = NoAhead;
     template <int COLS> __device__ void ahead(const TileOut &, Ahead &) const {}
     template <int COLS> __device__ void tile(const TileOut &o, Ahead &) const {

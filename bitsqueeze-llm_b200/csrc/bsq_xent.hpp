@@ -9,8 +9,8 @@ namespace bsq {
 
 enum XentReduction : int { kXentNone = 0, kXentSum = 1, kXentMean = 2 };
 
-constexpr uint64_t kXentMaxCols = 65536;                         // a logit is one chain of sums in tensor memory
-// ... and an element of dW one over the tokens: FP16 and BF16 (see the chains of the other gradient products)
+// Sums in tensor memory are in chains of 1024 of K or so (logits of the loss) or 4096 (logits of the gradient, dx and dW).  At most so many columns, and tokens in FP16 and BF16
+constexpr uint64_t kXentMaxCols = 65536;
 inline uint64_t xent_max_tokens(int type) { return type == 1 ? 65536 : 524288; }
 
 struct XentCall {

@@ -304,7 +304,8 @@ int bsq_grad_norm_clip(const void *const *d_grads, const uint64_t *counts, const
  * 2 the sum over the number of tokens that are not ignored (none: NaN).  d_stats: 2 * tokens + 1 floats that the gradient wants.  Sums are FP32 (of one token) and FP64 (of many).
  * Gradient: with d_grad the gradient of d_loss (one float, or one for each token), d_dx (tokens x cols) and d_dw (vocab x cols), either nullable, in the type of x:
  *   dx = dl W,  dW = dl^T x,  dl_tv = g_t (exp(l_tv - lse_t) - (1 - smoothing) [v = target] - smoothing / vocab)
- * dl is rounded to the operands' type, sums are FP32, results rounded once.  Ignored tokens have a dx of 0; their x is multiplied by 0 for dW and has to be finite.
+ * dl is rounded to the operands' type (times a power that the largest g sets), sums are FP32 in chains of some 4096 that are added up rounded (up to 2e-5 of a sum of one sign is lost), results
+ * rounded once.  Ignored tokens have a dx of 0; their x is multiplied by 0 for dW and has to be finite.
  * At most 65536 columns, and 65536 (FP16) or 524288 (BF16) tokens.  Calls enqueue on `stream` and return; they allocate nothing, keep nothing and may be captured.  d_scratch: as many bytes as the
  * function beside it says for the same arguments (pointers and strides included), on a 128-byte boundary.  d_status as for bsq_fp4_matmul. */
 size_t bsq_linear_xent_scratch_bytes(int type, const void *d_x, uint64_t tokens, uint64_t cols, uint64_t ld_x, const void *d_w, uint64_t vocab, uint64_t ld_w, double smoothing);
