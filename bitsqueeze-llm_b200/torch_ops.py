@@ -23,6 +23,7 @@ from array import array
 from operator import attrgetter
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from . import MXFP4, NVFP4, lib
 
@@ -366,7 +367,7 @@ def linear_cross_entropy(x, weight, target, ignore_index=-100, label_smoothing=0
     NaN).  A target outside 0 .. V - 1 gives NaN for its token.  Logits are FP32 sums; the backward pass computes them again, rounds their gradient to the type of x and returns the gradients of x and
     weight in it, rounded once.  Hidden states of ignored tokens get a gradient of 0; they are multiplied by 0 on the way to the weight's and have to be finite.
     At most 65536 columns and 65536 (float16) or 524288 (bfloat16) tokens.  Tensors that do not lie as the rows of one matrix are copied first.  Autocast does not change what is
-    asked of x: pass it and the weight in 16 bits."""
+    asked of x: pass it and the weight in 16 bits.  Forward-mode derivatives are refused (NotImplementedError)."""
     if x.dtype not in _XENT_TOKENS or not x.is_cuda or x.dim() == 0 or x.size(-1) == 0:
         raise ValueError("x must be a float16 or bfloat16 CUDA tensor with at least one column")
     if weight.dim() != 2 or weight.dtype != x.dtype or weight.device != x.device or weight.size(1) != x.size(-1) or not weight.size(0):
@@ -381,7 +382,8 @@ def linear_cross_entropy(x, weight, target, ignore_index=-100, label_smoothing=0
     if x.size(-1) > _XENT_COLS or target.numel() > _XENT_TOKENS[x.dtype]:
         raise ValueError("at most %d columns and %d tokens: split the batch" % (_XENT_COLS, _XENT_TOKENS[x.dtype]))
     call = _laid_out(x) if x.numel() else x, _laid_out(weight), target.contiguous(), ignore_index, label_smoothing, _REDUCTIONS[reduction]
-    if (x.requires_grad or weight.requires_grad) and torch.is_grad_enabled():
+    # (a tensor with a forward-mode tangent need not require a gradient: the function refuses it)
+    if (x.requires_grad or weight.requires_grad) and torch.is_grad_enabled() or unpack_dual(x).tangent is not None or unpack_dual(weight).tangent is not None:
         return _LinearCrossEntropy.apply(*call)
     return _xent_loss(*call)[0]
 
@@ -477,7 +479,7 @@ def orthogonalize(updates, steps=5, coefficients=_QUINTIC, eps=1e-7, scale=1.0, 
     bfloat16 results are off by at most about half their own rounding beside it: X is held in 2 x 16 bits, products read 16 and sum in FP32 (a side of up to 128: products of 22 bits); of exactly
     rank one up to 3.5e-3 in all, 5e-3 where the elements take few values, whose roundings do not average out.
     float32 and float16 results come from products of 2 x 16 bits of every operand, three times the work (1e-6 to 2e-4 off, more the further singular values lie apart; up to 6e-4 for rank one of few values).  An Inf or NaN makes its whole matrix NaN; zeros stay zeros, and where |G| is far below eps the result may be 0.
-    Matrices whose rows are not contiguous are copied first.  The result needs no gradient and gives none to the updates.  Sides of at most 65536, 1 to 64 steps."""
+    Matrices whose rows are not contiguous are copied first.  The result needs no gradient and gives none to the updates, backwards or forwards.  Sides of at most 65536, 1 to 64 steps."""
     single = isinstance(updates, torch.Tensor)
     updates = [updates] if single else list(updates)
     if not 1 <= steps <= _ORTH_STEPS or int(steps) != steps:
