@@ -474,7 +474,7 @@ def orthogonalize(updates, steps=5, coefficients=_QUINTIC, eps=1e-7, scale=1.0, 
     right with X^T X where G has more rows than columns), times `scale`.  `updates`: a tensor of at least two dimensions (the leading ones are a stack of matrices) or a list of them
     (float32, float16 or bfloat16 CUDA tensors of one device, of any shapes); the result is of the same form, in `dtype`.  Matrices of one shape and type go through together.  coefficients: (a, b, c)
     for all steps, or one triple for each; they must keep singular values from 0 to 1 below 1000.  `out`: tensors to write, apart from each other and from the updates (without it,
-    results of one shape that follow one another in a list share an allocation).
+    results of one shape that follow one another in a list lie in one allocation, which is freed with the last of them).
 
     bfloat16 results are off by at most about half their own rounding beside it: X is held in 2 x 16 bits, products read 16 and sum in FP32 (a side of up to 128: products of 22 bits); of exactly
     rank one up to 3.5e-3 in all, 5e-3 where the elements take few values, whose roundings do not average out.
@@ -503,10 +503,11 @@ def orthogonalize(updates, steps=5, coefficients=_QUINTIC, eps=1e-7, scale=1.0, 
     if out is None:
         outs, at = [], 0
         while at < n:                                            # (neighbours of one shape from one allocation: a call of the allocator costs more than a matrix's other arguments)
-            end = at + 1
-            while end < n and shapes[end] == shapes[at]:
+            shape, end = shapes[at], at + 1
+            while end < n and shapes[end] == shape and shape[0]:
                 end += 1
-            outs += [torch.empty(shapes[at], dtype=dtype, device=device)] if end == at + 1 else torch.empty((end - at,) + shapes[at], dtype=dtype, device=device).unbind(0)
+            some = torch.empty((shape[0] * (end - at),) + shape[1:], dtype=dtype, device=device)
+            outs += [some] if end == at + 1 else some.unsafe_split(shape[0])                      # (tensors of their own, not views of one that count their changes together)
             at = end
     else:
         outs = [out] if isinstance(out, torch.Tensor) else list(out)

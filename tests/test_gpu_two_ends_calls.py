@@ -33,3 +33,19 @@ def test_forward_mode_is_refused(ops, which, grad):
         with pytest.raises(NotImplementedError):
             ops.linear_cross_entropy(x, w, t)
         assert torch.isfinite(ops.linear_cross_entropy(*operands()))            # nothing carries a tangent
+
+
+def test_results_of_a_list_are_tensors_of_their_own(ops):
+    """Changing one in place is no change of another, and is allowed with a tensor that requires a gradient."""
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    updates = [torch.randn(*s, generator=gen, device="cuda") for s in ((64, 80), (64, 80), (64, 80), (2, 200, 150), (2, 200, 150), (64, 80), (0, 5), (0, 5), (3, 0), (3, 0))]
+    out = ops.orthogonalize(updates)
+    assert [o.shape for o in out] == [u.shape for u in updates] and all(o.is_contiguous() and not o._is_view() for o in out)
+    assert all(torch.equal(a, ops.orthogonalize(b)) for a, b in zip(out, updates) if b.numel())
+    p, kept = torch.ones(64, 80, dtype=torch.bfloat16, device="cuda", requires_grad=True), out[0].clone()
+    y = (p * out[0]).sum()                                         # saves out[0]
+    out[1].mul_(2), out[3].zero_()
+    y.backward()
+    assert torch.equal(p.grad, kept) and [o._version for o in out[:5]] == [0, 1, 0, 1, 0]
+    out[2].mul_(p)
+    assert out[2].requires_grad
