@@ -130,6 +130,7 @@ SIGNATURES = {
     "bsq_linear_xent_grad_scratch_bytes": (_sz, [_i, _vp, _u64, _u64, _u64, _vp, _u64, _u64, _i]),
     "bsq_linear_xent_grad": (_i, [_i, _vp, _u64, _u64, _u64, _vp, _u64, _u64, _vp, C.c_int64, C.c_double, _i, _vp, _vp, _vp, _u64, _vp, _u64, _vp, _vp, _vp]),
     "bsq_orthogonalize_scratch_bytes": (_sz, [_vp, _vp, _vp, _i, _i]),
+    "bsq_orthogonalize_check": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _vp, C.c_double, _f]),
     "bsq_orthogonalize": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _vp, C.c_double, _f, _vp, _vp, _vp]),
     "bsq_test_inject_status": (None, [_i, _u32]),
     "bsq_test_inject_lane_status": (None, [_vp, _i, _u32]),

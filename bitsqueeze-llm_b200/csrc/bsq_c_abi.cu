@@ -289,36 +289,81 @@ size_t bsq_orthogonalize_scratch_bytes(const uint64_t *rows, const uint64_t *col
         return 0;
     }
 }
+namespace {
+// Where a matrix lies, in bytes: `rows` rows of `width`, `pitch` apart
+struct Lies {
+    uintptr_t begin, end;
+    uint64_t pitch, width, rows;
+    bool out;
+};
+// Whether two matrices share a byte.  Where one begins before the other ends they do not if their rows are equally far apart and their columns lie beside one another (or one is a single row that lies
+// beside the other's columns); rows at other distances that pass one another count as sharing.
+bool share(const Lies &a, const Lies &b) {
+    if (a.end <= b.begin || b.end <= a.begin) return false;
+    if (a.rows > 1 && b.rows > 1 && a.pitch != b.pitch) return true;
+    const uint64_t pitch = a.rows > 1 ? a.pitch : b.pitch;
+    if (a.rows == 1 && b.rows == 1) return true;
+    const uint64_t at = a.begin <= b.begin ? (b.begin - a.begin) % pitch : (pitch - (a.begin - b.begin) % pitch) % pitch;          // b's columns, from a's first
+    return at < a.width || at + b.width > pitch;
+}
+// Whether a matrix that is written shares a byte with another one
+bool written_shared(std::vector<Lies> &all) {
+    std::sort(all.begin(), all.end(), [](const Lies &a, const Lies &b) { return a.begin < b.begin; });
+    std::vector<const Lies *> open[2];                            // of what came before: what has not ended yet, inputs and outputs
+    for (const Lies &m : all) {
+        for (int out = 0; out < 2; ++out) {
+            std::vector<const Lies *> &o = open[out];
+            if (!m.out && !out) continue;
+            o.erase(std::remove_if(o.begin(), o.end(), [&](const Lies *p) { return p->end <= m.begin; }), o.end());
+            for (const Lies *p : o)
+                if (share(*p, m)) return true;
+        }
+        open[m.out].push_back(&m);
+    }
+    return false;
+}
+enum { kFine = 0, kRefused = 1, kSteps = 2, kShared = 3 };
+int orth_call(const void *const *d_in, const uint64_t *rows, const uint64_t *cols, const uint64_t *lds, const int *types, int n, void *const *d_out, const uint64_t *ld_outs, int out_type, int steps,
+              const float *coefficients, double eps, float scale, std::vector<OrthMatrix> *m) {
+    if (n < 0 || (n && (!d_in || !rows || !cols || !lds || !types || !d_out || !ld_outs)) || !op_bytes(out_type)) return kRefused;
+    if (steps < 1 || steps > kOrthMaxSteps || !coefficients || !(eps >= 0.0) || std::isinf(eps) || !std::isfinite(scale)) return kRefused;
+    m->resize((size_t)n);
+    std::vector<Lies> all;
+    for (int i = 0; i < n; ++i) {
+        const uint64_t r = rows[i], c = cols[i], in = r > 1 ? lds[i] : c, out = r > 1 ? ld_outs[i] : c;
+        if (!op_bytes(types[i]) || r > kOrthMaxDim || c > kOrthMaxDim) return kRefused;
+        if (r && c && (!op_rows_ok(d_in[i], types[i], r, c, in) || !op_rows_ok(d_out[i], out_type, r, c, out))) return kRefused;
+        (*m)[(size_t)i] = {d_in[i], d_out[i], r, c, in, out, types[i]};
+        if (!r || !c) continue;
+        const auto lies = [&](const void *p, uint64_t ld, int type, bool written) {
+            const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+            const uint64_t size = (uint64_t)op_bytes(type);
+            all.push_back({at, at + ((r - 1) * ld + c) * size, ld * size, c * size, r, written});
+        };
+        lies(d_in[i], in, types[i], false);
+        lies(d_out[i], out, out_type, true);
+    }
+    return written_shared(all) ? kShared : kFine;
+}
+}  // namespace
+
+int bsq_orthogonalize_check(const void *const *d_in, const uint64_t *rows, const uint64_t *cols, const uint64_t *lds, const int *types, int n, void *const *d_out, const uint64_t *ld_outs,
+                            int out_type, int steps, const float *coefficients, double eps, float scale) {
+    try {
+        std::vector<OrthMatrix> m;
+        const int why = orth_call(d_in, rows, cols, lds, types, n, d_out, ld_outs, out_type, steps, coefficients, eps, scale, &m);
+        return why != kRefused && !orth_steps_ok(coefficients, steps) ? kSteps : why;
+    } catch (...) {
+        return kRefused;
+    }
+}
 int bsq_orthogonalize(const void *const *d_in, const uint64_t *rows, const uint64_t *cols, const uint64_t *lds, const int *types, int n, void *const *d_out, const uint64_t *ld_outs,
                       int out_type, int steps, const float *coefficients, double eps, float scale, void *d_scratch, uint32_t *d_status, void *stream) {
-    if (n < 0 || (n && (!d_in || !rows || !cols || !lds || !types || !d_out || !ld_outs)) || !op_bytes(out_type)) return 1;
-    if (steps < 1 || steps > kOrthMaxSteps || !coefficients || !(eps >= 0.0) || std::isinf(eps) || !std::isfinite(scale)) return 1;
     try {
-        struct Span {
-            uintptr_t begin, end;
-            bool out;
-        };
-        std::vector<OrthMatrix> m((size_t)n);
-        std::vector<Span> spans;
-        for (int i = 0; i < n; ++i) {
-            const uint64_t r = rows[i], c = cols[i], in = r > 1 ? lds[i] : c, out = r > 1 ? ld_outs[i] : c;
-            if (!op_bytes(types[i]) || r > kOrthMaxDim || c > kOrthMaxDim) return 1;
-            if (r && c && (!op_rows_ok(d_in[i], types[i], r, c, in) || !op_rows_ok(d_out[i], out_type, r, c, out))) return 1;
-            m[(size_t)i] = {d_in[i], d_out[i], r, c, in, out, types[i]};
-            if (!r || !c) continue;
-            const uintptr_t a = reinterpret_cast<uintptr_t>(d_in[i]), b = reinterpret_cast<uintptr_t>(d_out[i]);
-            spans.push_back({a, a + ((r - 1) * in + c) * (uint64_t)op_bytes(types[i]), false});
-            spans.push_back({b, b + ((r - 1) * out + c) * (uint64_t)op_bytes(out_type), true});
-        }
-        if (spans.empty()) return 0;
+        std::vector<OrthMatrix> m;
+        if (orth_call(d_in, rows, cols, lds, types, n, d_out, ld_outs, out_type, steps, coefficients, eps, scale, &m) != kFine) return 1;
+        if (std::none_of(m.begin(), m.end(), [](const OrthMatrix &a) { return a.rows && a.cols; })) return 0;
         if (!on_bytes(d_scratch, 128)) return 1;
-        std::sort(spans.begin(), spans.end(), [](const Span &a, const Span &b) { return a.begin < b.begin; });
-        uintptr_t any = 0, written = 0;                          // where what came before ends
-        for (const Span &s : spans) {
-            if (s.begin < (s.out ? any : written)) return 1;
-            any = std::max(any, s.end);
-            if (s.out) written = std::max(written, s.end);
-        }
         return rc(orthogonalize({m.data(), n, out_type, steps, coefficients, eps, scale}, d_scratch, d_status, device_sm_count(), as_stream(stream)));
     } catch (...) {
         return 1;

@@ -724,6 +724,11 @@ cudaError_t run_group(const OrthCall &c, const std::vector<StepScale> &scales, c
 
 }  // namespace
 
+bool orth_steps_ok(const float *coefficients, int steps) {
+    std::vector<StepScale> scales;
+    return scales_of(coefficients, steps, &scales);
+}
+
 size_t orth_scratch_bytes(const OrthCall &c) {
     size_t most = 0;
     const Plan p = plan_of(c);

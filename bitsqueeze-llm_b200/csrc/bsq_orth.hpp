@@ -26,7 +26,9 @@ struct OrthCall {
 };
 
 size_t orth_scratch_bytes(const OrthCall &c);
-// cudaErrorInvalidValue where the steps do not keep singular values that start within 0 and 1 below 1000: nothing is launched then
+// Whether the steps keep singular values that start within 0 and 1 below 1000
+bool orth_steps_ok(const float *coefficients, int steps);
+// ... else cudaErrorInvalidValue: nothing is launched then
 cudaError_t orthogonalize(const OrthCall &c, void *scratch, unsigned *status, int sm_count, cudaStream_t stream);
 
 }  // namespace bsq

@@ -473,7 +473,7 @@ def orthogonalize(updates, steps=5, coefficients=_QUINTIC, eps=1e-7, scale=1.0, 
     """Updates with their singular values brought near 1 by Newton-Schulz steps: X = G / (|G| + eps), then `steps` times X <- a X + (b A + c A^2) X with A = X X^T (from the
     right with X^T X where G has more rows than columns), times `scale`.  `updates`: a tensor of at least two dimensions (the leading ones are a stack of matrices) or a list of them
     (float32, float16 or bfloat16 CUDA tensors of one device, of any shapes); the result is of the same form, in `dtype`.  Matrices of one shape and type go through together.  coefficients: (a, b, c)
-    for all steps, or one triple for each; they must keep singular values from 0 to 1 below 1000.  `out`: tensors to write, apart from each other and from the updates (without it,
+    for all steps, or one triple for each; they must keep singular values from 0 to 1 below 1000.  `out`: tensors to write, apart from each other and from the updates (side by side in the rows of one tensor they may lie; without it,
     results of one shape that follow one another in a list lie in one allocation, which is freed with the last of them).
 
     bfloat16 results are off by at most about half their own rounding beside it: X is held in 2 x 16 bits, products read 16 and sum in FP32 (a side of up to 128: products of 22 bits); of exactly
@@ -541,12 +541,14 @@ def orthogonalize(updates, steps=5, coefficients=_QUINTIC, eps=1e-7, scale=1.0, 
         flat = array("f", [v for t in table for v in t])
         arrays = [a.buffer_info()[0] for a in (ins, rows, cols, lds, types, tos, ld_outs, flat)]
         scratch = _scratch("bsq_orthogonalize_scratch_bytes", device, arrays[1], arrays[2], arrays[4], len(ins), _TYPES[dtype])
+        call = (*arrays[:5], len(ins), *arrays[5:7], _TYPES[dtype], int(steps), arrays[7], eps, scale)
         try:
-            _call("bsq_orthogonalize", index, *arrays[:5], len(ins), *arrays[5:7], _TYPES[dtype], int(steps), arrays[7], eps, scale, scratch.data_ptr(), None)
+            _call("bsq_orthogonalize", index, *call, scratch.data_ptr(), None)
         except RuntimeError:
-            if not _steps_ok(table):
+            why = lib().bsq_orthogonalize_check(*call)
+            if why == 2:
                 raise ValueError("coefficients must keep singular values from 0 to 1 below 1000") from None
-            if out is not None:
+            if why == 3:
                 raise ValueError("the matrices that are written must lie apart from one another and from the updates") from None
             raise
     if out is not None:
@@ -565,15 +567,3 @@ def _matrices(t):
     for n, s in zip(t.shape[:-2], t.stride()[:-2]):
         at = [a + i * s for a in at for i in range(n)]
     return at
-
-
-def _steps_ok(table):
-    """As the library looks at coefficients: the largest singular value that each step may meet."""
-    most = 1.0
-    for a, b, c in table:
-        s = [most * 1.02 * i / 256 for i in range(257)]
-        p = [b * v * v + c * v ** 4 for v in s]
-        most = max(abs((a + q) * v) for q, v in zip(p, s))
-        if not most < 1000.0 or any(not abs(q) < 1e6 for q in p):
-            return False
-    return True

@@ -325,9 +325,13 @@ int bsq_linear_xent_grad(int type, const void *d_x, uint64_t tokens, uint64_t co
  * to 128: the steps as one polynomial of A_0, with FP32 sums and products of 22 bits (2^-11 at most beside the rounding), where the coefficients keep that polynomial below 1024; else from both
  * halves.  Exactly rank one, in BF16: up to 3.5e-3 in all, 5e-3 where the elements take few values, whose roundings do not average out.
  * An Inf or NaN makes its whole matrix NaN; a matrix of zeros stays one; where |G| is below 2^-20 * eps the result may be 0.  Sides of at most 65536, 1 to 64 steps; matrices without
- * elements are passed over.  Results must not overlap one another or an input.  Arrays are read before the call returns.  The call enqueues on `stream`, allocates nothing on the device, keeps
+ * elements are passed over.  Results must not overlap one another or an input (matrices that
+ * lie beside one another, column by column, in rows equally far apart are fine; rows at different distances that pass one another are refused).  Arrays are read before the call returns.  The call enqueues on `stream`, allocates nothing on the device, keeps
  * nothing and may be captured.  d_scratch: bsq_orthogonalize_scratch_bytes on a 128-byte boundary (matrices of one shape go together, up to 1 GB of scratch).  d_status as for bsq_fp4_matmul. */
 size_t bsq_orthogonalize_scratch_bytes(const uint64_t *rows, const uint64_t *cols, const int *types, int n, int out_type);
+/* What bsq_orthogonalize would say to these arguments, without a launch: 0 nothing, 1 refused, 2 the coefficients do not keep singular values below 1000, 3 a matrix that is written overlaps another. */
+int bsq_orthogonalize_check(const void *const *d_in, const uint64_t *rows, const uint64_t *cols, const uint64_t *lds, const int *types, int n, void *const *d_out, const uint64_t *ld_outs,
+                            int out_type, int steps, const float *coefficients, double eps, float scale);
 int bsq_orthogonalize(const void *const *d_in, const uint64_t *rows, const uint64_t *cols, const uint64_t *lds, const int *types, int n, void *const *d_out, const uint64_t *ld_outs,
                       int out_type, int steps, const float *coefficients, double eps, float scale, void *d_scratch, uint32_t *d_status, void *stream);
 

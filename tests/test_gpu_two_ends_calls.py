@@ -49,3 +49,41 @@ def test_results_of_a_list_are_tensors_of_their_own(ops):
     assert torch.equal(p.grad, kept) and [o._version for o in out[:5]] == [0, 1, 0, 1, 0]
     out[2].mul_(p)
     assert out[2].requires_grad
+
+
+@pytest.mark.parametrize("m,k,n", [(64, 3, 80), (300, 2, 200), (150, 5, 33), (40, 70, 8)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_results_side_by_side(ops, dtype, m, k, n):
+    """Written by columns of one tensor, as a list and as a stack; input and output as halves of one."""
+    gen = torch.Generator(device="cuda").manual_seed(m)
+    updates = torch.randn(k, m, n, generator=gen, device="cuda")
+    want = ops.orthogonalize(updates, dtype=dtype)
+    big = torch.full((m, k, n), -7.0, dtype=dtype, device="cuda")
+    assert torch.equal(ops.orthogonalize(updates, dtype=dtype, out=big.transpose(0, 1)), want) and torch.equal(big.transpose(0, 1), want)
+    big = torch.full((m, k * n + 1), -7.0, dtype=dtype, device="cuda")
+    outs = [big[:, i * n: (i + 1) * n] for i in range(k)][::-1]
+    got = ops.orthogonalize(list(updates)[::-1], dtype=dtype, out=outs)
+    assert all(a is b for a, b in zip(got, outs)) and torch.equal(torch.stack(outs[::-1]), want) and (big[:, -1] == -7).all()
+    both = torch.zeros(m, 2 * n, dtype=dtype, device="cuda")
+    both[:, :n] = updates[0]
+    one = ops.orthogonalize(both[:, :n].clone(), dtype=dtype)
+    ops.orthogonalize(both[:, :n], dtype=dtype, out=both[:, n:])
+    assert torch.equal(both[:, n:], one) and torch.equal(both[:, :n], updates[0].to(dtype))
+
+
+def test_what_is_said_of_a_call_that_fails(ops, monkeypatch):
+    """An overlap where there is one; the library's own error otherwise, also with `out`."""
+    g = torch.randn(64, 64, device="cuda").bfloat16()
+    out = torch.empty(2, 64, 64, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError, match="apart"):
+        ops.orthogonalize([g, g], out=[out[0], out[0]])
+    with pytest.raises(ValueError, match="apart"):
+        ops.orthogonalize([g, g], out=[out.view(64, 128)[:, :64], out.view(64, 128)[:, 60:124]])
+    with pytest.raises(ValueError, match="coefficients"):
+        ops.orthogonalize(g, out=out[0], coefficients=(10.0, 10.0, 10.0))
+
+    def fails(*args):
+        raise RuntimeError("bsq_orthogonalize failed")
+    monkeypatch.setattr(ops, "_call", fails)
+    with pytest.raises(RuntimeError, match="failed"):
+        ops.orthogonalize(g, out=out[0])
