@@ -87,3 +87,57 @@ def test_what_is_said_of_a_call_that_fails(ops, monkeypatch):
     monkeypatch.setattr(ops, "_call", fails)
     with pytest.raises(RuntimeError, match="failed"):
         ops.orthogonalize(g, out=out[0])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("m,n", [(64, 100), (300, 513), (513, 300), (1100, 1100)])
+def test_products_of_both_halves_of_several(ops, dtype, m, n):
+    """FP32 and FP16 results of a list and of a stack: what each gives alone, and X's formula."""
+    gen = torch.Generator(device="cuda").manual_seed(m + n)
+    updates = [torch.randn(m, n, generator=gen, device="cuda") * 10.0 ** i for i in range(5)]
+    alone = [ops.orthogonalize(u, dtype=dtype) for u in updates]
+    assert all(torch.equal(a, b) for a, b in zip(ops.orthogonalize(updates, dtype=dtype), alone))
+    assert torch.equal(ops.orthogonalize(torch.stack(updates), dtype=dtype), torch.stack(alone))
+    for u, a in zip(updates, alone):
+        x = u.double() / u.double().norm()
+        for _ in range(5):
+            s = x @ x.t()
+            x = 3.4445 * x + (-4.7750 * s + 2.0315 * s @ s) @ x
+        # noise keeps its digits: sums of FP32 and operands of 22 bits, 2^-13 at most, and the result's rounding
+        assert (a.double() - x).norm() <= (2.0 ** -13 + torch.finfo(dtype).eps / 2) * x.norm()
+
+
+@pytest.mark.parametrize("m,n,dtype", [(1024, 4096, torch.bfloat16), (4096, 1024, torch.float32), (128, 65536, torch.bfloat16)])
+def test_more_than_share_the_scratch(ops, m, n, dtype):
+    """More matrices than 1 GB of scratch takes: several runs, one behind the other."""
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    two = [torch.randn(m, n, generator=gen, device="cuda").bfloat16() for _ in range(2)]
+    want = [ops.orthogonalize(u, dtype=dtype) for u in two]
+    got = ops.orthogonalize([two[i % 2] for i in range(61)], dtype=dtype)
+    assert all(torch.equal(g, want[i % 2]) for i, g in enumerate(got))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("e", [0.1, 1.0])
+@pytest.mark.parametrize("tokens,cols,vocab", [(300, 64, 70001), (2, 40, 140000), (1025, 72, 66000)])
+def test_smoothing_over_several_pieces(ops, dtype, e, tokens, cols, vocab):
+    """dl = p - e / V, less 1 - e at the target, a piece of the vocabulary at a time: against the formula in 64 bits."""
+    x, w, t = operands(tokens, cols, vocab, dtype)
+    t[0], t[-1] = vocab - 1, -100
+    live = t != -100
+    l = x.double() @ w.double().t()
+    logp = torch.log_softmax(l, 1)
+    want = torch.full_like(l, e / vocab)
+    want[live.nonzero()[:, 0], t[live]] += 1 - e
+    loss = -(want * logp).sum(1) * live
+    dl = (torch.exp(logp) - want) * live[:, None]
+    dx, dw = dl @ w.double(), dl.t() @ x.double()
+    x.requires_grad_(), w.requires_grad_()
+    got = ops.linear_cross_entropy(x, w, t, label_smoothing=e, reduction="none")
+    a, b = torch.autograd.grad(got.sum(), (x, w))
+    assert ((got - loss).abs() <= 1e-4).all()                      # (sums of 1100 products and of 140000 terms in FP32: a few 2^-23 of 12, 300 additions of 2^-24)
+    # each row or column of the gradients: dl and the result rounded once each, 2^-8 or 2^-11, and 2^-20 of what e / V takes from p before dl is rounded
+    half = torch.finfo(dtype).eps / 2
+    near = (dl.abs() @ w.double().abs(), dl.abs().t() @ x.double().abs())
+    for got, want, by in ((a, dx, near[0]), (b, dw, near[1])):
+        assert ((got.double() - want).norm(dim=1) <= 2.02 * half * by.norm(dim=1) + 2.0 ** -20 * (x.abs().max() + w.abs().max()) * by.size(1) ** 0.5).all()
