@@ -477,8 +477,8 @@ def orthogonalize(updates, steps=5, coefficients=_QUINTIC, eps=1e-7, scale=1.0, 
     results of one shape that follow one another in a list lie in one allocation, which is freed with the last of them).
 
     bfloat16 results are off by at most about half their own rounding beside it: X is held in 2 x 16 bits, products read 16 and sum in FP32 (a side of up to 128: products of 22 bits); of exactly
-    rank one up to 3.5e-3 in all, 5e-3 where the elements take few values, whose roundings do not average out.
-    float32 and float16 results come from products of 2 x 16 bits of every operand, three times the work (1e-6 to 2e-4 off, more the further singular values lie apart; up to 6e-4 for rank one of few values).  An Inf or NaN makes its whole matrix NaN; zeros stay zeros, and where |G| is far below eps the result may be 0.
+    rank one up to 3.5e-3 in all, with both sides above 128 up to 1.2e-2 where those of a row or column take few values, whose roundings do not average out.
+    float32 and float16 results come from products of 2 x 16 bits of every operand, three times the work (1e-6 to 2e-4 off, more the further singular values lie apart; up to 1.2e-3 for rank one of few values).  An Inf or NaN makes its whole matrix NaN; zeros stay zeros, and where |G| is far below eps the result may be 0.
     Matrices whose rows are not contiguous are copied first.  The result needs no gradient and gives none to the updates, backwards or forwards.  Sides of at most 65536, 1 to 64 steps."""
     single = isinstance(updates, torch.Tensor)
     updates = [updates] if single else list(updates)

@@ -321,9 +321,9 @@ int bsq_linear_xent_grad(int type, const void *d_x, uint64_t tokens, uint64_t co
  * for each step's coefficients (a, b, c; 3 * steps floats)  A = X X^T,  X <- a X + (b A + c A^2) X  (with X^T X from the right where G has more rows than columns);
  * out = scale * X in out_type.  The coefficients must keep singular values from 0 to 1 below 1000 all the way (else 1).  X is held in two times 16 bits; products read 16 bits of each operand and
  * sum in FP32: results in BF16 are off by at most about half their own rounding.  FP32 and FP16 results come from products of both halves (2^-19 where
- * singular values are alike; up to 2^-12 in the 2-norm where a few stand a hundred times above the others, 6e-4 for rank one of few values).  BF16 results of matrices with a side of up
+ * singular values are alike; up to 2^-12 in the 2-norm where a few stand a hundred times above the others, 1.2e-3 for rank one of few values).  BF16 results of matrices with a side of up
  * to 128: the steps as one polynomial of A_0, with FP32 sums and products of 22 bits (2^-11 at most beside the rounding), where the coefficients keep that polynomial below 1024; else from both
- * halves.  Exactly rank one, in BF16: up to 3.5e-3 in all, 5e-3 where the elements take few values, whose roundings do not average out.
+ * halves.  Exactly rank one, in BF16: up to 3.5e-3 in all, with both sides above 128 up to 1.2e-2 where those of a row or column take few values, whose roundings do not average out.
  * An Inf or NaN makes its whole matrix NaN; a matrix of zeros stays one; where |G| is below 2^-20 * eps the result may be 0.  Sides of at most 65536, 1 to 64 steps; matrices without
  * elements are passed over.  Results must not overlap one another or an input (matrices that
  * lie beside one another, column by column, in rows equally far apart are fine; rows at different distances that pass one another are refused).  Arrays are read before the call returns.  The call enqueues on `stream`, allocates nothing on the device, keeps

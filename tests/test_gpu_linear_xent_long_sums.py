@@ -98,3 +98,20 @@ def test_input_gradient_of_a_large_vocabulary(ops, dtype, tokens, cols, vocab):
     off = 4 * USUAL_BACK + 15 * USUAL + (vocab // 1024 + 70) * 2.0 ** -24 + 2.0 ** -20     # (logits of some 3 and the sum; lse of some 15)
     assert rel.abs().max() <= off + half * 1.2
     assert rel.mean().abs() <= off + half / 10
+
+
+@pytest.mark.parametrize("tokens,cols,vocab", [(40, 9000, 700), (300, 13000, 515), (9000, 64, 300)])
+def test_waits_that_run_out_between_chains(ops, lib, tokens, cols, vocab):
+    """Sums of several chains, given up: NaN, and the next call is as before."""
+    gen = torch.Generator(device="cuda").manual_seed(tokens)
+    x, w = torch.randn(tokens, cols, generator=gen, device="cuda").bfloat16().requires_grad_(), (torch.randn(vocab, cols, generator=gen, device="cuda") / cols ** 0.5).bfloat16().requires_grad_()
+    t = torch.randint(0, vocab, (tokens,), generator=gen, device="cuda")
+    want = torch.autograd.grad(ops.linear_cross_entropy(x, w, t), (x, w))
+    try:
+        lib.bsq_test_limit_waits(0)
+        got = torch.autograd.grad(ops.linear_cross_entropy(x, w, t), (x, w))
+        assert all(torch.isnan(g).all() for g in got)
+        torch.cuda.synchronize()
+    finally:
+        lib.bsq_test_limit_waits(1 << 16)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(ops.linear_cross_entropy(x, w, t), (x, w)), want))
