@@ -4,11 +4,11 @@
 //
 // Loss: one product whose epilogue leaves, for each token and 128 (64) columns of the vocabulary, the largest logit and the sum of exponentials against it, and the target's
 // logit; xent_join_kernel joins a token's parts (8 bytes for 128 logits are all that is written of them).
-// Gradient: the vocabulary goes by in pieces of some 128 MB of dl.  Of a piece the logits are computed again, the epilogue turns them into dl in 16 bits (the
+// Gradient: the vocabulary goes by in pieces of some 128 MB of dl (1024 columns at least).  Of a piece the logits are computed again, the epilogue turns them into dl in 16 bits (the
 // rounding that a 16-bit gradient of logits has anyway; scaled, see XentScale), then dW of the piece is complete, and dx is summed over the pieces in FP32.
 //
 // Bound by the tensor core, then by power: the loss of 8192 x 4096 x 32000 1267 us from rest (1695 TFLOP/s, 1.02 of the measured burst rate of a library product; the tensor core is busy 98 %
-// of the time), 1510 to 1530 one after the other (1410); loss and gradients of 4096 x 4096 x 32000 3.24 to 3.3 ms (8 T D V: 1300 to 1330 TFLOP/s).  Few tokens by the weight's bytes: 64 x 4096 x
+// of the time), 1510 to 1530 one after the other (1410); loss and gradients of 4096 x 4096 x 32000 3.3 to 3.35 ms (8 T D V: 1280 to 1300 TFLOP/s).  Few tokens by the weight's bytes: 64 x 4096 x
 // 131072 193 us (5.6 TB/s), one token 43 us for 262 MB (xent_few_kernel).
 //
 // Exponents are taken in base 2, and the reference of a tile is the rounded product of its largest logit and log2(e), so that the rounding cancels.

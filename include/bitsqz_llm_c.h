@@ -304,8 +304,8 @@ int bsq_grad_norm_clip(const void *const *d_grads, const uint64_t *counts, const
  * 2 the sum over the number of tokens that are not ignored (none: NaN).  d_stats: 2 * tokens + 1 floats that the gradient wants.  Sums are FP32 (of one token) and FP64 (of many).
  * Gradient: with d_grad the gradient of d_loss (one float, or one for each token), d_dx (tokens x cols) and d_dw (vocab x cols), either nullable, in the type of x:
  *   dx = dl W,  dW = dl^T x,  dl_tv = g_t (exp(l_tv - lse_t) - (1 - smoothing) [v = target] - smoothing / vocab)
- * dl is rounded to the operands' type (times a power that the largest g sets), sums are FP32 in chains of some 4096 that are added up rounded (up to 2e-5 of a sum of one sign is lost), results
- * rounded once.  Ignored tokens have a dx of 0; their x is multiplied by 0 for dW and has to be finite.
+ * dl is rounded to the operands' type (scaled by the largest g; in FP16 tokens whose g is 10^6 times smaller lose digits), sums are FP32 in chains of some 4096 that are added
+ * up rounded (up to 2e-5 of a sum of one sign is lost), results rounded once.  Ignored tokens have a dx of 0; their x is multiplied by 0 for dW and has to be finite.
  * At most 65536 columns, and 65536 (FP16) or 524288 (BF16) tokens.  Calls enqueue on `stream` and return; they allocate nothing, keep nothing and may be captured.  d_scratch: as many bytes as the
  * function beside it says for the same arguments (pointers and strides included), on a 128-byte boundary.  d_status as for bsq_fp4_matmul. */
 size_t bsq_linear_xent_scratch_bytes(int type, const void *d_x, uint64_t tokens, uint64_t cols, uint64_t ld_x, const void *d_w, uint64_t vocab, uint64_t ld_w, double smoothing);
@@ -325,9 +325,8 @@ int bsq_linear_xent_grad(int type, const void *d_x, uint64_t tokens, uint64_t co
  * to 128: the steps as one polynomial of A_0, with FP32 sums and products of 22 bits (2^-11 at most beside the rounding), where the coefficients keep that polynomial below 1024; else from both
  * halves.  Exactly rank one, in BF16: up to 3.5e-3 in all, with both sides above 128 up to 1.2e-2 where those of a row or column take few values, whose roundings do not average out.
  * An Inf or NaN makes its whole matrix NaN; a matrix of zeros stays one; where |G| is below 2^-20 * eps the result may be 0.  Sides of at most 65536, 1 to 64 steps; matrices without
- * elements are passed over.  Results must not overlap one another or an input (matrices that
- * lie beside one another, column by column, in rows equally far apart are fine; rows at different distances that pass one another are refused).  Arrays are read before the call returns.  The call enqueues on `stream`, allocates nothing on the device, keeps
- * nothing and may be captured.  d_scratch: bsq_orthogonalize_scratch_bytes on a 128-byte boundary (matrices of one shape go together, up to 1 GB of scratch).  d_status as for bsq_fp4_matmul. */
+ * elements are passed over.  Results must not overlap one another or an input (matrices that lie beside one another, column by column, in rows equally far apart are fine;
+ * rows at different distances that pass one another are refused).  Arrays are read before the call returns.  The call enqueues on `stream`, allocates nothing on the device, keeps nothing and may be captured.  d_scratch: bsq_orthogonalize_scratch_bytes on a 128-byte boundary (matrices of one shape go together, up to 1 GB of scratch).  d_status as for bsq_fp4_matmul. */
 size_t bsq_orthogonalize_scratch_bytes(const uint64_t *rows, const uint64_t *cols, const int *types, int n, int out_type);
 /* What bsq_orthogonalize would say to these arguments, without a launch: 0 nothing, 1 refused, 2 the coefficients do not keep singular values below 1000, 3 a matrix that is written overlaps another. */
 int bsq_orthogonalize_check(const void *const *d_in, const uint64_t *rows, const uint64_t *cols, const uint64_t *lds, const int *types, int n, void *const *d_out, const uint64_t *ld_outs,
