@@ -11,7 +11,7 @@
 // Others have no room for 128 sums beside what they hold (up to 4 KB a thread spill).  kBack: a function of its own adds them up and writes them back to where the last chain lies; the tile is taken from
 // there while the next one's first chain is summed.  kTotals (chains of Gemm16::chain): they are added up, rounded, in the other half of tensor memory, where the tile is then taken from.
 //
-// An operand may come in two parts, high + low (splits): the product is then high x high + high x low + low x high, three walks along K into the same sums.
+// An operand may come in two parts, high + low (splits): the product is then high x high + high x low + low x high, three walks along K into the same sums; or two, with the low part of one operand only.
 //
 // Bound by the tensor core, then by power: see the products that use it.
 #pragma once
@@ -34,7 +34,8 @@ constexpr int kG16Band = 16;                                     // rows of tile
 struct Gemm16 {
     int M, N;                        // of one matrix of the stack
     int m_tiles, n_tiles, batch;
-    int k_stages, parts;             // stages along K of a tile, walks along K (1, or 3 of split operands)
+    int k_stages, parts;             // stages along K of a tile, walks along K (1, 2 with one operand's low part, or 3 of split operands)
+    bool low_a;                      // of two walks: the low part is A's, else B's
     int chain;                       // stages of a chain of sums, about; 0: one chain (kTotals)
     int splits;                      // a matrix's tiles are this many, each with k_stages of K, one behind the other: z = matrix * splits + slice
     bool a_kmajor, b_kmajor;         // contiguous along K, or along M / N
@@ -44,7 +45,7 @@ struct Gemm16 {
 };
 
 struct Gemm16Maps {
-    CUtensorMap a[2], b[2];          // high and low parts (low: only with parts == 3)
+    CUtensorMap a[2], b[2];          // high and low parts (low: with more than one walk)
 };
 
 struct Gemm16Bars {
@@ -310,7 +311,8 @@ __global__ void __launch_bounds__(kG16Threads, 1) gemm16_kernel(const __grid_con
                 const TileAt at = tile_at(g, t);
                 const int a0 = at.i * kTile + half * 128, b0 = at.j * kTile + half * 128, z = at.z / g.splits, d0 = at.z % g.splits * g.k_stages;
                 for (int p = 0; p < g.parts && ok; ++p) {
-                    const CUtensorMap *ma = &maps.a[p == 2], *mb = &maps.b[p == 1];
+                    const bool low_a = p == 2 || (p == 1 && g.low_a);
+                    const CUtensorMap *ma = &maps.a[low_a], *mb = &maps.b[p && !low_a];
                     for (int d = 0; d < g.k_stages; ++d, ++filled, r.next()) {
                         if (r.wrapped) ok = mbar_wait_asleep(&bars.empty[r.pos], r.par ^ 1u, status);
                         if (!ok) break;

@@ -3,7 +3,7 @@
 //
 // What 16-bit operands cost, and what is done about it (the steps pull small singular values up by 3.4 each, and with them whatever rounding has left there):
 //   * FP16, not BF16: entries are bounded, a power of two brings them into its range, and it has three bits more at the same rate;
-//   * X is kept as high + low, two FP16 words of 22 bits.  Products read the high part; a X is added up from both in the epilogue.  With one word the
+//   * X is kept as high + low, two FP16 words of 22 bits.  Products read the high part (P X both, where the side is short); a X is added up from both in the epilogue.  With one word the
 //     large singular values' rounding is what the small ones start from (rank-8 gradients with noise: 4e-3 off after five steps, this way 1e-4);
 //   * the diagonals of A and of P = b A + c A^2, of size 1 where everything else is small, are kept in FP32: what rounding takes from them, and what the
 //     products leave out of the low part (P_ii X_low), goes back in the epilogues (noise: 1.9e-3 off without, 0.2e-3 to 0.7e-3 with it; a rounding to BF16 is 1.7e-3).
@@ -28,6 +28,10 @@ constexpr uint64_t kOrthRoom = 1ull << 30;                       // scratch that
 // Stages of a chain of sums (4096 of K, of split operands 1024).  What the tensor core cuts off where a sum's terms have one sign is not of X's rank, and each step pulls it up by 3.4: rank one,
 // 65536 x 33000, was 8.8e-3 off in BF16 and 3.1e-2 in FP32 with one chain for all of K, and is 2.8e-3 (its rounding to BF16 is 2e-3 of that) and 1.7e-4.  Up to 6100 of K BF16 has one chain still
 template <bool SPLIT> constexpr int kOrthChain = (SPLIT ? 1024 : 4096) / kG16K;
+// Short sides up to which P goes with X's low part too, in a second walk along K.  Behind it only P's diagonal does: of rank one that is not of X's rank, and each later step pulls it up by a.
+// With Gaussian factors it leaves 0.43 / s beside the rounding of 1.7e-3: 129 x 357 3.7e-3 in all (up to 6e-3) without the second walk, 1.7e-3 with it; 1000 x 1000 1.75e-3 without.
+// 129 x 129 112 us without, 116 with it; 300 x 2000 some 3 %, 512 x 1024 142 and 153; 1024 x 4096 would take a fifth more.
+constexpr uint64_t kOrthLowSide = 512;
 constexpr int kNormThreads = 512;
 constexpr uint64_t kNormChunk = 16384;                           // elements of a CTA of the pass that finds the norms, at least
 constexpr int kNormParts = kNormThreads;
@@ -632,7 +636,7 @@ cudaError_t run_small(const OrthCall &c, const OrthSmallSteps &steps, const Orth
 template <bool SPLIT>
 cudaError_t run_group(const OrthCall &c, const std::vector<StepScale> &scales, const OrthMatrix *const *m, int count, void *scratch, unsigned *status, int sm_count, cudaStream_t stream) {
     const uint64_t rows = m[0]->rows, cols = m[0]->cols, s = std::min(rows, cols);
-    const bool tall = rows > cols;
+    const bool tall = rows > cols, low = !SPLIT && s <= kOrthLowSide;
     const Room r = room_of(*m[0], SPLIT ? kSplit : kHigh, count, scratch);
     OrthIn in;
     OrthOut out = {};
@@ -691,8 +695,13 @@ cudaError_t run_group(const OrthCall &c, const std::vector<StepScale> &scales, c
         if ((err = launch_gemm16(ops, poly, g, s, pairs_s, status, sm_count, stream)) != cudaSuccess) return err;
         // X
         for (int i = 0; i < 2; ++i) {
-            const Stack p = {r.p[SPLIT ? i : 0], s, s, r.ld_a, (uint64_t)count, r.apart_a}, x = {i && SPLIT ? r.low[now] : r.high[now], cols, rows, r.ld_x, (uint64_t)count, r.apart_x};
+            const Stack p = {r.p[SPLIT ? i : 0], s, s, r.ld_a, (uint64_t)count, r.apart_a}, x = {i && (SPLIT || low) ? r.low[now] : r.high[now], cols, rows, r.ld_x, (uint64_t)count, r.apart_x};
             if (!map_operand(tall ? &ops.b[i] : &ops.a[i], p, false, true) || !map_operand(tall ? &ops.a[i] : &ops.b[i], x, false, tall)) return cudaErrorInvalidValue;
+        }
+        const Gemm16 one = g;
+        if (low) {
+            g.parts = 2;
+            g.low_a = tall;
         }
         g.M = (int)rows;
         g.N = (int)cols;
@@ -714,10 +723,11 @@ cudaError_t run_group(const OrthCall &c, const std::vector<StepScale> &scales, c
         e.back = std::ldexp(1.0f, -k.p);
         e.scale = last ? c.scale : std::ldexp(1.0f, scales[(size_t)step + 1].x);
         e.of_high = r.of_high;
-        e.of_low = r.of_low;
+        e.of_low = low ? r.of_high : r.of_low;
         e.ld_p = r.ld_a;
         e.out = out;
         if ((err = launch_gemm16(ops, e, g, s, pairs_x, status, sm_count, stream)) != cudaSuccess) return err;
+        g = one;
     }
     return cudaSuccess;
 }
