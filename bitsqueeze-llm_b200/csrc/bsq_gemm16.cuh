@@ -468,6 +468,17 @@ __global__ void __launch_bounds__(kG16Threads, 1) gemm16_kernel(const __grid_con
 }
 
 // ---- host ----
+inline uint64_t padded(uint64_t n, uint64_t to) { return (n + to - 1) / to * to; }
+// Scratch, handed out piece by piece on 128 bytes
+struct Scratch {
+    unsigned char *base;
+    size_t used = 0;
+    template <class T> T *take(uint64_t count) {
+        T *p = reinterpret_cast<T *>(base + used);
+        used += padded(count * sizeof(T), 128);
+        return p;
+    }
+};
 template <class EPI> constexpr size_t g16_smem() { return 1024 + g16_stages<EPI>() * kG16Stage + (EPI::kBoxes ? kG16Warps * 2 * kG16Box : 0) + sizeof(Gemm16Bars) + 64; }
 
 // A stack of matrices of 16- or 32-bit elements in memory: `rows` rows of `cols` elements, `ld` apart, matrices `apart` elements apart

@@ -428,8 +428,6 @@ template <bool SPLIT> struct StepOut {
 };
 
 // ---- host ----
-uint64_t up(uint64_t n, uint64_t to) { return (n + to - 1) / to * to; }
-
 // Powers of two that X, A and P of a step are held times: largest magnitudes below 2^15
 struct StepScale {
     int x, a, p;
@@ -483,39 +481,35 @@ struct Room {
 };
 Room room_of(const OrthMatrix &m, Way way, int count, void *scratch) {
     Room r = {};
+    Scratch room = {static_cast<unsigned char *>(scratch)};
     const uint64_t s = std::min(m.rows, m.cols), n = (uint64_t)count;
-    unsigned char *base = static_cast<unsigned char *>(scratch);
-    const auto take = [&](uint64_t bytes) {
-        unsigned char *p = base + r.bytes;
-        r.bytes += up(bytes, 128);
-        return p;
-    };
-    r.parts = reinterpret_cast<double *>(take(n * kNormParts * 8));
+    r.parts = room.take<double>(n * kNormParts);
     if (way == kSmall) {
         r.small.slices = orth_small_slices(std::max(m.rows, m.cols), &r.small.per);
-        r.small.sums = reinterpret_cast<float *>(take(n * (uint64_t)r.small.slices * s * s * 4));
-        r.small.sum = reinterpret_cast<float *>(take(n * s * s * 4));
-        r.small.r = reinterpret_cast<float *>(take(n * s * s * 4));
-        r.small.identity = reinterpret_cast<float *>(take(n * 4));
+        r.small.sums = room.take<float>(n * (uint64_t)r.small.slices * s * s);
+        r.small.sum = room.take<float>(n * s * s);
+        r.small.r = room.take<float>(n * s * s);
+        r.small.identity = room.take<float>(n);
+        r.bytes = room.used;
         return r;
     }
-    const bool split = way == kSplit;
-    r.ld_x = up(m.cols, 16);
+    r.ld_x = padded(m.cols, 16);
     r.apart_x = m.rows * r.ld_x;
-    r.ld_a = up(s, 16);
+    r.ld_a = padded(s, 16);
     r.apart_a = s * r.ld_a;
     for (int i = 0; i < 2; ++i) {
-        r.high[i] = reinterpret_cast<unsigned short *>(take(n * r.apart_x * 2));
-        r.low[i] = reinterpret_cast<unsigned short *>(take(n * r.apart_x * 2));
+        r.high[i] = room.take<unsigned short>(n * r.apart_x);
+        r.low[i] = room.take<unsigned short>(n * r.apart_x);
     }
-    for (int i = 0; i < (split ? 2 : 1); ++i) {
-        r.a[i] = reinterpret_cast<unsigned short *>(take(n * r.apart_a * 2));
-        r.p[i] = reinterpret_cast<unsigned short *>(take(n * r.apart_a * 2));
+    for (int i = 0; i < (way == kSplit ? 2 : 1); ++i) {
+        r.a[i] = room.take<unsigned short>(n * r.apart_a);
+        r.p[i] = room.take<unsigned short>(n * r.apart_a);
     }
-    r.factor = reinterpret_cast<float *>(take(n * 4));
-    r.rest = reinterpret_cast<float *>(take(n * r.ld_a * 4));
-    r.of_high = reinterpret_cast<float *>(take(n * r.ld_a * 4));
-    r.of_low = reinterpret_cast<float *>(take(n * r.ld_a * 4));
+    r.factor = room.take<float>(n);
+    r.rest = room.take<float>(n * r.ld_a);
+    r.of_high = room.take<float>(n * r.ld_a);
+    r.of_low = room.take<float>(n * r.ld_a);
+    r.bytes = room.used;
     return r;
 }
 

@@ -498,19 +498,7 @@ __global__ void __launch_bounds__(256) align_rows_kernel(const unsigned short *i
 }
 
 // ---- host ----
-uint64_t padded(uint64_t n, uint64_t to) { return (n + to - 1) / to * to; }
 bool needs_copy(const void *p, uint64_t rows, uint64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 != 0 || (rows > 1 && ld % 8 != 0); }
-
-// Scratch, handed out piece by piece on 128 bytes
-struct Scratch {
-    unsigned char *base;
-    size_t used = 0;
-    template <class T> T *take(uint64_t count) {
-        T *p = reinterpret_cast<T *>(base + used);
-        used += padded(count * sizeof(T), 128);
-        return p;
-    }
-};
 
 struct Operands {
     Stack x, w;
